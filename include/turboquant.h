@@ -444,6 +444,106 @@ int tq_launch_attention_ref(const uint16_t* query, const uint16_t* key, const ui
                             int num_queries, int num_kv_tokens, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* Operators of a speculative decode step around the paged caches (superset  */
+/* of the reference ABI, whose entries take keys that are already rotated    */
+/* and give every query row one contiguous kv length): per-head norm and     */
+/* rotation of queries and keys, the same with the append to dense pages,    */
+/* and the attention of a tree of drafted tokens.  Inference only.           */
+/* ---------------------------------------------------------------------- */
+
+/* 16-bit element types of the entries below (dense pages hold either). */
+enum { TQ_DTYPE_FP16 = 0, TQ_DTYPE_BF16 = 1 };
+
+typedef struct TQRopeConfig {
+    int dtype;        /* TQ_DTYPE_* of query, key, value, weights and outputs          */
+    int num_q_heads;  /* query heads (the kv heads and head_dim are TQConfig's)         */
+    int rot_dim;      /* rotated leading dims of a head: even, 2 <= rot_dim <= head_dim */
+    int interleaved;  /* 0: pairs (i, i + rot_dim/2); otherwise pairs (2i, 2i + 1)      */
+    int max_position; /* rows of the cos_sin table                                      */
+    float eps;        /* of the RMS norm, >= 0                                          */
+} TQRopeConfig;
+
+/* Per (token, head) row x of query [num_tokens, num_q_heads, D] and key
+ * [num_tokens, H, D]: if its weight (D values) is not NULL,
+ * x * w / sqrt(mean(x^2) + eps); then every pair (a, b) of the first rot_dim
+ * dims becomes (a cos - b sin, a sin + b cos) with the angle of pair i at the
+ * token's position: cos = cos_sin[position][i], sin =
+ * cos_sin[position][rot_dim/2 + i] (fp32 [max_position, rot_dim]).  Computed
+ * in fp32 and rounded once.  Strides are elements from one token to the next
+ * (heads are contiguous), so query and key may be views of a fused projection.
+ * An output may be its own input (same pointer and stride); otherwise outputs
+ * overlap neither inputs nor each other.  A token whose position is outside
+ * [0, max_position) is skipped: its outputs stay as they were.  num_tokens 0
+ * does nothing.  Any head_dim a power of two in [2, 128]; fastest with head_dim
+ * 64 or 128 = rot_dim and 16-byte aligned pointers and strides. */
+int tq_launch_qk_norm_rope(const void* query, int64_t query_stride, const void* key,
+                           int64_t key_stride, const void* q_weight, const void* k_weight,
+                           const float* cos_sin, const int32_t* positions, void* out_query,
+                           int64_t out_query_stride, void* out_key, int64_t out_key_stride,
+                           const TQRopeConfig* rope, const TQConfig* cfg, int num_tokens,
+                           void* stream);
+
+/* tq_launch_qk_norm_rope with the rotated keys, and the values
+ * [num_tokens, H, D] as they are, written into the dense pages named by
+ * slot_mapping (as tq_launch_dense_store_kv; the pages hold rope->dtype).
+ * query and out_query may both be NULL (keys and values only).  A token with a
+ * negative slot stores nothing (its query is still rotated); one with a
+ * position outside the table is skipped whole.  Slots are distinct. */
+int tq_launch_dense_rope_append_kv(const void* query, int64_t query_stride, const void* key,
+                                   int64_t key_stride, const void* value, int64_t value_stride,
+                                   const void* q_weight, const void* k_weight,
+                                   const float* cos_sin, const int32_t* positions,
+                                   const int32_t* slot_mapping, uint8_t* page_pool,
+                                   void* out_query, int64_t out_query_stride,
+                                   const TQDensePageLayout* layout, const TQRopeConfig* rope,
+                                   const TQConfig* cfg, int num_tokens, void* stream);
+
+/* Attention of drafted token trees over a paged cache: softmax(q k^T /
+ * sqrt(D)) v.  query / output [num_tokens, num_q_heads, D]; query head i reads
+ * kv head i / (num_q_heads / H) (num_q_heads a multiple of H).  Sequence s
+ * owns the rows row_start[s] .. row_start[s + 1] - 1 (row_start: num_seqs + 1
+ * non-decreasing values from 0), its n_s drafted tokens, whose keys and values
+ * are in its pages behind its prefix_len[s] (>= 0) committed tokens: drafted
+ * token j is token prefix_len[s] + j of the sequence (pages as in the paged
+ * entries: token t at position t % block_size of page
+ * block_tables[s * max_blocks_per_seq + t / block_size]).  A row attends the
+ * whole prefix and drafted token j < n_s of its sequence where bit j % 32 of
+ * tree_mask[row * mask_words + j / 32] is set: a row attends itself only if its
+ * own bit says so.  Tokens past 32 * mask_words drafted ones have no bit.  Rows
+ * that attend nothing get 0; rows past row_start[num_seqs] stay as they were.
+ * max_kv_len >= every prefix_len[s] + n_s sizes the launch (tokens past it are
+ * not attended) and must fit in max_blocks_per_seq pages.  A token whose page
+ * id is negative is not attended; other page ids are valid.  Masked and unused
+ * tokens never reach a row, whatever their pages hold (NaN, infinities).
+ * head_dim 64 or 128; page_pool, the page size and the regions' offsets 16-byte
+ * aligned for dense pages, 2-byte aligned for compressed ones; query and output
+ * 16-byte aligned.  The dense entry takes fp16 or bf16 (dtype, TQ_DTYPE_*, of
+ * query, pages and output), the others fp16.  num_seqs or num_tokens 0 does
+ * nothing.  Split-K partials in the per-stream workspace, as the other
+ * attention entries (tq_workspace_release). */
+int tq_launch_dense_tree_attention(const void* query, const uint8_t* page_pool,
+                                   const int32_t* block_tables, int max_blocks_per_seq,
+                                   const int32_t* row_start, const int32_t* prefix_len,
+                                   const int32_t* tree_mask, int mask_words, void* output,
+                                   const TQDensePageLayout* layout, const TQConfig* cfg, int dtype,
+                                   int num_q_heads, int num_seqs, int num_tokens, int max_kv_len,
+                                   void* stream);
+int tq_launch_turbo_prod_tree_attention(const uint16_t* query, const uint8_t* page_pool,
+                                        const int32_t* block_tables, int max_blocks_per_seq,
+                                        const int32_t* row_start, const int32_t* prefix_len,
+                                        const int32_t* tree_mask, int mask_words, uint16_t* output,
+                                        const TQTurboProdPageLayout* layout, const TQConfig* cfg,
+                                        int num_q_heads, int num_seqs, int num_tokens,
+                                        int max_kv_len, void* stream);
+int tq_launch_turbo_mse_tree_attention(const uint16_t* query, const uint8_t* page_pool,
+                                       const int32_t* block_tables, int max_blocks_per_seq,
+                                       const int32_t* row_start, const int32_t* prefix_len,
+                                       const int32_t* tree_mask, int mask_words, uint16_t* output,
+                                       const TQTurbomsePageLayout* layout, const TQConfig* cfg,
+                                       int num_q_heads, int num_seqs, int num_tokens,
+                                       int max_kv_len, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* On-disk CAG store (superset of the reference ABI).  The reference reads  */
 /* and writes these files in Python (tq_backend/cag_store.py); these        */
 /* entries produce and consume the same files from C/C++:                   */

@@ -37,7 +37,8 @@ HIPCC_FLAGS = [
 ]
 
 SOURCES = ["tq_capi.cpp", "tq_pool.cpp", "tq_loader.cpp", "tq_store.cpp", "tq_launch_cxx.cpp",
-           "tq_codec.hip", "tq_legacy.hip", "tq_attention.hip", "tq_noalloc.hip"]
+           "tq_codec.hip", "tq_legacy.hip", "tq_attention.hip", "tq_noalloc.hip", "tq_rope.hip",
+           "tq_tree.hip"]
 
 
 def _hipcc() -> str:

@@ -95,6 +95,19 @@ class TQDensePageLayout(ctypes.Structure):
         "elem_bytes", "k_offset", "v_offset", "k_bytes", "v_bytes", "page_size_bytes")]
 
 
+class TQRopeConfig(ctypes.Structure):
+    """include/turboquant.h: the norm and rotation of queries and keys."""
+
+    _fields_ = [
+        ("dtype", c_int),  # 0 fp16, 1 bf16
+        ("num_q_heads", c_int),
+        ("rot_dim", c_int),
+        ("interleaved", c_int),
+        ("max_position", c_int),
+        ("eps", c_float),
+    ]
+
+
 class TQStoreFormat(ctypes.Structure):
     """Format record of the on-disk store (.bin footer, .meta keys)."""
 
@@ -218,6 +231,26 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                                  _P(TQDensePageLayout), _P(TQConfig), c_int, c_void_p], c_int),
     "tq_launch_attention_ref": ([c_void_p, c_void_p, c_void_p, c_void_p, _P(c_float),
                                  _P(TQConfig), c_int, c_int, c_void_p], c_int),
+    # a speculative step around the caches: norm + rotation, append, tree attention
+    "tq_launch_qk_norm_rope": ([c_void_p, _I64, c_void_p, _I64, c_void_p, c_void_p, _P(c_float),
+                                _P(c_int32), c_void_p, _I64, c_void_p, _I64, _P(TQRopeConfig),
+                                _P(TQConfig), c_int, c_void_p], c_int),
+    "tq_launch_dense_rope_append_kv": ([c_void_p, _I64, c_void_p, _I64, c_void_p, _I64, c_void_p,
+                                        c_void_p, _P(c_float), _P(c_int32), _P(c_int32),
+                                        _P(c_uint8), c_void_p, _I64, _P(TQDensePageLayout),
+                                        _P(TQRopeConfig), _P(TQConfig), c_int, c_void_p], c_int),
+    "tq_launch_dense_tree_attention": ([c_void_p, _P(c_uint8), _P(c_int32), c_int, _P(c_int32),
+                                        _P(c_int32), _P(c_int32), c_int, c_void_p,
+                                        _P(TQDensePageLayout), _P(TQConfig), c_int, c_int, c_int,
+                                        c_int, c_int, c_void_p], c_int),
+    "tq_launch_turbo_prod_tree_attention": ([c_void_p, _P(c_uint8), _P(c_int32), c_int,
+                                             _P(c_int32), _P(c_int32), _P(c_int32), c_int,
+                                             c_void_p, _P(TQTurboProdPageLayout), _P(TQConfig),
+                                             c_int, c_int, c_int, c_int, c_void_p], c_int),
+    "tq_launch_turbo_mse_tree_attention": ([c_void_p, _P(c_uint8), _P(c_int32), c_int,
+                                            _P(c_int32), _P(c_int32), _P(c_int32), c_int,
+                                            c_void_p, _P(TQTurbomsePageLayout), _P(TQConfig),
+                                            c_int, c_int, c_int, c_int, c_void_p], c_int),
     # on-disk store (tq_backend/cag_store.py formats)
     "tq_store_sha256_hex": ([c_void_p, c_size_t, ctypes.c_char_p], c_int),
     "tq_store_key": ([ctypes.c_char_p, c_int, ctypes.c_char_p, ctypes.c_char_p, c_size_t], c_int),
@@ -248,6 +281,44 @@ def _ready(t, dtype: torch.dtype, numel: int) -> bool:
     "cuda", without making a device object and its string on every call)."""
     return (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.is_contiguous()
             and t.numel() >= numel)
+
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # TQ_DTYPE_*
+
+
+def rope_table(max_position: int, rot_dim: int, base: float = 10000.0, inv_freq=None,
+               device=None) -> torch.Tensor:
+    """The cos_sin table of the rotation entries: [max_position, rot_dim] fp32,
+    row p holding cos(p f_i) then sin(p f_i) for i < rot_dim / 2, with
+    f_i = base^(-2i / rot_dim), or inv_freq's values (scaled frequencies).
+    Angles in float64: a fp32 angle of position 32,768 is off by up to 2e-3."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rope_table: rot_dim must be even and >= 2")
+    if inv_freq is None:
+        f = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    else:
+        f = torch.as_tensor(inv_freq).detach().to("cpu", torch.float64)
+        if f.shape != (rot_dim // 2,):
+            raise ValueError(f"rope_table: inv_freq must hold {rot_dim // 2} values")
+    a = torch.arange(max_position, dtype=torch.float64)[:, None] * f
+    return torch.cat([a.cos(), a.sin()], 1).to(device=device, dtype=torch.float32)
+
+
+def tree_mask_from_parents(parents) -> torch.Tensor:
+    """The tree_mask rows of one sequence's drafted tokens, [n, ceil(n / 32)]
+    int32 (on the CPU): parents[j] is the index of token j's parent among them
+    (< j), or -1 for a child of the prefix; bit i of row j is set for j and its
+    ancestors."""
+    p = [int(x) for x in parents]
+    words = max(1, (len(p) + 31) // 32)
+    rows = []
+    for j, up in enumerate(p):
+        if not -1 <= up < j:
+            raise ValueError(f"tree_mask_from_parents: parents[{j}] = {up} is not in [-1, {j})")
+        rows.append((rows[up] if up >= 0 else 0) | 1 << j)
+    out = [[(r >> 32 * w & 0xFFFFFFFF) - (r >> 32 * w + 31 & 1) * (1 << 32) for w in range(words)]
+           for r in rows]
+    return torch.tensor(out, dtype=torch.int32).reshape(len(p), words)
 
 
 def _ready_pointers(tensors, dtype: torch.dtype, numel: int):
@@ -644,6 +715,172 @@ class TurboQuantWrapper:
                 self._stream(stream))
         if rc != 0:
             self._kernel_raise(rc, scheme, "paged_attn_output")
+
+    # ── a speculative step: norm + rotation, append, tree attention ──── #
+
+    @staticmethod
+    def _token_rows(scheme, op, name, t, dtype, tokens, heads, dim):
+        """(pointer, token stride) of [tokens, heads, dim] rows: dims and heads
+        contiguous, any distance between tokens (a view of a fused projection)."""
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{scheme} {op}: {name} must be a GPU tensor")
+        if t.dtype is not dtype:
+            raise ValueError(f"{scheme} {op}: {name} must be {dtype}, got {t.dtype}")
+        if t.shape != (tokens, heads, dim):
+            raise ValueError(f"{scheme} {op}: {name} must be [{tokens}, {heads}, {dim}], got "
+                             f"{list(t.shape)}")
+        st = t.stride()
+        if tokens and (st[2] != 1 or (st[1] != dim and heads > 1)
+                       or (tokens > 1 and st[0] < heads * dim)):
+            raise ValueError(f"{scheme} {op}: {name} must have contiguous heads and distinct tokens")
+        return t.data_ptr(), st[0]
+
+    @staticmethod
+    def _on_one_device(scheme, op, first, *others):
+        """A launch runs on the current device: every tensor must live there."""
+        dev = first.get_device()
+        for t in others:
+            if t is not None and t.get_device() != dev:
+                raise ValueError(f"{scheme} {op}: tensors on different GPUs")
+        if dev != torch.cuda.current_device():
+            raise ValueError(f"{scheme} {op}: tensors on GPU {dev}, the current device is "
+                             f"{torch.cuda.current_device()}")
+
+    def _rope_args(self, scheme, op, key, positions, cos_sin, cfg, q_heads, q_weight, k_weight, eps,
+                   interleaved):
+        """(TQRopeConfig, weight pointers) after the checks both rotation entries share."""
+        if not isinstance(key, torch.Tensor) or key.dtype not in _DTYPES:
+            raise ValueError(f"{scheme} {op}: key must be a float16 or bfloat16 tensor")
+        if key.dim() != 3:
+            raise ValueError(f"{scheme} {op}: key must be [num_tokens, num_kv_heads, head_dim]")
+        N, D = key.shape[0], cfg.head_dim
+        if not isinstance(cos_sin, torch.Tensor) or cos_sin.dim() != 2:
+            raise ValueError(f"{scheme} {op}: cos_sin must be [max_position, rot_dim]")
+        self._check(scheme, op, positions=(positions, torch.int32, N),
+                    cos_sin=(cos_sin, torch.float32, cos_sin.numel()))
+        w = []
+        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None:
+                self._check(scheme, op, **{name: (t, key.dtype, D)})
+            w.append(t.data_ptr() if t is not None else None)
+        rope = TQRopeConfig(_DTYPES[key.dtype], q_heads, cos_sin.shape[1], int(bool(interleaved)),
+                            cos_sin.shape[0], eps)
+        return rope, w
+
+    def qk_norm_rope(self, query, key, positions, cos_sin, out_query, out_key, cfg, q_weight=None,
+                     k_weight=None, eps: float = 1e-6, interleaved: bool = False,
+                     stream: int = 0) -> None:
+        """Per-head RMS norm (where a weight [D] is given) and rotation of query
+        [N, Hq, D] and key [N, H, D] (fp16 or bf16; views of a fused projection
+        allowed) at the tokens' positions, into out_query and out_key (which may
+        be the inputs).  cos_sin: rope_table's; its width is the rotated part of
+        a head.  A token at a position outside the table is skipped."""
+        op = "qk_norm_rope"
+        if not isinstance(query, torch.Tensor) or query.dim() != 3:
+            raise ValueError(f"rope {op}: query must be [num_tokens, num_q_heads, head_dim]")
+        N, Hq = query.shape[:2]
+        H, D = cfg.num_kv_heads, cfg.head_dim
+        rope, w = self._rope_args("rope", op, key, positions, cos_sin, cfg, Hq, q_weight, k_weight,
+                                  eps, interleaved)
+        q, qs = self._token_rows("rope", op, "query", query, key.dtype, N, Hq, D)
+        k, ks = self._token_rows("rope", op, "key", key, key.dtype, N, H, D)
+        oq, oqs = self._token_rows("rope", op, "out_query", out_query, key.dtype, N, Hq, D)
+        ok, oks = self._token_rows("rope", op, "out_key", out_key, key.dtype, N, H, D)
+        self._on_one_device("rope", op, query, key, positions, cos_sin, out_query, out_key, q_weight,
+                            k_weight)
+        if N == 0:
+            return
+        rc = self._fast.tq_launch_qk_norm_rope(
+            q, qs, k, ks, w[0], w[1], cos_sin.data_ptr(), positions.data_ptr(), oq, oqs, ok, oks,
+            ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
+        if rc != 0:
+            self._kernel_raise(rc, "rope", op)
+
+    def dense_rope_append(self, query, key, value, positions, slot_mapping, cos_sin, out_query,
+                          page_pool, layout, cfg, q_weight=None, k_weight=None, eps: float = 1e-6,
+                          interleaved: bool = False, stream: int = 0) -> None:
+        """qk_norm_rope with the rotated keys, and the values as they are, written
+        into the dense pages named by slot_mapping (pages of key's dtype); query
+        and out_query may both be None.  A negative slot stores nothing."""
+        op = "rope_append"
+        if (query is None) != (out_query is None):
+            raise ValueError(f"dense {op}: query and out_query go together")
+        if query is not None and (not isinstance(query, torch.Tensor) or query.dim() != 3):
+            raise ValueError(f"dense {op}: query must be [num_tokens, num_q_heads, head_dim]")
+        H, D = cfg.num_kv_heads, cfg.head_dim
+        Hq = query.shape[1] if query is not None else 1
+        rope, w = self._rope_args("dense", op, key, positions, cos_sin, cfg, Hq, q_weight, k_weight,
+                                  eps, interleaved)
+        N = key.shape[0]
+        self._check("dense", op, slot_mapping=(slot_mapping, torch.int32, N),
+                    page_pool=(page_pool, torch.uint8, 0))
+        q, qs, oq, oqs = None, 0, None, 0
+        if query is not None:
+            q, qs = self._token_rows("dense", op, "query", query, key.dtype, N, Hq, D)
+            oq, oqs = self._token_rows("dense", op, "out_query", out_query, key.dtype, N, Hq, D)
+        k, ks = self._token_rows("dense", op, "key", key, key.dtype, N, H, D)
+        v, vs = self._token_rows("dense", op, "value", value, key.dtype, N, H, D)
+        self._on_one_device("dense", op, key, query, value, positions, slot_mapping, cos_sin,
+                            out_query, page_pool, q_weight, k_weight)
+        if N == 0:
+            return
+        rc = self._fast.tq_launch_dense_rope_append_kv(
+            q, qs, k, ks, v, vs, w[0], w[1], cos_sin.data_ptr(), positions.data_ptr(),
+            slot_mapping.data_ptr(), page_pool.data_ptr(), oq, oqs, ctypes.byref(layout),
+            ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
+        if rc != 0:
+            self._kernel_raise(rc, "dense", op)
+
+    def tree_attn_output(self, scheme: str, query, page_pool, block_tables, row_start, prefix_len,
+                         tree_mask, output, layout, cfg, max_kv_len: int, stream: int = 0) -> None:
+        """Attention of every sequence's drafted tokens over its prefix and, by
+        tree_mask, its drafted tokens (one launch and a merge).
+
+        scheme "dense" (query fp16 or bf16, the pages' type), "turbo_prod" or
+        "turbo_mse" (fp16).  query / output [num_tokens, Hq, D]; sequence s owns
+        rows row_start[s] .. row_start[s + 1] - 1, its drafted tokens, cached
+        behind its prefix_len[s] tokens; row r attends drafted token j where bit
+        j % 32 of tree_mask[r, j // 32] is set (tree_mask_from_parents).
+        block_tables [num_seqs, max_blocks] int32 page ids."""
+        op = "tree_attn_output"
+        if scheme not in ("dense", "turbo_prod", "turbo_mse"):
+            raise ValueError(f"{scheme} {op}: no such scheme")
+        D = cfg.head_dim
+        if not isinstance(query, torch.Tensor) or query.dim() != 3 or query.shape[2] != D:
+            raise ValueError(f"{scheme} {op}: query must be [num_tokens, num_q_heads, {D}]")
+        if query.dtype not in (_DTYPES if scheme == "dense" else (torch.float16,)):
+            raise ValueError(f"{scheme} {op}: query must not be {query.dtype}")
+        for name, t in (("block_tables", block_tables), ("tree_mask", tree_mask)):
+            if not isinstance(t, torch.Tensor) or t.dim() != 2:
+                raise ValueError(f"{scheme} {op}: {name} must have two dimensions")
+        N, Hq = query.shape[:2]
+        S = block_tables.shape[0]
+        if tree_mask.shape[0] < N:
+            raise ValueError(f"{scheme} {op}: tree_mask has {tree_mask.shape[0]} rows, needs {N}")
+        self._check(scheme, op, query=(query, query.dtype, N * Hq * D),
+                    page_pool=(page_pool, torch.uint8, 0),
+                    block_tables=(block_tables, torch.int32, 0),
+                    row_start=(row_start, torch.int32, S + 1),
+                    prefix_len=(prefix_len, torch.int32, S),
+                    tree_mask=(tree_mask, torch.int32, 0),
+                    output=(output, query.dtype, N * Hq * D))
+        self._on_one_device(scheme, op, query, page_pool, block_tables, row_start, prefix_len,
+                            tree_mask, output)
+        if N == 0 or S == 0:
+            return
+        args = [query.data_ptr(), page_pool.data_ptr(), block_tables.data_ptr(),
+                block_tables.shape[1], row_start.data_ptr(), prefix_len.data_ptr(),
+                tree_mask.data_ptr(), tree_mask.shape[1], output.data_ptr(), ctypes.byref(layout),
+                ctypes.byref(cfg)]
+        tail = [Hq, S, N, max_kv_len, self._stream(stream)]
+        if scheme == "dense":
+            rc = self._fast.tq_launch_dense_tree_attention(*args, _DTYPES[query.dtype], *tail)
+        elif scheme == "turbo_prod":
+            rc = self._fast.tq_launch_turbo_prod_tree_attention(*args, *tail)
+        else:
+            rc = self._fast.tq_launch_turbo_mse_tree_attention(*args, *tail)
+        if rc != 0:
+            self._kernel_raise(rc, scheme, op)
 
     # ── the reference's unexported kernels ──────────────────────────── #
     # QJL-1b (include/tq_qjl.cuh), legacy INT4 (include/tq_layout.h), dense
