@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tq_device.h"
 
@@ -26,129 +27,904 @@ struct TreeArgs {
     const int32_t *tables, *row_start, *prefix, *mask;
     uint16_t* out;
     PageGeom g;  // dense pages: kc_off, vc_off and code_stride of fp16/bf16 rows
-    int max_blocks, mask_words, hq, seqs, tokens, max_kv;
+    int max_blocks, mask_words, hq, group, seqs, tokens, max_kv;  // group: query heads per kv head
 };
 
+// Base-2 exponent and logarithm as the hardware computes them (~1 ulp).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) u4 lds_u4;
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+// C += A B, A [16 x 32] by rows, B [32 x 16] by columns: lane l holds row
+// (column) l % 16, k = 8 (l / 16) + 0..7; of C column l % 16, rows
+// 4 (l / 16) + 0..3.
 template <bool BF>
-__device__ __forceinline__ float to_float(uint16_t x) {
-    return BF ? __uint_as_float((uint32_t)x << 16) : h2f(x);
-}
-template <bool BF>
-__device__ __forceinline__ uint16_t from_float(float f) {
-    if constexpr (BF) return __builtin_bit_cast(uint16_t, (__bf16)f);
-    return f2h(f);
+__device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a),
+                                                       __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
+                                                      __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// Element d of a cell's K or V row.
-template <int FMT>
-__device__ float cell_value(const TreeArgs& a, const uint8_t* page, int cell, int d, bool key) {
-    const PageGeom& g = a.g;
-    const uint8_t* row = page + (key ? g.kc_off : g.vc_off) + (size_t)cell * g.code_stride;
-    if constexpr (FMT == kFp16 || FMT == kBf16) return to_float<FMT == kBf16>(ld_u16(row + 2 * d));
-    const int n = (row[d >> 1] >> (4 * (d & 1))) & 15;
-    const float s = h2f(ld_u16(page + (key ? g.ks_off : g.vs_off) + (size_t)cell * 2));
-    if (FMT == kProd && key) {
-        const float e = h2f(ld_u16(page + g.kres_off + (size_t)cell * 2));
-        return (pick(kK3, n & 7) + (n & 8 ? e : -e)) * s;
+// Two fp32 -> packed fp16 or bf16, to nearest even, a in the low half.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF) {
+        typedef float f2v __attribute__((ext_vector_type(2)));
+        typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v){a, b}, b2v));
+    } else {
+        return f2h2(a, b);
     }
-    return pick(kV4, n) * s;
 }
 
-// One wave per (row, query head).
-template <int FMT, int D>
-__global__ __launch_bounds__(64) void tree_rows_kernel(const TreeArgs a, float inv) {
-    __shared__ float q[D];
-    const int r = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x;
-    const int h = hq / (a.hq / a.g.H);
-    // The row's sequence: the starts are non-decreasing.
-    int s = 0;
-    for (int b = 0; b < a.seqs; b += 64)
-        s += __popcll(__ballot(b + lane < a.seqs && a.row_start[1 + b + lane] <= r));
-    if (s >= a.seqs || r < a.row_start[s]) return;
-    const int n = min(a.row_start[s + 1], a.tokens) - a.row_start[s];
-    const int L = max(a.prefix[s], 0);
-    const int end = (int)min((long long)L + n, (long long)a.max_kv);
-    constexpr bool turned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
-    auto rotate = [&] {  // q = WHT(q) / sqrt(D), lane pairs through LDS
-        for (int m = 1; m < D; m <<= 1) {
-            __syncthreads();
-            for (int i = lane; i < D / 2; i += 64) {
-                const int lo = (i / m) * 2 * m + i % m;
-                const float u = q[lo], w = q[lo + m];
-                q[lo] = u + w;
-                q[lo + m] = u - w;
+// All ones in the halves of x that are infinite or NaN.
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    return ((x & E) == E ? 0xffffu : 0u) | ((x >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+// 1.0 in the halves of x that are NaN or infinite with sign `neg`.
+template <bool BF>
+__device__ __forceinline__ uint32_t infinite_ones(uint32_t x, uint32_t neg) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u, one = BF ? 0x3f80u : 0x3c00u;
+    uint32_t r = 0;
+#pragma unroll
+    for (int k = 0; k < 32; k += 16) {
+        const uint32_t v = x >> k & 0xffffu, m = v & 0x7fffu;
+        r |= (m > E || (m == E && v >> 15 == neg)) ? one << k : 0u;
+    }
+    return r;
+}
+
+// One butterfly stage with lane ^ M.
+template <int M>
+__device__ __forceinline__ float butterfly(float v, int lane) {
+    const float o = lane_xor<M>(v);
+    return (lane & M) ? o - v : v + o;
+}
+
+// ---------------------------------------------------------------------------
+// Work of a launch.  An item is one (kv head, sequence, tile of M query rows),
+// its chunks of C tokens.  Items lie one behind the other (by head, sequence,
+// tile), and workgroup w takes the chunks [w per, (w + 1) per) of that line:
+// the same work for every workgroup, whatever the lengths, which only the
+// device knows.  A piece is a workgroup's part of an item; only its first and
+// its last piece can be cut.
+// ---------------------------------------------------------------------------
+struct Tiling {
+    int m_log, c_log;  // log2 of M, C
+    int groups;        // workgroups of the split launch
+    int least;         // fewest chunks a workgroup takes
+};
+struct Plan {
+    int total;  // chunks of one head's items
+    int per;    // chunks of a workgroup
+};
+// One sequence per lane, from sequence `first` on.
+struct SeqBlock {
+    int first;
+    int row0, rows, L, end;  // first token row, drafted tokens, prefix length, kv end
+    int chunks, tiles;
+    int before;  // chunks of the head's items before this sequence
+};
+
+__device__ __forceinline__ SeqBlock load_seqs(const TreeArgs& a, const Tiling& g, int first,
+                                              int before, int lane, int& after) {
+    SeqBlock b;
+    b.first = first;
+    const int s = min(first + lane, a.seqs - 1);
+    const int r0 = a.row_start[s], r1 = a.row_start[s + 1], L = a.prefix[s];
+    b.row0 = min(max(r0, 0), a.tokens);
+    b.rows = first + lane < a.seqs ? max(min(r1, a.tokens) - b.row0, 0) : 0;
+    b.L = max(L, 0);
+    b.end = (int)min((long long)b.L + b.rows, (long long)a.max_kv);
+    b.chunks = max((b.end + (1 << g.c_log) - 1) >> g.c_log, 1);
+    b.tiles = (b.rows * a.group + (1 << g.m_log) - 1) >> g.m_log;
+    const int cost = b.tiles * b.chunks;
+    int up = cost;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int u = __shfl_up(up, m, 64);
+        up += lane >= m ? u : 0;
+    }
+    b.before = before + up - cost;
+    after = before + __builtin_amdgcn_readlane(up, 63);
+    return b;
+}
+
+__device__ __forceinline__ Plan make_plan(const TreeArgs& a, const Tiling& g, int total) {
+    Plan p;
+    p.total = total;
+    const long long all = (long long)total * a.g.H;
+    p.per = max((int)((all + g.groups - 1) / g.groups), g.least);
+    return p;
+}
+
+// A piece, the same in every lane.
+struct Piece {
+    int h, s, row0, rows, L, end;
+    int tile, chunk, chunks;  // first chunk of the piece; chunks of its item
+};
+__device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, const Plan& p, int at,
+                                        int lane, SeqBlock& b) {
+    Piece o;
+    o.h = at / p.total;
+    const int x = at - o.h * p.total;
+    if (a.seqs > 64) {
+        int after;
+        if (__builtin_amdgcn_readlane(b.before, 0) > x)  // the next head: from the start
+            b = load_seqs(a, g, 0, 0, lane, after);
+        while (true) {
+            after = __builtin_amdgcn_readlane(b.before + b.tiles * b.chunks, 63);
+            if (x < after || b.first + 64 >= a.seqs) break;
+            b = load_seqs(a, g, b.first + 64, after, lane, after);
+        }
+    }
+    // The last sequence that begins at or before x: one without work begins
+    // where its successor does, so it is the last only if x is past all work.
+    const int k = max(__popcll(__ballot(b.before <= x && b.first + lane < a.seqs)) - 1, 0);
+    o.s = b.first + k;
+    o.row0 = __builtin_amdgcn_readlane(b.row0, k);
+    o.rows = __builtin_amdgcn_readlane(b.rows, k);
+    o.L = __builtin_amdgcn_readlane(b.L, k);
+    o.end = __builtin_amdgcn_readlane(b.end, k);
+    o.chunks = __builtin_amdgcn_readlane(b.chunks, k);
+    const int y = x - __builtin_amdgcn_readlane(b.before, k);
+    o.tile = y / o.chunks;
+    o.chunk = y - o.tile * o.chunks;
+    return o;
+}
+
+// ---------------------------------------------------------------------------
+// The split kernel: four waves, WR of them side by side over the tile's rows
+// (16 RT each), 4 / WR over a chunk's tokens (T each).  Both products run
+// transposed: S' = K Q' has a query row per lane column and four tokens in a
+// lane's registers, so a row's softmax is in-lane but for two lane swaps, and
+// the registers are the B operand of O' = V' P' as they are (the k-order of a
+// 32-token step is 4 (l / 16) + 0..3 of either 16 tokens; V' is read from its
+// token rows in that order by transposing LDS loads).
+// ---------------------------------------------------------------------------
+template <int FMT, int D, int RT, int WR>
+struct Shape {
+    static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
+    static constexpr int WT = 4 / WR;
+    static constexpr int T = WR == 4 ? 64 : 32, C = T * WT, M = 16 * RT * WR;
+    static constexpr int kRow = 2 * D, kTile = C * kRow;
+    static constexpr int kTiles = kTurned ? 3 : 4;  // K hi, K lo, V; or K, V twice
+    static constexpr int kMerge = WT > 1 ? WT * M * (D + 4) * 4 : 0;
+    static constexpr int kLds = kTiles * kTile > kMerge ? kTiles * kTile : kMerge;
+};
+
+constexpr float kAlphaV = 1.5982153f;  // alpha V4[c] is fp16-exact to 9.2e-5 for every c
+
+// 16 bytes per lane from p straight into LDS at byte `lds` + 16 lane.
+__device__ __forceinline__ void load_to_lds(const uint8_t* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void wait_vmem() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+struct DecodeTables {
+    uint32_t v[256];  // code byte -> fp16 pair of alpha V4 (low nibble first)
+    uint2 k[256];     // turbo_mse: fp16 pairs of V4, hi and lo; turbo_prod: fp32 pair of K3
+};
+struct alignas(16) TokenScales {
+    float k[128], v[128], lv[128];  // of a chunk's tokens; lv = max(log2 |v|, -25)
+};
+struct Nothing {};
+
+template <int FMT, int D, int RT, int WR>
+__global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, const Tiling tl,
+                                                            float* __restrict__ ws, float scale,
+                                                            float inv) {
+    using S = Shape<FMT, D, RT, WR>;
+    constexpr bool BF = S::BF, kTurned = S::kTurned;
+    constexpr int T = S::T, C = S::C, M = S::M, WT = S::WT, NS = T / 16, kRow = S::kRow;
+    constexpr float kOff = BF ? 0.0f : 14.0f;  // weights up to 2^14: small ones stay normal in fp16
+    __shared__ __attribute__((aligned(1024))) uint8_t mem[S::kLds];
+    __shared__ float2 ml[WT][M];
+    __shared__ typename std::conditional<kTurned, DecodeTables, Nothing>::type tab;
+    __shared__ typename std::conditional<kTurned, TokenScales, Nothing>::type tsc;
+
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, gq = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, wt = wv / WR;
+    const PageGeom& g = a.g;
+    const uint32_t mem0 = (uint32_t)(uintptr_t)(lds_u8*)mem;
+    // Chunks of a token group's rows lie in 16-byte pieces exchanged by an
+    // exclusive or with the row: the 16 rows that a load touches at one column
+    // are in different banks.
+    const auto swz = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+    const uint32_t k_at = mem0 + (wt * T + i) * kRow + ((gq ^ swz(i)) * 16);
+    const int vrow = 4 * gq + (i >> 2);
+    const uint32_t v_at = mem0 + (wt * T + vrow) * kRow + ((((i >> 1) & 1) ^ swz(vrow)) * 16) + (i & 1) * 8;
+
+    if constexpr (kTurned) {
+        const int lo = tid & 15, hi = tid >> 4;
+        tab.v[tid] = f2h2(kAlphaV * pick(kV4, lo), kAlphaV * pick(kV4, hi));
+        if constexpr (FMT == kMse) {
+            const float x = pick(kV4, lo), y = pick(kV4, hi);
+            const uint32_t h = f2h2(x, y);
+            tab.k[tid] = make_uint2(h, f2h2(x - h2f(h & 0xffff), y - h2f(h >> 16)));
+        } else {
+            tab.k[tid] = make_uint2(__float_as_uint(pick(kK3, lo & 7)), __float_as_uint(pick(kK3, hi & 7)));
+        }
+    }
+
+    SeqBlock sb;
+    int total;
+    sb = load_seqs(a, tl, 0, 0, lane, total);
+    for (int f = 64; f < a.seqs; f += 64) (void)load_seqs(a, tl, f, total, lane, total);
+    const Plan plan = make_plan(a, tl, total);
+    const int all = plan.total * g.H;
+    const long long begin = (long long)blockIdx.x * plan.per;
+    const int stop = (int)min(begin + plan.per, (long long)all);
+
+    // Bytes that can always be read, as an offset from the pool: the query's.
+    const uint64_t dummy = (uint64_t)(reinterpret_cast<uintptr_t>(a.query) - reinterpret_cast<uintptr_t>(a.pool));
+
+    bool first = true;
+    for (int at = (int)min(begin, (long long)all); at < stop;) {
+        const Piece pc = locate(a, tl, plan, at, lane, sb);
+        const int c0 = pc.chunk, c1 = min(pc.chunk + (stop - at), pc.chunks);
+        const bool whole = c1 - c0 == pc.chunks;
+        const int R = pc.rows * a.group, h = pc.h;
+        const int32_t* __restrict__ table = a.tables + (size_t)pc.s * a.max_blocks;
+        __syncthreads();  // the last piece's LDS is free (and the tables are written)
+
+        // This lane's query rows.
+        int row[RT];
+        size_t qo[RT];
+        const int32_t* mrow[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            row[rt] = pc.tile * M + (wr * RT + rt) * 16 + i;
+            const int rr = min(row[rt], R - 1), tok = rr / a.group;
+            qo[rt] = ((size_t)(pc.row0 + tok) * a.hq + h * a.group + (rr - tok * a.group)) * D;
+            mrow[rt] = a.mask + (size_t)(pc.row0 + tok) * a.mask_words;
+        }
+        const auto token_of = [&](int c) { return c * C + wt * T + (lane & (T - 1)); };
+        const auto page_of = [&](int t, int& tib) {
+            const int tc = max(min(t, pc.end - 1), 0);
+            const int pg = g.bs_shift >= 0 ? tc >> g.bs_shift : tc / g.block_size;
+            tib = tc - pg * g.block_size;
+            return pg;
+        };
+        int tib;
+        int id = table[page_of(token_of(c0), tib)];
+        const auto readable = [&](int t, int pid) { return t < pc.end && pid >= 0; };
+
+        // Compressed pages: the codes and scales of this lane's units of the
+        // next chunk (unit u: a quarter of the codes of token u / 4).
+        constexpr int KU = kTurned ? T * 4 / (WR * 64) : 1;
+        typedef uint32_t code_t __attribute__((ext_vector_type(D / 32), aligned(2)));
+        code_t kc[KU], vc[KU];
+        uint16_t ks[KU], kr[KU], vs[KU];
+        int uid[KU];
+        const auto unit_token = [&](int c, int k) {
+            return c * C + wt * T + (((wr + k * WR) * 64 + lane) >> 2);
+        };
+        const auto unit_ids = [&](int c) {
+            if constexpr (kTurned) {
+#pragma unroll
+                for (int k = 0; k < KU; ++k) {
+                    int tb;
+                    uid[k] = table[page_of(unit_token(c, k), tb)];
+                }
+            }
+        };
+        const auto fetch = [&](int c) {
+            if constexpr (kTurned) {
+#pragma unroll
+                for (int k = 0; k < KU; ++k) {
+                    int tb;
+                    const int t = unit_token(c, k);
+                    (void)page_of(t, tb);
+                    const bool ok = readable(t, uid[k]);
+                    const uint64_t page = (uint64_t)max(uid[k], 0) * g.page_size;
+                    const uint64_t cell = (uint64_t)(tb * g.H + h);
+                    const int part = (lane & 3) * (D / 8);
+                    const auto at_of = [&](uint64_t off, uint64_t n) {
+                        return a.pool + (ok ? page + off + cell * n : dummy);
+                    };
+                    kc[k] = *reinterpret_cast<const code_t*>(at_of(g.kc_off, D / 2) + part);
+                    vc[k] = *reinterpret_cast<const code_t*>(at_of(g.vc_off, D / 2) + part);
+                    ks[k] = ld_u16(at_of(g.ks_off, 2));
+                    if (FMT == kProd) kr[k] = ld_u16(at_of(g.kres_off, 2));
+                    vs[k] = ld_u16(at_of(g.vs_off, 2));
+                }
+            }
+        };
+        const auto decode = [&] {
+            if constexpr (kTurned) {
+#pragma unroll
+                for (int k = 0; k < KU; ++k) {
+                    const int r = ((wr + k * WR) * 64 + lane) >> 2;  // token of the group
+                    const int part = lane & 3;
+                    if (part == 0) tsc.k[wt * T + r] = h2f(ks[k]);
+                    if (part == 1) {
+                        const float v = h2f(vs[k]);
+                        tsc.v[wt * T + r] = v;
+                        tsc.lv[wt * T + r] = fmaxf(log2_hw(fabsf(v)), -25.0f);
+                    }
+                    uint8_t* to = mem + (wt * T + r) * kRow;
+                    const uint32_t re = FMT == kProd ? __float_as_uint(h2f(kr[k])) : 0u;
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {  // a code dword: 8 values, 16 bytes
+                        u4 hi, lo, v;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint32_t kb = kc[k][q] >> (8 * b) & 255, vb = vc[k][q] >> (8 * b) & 255;
+                            v[b] = tab.v[vb];
+                            const uint2 e = tab.k[kb];
+                            if constexpr (FMT == kMse) {
+                                hi[b] = e.x;
+                                lo[b] = e.y;
+                            } else {  // level + (sign ? re : -re)
+                                const float x = __uint_as_float(e.x) +
+                                                __uint_as_float(re ^ ((~kb & 8u) << 28));
+                                const float y = __uint_as_float(e.y) +
+                                                __uint_as_float(re ^ ((~kb & 128u) << 24));
+                                hi[b] = f2h2(x, y);
+                                lo[b] = f2h2(x - h2f(hi[b] & 0xffff), y - h2f(hi[b] >> 16));
+                            }
+                        }
+                        const int piece = ((part * (D / 32) + q) ^ swz(r)) * 16;
+                        *reinterpret_cast<u4*>(to + piece) = hi;
+                        *reinterpret_cast<u4*>(to + S::kTile + piece) = lo;
+                        *reinterpret_cast<u4*>(to + 2 * S::kTile + piece) = v;
+                    }
+                }
+            }
+        };
+        // Dense pages: the group's rows of chunk c straight into buffer c % 2.
+        const auto stage = [&](int c, int pid) {
+            if constexpr (!kTurned) {
+                int tb;
+                const int t = token_of(c);
+                (void)page_of(t, tb);
+                const uint64_t off = readable(t, pid)
+                                         ? (uint64_t)pid * g.page_size + g.kc_off +
+                                               (uint64_t)(tb * g.H + h) * kRow
+                                         : dummy;
+                const int off_lo = (int)(uint32_t)off, off_hi = (int)(off >> 32);
+                constexpr int kRows = 1024 / kRow;  // rows of one load
+                const uint32_t to = mem0 + (c & 1) * 2 * S::kTile + (wt * T + wr * (T / WR)) * kRow;
+#pragma unroll
+                for (int k = 0; k < T / WR / kRows; ++k) {
+                    const int r = wr * (T / WR) + k * kRows + lane / (kRow / 16);
+                    const uint64_t o = (uint64_t)(uint32_t)__shfl(off_lo, r, 64) |
+                                       (uint64_t)(uint32_t)__shfl(off_hi, r, 64) << 32;
+                    const int piece = ((lane % (kRow / 16)) ^ swz(r)) * 16;
+                    const uint64_t ov = o == dummy ? dummy : o + (g.vc_off - g.kc_off);
+                    load_to_lds(a.pool + o + piece, to + k * 1024);
+                    load_to_lds(a.pool + ov + piece, to + S::kTile + k * 1024);
+                }
+            }
+        };
+
+        unit_ids(c0);
+        // Query operands.
+        constexpr int KK = D / 32;
+        u4 qh[RT][KK], ql[kTurned ? RT : 1][KK];
+        float qs[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            u4 raw[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+                raw[kk] = *reinterpret_cast<const u4*>(a.query + qo[rt] + kk * 32 + gq * 8);
+            qs[rt] = scale;
+            if constexpr (!kTurned) {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) qh[rt][kk] = raw[kk];
+            } else {
+                // WHT(q s) / sqrt(D): value kk * 32 + gq * 8 + e.
+                float x[KK][8];
+                const float sh = (h & 1) ? -inv : inv;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = h2f(raw[kk][e] & 0xffff) * sh, w = h2f(raw[kk][e] >> 16) * -sh;
+                        x[kk][2 * e] = u + w;
+                        x[kk][2 * e + 1] = u - w;
+                    }
+                float top = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+                    for (int m = 2; m < 8; m <<= 1)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (!(e & m)) {
+                                const float u = x[kk][e], w = x[kk][e + m];
+                                x[kk][e] = u + w;
+                                x[kk][e + m] = u - w;
+                            }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[kk][e] = butterfly<16>(x[kk][e], lane);
+                        x[kk][e] = butterfly<32>(x[kk][e], lane);
+                    }
+                }
+#pragma unroll
+                for (int m = 1; m < KK; m <<= 1)
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk)
+                        if (!(kk & m))
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float u = x[kk][e], w = x[kk + m][e];
+                                x[kk][e] = u + w;
+                                x[kk + m][e] = u - w;
+                            }
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[kk][e]));
+                top = lane_xor_reduce<16>(top, [](float u, float w) { return fmaxf(u, w); });
+                top = lane_xor_reduce<32>(top, [](float u, float w) { return fmaxf(u, w); });
+                // A power of two brings the row's largest value into [2^13, 2^14),
+                // so hi + lo keep 22 bits of it and no row leaves fp16's range.
+                const int ex = (int)(__float_as_uint(top) >> 23) - 127;
+                const int sh2 = top > 0.0f && ex < 128 ? 13 - max(ex, -100) : 0;
+                const float up = __uint_as_float((uint32_t)(sh2 + 127) << 23);
+                qs[rt] = scale * __uint_as_float((uint32_t)(127 - sh2) << 23);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = x[kk][2 * e] * up, w = x[kk][2 * e + 1] * up;
+                        const uint32_t p = f2h2(u, w);
+                        qh[rt][kk][e] = p;
+                        ql[rt][kk][e] = f2h2(u - h2f(p & 0xffff), w - h2f(p >> 16));
+                    }
             }
         }
-        __syncthreads();
-        for (int d = lane; d < D; d += 64) q[d] *= inv;
-    };
-    const size_t ro = ((size_t)r * a.hq + hq) * D;
-    for (int d = lane; d < D; d += 64)
-        q[d] = to_float<BF>(a.query[ro + d]) * (turned ? sign_of(d, h) : 1.0f);
-    if (turned) rotate();
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[D / 64] = {};
-    for (int t0 = 0; t0 < end; t0 += 64) {
-        const int t = t0 + lane;
-        bool seen = t < end;
-        if (seen && t >= L) {
-            const int j = t - L;
-            seen = j < 32 * a.mask_words && (a.mask[(size_t)r * a.mask_words + (j >> 5)] >> (j & 31) & 1);
+
+        float m[RT], l[RT];
+        f4 o[RT][D / 16];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -INFINITY;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        int id = -1;
-        if (seen) id = a.tables[(size_t)s * a.max_blocks + t / a.g.block_size];
-        seen = seen && id >= 0;
-        const uint8_t* page = a.pool + (size_t)max(id, 0) * a.g.page_size;
-        const int cell = (t % a.g.block_size) * a.g.H + h;
-        float x = -INFINITY;
-        if (seen) {
-            x = 0.0f;
-            for (int d = 0; d < D; ++d) x = fmaf(q[d], cell_value<FMT>(a, page, cell, d, true), x);
-            x *= inv;
+
+        stage(c0, id);
+        fetch(c0);
+        int next = id;
+        if (c0 + 1 < c1) {
+            next = table[page_of(token_of(c0 + 1), tib)];
+            unit_ids(c0 + 1);
         }
-        const float mn = fmaxf(m, max_lanes<64>(x));
-        const float p = seen ? expf(x - mn) : 0.0f, f = mn == -INFINITY ? 1.0f : expf(m - mn);
-        l = l * f + sum_lanes<64>(p);
-        m = mn;
-        for (int i = 0; i < D / 64; ++i) o[i] *= f;
-        const unsigned long long all = __ballot(seen);
-        for (int k = 0; k < 64; ++k) {
-            if (!(all >> k & 1)) continue;
-            const float pk = __shfl(p, k);
-            const uint8_t* pg = a.pool + (size_t)__shfl(id, k) * a.g.page_size;
-            const int c = __shfl(cell, k);
-            for (int i = 0; i < D / 64; ++i)
-                o[i] = fmaf(pk, cell_value<FMT>(a, pg, c, lane + 64 * i, false), o[i]);
+        for (int c = c0; c < c1; ++c) {
+            const int t = token_of(c);
+            const int tb0 = c * C + wt * T;  // the wave's first token
+            uint64_t live = __ballot(readable(t, id));
+            if (T < 64) live &= (1ull << (T & 63)) - 1;
+            constexpr uint64_t kAll = T == 64 ? ~0ull : (1ull << (T & 63)) - 1;
+            const bool plain = live == kAll && tb0 + T <= pc.L;
+            // The chunk's tiles are in LDS: loaded by its waves, or decoded now.
+            if constexpr (kTurned) {
+                decode();
+            } else {
+                wait_vmem();
+            }
+            if constexpr (WR > 1) {
+                __syncthreads();
+            } else {
+                // (the wave's own tiles: its last reads of the buffer that is
+                // loaded next have arrived, its decoded values are written)
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+            id = next;
+            if (c + 1 < c1) {
+                stage(c + 1, next);
+                fetch(c + 1);
+                if (c + 2 < c1) {
+                    next = table[page_of(token_of(c + 2), tib)];
+                    unit_ids(c + 2);
+                }
+            }
+            const uint32_t kb = k_at + (kTurned ? 0 : (c & 1) * 2 * S::kTile);
+            const uint32_t vb = v_at + (kTurned ? 2 * S::kTile : ((c & 1) * 2 + 1) * S::kTile);
+
+            f4 x[RT][NS];
+#pragma unroll
+            for (int ns = 0; ns < NS; ++ns) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) x[rt][ns] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    const u4 k0 = *(lds_u4*)(uintptr_t)((kb ^ (kk * 64)) + ns * 16 * kRow);
+                    if constexpr (kTurned) {
+                        const u4 k1 = *(lds_u4*)(uintptr_t)((kb ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            x[rt][ns] = mfma<false>(k1, qh[rt][kk], x[rt][ns]);
+                            x[rt][ns] = mfma<false>(k0, ql[rt][kk], x[rt][ns]);
+                        }
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<BF>(k0, qh[rt][kk], x[rt][ns]);
+                }
+            }
+            // Logits in units of log2; per token: K's scale.
+            f4 sv[kTurned ? NS : 1], lv[kTurned ? NS : 1];
+            if constexpr (kTurned) {
+#pragma unroll
+                for (int ns = 0; ns < NS; ++ns) {
+                    const int tk = wt * T + ns * 16 + gq * 4;
+                    const f4 sk = *reinterpret_cast<const f4*>(&tsc.k[tk]);
+                    sv[ns] = *reinterpret_cast<const f4*>(&tsc.v[tk]);
+                    lv[ns] = *reinterpret_cast<const f4*>(&tsc.lv[tk]);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[rt][ns][r] *= sk[r] * qs[rt];
+                }
+            }
+            uint64_t see[RT];
+            if (!plain) {
+                const int j0 = tb0 - pc.L;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    see[rt] = live;
+                    if (j0 + T > 0) {  // (words before the drafted tokens: the prefix)
+                        const int w0 = j0 >> 5;
+                        uint32_t w[3];
+#pragma unroll
+                        for (int k = 0; k < 3; ++k)
+                            w[k] = w0 + k < 0 ? ~0u : w0 + k < a.mask_words ? (uint32_t)mrow[rt][w0 + k] : 0u;
+                        const int sh = j0 & 31;
+                        const uint32_t b0 = (uint32_t)(((uint64_t)w[1] << 32 | w[0]) >> sh);
+                        const uint32_t b1 = (uint32_t)(((uint64_t)w[2] << 32 | w[1]) >> sh);
+                        see[rt] &= (uint64_t)b1 << 32 | b0;
+                    }
+#pragma unroll
+                    for (int ns = 0; ns < NS; ++ns)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!(see[rt] >> (ns * 16 + gq * 4 + r) & 1)) x[rt][ns][r] = -INFINITY;
+                }
+            }
+            // Running maximum.  Compressed pages: of logit + log2 |V's scale|, so
+            // that the weights times their scales, what PV takes, are at most 2^14
+            // whatever the scales are (-25: scales of zero take part too).
+            u4 pw[RT][NS / 2];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int ns = 0; ns < NS; ++ns)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        top = fmaxf(top, kTurned ? x[rt][ns][r] + lv[ns][r] : x[rt][ns][r]);
+                if (!kTurned) top *= scale;
+                top = lane_xor_reduce<16>(top, [](float u, float w) { return fmaxf(u, w); });
+                top = lane_xor_reduce<32>(top, [](float u, float w) { return fmaxf(u, w); });
+                if (__ballot(top > m[rt])) {
+                    const float mn = fmaxf(m[rt], top);
+                    const float f = mn > m[rt] ? exp2_hw(m[rt] - mn) : 1.0f;
+                    m[rt] = mn;
+                    l[rt] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
+                }
+                const float ref = kOff - (m[rt] == -INFINITY ? 0.0f : m[rt]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int ns = 0; ns < NS; ++ns) {
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[r] = exp2_hw(kTurned ? x[rt][ns][r] + ref : fmaf(x[rt][ns][r], scale, ref));
+                        sum += p[r];
+                        if constexpr (kTurned) {
+                            p[r] *= sv[ns][r];
+                            if (!plain && !(see[rt] >> (ns * 16 + gq * 4 + r) & 1)) p[r] = 0.0f;
+                        }
+                    }
+                    pw[rt][ns / 2][(ns & 1) * 2] = pack2<BF>(p[0], p[1]);
+                    pw[rt][ns / 2][(ns & 1) * 2 + 1] = pack2<BF>(p[2], p[3]);
+                }
+                l[rt] += sum;
+            }
+            // Dense pages hold any bits, also where a row sees nothing, and 0 * NaN
+            // is NaN: chunks with masked tokens look for such values first.
+            bool odd = false;
+            if constexpr (!kTurned) {
+                if (!plain) {
+                    uint32_t bad = 0;
+#pragma unroll 4
+                    for (int k = 0; k < T * kRow / 1024; ++k) {
+                        const u4 w = *(lds_u4*)(uintptr_t)(mem0 + ((c & 1) * 2 + 1) * S::kTile + wt * T * kRow +
+                                                           k * 1024 + lane * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) bad |= not_finite<BF>(w[e]);
+                    }
+                    odd = __ballot(bad != 0) != 0;
+                }
+            }
+#pragma unroll
+            for (int st = 0; st < T / 32; ++st) {
+                u4 ones[RT];  // 1 where a row sees the token
+                if (!kTurned && odd) {
+                    constexpr uint32_t one = BF ? 0x3f80u : 0x3c00u;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int b = st * 32 + (e >> 1) * 16 + gq * 4 + (e & 1) * 2;
+                            ones[rt][e] = (see[rt] >> b & 1 ? one : 0u) | (see[rt] >> (b + 1) & 1 ? one << 16 : 0u);
+                        }
+                }
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt) {
+                    const uint32_t p = (vb ^ (dt * 32)) + st * 32 * kRow;
+                    const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)p);
+                    const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(p + 16 * kRow));
+                    const u2 w0 = __builtin_bit_cast(u2, v0), w1 = __builtin_bit_cast(u2, v1);
+                    u4 v = {w0[0], w0[1], w1[0], w1[1]};
+                    if (!kTurned && odd) {
+                        u4 pos, neg;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            pos[e] = infinite_ones<BF>(v[e], 0u);
+                            neg[e] = infinite_ones<BF>(v[e], 1u);
+                            v[e] &= ~not_finite<BF>(v[e]);
+                        }
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                            const f4 np = mfma<BF>(pos, ones[rt], zero), nn = mfma<BF>(neg, ones[rt], zero);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                if (np[r] > 0.0f) o[rt][dt][r] += INFINITY;
+                                if (nn[r] > 0.0f) o[rt][dt][r] -= INFINITY;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(v, pw[rt][st], o[rt][dt]);
+                }
+            }
+            if (kTurned && WR > 1) __syncthreads();  // the tiles are decoded again
+        }
+
+        // A row's sum over its four lanes.
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            l[rt] = lane_xor_reduce<16>(l[rt], [](float u, float w) { return u + w; });
+            l[rt] = lane_xor_reduce<32>(l[rt], [](float u, float w) { return u + w; });
+            if constexpr (kTurned) {
+                // Rotated back (linear: before any merge): value dt * 16 + gq * 4 + r.
+                const float sh = ((h & 1) ? -inv : inv) * (1.0f / kAlphaV);
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt) {
+                    f4 y = o[rt][dt];
+                    f4 z = {y[0] + y[1], y[0] - y[1], y[2] + y[3], y[2] - y[3]};
+                    y = f4{z[0] + z[2], z[1] + z[3], z[0] - z[2], z[1] - z[3]};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        y[r] = butterfly<16>(y[r], lane);
+                        y[r] = butterfly<32>(y[r], lane);
+                    }
+                    o[rt][dt] = y;
+                }
+#pragma unroll
+                for (int k = 1; k < D / 16; k <<= 1)
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt)
+                        if (!(dt & k)) {
+                            const f4 u = o[rt][dt], w = o[rt][dt + k];
+                            o[rt][dt] = u + w;
+                            o[rt][dt + k] = u - w;
+                        }
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
+                    o[rt][dt] *= f4{sh, -sh, sh, -sh};
+            }
+        }
+        const int piece = 2 * blockIdx.x + (first ? 0 : 1);
+        float* po = ws + (size_t)piece * M * D;
+        float2* pm = reinterpret_cast<float2*>(ws + (size_t)2 * tl.groups * M * D) + (size_t)piece * M;
+        if constexpr (WT == 1) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (row[rt] >= R) continue;
+                if (whole) {
+                    const float f = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt) {
+                        const f4 y = o[rt][dt] * f;
+                        *reinterpret_cast<u2*>(a.out + qo[rt] + dt * 16 + gq * 4) =
+                            u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
+                    }
+                } else {
+                    const int r = (wr * RT + rt) * 16 + i;
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt)
+                        *reinterpret_cast<f4*>(po + r * D + dt * 16 + gq * 4) = o[rt][dt];
+                    if (gq == 0) pm[r] = make_float2(m[rt], l[rt]);
+                }
+            }
+        } else {
+            __syncthreads();  // every wave is done with the tiles
+            float* mo = reinterpret_cast<float*>(mem);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const int r = (wr * RT + rt) * 16 + i;
+                if (gq == 0) ml[wt][r] = make_float2(m[rt], l[rt]);
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
+                    *reinterpret_cast<f4*>(mo + (wt * M + r) * (D + 4) + dt * 16 + gq * 4) = o[rt][dt];
+            }
+            __syncthreads();
+#pragma unroll 2
+            for (int u = tid; u < M * (D / 4); u += 256) {
+                const int r = u / (D / 4), d = u % (D / 4) * 4, rr = pc.tile * M + r;
+                if (rr >= R) break;
+                float mm = -INFINITY, lsum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WT; ++w) mm = fmaxf(mm, ml[w][r].x);
+                f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < WT; ++w) {
+                    const float2 e = ml[w][r];
+                    const float f = e.x == -INFINITY ? 0.0f : exp2_hw(e.x - mm);
+                    // (an empty part holds zeros, but for a NaN logit)
+                    lsum += e.x == -INFINITY ? e.y : e.y * f;
+                    y += *reinterpret_cast<const f4*>(mo + (w * M + r) * (D + 4) + d) * (e.x == -INFINITY ? 1.0f : f);
+                }
+                if (whole) {
+                    const int tok = rr / a.group;
+                    const size_t to = ((size_t)(pc.row0 + tok) * a.hq + h * a.group + (rr - tok * a.group)) * D + d;
+                    y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
+                    *reinterpret_cast<u2*>(a.out + to) = u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
+                } else {
+                    *reinterpret_cast<f4*>(po + r * D + d) = y;
+                    if (d == 0) pm[r] = make_float2(mm, lsum);
+                }
+            }
+        }
+        at += c1 - c0;
+        first = false;
+    }
+}
+
+// Merge of the items that were cut: one wave per query row, D / 4 lanes per
+// piece of it.
+template <bool BF, int D>
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
+                                                         const float* __restrict__ ws) {
+    const int lane = threadIdx.x & 63;
+    const int flat = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (flat >= a.tokens * a.hq) return;
+    const int tok = flat / a.hq, qh = flat - tok * a.hq, h = qh / a.group;
+    int total = 0, row0 = -1, before = 0, chunks = 1;
+    for (int f = 0; f < a.seqs; f += 64) {
+        const SeqBlock b = load_seqs(a, tl, f, total, lane, total);
+        const uint64_t hit = __ballot(b.row0 <= tok && tok < b.row0 + b.rows);
+        if (hit && row0 < 0) {
+            const int k = __ffsll((unsigned long long)hit) - 1;
+            row0 = __builtin_amdgcn_readlane(b.row0, k);
+            before = __builtin_amdgcn_readlane(b.before, k);
+            chunks = __builtin_amdgcn_readlane(b.chunks, k);
         }
     }
-    __syncthreads();
-    for (int i = 0; i < D / 64; ++i) q[lane + 64 * i] = l == 0.0f ? 0.0f : o[i] / l;
-    if (turned) rotate();
-    __syncthreads();
-    for (int d = lane; d < D; d += 64)
-        a.out[ro + d] = from_float<BF>(q[d] * (turned ? sign_of(d, h) : 1.0f));
+    if (row0 < 0) return;  // behind the last sequence
+    const Plan p = make_plan(a, tl, total);
+    const int rr = (tok - row0) * a.group + (qh - h * a.group);
+    const int tile = rr >> tl.m_log, r = rr & ((1 << tl.m_log) - 1);
+    const int from = h * total + before + tile * chunks;
+    const int w0 = from / p.per, w1 = (from + chunks - 1) / p.per;
+    if (w0 == w1 || w1 >= tl.groups) return;  // whole: written by the split kernel
+    const size_t M = (size_t)1 << tl.m_log;
+    const float2* pm = reinterpret_cast<const float2*>(ws + (size_t)2 * tl.groups * M * D);
+    const auto piece_of = [&](int w) { return (size_t)2 * w + (w == w0 && from != w * p.per ? 1 : 0); };
+    constexpr int kLanes = D / 4, kSide = 64 / kLanes;
+    const int side = lane / kLanes, d = lane % kLanes * 4;
+    float mm = -INFINITY, lsum = 0.0f;
+    f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w = w0 + side; w <= w1; w += kSide) {
+        const size_t q = piece_of(w) * M + r;
+        const float2 e = pm[q];
+        const f4 v = *reinterpret_cast<const f4*>(ws + q * D + d);
+        const float mn = fmaxf(mm, e.x);
+        const float fo = mm == -INFINITY ? 1.0f : exp2_hw(mm - mn);
+        const float fn = e.x == -INFINITY ? 1.0f : exp2_hw(e.x - mn);
+        y = y * fo + v * fn;
+        lsum = lsum * fo + e.y * fn;
+        mm = mn;
+    }
+#pragma unroll
+    for (int k = kLanes; k < 64; k <<= 1) {
+        const float om = __shfl_xor(mm, k, 64), ol = __shfl_xor(lsum, k, 64);
+        const float mn = fmaxf(mm, om);
+        const float fo = mm == -INFINITY ? 1.0f : exp2_hw(mm - mn);
+        const float fn = om == -INFINITY ? 1.0f : exp2_hw(om - mn);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = y[c] * fo + __shfl_xor(y[c], k, 64) * fn;
+        lsum = lsum * fo + ol * fn;
+        mm = mn;
+    }
+    if (side == 0) {
+        y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
+        *reinterpret_cast<u2*>(a.out + (size_t)flat * D + d) =
+            u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
+    }
+}
+
+template <int FMT, int D, int RT, int WR>
+void launch_shape(const TreeArgs& a, hipStream_t stream) {
+    using S = Shape<FMT, D, RT, WR>;
+    const auto log2i = [](int x) { return __builtin_ctz((unsigned)x); };
+    Tiling t;
+    t.m_log = log2i(S::M);
+    t.c_log = log2i(S::C);
+    t.least = std::max(1, 128 / S::C);
+    // The line's length is known to the device only; here its bound.
+    const long long chunks = std::max<long long>(1, ((long long)a.max_kv + S::C - 1) / S::C);
+    const long long items =
+        (((long long)a.tokens * a.group) / S::M + std::min(a.seqs, a.tokens)) * a.g.H;
+    if (items * chunks >= (1LL << 31) - (1 << 24))
+        throw Error("tree_attention: too many (row tile, token chunk) pairs (2^31)");
+    t.groups = (int)std::max<long long>(
+        1, std::min<long long>((long long)num_cus() * 2, (items * chunks + t.least - 1) / t.least));
+    constexpr size_t kPiece = (size_t)S::M * (D + 2) * sizeof(float);
+    float* ws = nullptr;
+    const bool cut = chunks > 1;  // an item of one chunk is never cut
+    if (cut)
+        ws = static_cast<float*>(Scratch{}.get(stream, 2 * (size_t)t.groups * kPiece, "tree attention",
+                                               4 * (size_t)num_cus() * 128 * (D + 2) * sizeof(float)));
+    hipLaunchKernelGGL((tree_split_kernel<FMT, D, RT, WR>), dim3(t.groups), dim3(256), 0, stream, a, t,
+                       ws, 1.44269504f * inv_sqrt_d(D), inv_sqrt_d(D));
+    check_launch("tree_attention_kernel");
+    if (!cut) return;
+    hipLaunchKernelGGL((tree_merge_kernel<S::BF, D>), dim3((unsigned)(((long long)a.tokens * a.hq + 3) / 4)),
+                       dim3(256), 0, stream, a, t, ws);
+    check_launch("tree_attention_merge_kernel");
+}
+
+// Query rows per tile: the fewest that hold an average sequence's rows.
+template <int FMT, int D>
+void launch_format(const TreeArgs& a, hipStream_t stream) {
+    const long long rows = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
+    if (rows <= 16) return launch_shape<FMT, D, 1, 1>(a, stream);
+    if (rows <= 32) return launch_shape<FMT, D, 2, 1>(a, stream);
+    if (rows <= 64) return launch_shape<FMT, D, 2, 2>(a, stream);
+    return launch_shape<FMT, D, 2, 4>(a, stream);
 }
 
 void launch_tree(int fmt, const TreeArgs& a, hipStream_t stream) {
-    const dim3 grid(a.tokens, a.hq);
-    const float inv = inv_sqrt_d(a.g.D);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(64), 0, stream, a, inv);
-        check_launch("tree_attention_kernel");
-    };
     if (a.g.D == 128) {
         switch (fmt) {
-            case kFp16: return go(tree_rows_kernel<kFp16, 128>);
-            case kBf16: return go(tree_rows_kernel<kBf16, 128>);
-            case kProd: return go(tree_rows_kernel<kProd, 128>);
-            default: return go(tree_rows_kernel<kMse, 128>);
+            case kFp16: return launch_format<kFp16, 128>(a, stream);
+            case kBf16: return launch_format<kBf16, 128>(a, stream);
+            case kProd: return launch_format<kProd, 128>(a, stream);
+            default: return launch_format<kMse, 128>(a, stream);
         }
     }
     switch (fmt) {
-        case kFp16: return go(tree_rows_kernel<kFp16, 64>);
-        case kBf16: return go(tree_rows_kernel<kBf16, 64>);
-        case kProd: return go(tree_rows_kernel<kProd, 64>);
-        default: return go(tree_rows_kernel<kMse, 64>);
+        case kFp16: return launch_format<kFp16, 64>(a, stream);
+        case kBf16: return launch_format<kBf16, 64>(a, stream);
+        case kProd: return launch_format<kProd, 64>(a, stream);
+        default: return launch_format<kMse, 64>(a, stream);
     }
 }
 
@@ -207,6 +983,7 @@ int tree_entry(const char* name, int fmt, Geom&& geom, const void* query, const 
         a.max_blocks = max_blocks;
         a.mask_words = mask_words;
         a.hq = hq;
+        a.group = hq / g.H;
         a.seqs = seqs;
         a.tokens = tokens;
         a.max_kv = max_kv;
