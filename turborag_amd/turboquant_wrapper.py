@@ -729,22 +729,20 @@ class TurboQuantWrapper:
         if t.shape != (tokens, heads, dim):
             raise ValueError(f"{scheme} {op}: {name} must be [{tokens}, {heads}, {dim}], got "
                              f"{list(t.shape)}")
-        st = t.stride()
-        if tokens and (st[2] != 1 or (st[1] != dim and heads > 1)
-                       or (tokens > 1 and st[0] < heads * dim)):
+        s0, s1, s2 = t.stride()
+        if tokens and (s2 != 1 or (s1 != dim and heads > 1)
+                       or (tokens > 1 and s0 < heads * dim)):
             raise ValueError(f"{scheme} {op}: {name} must have contiguous heads and distinct tokens")
-        return t.data_ptr(), st[0]
+        return t.data_ptr(), s0
 
     @staticmethod
-    def _on_one_device(scheme, op, first, *others):
+    def _on_current_device(scheme, op, *tensors):
         """A launch runs on the current device: every tensor must live there."""
-        dev = first.get_device()
-        for t in others:
+        dev = torch.cuda.current_device()
+        for t in tensors:
             if t is not None and t.get_device() != dev:
-                raise ValueError(f"{scheme} {op}: tensors on different GPUs")
-        if dev != torch.cuda.current_device():
-            raise ValueError(f"{scheme} {op}: tensors on GPU {dev}, the current device is "
-                             f"{torch.cuda.current_device()}")
+                raise ValueError(f"{scheme} {op}: a tensor on GPU {t.get_device()}, the current "
+                                 f"device is {dev}")
 
     def _rope_args(self, scheme, op, key, positions, cos_sin, cfg, q_heads, q_weight, k_weight, eps,
                    interleaved):
@@ -756,16 +754,20 @@ class TurboQuantWrapper:
         N, D = key.shape[0], cfg.head_dim
         if not isinstance(cos_sin, torch.Tensor) or cos_sin.dim() != 2:
             raise ValueError(f"{scheme} {op}: cos_sin must be [max_position, rot_dim]")
-        self._check(scheme, op, positions=(positions, torch.int32, N),
-                    cos_sin=(cos_sin, torch.float32, cos_sin.numel()))
-        w = []
-        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if t is not None:
-                self._check(scheme, op, **{name: (t, key.dtype, D)})
-            w.append(t.data_ptr() if t is not None else None)
-        rope = TQRopeConfig(_DTYPES[key.dtype], q_heads, cos_sin.shape[1], int(bool(interleaved)),
-                            cos_sin.shape[0], eps)
-        return rope, w
+        if not (_ready(positions, torch.int32, N) and _ready(cos_sin, torch.float32, 0)):
+            self._check(scheme, op, positions=(positions, torch.int32, N),
+                        cos_sin=(cos_sin, torch.float32, 0))
+        qw = kw = None
+        if q_weight is not None:
+            if not _ready(q_weight, key.dtype, D):
+                self._check(scheme, op, q_weight=(q_weight, key.dtype, D))
+            qw = q_weight.data_ptr()
+        if k_weight is not None:
+            if not _ready(k_weight, key.dtype, D):
+                self._check(scheme, op, k_weight=(k_weight, key.dtype, D))
+            kw = k_weight.data_ptr()
+        rows, rot = cos_sin.shape
+        return TQRopeConfig(_DTYPES[key.dtype], q_heads, rot, bool(interleaved), rows, eps), qw, kw
 
     def qk_norm_rope(self, query, key, positions, cos_sin, out_query, out_key, cfg, q_weight=None,
                      k_weight=None, eps: float = 1e-6, interleaved: bool = False,
@@ -778,20 +780,21 @@ class TurboQuantWrapper:
         op = "qk_norm_rope"
         if not isinstance(query, torch.Tensor) or query.dim() != 3:
             raise ValueError(f"rope {op}: query must be [num_tokens, num_q_heads, head_dim]")
-        N, Hq = query.shape[:2]
+        N, Hq, _ = query.shape
         H, D = cfg.num_kv_heads, cfg.head_dim
-        rope, w = self._rope_args("rope", op, key, positions, cos_sin, cfg, Hq, q_weight, k_weight,
-                                  eps, interleaved)
-        q, qs = self._token_rows("rope", op, "query", query, key.dtype, N, Hq, D)
-        k, ks = self._token_rows("rope", op, "key", key, key.dtype, N, H, D)
-        oq, oqs = self._token_rows("rope", op, "out_query", out_query, key.dtype, N, Hq, D)
-        ok, oks = self._token_rows("rope", op, "out_key", out_key, key.dtype, N, H, D)
-        self._on_one_device("rope", op, query, key, positions, cos_sin, out_query, out_key, q_weight,
-                            k_weight)
+        rope, qw, kw = self._rope_args("rope", op, key, positions, cos_sin, cfg, Hq, q_weight,
+                                       k_weight, eps, interleaved)
+        dtype, rows = key.dtype, self._token_rows
+        q, qs = rows("rope", op, "query", query, dtype, N, Hq, D)
+        k, ks = rows("rope", op, "key", key, dtype, N, H, D)
+        oq, oqs = rows("rope", op, "out_query", out_query, dtype, N, Hq, D)
+        ok, oks = rows("rope", op, "out_key", out_key, dtype, N, H, D)
+        self._on_current_device("rope", op, query, key, positions, cos_sin, out_query, out_key,
+                                q_weight, k_weight)
         if N == 0:
             return
         rc = self._fast.tq_launch_qk_norm_rope(
-            q, qs, k, ks, w[0], w[1], cos_sin.data_ptr(), positions.data_ptr(), oq, oqs, ok, oks,
+            q, qs, k, ks, qw, kw, cos_sin.data_ptr(), positions.data_ptr(), oq, oqs, ok, oks,
             ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
         if rc != 0:
             self._kernel_raise(rc, "rope", op)
@@ -809,23 +812,24 @@ class TurboQuantWrapper:
             raise ValueError(f"dense {op}: query must be [num_tokens, num_q_heads, head_dim]")
         H, D = cfg.num_kv_heads, cfg.head_dim
         Hq = query.shape[1] if query is not None else 1
-        rope, w = self._rope_args("dense", op, key, positions, cos_sin, cfg, Hq, q_weight, k_weight,
-                                  eps, interleaved)
-        N = key.shape[0]
-        self._check("dense", op, slot_mapping=(slot_mapping, torch.int32, N),
-                    page_pool=(page_pool, torch.uint8, 0))
+        rope, qw, kw = self._rope_args("dense", op, key, positions, cos_sin, cfg, Hq, q_weight,
+                                       k_weight, eps, interleaved)
+        N, dtype, rows = key.shape[0], key.dtype, self._token_rows
+        if not (_ready(slot_mapping, torch.int32, N) and _ready(page_pool, torch.uint8, 0)):
+            self._check("dense", op, slot_mapping=(slot_mapping, torch.int32, N),
+                        page_pool=(page_pool, torch.uint8, 0))
         q, qs, oq, oqs = None, 0, None, 0
         if query is not None:
-            q, qs = self._token_rows("dense", op, "query", query, key.dtype, N, Hq, D)
-            oq, oqs = self._token_rows("dense", op, "out_query", out_query, key.dtype, N, Hq, D)
-        k, ks = self._token_rows("dense", op, "key", key, key.dtype, N, H, D)
-        v, vs = self._token_rows("dense", op, "value", value, key.dtype, N, H, D)
-        self._on_one_device("dense", op, key, query, value, positions, slot_mapping, cos_sin,
-                            out_query, page_pool, q_weight, k_weight)
+            q, qs = rows("dense", op, "query", query, dtype, N, Hq, D)
+            oq, oqs = rows("dense", op, "out_query", out_query, dtype, N, Hq, D)
+        k, ks = rows("dense", op, "key", key, dtype, N, H, D)
+        v, vs = rows("dense", op, "value", value, dtype, N, H, D)
+        self._on_current_device("dense", op, key, query, value, positions, slot_mapping, cos_sin,
+                                out_query, page_pool, q_weight, k_weight)
         if N == 0:
             return
         rc = self._fast.tq_launch_dense_rope_append_kv(
-            q, qs, k, ks, v, vs, w[0], w[1], cos_sin.data_ptr(), positions.data_ptr(),
+            q, qs, k, ks, v, vs, qw, kw, cos_sin.data_ptr(), positions.data_ptr(),
             slot_mapping.data_ptr(), page_pool.data_ptr(), oq, oqs, ctypes.byref(layout),
             ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
         if rc != 0:
@@ -857,15 +861,15 @@ class TurboQuantWrapper:
         S = block_tables.shape[0]
         if tree_mask.shape[0] < N:
             raise ValueError(f"{scheme} {op}: tree_mask has {tree_mask.shape[0]} rows, needs {N}")
-        self._check(scheme, op, query=(query, query.dtype, N * Hq * D),
-                    page_pool=(page_pool, torch.uint8, 0),
-                    block_tables=(block_tables, torch.int32, 0),
-                    row_start=(row_start, torch.int32, S + 1),
-                    prefix_len=(prefix_len, torch.int32, S),
-                    tree_mask=(tree_mask, torch.int32, 0),
-                    output=(output, query.dtype, N * Hq * D))
-        self._on_one_device(scheme, op, query, page_pool, block_tables, row_start, prefix_len,
-                            tree_mask, output)
+        want = ((query, query.dtype, N * Hq * D), (page_pool, torch.uint8, 0),
+                (block_tables, torch.int32, 0), (row_start, torch.int32, S + 1),
+                (prefix_len, torch.int32, S), (tree_mask, torch.int32, 0),
+                (output, query.dtype, N * Hq * D))
+        if not all(_ready(*w) for w in want):
+            self._check(scheme, op, **dict(zip(("query", "page_pool", "block_tables", "row_start",
+                                                "prefix_len", "tree_mask", "output"), want)))
+        self._on_current_device(scheme, op, query, page_pool, block_tables, row_start, prefix_len,
+                                tree_mask, output)
         if N == 0 or S == 0:
             return
         args = [query.data_ptr(), page_pool.data_ptr(), block_tables.data_ptr(),
