@@ -160,9 +160,10 @@ def tree_attention(scheme, query, pool, tables, row_start, prefix, mask, layout,
             # (weights and their sum each move by arg; 64 U32 the sums' own roundings, which
             # grow with the logarithm of the tokens: chunks, lanes and waves are summed apart)
             e = big * (unit(query.dtype) + 2 * arg + 64 * U32 + (2.0 ** -13 if turned else 0.0))
-            # fp16 weights 2^-14 and more below a row's largest are subnormal: 2^-24 / 2^14 each
+            # fp16 weights are multiples of 2^-24 where they are subnormal, so half of that off; a
+            # row's largest weight is 2^11 or more: 2^-25 / 2^11 of it each
             if query.dtype == torch.float16:
-                e = e + 2.0 ** -38 * vv.abs().nan_to_num(0.0, 0.0, 0.0).sum(0)
+                e = e + 2.0 ** -36 * vv.abs().nan_to_num(0.0, 0.0, 0.0).sum(0)
             if turned:
                 o = (o @ had) * signs(h, D)
                 e = e.sum(1, keepdim=True).expand_as(e) / math.sqrt(D)

@@ -65,7 +65,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
         typedef __bf16 b2v __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v){a, b}, b2v));
     } else {
-        return f2h2(a, b);
+        typedef float f2v __attribute__((ext_vector_type(2)));
+        typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v){a, b}, h2v));
     }
 }
 
@@ -196,10 +198,10 @@ __device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, cons
 // 32-token step is 4 (l / 16) + 0..3 of either 16 tokens; V' is read from its
 // token rows in that order by transposing LDS loads).
 // ---------------------------------------------------------------------------
-template <int FMT, int D, int RT, int WR>
+template <int FMT, int D, int RT, int WR, int NW>
 struct Shape {
     static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
-    static constexpr int WT = 4 / WR;
+    static constexpr int WT = NW / WR;
     static constexpr int T = WR == 4 ? 64 : 32, C = T * WT, M = 16 * RT * WR;
     static constexpr int kRow = 2 * D, kTile = C * kRow;
     static constexpr int kTiles = kTurned ? 3 : 4;  // K hi, K lo, V; or K, V twice
@@ -224,15 +226,22 @@ struct alignas(16) TokenScales {
     float k[128], v[128], lv[128];  // of a chunk's tokens; lv = max(log2 |v|, -25)
 };
 struct Nothing {};
+#ifndef TQ_SUB_UNROLL
+#define TQ_SUB_UNROLL 1
+#endif
 
-template <int FMT, int D, int RT, int WR>
-__global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, const Tiling tl,
+template <int FMT, int D, int RT, int WR, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a, const Tiling tl,
                                                             float* __restrict__ ws, float scale,
                                                             float inv) {
-    using S = Shape<FMT, D, RT, WR>;
+    using S = Shape<FMT, D, RT, WR, NW>;
     constexpr bool BF = S::BF, kTurned = S::kTurned;
-    constexpr int T = S::T, C = S::C, M = S::M, WT = S::WT, NS = T / 16, kRow = S::kRow;
-    constexpr float kOff = BF ? 0.0f : 14.0f;  // weights up to 2^14: small ones stay normal in fp16
+    constexpr int T = S::T, C = S::C, M = S::M, WT = S::WT, kRow = S::kRow;
+    // The reference of a row's weights follows its running maximum once that is
+    // kSlack above it (rescaling the sums of 16 rows at every new maximum of one
+    // of them took a quarter of the instructions).  Weights are 2^kOff at the
+    // reference: at most 2^15 in fp16, where small ones stay normal.
+    constexpr float kSlack = 4.0f, kOff = BF ? 0.0f : 11.0f;
     __shared__ __attribute__((aligned(1024))) uint8_t mem[S::kLds];
     __shared__ float2 ml[WT][M];
     __shared__ typename std::conditional<kTurned, DecodeTables, Nothing>::type tab;
@@ -250,16 +259,18 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
     const int vrow = 4 * gq + (i >> 2);
     const uint32_t v_at = mem0 + (wt * T + vrow) * kRow + ((((i >> 1) & 1) ^ swz(vrow)) * 16) + (i & 1) * 8;
 
-    if constexpr (kTurned) {
+    if (kTurned && tid < 256) {
+      if constexpr (kTurned) {
         const int lo = tid & 15, hi = tid >> 4;
-        tab.v[tid] = f2h2(kAlphaV * pick(kV4, lo), kAlphaV * pick(kV4, hi));
+        tab.v[tid] = pack2<false>(kAlphaV * pick(kV4, lo), kAlphaV * pick(kV4, hi));
         if constexpr (FMT == kMse) {
             const float x = pick(kV4, lo), y = pick(kV4, hi);
-            const uint32_t h = f2h2(x, y);
-            tab.k[tid] = make_uint2(h, f2h2(x - h2f(h & 0xffff), y - h2f(h >> 16)));
+            const uint32_t h = pack2<false>(x, y);
+            tab.k[tid] = make_uint2(h, pack2<false>(x - h2f(h & 0xffff), y - h2f(h >> 16)));
         } else {
             tab.k[tid] = make_uint2(__float_as_uint(pick(kK3, lo & 7)), __float_as_uint(pick(kK3, hi & 7)));
         }
+      }
     }
 
     SeqBlock sb;
@@ -302,7 +313,9 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
             return pg;
         };
         int tib;
-        int id = table[page_of(token_of(c0), tib)];
+        int id = table[page_of(token_of(c0), tib)], id2 = -1;
+        constexpr bool kPair = WR > 1 && WT > 1;
+        if (kPair) id2 = table[page_of(token_of(c0) + (wt ? -T : T), tib)];
         const auto readable = [&](int t, int pid) { return t < pc.end && pid >= 0; };
 
         // Compressed pages: the codes and scales of this lane's units of the
@@ -376,8 +389,8 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
                                                 __uint_as_float(re ^ ((~kb & 8u) << 28));
                                 const float y = __uint_as_float(e.y) +
                                                 __uint_as_float(re ^ ((~kb & 128u) << 24));
-                                hi[b] = f2h2(x, y);
-                                lo[b] = f2h2(x - h2f(hi[b] & 0xffff), y - h2f(hi[b] >> 16));
+                                hi[b] = pack2<false>(x, y);
+                                lo[b] = pack2<false>(x - h2f(hi[b] & 0xffff), y - h2f(hi[b] >> 16));
                             }
                         }
                         const int piece = ((part * (D / 32) + q) ^ swz(r)) * 16;
@@ -487,15 +500,16 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float u = x[kk][2 * e] * up, w = x[kk][2 * e + 1] * up;
-                        const uint32_t p = f2h2(u, w);
+                        const uint32_t p = pack2<false>(u, w);
                         qh[rt][kk][e] = p;
-                        ql[rt][kk][e] = f2h2(u - h2f(p & 0xffff), w - h2f(p >> 16));
+                        ql[rt][kk][e] = pack2<false>(u - h2f(p & 0xffff), w - h2f(p >> 16));
                     }
             }
         }
 
         float m[RT], l[RT];
         f4 o[RT][D / 16];
+        uint32_t plus[RT] = {}, minus[RT] = {};  // sums that hold +infinity, -infinity (bit dt * 4 + r)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             m[rt] = -INFINITY;
@@ -506,18 +520,24 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
 
         stage(c0, id);
         fetch(c0);
-        int next = id;
+        int next = id, next2 = id2;
         if (c0 + 1 < c1) {
             next = table[page_of(token_of(c0 + 1), tib)];
+            if (kPair) next2 = table[page_of(token_of(c0 + 1) + (wt ? -T : T), tib)];
             unit_ids(c0 + 1);
         }
         for (int c = c0; c < c1; ++c) {
-            const int t = token_of(c);
             const int tb0 = c * C + wt * T;  // the wave's first token
-            uint64_t live = __ballot(readable(t, id));
-            if (T < 64) live &= (1ull << (T & 63)) - 1;
             constexpr uint64_t kAll = T == 64 ? ~0ull : (1ull << (T & 63)) - 1;
+            const uint64_t live = __ballot(readable(token_of(c), id)) & kAll;
             const bool plain = live == kAll && tb0 + T <= pc.L;
+            // (the same in every wave: two token groups know each other's tokens)
+            bool plain_all = plain;
+            if constexpr (WR > 1 && WT > 1) {
+                static_assert(WT == 2, "two token groups");
+                const uint64_t other = __ballot(readable(token_of(c) + (wt ? -T : T), id2)) & kAll;
+                plain_all = live == kAll && other == kAll && c * C + C <= pc.L;
+            }
             // The chunk's tiles are in LDS: loaded by its waves, or decoded now.
             if constexpr (kTurned) {
                 decode();
@@ -532,52 +552,27 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
             id = next;
+            id2 = next2;
             if (c + 1 < c1) {
                 stage(c + 1, next);
                 fetch(c + 1);
                 if (c + 2 < c1) {
                     next = table[page_of(token_of(c + 2), tib)];
+                    if (kPair) next2 = table[page_of(token_of(c + 2) + (wt ? -T : T), tib)];
                     unit_ids(c + 2);
                 }
             }
             const uint32_t kb = k_at + (kTurned ? 0 : (c & 1) * 2 * S::kTile);
             const uint32_t vb = v_at + (kTurned ? 2 * S::kTile : ((c & 1) * 2 + 1) * S::kTile);
 
-            f4 x[RT][NS];
-#pragma unroll
-            for (int ns = 0; ns < NS; ++ns) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) x[rt][ns] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    const u4 k0 = *(lds_u4*)(uintptr_t)((kb ^ (kk * 64)) + ns * 16 * kRow);
-                    if constexpr (kTurned) {
-                        const u4 k1 = *(lds_u4*)(uintptr_t)((kb ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            x[rt][ns] = mfma<false>(k1, qh[rt][kk], x[rt][ns]);
-                            x[rt][ns] = mfma<false>(k0, ql[rt][kk], x[rt][ns]);
-                        }
-                    }
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<BF>(k0, qh[rt][kk], x[rt][ns]);
-                }
-            }
-            // Logits in units of log2; per token: K's scale.
-            f4 sv[kTurned ? NS : 1], lv[kTurned ? NS : 1];
-            if constexpr (kTurned) {
-#pragma unroll
-                for (int ns = 0; ns < NS; ++ns) {
-                    const int tk = wt * T + ns * 16 + gq * 4;
-                    const f4 sk = *reinterpret_cast<const f4*>(&tsc.k[tk]);
-                    sv[ns] = *reinterpret_cast<const f4*>(&tsc.v[tk]);
-                    lv[ns] = *reinterpret_cast<const f4*>(&tsc.lv[tk]);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) x[rt][ns][r] *= sk[r] * qs[rt];
-                }
-            }
+            const auto values = [&](int st, int dt) {
+                const uint32_t p = (vb ^ (dt * 32)) + st * 32 * kRow;
+                const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)p);
+                const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(p + 16 * kRow));
+                const u2 w0 = __builtin_bit_cast(u2, v0), w1 = __builtin_bit_cast(u2, v1);
+                return u4{w0[0], w0[1], w1[0], w1[1]};
+            };
+            // The tokens that each row sees.
             uint64_t see[RT];
             if (!plain) {
                 const int j0 = tb0 - pc.L;
@@ -595,112 +590,182 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
                         const uint32_t b1 = (uint32_t)(((uint64_t)w[2] << 32 | w[1]) >> sh);
                         see[rt] &= (uint64_t)b1 << 32 | b0;
                     }
-#pragma unroll
-                    for (int ns = 0; ns < NS; ++ns)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (!(see[rt] >> (ns * 16 + gq * 4 + r) & 1)) x[rt][ns][r] = -INFINITY;
                 }
             }
-            // Running maximum.  Compressed pages: of logit + log2 |V's scale|, so
-            // that the weights times their scales, what PV takes, are at most 2^14
-            // whatever the scales are (-25: scales of zero take part too).
-            u4 pw[RT][NS / 2];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int ns = 0; ns < NS; ++ns)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        top = fmaxf(top, kTurned ? x[rt][ns][r] + lv[ns][r] : x[rt][ns][r]);
-                if (!kTurned) top *= scale;
-                top = lane_xor_reduce<16>(top, [](float u, float w) { return fmaxf(u, w); });
-                top = lane_xor_reduce<32>(top, [](float u, float w) { return fmaxf(u, w); });
-                if (__ballot(top > m[rt])) {
-                    const float mn = fmaxf(m[rt], top);
-                    const float f = mn > m[rt] ? exp2_hw(m[rt] - mn) : 1.0f;
-                    m[rt] = mn;
-                    l[rt] *= f;
-#pragma unroll
-                    for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
-                }
-                const float ref = kOff - (m[rt] == -INFINITY ? 0.0f : m[rt]);
-                float sum = 0.0f;
-#pragma unroll
-                for (int ns = 0; ns < NS; ++ns) {
-                    float p[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        p[r] = exp2_hw(kTurned ? x[rt][ns][r] + ref : fmaf(x[rt][ns][r], scale, ref));
-                        sum += p[r];
-                        if constexpr (kTurned) {
-                            p[r] *= sv[ns][r];
-                            if (!plain && !(see[rt] >> (ns * 16 + gq * 4 + r) & 1)) p[r] = 0.0f;
-                        }
-                    }
-                    pw[rt][ns / 2][(ns & 1) * 2] = pack2<BF>(p[0], p[1]);
-                    pw[rt][ns / 2][(ns & 1) * 2 + 1] = pack2<BF>(p[2], p[3]);
-                }
-                l[rt] += sum;
-            }
-            // Dense pages hold any bits, also where a row sees nothing, and 0 * NaN
-            // is NaN: chunks with masked tokens look for such values first.
-            bool odd = false;
+            // Dense pages hold any bits, also where a row sees nothing, and 0 * NaN is
+            // NaN: a chunk with masked tokens is searched for infinities and NaN.
+            // Where a row sees one (counted by a product of ones) its sums are
+            // marked; then the values become zeros.
             if constexpr (!kTurned) {
-                if (!plain) {
+                if (WR > 1 ? !plain_all : !plain) {
+                    const uint32_t tile = mem0 + ((c & 1) * 2 + 1) * S::kTile +
+                                          (WR > 1 ? wv * (S::kTile / NW) : wt * T * kRow) + lane * 16;
+                    constexpr int kLoads = (WR > 1 ? S::kTile / NW : T * kRow) / 1024;
                     uint32_t bad = 0;
 #pragma unroll 4
-                    for (int k = 0; k < T * kRow / 1024; ++k) {
-                        const u4 w = *(lds_u4*)(uintptr_t)(mem0 + ((c & 1) * 2 + 1) * S::kTile + wt * T * kRow +
-                                                           k * 1024 + lane * 16);
+                    for (int k = 0; k < kLoads; ++k) {
+                        const u4 w = *(lds_u4*)(uintptr_t)(tile + k * 1024);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) bad |= not_finite<BF>(w[e]);
                     }
-                    odd = __ballot(bad != 0) != 0;
+                    const bool odd = WR > 1 ? __syncthreads_or(bad != 0) : __ballot(bad != 0) != 0;
+                    if (odd) {
+                        constexpr uint32_t one = BF ? 0x3f80u : 0x3c00u;
+#pragma unroll 1
+                        for (int dt = 0; dt < T / 32 * (D / 16); ++dt) {
+                            const int st = dt / (D / 16), dd = dt % (D / 16);
+                            const u4 v = values(st, dd);
+                            u4 pos, neg;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                pos[e] = infinite_ones<BF>(v[e], 0u);
+                                neg[e] = infinite_ones<BF>(v[e], 1u);
+                            }
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) {
+                                u4 ones;
+                                const uint32_t sees = (uint32_t)(see[rt] >> (st * 32)) >> (gq * 4);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t b = sees >> ((e >> 1) * 16 + (e & 1) * 2);
+                                    ones[e] = (b & 1 ? one : 0u) | (b & 2 ? one << 16 : 0u);
+                                }
+                                const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                                const f4 np = mfma<BF>(pos, ones, zero), nn = mfma<BF>(neg, ones, zero);
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    if (np[r] > 0.0f) plus[rt] |= 1u << (dd * 4 + r);
+                                    if (nn[r] > 0.0f) minus[rt] |= 1u << (dd * 4 + r);
+                                }
+                            }
+                        }
+                        if (WR > 1) __syncthreads();
+#pragma unroll 1
+                        for (int k = 0; k < kLoads; ++k) {
+                            u4 w = *(lds_u4*)(uintptr_t)(tile + k * 1024);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] &= ~not_finite<BF>(w[e]);
+                            *(lds_u4*)(uintptr_t)(tile + k * 1024) = w;
+                        }
+                        if (WR > 1) __syncthreads();
+                    }
                 }
             }
-#pragma unroll
+
+            // 32 tokens at a time: a row's logits, their weights, the values.
+#pragma unroll TQ_SUB_UNROLL
             for (int st = 0; st < T / 32; ++st) {
-                u4 ones[RT];  // 1 where a row sees the token
-                if (!kTurned && odd) {
-                    constexpr uint32_t one = BF ? 0x3f80u : 0x3c00u;
+                const uint32_t ks_at = kb + st * 32 * kRow;
+                const int tk = wt * T + st * 32 + gq * 4;  // this lane's tokens: tk + 16 ns + 0..3
+                f4 x[RT][2];
+#pragma unroll
+                for (int ns = 0; ns < 2; ++ns) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) x[rt][ns] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) {
+                        const u4 k0 = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + ns * 16 * kRow);
+                        if constexpr (kTurned) {
+                            const u4 k1 = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) {
+                                x[rt][ns] = mfma<false>(k1, qh[rt][kk], x[rt][ns]);
+                                x[rt][ns] = mfma<false>(k0, ql[rt][kk], x[rt][ns]);
+                            }
+                        }
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<BF>(k0, qh[rt][kk], x[rt][ns]);
+                    }
+                }
+                // Logits in units of log2 (dense pages: the factor enters below);
+                // compressed pages: K's scale per token.
+                if constexpr (kTurned) {
+#pragma unroll
+                    for (int ns = 0; ns < 2; ++ns) {
+                        const f4 sk = *reinterpret_cast<const f4*>(&tsc.k[tk + ns * 16]);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[rt][ns][r] *= sk[r] * qs[rt];
+                    }
+                }
+                uint32_t sees[RT];
+                if (!plain) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        sees[rt] = (uint32_t)(see[rt] >> (st * 32)) >> (gq * 4);
+#pragma unroll
+                        for (int ns = 0; ns < 2; ++ns)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (!(sees[rt] >> (ns * 16 + r) & 1)) x[rt][ns][r] = -INFINITY;
+                    }
+                }
+                // Running maximum.  Compressed pages: of logit + log2 |V's scale|, so
+                // that the weights times their scales, what PV takes, are at most 2^15
+                // whatever the scales are (-25: scales of zero take part too).
+                float top[RT], ref[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) top[rt] = -INFINITY;
+#pragma unroll
+                for (int ns = 0; ns < 2; ++ns) {
+                    f4 lv = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (kTurned) lv = *reinterpret_cast<const f4*>(&tsc.lv[tk + ns * 16]);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int b = st * 32 + (e >> 1) * 16 + gq * 4 + (e & 1) * 2;
-                            ones[rt][e] = (see[rt] >> b & 1 ? one : 0u) | (see[rt] >> (b + 1) & 1 ? one << 16 : 0u);
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            top[rt] = fmaxf(top[rt], kTurned ? x[rt][ns][r] + lv[r] : x[rt][ns][r]);
                 }
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) {
-                    const uint32_t p = (vb ^ (dt * 32)) + st * 32 * kRow;
-                    const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)p);
-                    const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(p + 16 * kRow));
-                    const u2 w0 = __builtin_bit_cast(u2, v0), w1 = __builtin_bit_cast(u2, v1);
-                    u4 v = {w0[0], w0[1], w1[0], w1[1]};
-                    if (!kTurned && odd) {
-                        u4 pos, neg;
+                for (int rt = 0; rt < RT; ++rt) {
+                    float t = kTurned ? top[rt] : top[rt] * scale;
+                    t = lane_xor_reduce<16>(t, [](float u, float w) { return fmaxf(u, w); });
+                    t = lane_xor_reduce<32>(t, [](float u, float w) { return fmaxf(u, w); });
+                    if (__ballot(t > m[rt] + kSlack)) {
+                        const float mn = t > m[rt] + kSlack ? t : m[rt];
+                        const float f = t > m[rt] + kSlack ? exp2_hw(m[rt] - mn) : 1.0f;
+                        m[rt] = mn;
+                        l[rt] *= f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            pos[e] = infinite_ones<BF>(v[e], 0u);
-                            neg[e] = infinite_ones<BF>(v[e], 1u);
-                            v[e] &= ~not_finite<BF>(v[e]);
-                        }
+                        for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
+                    }
+                    ref[rt] = kOff - (m[rt] == -INFINITY ? 0.0f : m[rt]);
+                }
+                u4 pw[RT];
+                const auto weights = [&](auto masked) {
+#pragma unroll
+                    for (int ns = 0; ns < 2; ++ns) {
+                        f4 sv = {1.0f, 1.0f, 1.0f, 1.0f};
+                        if constexpr (kTurned) sv = *reinterpret_cast<const f4*>(&tsc.v[tk + ns * 16]);
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) {
-                            const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                            const f4 np = mfma<BF>(pos, ones[rt], zero), nn = mfma<BF>(neg, ones[rt], zero);
+                            float p[4], sum = 0.0f;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                if (np[r] > 0.0f) o[rt][dt][r] += INFINITY;
-                                if (nn[r] > 0.0f) o[rt][dt][r] -= INFINITY;
+                                p[r] = exp2_hw(kTurned ? x[rt][ns][r] + ref[rt]
+                                                       : fmaf(x[rt][ns][r], scale, ref[rt]));
+                                sum += p[r];
+                                if constexpr (kTurned) {
+                                    p[r] *= sv[r];  // (not 0 * NaN where the row sees nothing)
+                                    if (masked && !(sees[rt] >> (ns * 16 + r) & 1)) p[r] = 0.0f;
+                                }
                             }
+                            l[rt] += sum;
+                            pw[rt][ns * 2] = pack2<BF>(p[0], p[1]);
+                            pw[rt][ns * 2 + 1] = pack2<BF>(p[2], p[3]);
                         }
                     }
+                };
+                if (!kTurned || plain)
+                    weights(std::false_type{});
+                else
+                    weights(std::true_type{});
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(v, pw[rt][st], o[rt][dt]);
+                for (int dt = 0; dt < D / 16; ++dt) {
+                    const u4 v = values(st, dt);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(v, pw[rt], o[rt][dt]);
                 }
             }
             if (kTurned && WR > 1) __syncthreads();  // the tiles are decoded again
@@ -709,6 +774,15 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
         // A row's sum over its four lanes.
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            if constexpr (!kTurned) {
+                if (__ballot((plus[rt] | minus[rt]) != 0)) {
+#pragma unroll
+                    for (int k = 0; k < D / 4; ++k) {
+                        if (plus[rt] >> k & 1) o[rt][k / 4][k % 4] += INFINITY;
+                        if (minus[rt] >> k & 1) o[rt][k / 4][k % 4] -= INFINITY;
+                    }
+                }
+            }
             l[rt] = lane_xor_reduce<16>(l[rt], [](float u, float w) { return u + w; });
             l[rt] = lane_xor_reduce<32>(l[rt], [](float u, float w) { return u + w; });
             if constexpr (kTurned) {
@@ -776,7 +850,7 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
             }
             __syncthreads();
 #pragma unroll 2
-            for (int u = tid; u < M * (D / 4); u += 256) {
+            for (int u = tid; u < M * (D / 4); u += 64 * NW) {
                 const int r = u / (D / 4), d = u % (D / 4) * 4, rr = pc.tile * M + r;
                 if (rr >= R) break;
                 float mm = -INFINITY, lsum = 0.0f;
@@ -807,13 +881,16 @@ __global__ __launch_bounds__(256, 2) void tree_split_kernel(const TreeArgs a, co
     }
 }
 
-// Merge of the items that were cut: one wave per query row, D / 4 lanes per
+// Merge of the items that were cut: WAVES waves per query row, D / 4 lanes per
 // piece of it.
-template <bool BF, int D>
+template <bool BF, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
                                                          const float* __restrict__ ws) {
-    const int lane = threadIdx.x & 63;
-    const int flat = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    constexpr int kLanes = D / 4, kSides = 64 * WAVES / kLanes, kRows = 4 / WAVES, kDeep = 4;
+    __shared__ float2 sml[kRows][kSides];
+    __shared__ f4 so[kRows][kSides][kLanes];
+    const int lane = threadIdx.x & 63, mine = threadIdx.x / (64 * WAVES);
+    const int flat = __builtin_amdgcn_readfirstlane(blockIdx.x * kRows + mine);
     if (flat >= a.tokens * a.hq) return;
     const int tok = flat / a.hq, qh = flat - tok * a.hq, h = qh / a.group;
     int total = 0, row0 = -1, before = 0, chunks = 1;
@@ -836,43 +913,47 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
     if (w0 == w1 || w1 >= tl.groups) return;  // whole: written by the split kernel
     const size_t M = (size_t)1 << tl.m_log;
     const float2* pm = reinterpret_cast<const float2*>(ws + (size_t)2 * tl.groups * M * D);
-    const auto piece_of = [&](int w) { return (size_t)2 * w + (w == w0 && from != w * p.per ? 1 : 0); };
-    constexpr int kLanes = D / 4, kSide = 64 / kLanes;
-    const int side = lane / kLanes, d = lane % kLanes * 4;
+    const int side = threadIdx.x % (64 * WAVES) / kLanes, d = threadIdx.x % kLanes;
     float mm = -INFINITY, lsum = 0.0f;
     f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int w = w0 + side; w <= w1; w += kSide) {
-        const size_t q = piece_of(w) * M + r;
-        const float2 e = pm[q];
-        const f4 v = *reinterpret_cast<const f4*>(ws + q * D + d);
-        const float mn = fmaxf(mm, e.x);
-        const float fo = mm == -INFINITY ? 1.0f : exp2_hw(mm - mn);
-        const float fn = e.x == -INFINITY ? 1.0f : exp2_hw(e.x - mn);
-        y = y * fo + v * fn;
-        lsum = lsum * fo + e.y * fn;
-        mm = mn;
-    }
-#pragma unroll
-    for (int k = kLanes; k < 64; k <<= 1) {
-        const float om = __shfl_xor(mm, k, 64), ol = __shfl_xor(lsum, k, 64);
+    const auto add = [&](float om, float ol, f4 v) {
         const float mn = fmaxf(mm, om);
         const float fo = mm == -INFINITY ? 1.0f : exp2_hw(mm - mn);
         const float fn = om == -INFINITY ? 1.0f : exp2_hw(om - mn);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = y[c] * fo + __shfl_xor(y[c], k, 64) * fn;
+        y = y * fo + v * fn;
         lsum = lsum * fo + ol * fn;
         mm = mn;
+    };
+    for (int w = w0 + side; w <= w1; w += kSides * kDeep) {
+        float2 e[kDeep];
+        f4 v[kDeep];
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) {
+            const int u = min(w + k * kSides, w1);
+            const size_t q = ((size_t)2 * u + (u == w0 && from != u * p.per ? 1 : 0)) * M + r;
+            e[k] = pm[q];
+            v[k] = *reinterpret_cast<const f4*>(ws + q * D + d * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k)
+            if (w + k * kSides <= w1) add(e[k].x, e[k].y, v[k]);
     }
-    if (side == 0) {
-        y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
-        *reinterpret_cast<u2*>(a.out + (size_t)flat * D + d) =
-            u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
-    }
+    so[mine][side][d] = y;
+    if (d == 0) sml[mine][side] = make_float2(mm, lsum);
+    if constexpr (WAVES > 1)
+        __syncthreads();  // (one row per workgroup: all of it is here)
+    else
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (side) return;
+    for (int k = 1; k < min(kSides, w1 - w0 + 1); ++k) add(sml[mine][k].x, sml[mine][k].y, so[mine][k][d]);
+    y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    *reinterpret_cast<u2*>(a.out + (size_t)flat * D + d * 4) =
+        u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
 }
 
-template <int FMT, int D, int RT, int WR>
+template <int FMT, int D, int RT, int WR, int NW>
 void launch_shape(const TreeArgs& a, hipStream_t stream) {
-    using S = Shape<FMT, D, RT, WR>;
+    using S = Shape<FMT, D, RT, WR, NW>;
     const auto log2i = [](int x) { return __builtin_ctz((unsigned)x); };
     Tiling t;
     t.m_log = log2i(S::M);
@@ -885,19 +966,22 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     if (items * chunks >= (1LL << 31) - (1 << 24))
         throw Error("tree_attention: too many (row tile, token chunk) pairs (2^31)");
     t.groups = (int)std::max<long long>(
-        1, std::min<long long>((long long)num_cus() * 2, (items * chunks + t.least - 1) / t.least));
+        1, std::min<long long>((long long)num_cus() * (8 / NW), (items * chunks + t.least - 1) / t.least));
     constexpr size_t kPiece = (size_t)S::M * (D + 2) * sizeof(float);
     float* ws = nullptr;
     const bool cut = chunks > 1;  // an item of one chunk is never cut
     if (cut)
         ws = static_cast<float*>(Scratch{}.get(stream, 2 * (size_t)t.groups * kPiece, "tree attention",
                                                4 * (size_t)num_cus() * 128 * (D + 2) * sizeof(float)));
-    hipLaunchKernelGGL((tree_split_kernel<FMT, D, RT, WR>), dim3(t.groups), dim3(256), 0, stream, a, t,
+    hipLaunchKernelGGL((tree_split_kernel<FMT, D, RT, WR, NW>), dim3(t.groups), dim3(64 * NW), 0, stream, a, t,
                        ws, 1.44269504f * inv_sqrt_d(D), inv_sqrt_d(D));
     check_launch("tree_attention_kernel");
     if (!cut) return;
-    hipLaunchKernelGGL((tree_merge_kernel<S::BF, D>), dim3((unsigned)(((long long)a.tokens * a.hq + 3) / 4)),
-                       dim3(256), 0, stream, a, t, ws);
+    const unsigned rows = (unsigned)(a.tokens * a.hq);
+    if (rows >= 8u * num_cus())  // enough rows to fill the CUs with a wave each
+        hipLaunchKernelGGL((tree_merge_kernel<S::BF, D, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, a, t, ws);
+    else
+        hipLaunchKernelGGL((tree_merge_kernel<S::BF, D, 4>), dim3(rows), dim3(256), 0, stream, a, t, ws);
     check_launch("tree_attention_merge_kernel");
 }
 
@@ -905,10 +989,10 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
 template <int FMT, int D>
 void launch_format(const TreeArgs& a, hipStream_t stream) {
     const long long rows = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
-    if (rows <= 16) return launch_shape<FMT, D, 1, 1>(a, stream);
-    if (rows <= 32) return launch_shape<FMT, D, 2, 1>(a, stream);
-    if (rows <= 64) return launch_shape<FMT, D, 2, 2>(a, stream);
-    return launch_shape<FMT, D, 2, 4>(a, stream);
+    if (rows <= 16) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
+    if (rows <= 32) return launch_shape<FMT, D, 2, 1, 4>(a, stream);
+    if (rows <= 64) return launch_shape<FMT, D, 2, 2, 4>(a, stream);
+    return launch_shape<FMT, D, 2, 4, 4>(a, stream);
 }
 
 void launch_tree(int fmt, const TreeArgs& a, hipStream_t stream) {
