@@ -90,7 +90,22 @@ __device__ __forceinline__ uint32_t infinite_ones(uint32_t x, uint32_t neg) {
     return r;
 }
 
-// One butterfly stage with lane ^ M.
+// One butterfly stage with lane ^ M (16 or 32) of two values: the swap brings a
+// value's two halves under each other, and back.
+template <int M>
+__device__ __forceinline__ void butterfly2(float& a, float& b) {
+    const auto swap = [](float u, float w) {
+        if constexpr (M == 16)
+            return __builtin_amdgcn_permlane16_swap(__float_as_uint(u), __float_as_uint(w), false, false);
+        else
+            return __builtin_amdgcn_permlane32_swap(__float_as_uint(u), __float_as_uint(w), false, false);
+    };
+    const auto x = swap(a, b);
+    const float u = __uint_as_float(x[0]), w = __uint_as_float(x[1]);
+    const auto y = swap(u + w, u - w);
+    a = __uint_as_float(y[0]);
+    b = __uint_as_float(y[1]);
+}
 template <int M>
 __device__ __forceinline__ float butterfly(float v, int lane) {
     const float o = lane_xor<M>(v);
@@ -202,11 +217,16 @@ template <int FMT, int D, int RT, int WR, int NW>
 struct Shape {
     static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
     static constexpr int WT = NW / WR;
-    static constexpr int T = WR == 4 ? 64 : 32, C = T * WT, M = 16 * RT * WR;
+    static constexpr int T = WR >= 4 ? 64 : 32, C = T * WT, M = 16 * RT * WR;
     static constexpr int kRow = 2 * D, kTile = C * kRow;
-    static constexpr int kTiles = kTurned ? 3 : 4;  // K hi, K lo, V; or K, V twice
+    // Buffers of a chunk's tiles (K, V; compressed pages K hi, K lo, V, one buffer
+    // where other workgroups of the CU work while it is filled).
+    static constexpr int kBufs = kTurned && WR < 8 ? 1 : 2, kTiles = kTurned ? 3 : 2;
     static constexpr int kMerge = WT > 1 ? WT * M * (D + 4) * 4 : 0;
-    static constexpr int kLds = kTiles * kTile > kMerge ? kTiles * kTile : kMerge;
+    static constexpr int kLds = kBufs * kTiles * kTile > kMerge ? kBufs * kTiles * kTile : kMerge;
+    // Bytes of codes that a lane decodes at a time, how many of them, lanes per token.
+    static constexpr int kLane = T * (D / 2) / (WR * 64), kUnit = kLane < 16 ? kLane : 16;
+    static constexpr int KU = kLane / kUnit, kParts = D / 2 / kUnit;
 };
 
 constexpr float kAlphaV = 1.5982153f;  // alpha V4[c] is fp16-exact to 9.2e-5 for every c
@@ -245,7 +265,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
     __shared__ __attribute__((aligned(1024))) uint8_t mem[S::kLds];
     __shared__ float2 ml[WT][M];
     __shared__ typename std::conditional<kTurned, DecodeTables, Nothing>::type tab;
-    __shared__ typename std::conditional<kTurned, TokenScales, Nothing>::type tsc;
+    __shared__ typename std::conditional<kTurned, TokenScales, Nothing>::type tscs[S::kBufs];
 
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, gq = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, wt = wv / WR;
@@ -319,15 +339,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
         const auto readable = [&](int t, int pid) { return t < pc.end && pid >= 0; };
 
         // Compressed pages: the codes and scales of this lane's units of the
-        // next chunk (unit u: a quarter of the codes of token u / 4).
-        constexpr int KU = kTurned ? T * 4 / (WR * 64) : 1;
-        typedef uint32_t code_t __attribute__((ext_vector_type(D / 32), aligned(2)));
+        // next chunk (unit u: a part of the codes of token u / kParts).
+        constexpr int KU = kTurned ? S::KU : 1, kUnit = S::kUnit, kParts = S::kParts;
+        typedef uint32_t code_t __attribute__((ext_vector_type(kUnit / 4), aligned(2)));
         code_t kc[KU], vc[KU];
         uint16_t ks[KU], kr[KU], vs[KU];
         int uid[KU];
-        const auto unit_token = [&](int c, int k) {
-            return c * C + wt * T + (((wr + k * WR) * 64 + lane) >> 2);
-        };
+        const auto unit_of = [&](int k) { return (wr + k * WR) * 64 + lane; };
+        const auto unit_token = [&](int c, int k) { return c * C + wt * T + unit_of(k) / kParts; };
         const auto unit_ids = [&](int c) {
             if constexpr (kTurned) {
 #pragma unroll
@@ -347,7 +366,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     const bool ok = readable(t, uid[k]);
                     const uint64_t page = (uint64_t)max(uid[k], 0) * g.page_size;
                     const uint64_t cell = (uint64_t)(tb * g.H + h);
-                    const int part = (lane & 3) * (D / 8);
+                    const int part = lane % kParts * kUnit;
                     const auto at_of = [&](uint64_t off, uint64_t n) {
                         return a.pool + (ok ? page + off + cell * n : dummy);
                     };
@@ -359,44 +378,66 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                 }
             }
         };
-        const auto decode = [&] {
+        // K's values lie in the order of the query's operand: 16-byte piece
+        // 4 kk + gq of a row holds dims 32 kk + 4 gq + 0..3 and 16 more.
+        const auto decode = [&](int buf) {
             if constexpr (kTurned) {
+                auto& tsc = tscs[buf];
 #pragma unroll
                 for (int k = 0; k < KU; ++k) {
-                    const int r = ((wr + k * WR) * 64 + lane) >> 2;  // token of the group
-                    const int part = lane & 3;
+                    const int r = unit_of(k) / kParts;  // token of the group
+                    const int part = lane % kParts;
                     if (part == 0) tsc.k[wt * T + r] = h2f(ks[k]);
                     if (part == 1) {
                         const float v = h2f(vs[k]);
                         tsc.v[wt * T + r] = v;
                         tsc.lv[wt * T + r] = fmaxf(log2_hw(fabsf(v)), -25.0f);
                     }
-                    uint8_t* to = mem + (wt * T + r) * kRow;
+                    uint8_t* to = mem + buf * S::kTiles * S::kTile + (wt * T + r) * kRow;
                     const uint32_t re = FMT == kProd ? __float_as_uint(h2f(kr[k])) : 0u;
+                    u4 hi[kUnit / 4], lo[kUnit / 4];
 #pragma unroll
-                    for (int q = 0; q < D / 32; ++q) {  // a code dword: 8 values, 16 bytes
-                        u4 hi, lo, v;
+                    for (int q = 0; q < kUnit / 4; ++q) {  // a code dword: 8 values
+                        u4 v;
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
                             const uint32_t kb = kc[k][q] >> (8 * b) & 255, vb = vc[k][q] >> (8 * b) & 255;
                             v[b] = tab.v[vb];
                             const uint2 e = tab.k[kb];
                             if constexpr (FMT == kMse) {
-                                hi[b] = e.x;
-                                lo[b] = e.y;
+                                hi[q][b] = e.x;
+                                lo[q][b] = e.y;
                             } else {  // level + (sign ? re : -re)
                                 const float x = __uint_as_float(e.x) +
                                                 __uint_as_float(re ^ ((~kb & 8u) << 28));
                                 const float y = __uint_as_float(e.y) +
                                                 __uint_as_float(re ^ ((~kb & 128u) << 24));
-                                hi[b] = pack2<false>(x, y);
-                                lo[b] = pack2<false>(x - h2f(hi[b] & 0xffff), y - h2f(hi[b] >> 16));
+                                hi[q][b] = pack2<false>(x, y);
+                                lo[q][b] = pack2<false>(x - h2f(hi[q][b] & 0xffff), y - h2f(hi[q][b] >> 16));
                             }
                         }
-                        const int piece = ((part * (D / 32) + q) ^ swz(r)) * 16;
-                        *reinterpret_cast<u4*>(to + piece) = hi;
-                        *reinterpret_cast<u4*>(to + S::kTile + piece) = lo;
+                        const int piece = ((part * (kUnit / 4) + q) ^ swz(r)) * 16;
                         *reinterpret_cast<u4*>(to + 2 * S::kTile + piece) = v;
+                    }
+                    if constexpr (kUnit == 16) {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            const int q = p >> 1, b = (p & 1) * 2, piece = ((part * 4 + p) ^ swz(r)) * 16;
+                            *reinterpret_cast<u4*>(to + piece) =
+                                u4{hi[q][b], hi[q][b + 1], hi[q + 2][b], hi[q + 2][b + 1]};
+                            *reinterpret_cast<u4*>(to + S::kTile + piece) =
+                                u4{lo[q][b], lo[q][b + 1], lo[q + 2][b], lo[q + 2][b + 1]};
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < kUnit / 4; ++q)
+#pragma unroll
+                            for (int b = 0; b < 4; b += 2) {
+                                const int f = part * (kUnit / 2) + q * 2 + b / 2;  // dims 4f..4f + 3
+                                const int piece = (((f >> 3) * 4 + (f & 3)) ^ swz(r)) * 16 + (f >> 2 & 1) * 8;
+                                *reinterpret_cast<u2*>(to + piece) = u2{hi[q][b], hi[q][b + 1]};
+                                *reinterpret_cast<u2*>(to + S::kTile + piece) = u2{lo[q][b], lo[q][b + 1]};
+                            }
                     }
                 }
             }
@@ -443,66 +484,48 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) qh[rt][kk] = raw[kk];
             } else {
-                // WHT(q s) / sqrt(D): value kk * 32 + gq * 8 + e.
-                float x[KK][8];
-                const float sh = (h & 1) ? -inv : inv;
+                // q's rotation H (q s) as a product: row dt * 16 + i of the operand
+                // holds (-1)^(popcount(row & d) + d + h) at d = 32 kk + 8 gq + e, i.e.
+                // one pattern of e per lane, negated by parity of row >> 3 & d >> 3.
+                uint32_t sg[4];
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float u = h2f(raw[kk][e] & 0xffff) * sh, w = h2f(raw[kk][e] >> 16) * -sh;
-                        x[kk][2 * e] = u + w;
-                        x[kk][2 * e + 1] = u - w;
-                    }
+                for (int e = 0; e < 8; e += 2) {
+                    const uint32_t par = (uint32_t)(h ^ ((i >> 3) & gq & 1)) & 1;
+                    const uint32_t s0 = (__popc(i & 7 & e) ^ par) & 1, s1 = (__popc(i & 7 & (e + 1)) ^ par ^ 1) & 1;
+                    sg[e / 2] = 0x3c003c00u | s0 << 15 | s1 << 31;
+                }
+                const uint32_t odd_rows = (gq & 2) ? 0x80008000u : 0u;
+                f4 x[D / 16];
                 float top = 0.0f;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
+                for (int dt = 0; dt < D / 16; ++dt) {
+                    x[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int m = 2; m < 8; m <<= 1)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (!(e & m)) {
-                                const float u = x[kk][e], w = x[kk][e + m];
-                                x[kk][e] = u + w;
-                                x[kk][e + m] = u - w;
-                            }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[kk][e] = butterfly<16>(x[kk][e], lane);
-                        x[kk][e] = butterfly<32>(x[kk][e], lane);
+                    for (int kk = 0; kk < KK; ++kk) {
+                        const uint32_t flip = ((dt & 1) ? odd_rows : 0u) ^
+                                              (__builtin_popcount((dt >> 1) & kk) & 1 ? 0x80008000u : 0u);
+                        x[dt] = mfma<false>(u4{sg[0] ^ flip, sg[1] ^ flip, sg[2] ^ flip, sg[3] ^ flip}, raw[kk],
+                                            x[dt]);
                     }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(x[dt][r]));
                 }
-#pragma unroll
-                for (int m = 1; m < KK; m <<= 1)
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk)
-                        if (!(kk & m))
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float u = x[kk][e], w = x[kk + m][e];
-                                x[kk][e] = u + w;
-                                x[kk + m][e] = u - w;
-                            }
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[kk][e]));
                 top = lane_xor_reduce<16>(top, [](float u, float w) { return fmaxf(u, w); });
                 top = lane_xor_reduce<32>(top, [](float u, float w) { return fmaxf(u, w); });
                 // A power of two brings the row's largest value into [2^13, 2^14),
                 // so hi + lo keep 22 bits of it and no row leaves fp16's range.
                 const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-                const int sh2 = top > 0.0f && ex < 128 ? 13 - max(ex, -100) : 0;
-                const float up = __uint_as_float((uint32_t)(sh2 + 127) << 23);
-                qs[rt] = scale * __uint_as_float((uint32_t)(127 - sh2) << 23);
+                const int sh = top > 0.0f && ex < 128 ? 13 - max(ex, -100) : 0;
+                const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+                qs[rt] = scale * inv * __uint_as_float((uint32_t)(127 - sh) << 23);
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
+                for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float u = x[kk][2 * e] * up, w = x[kk][2 * e + 1] * up;
+                    for (int e = 0; e < 2; ++e) {
+                        const float u = x[dt][2 * e] * up, w = x[dt][2 * e + 1] * up;
                         const uint32_t p = pack2<false>(u, w);
-                        qh[rt][kk][e] = p;
-                        ql[rt][kk][e] = pack2<false>(u - h2f(p & 0xffff), w - h2f(p >> 16));
+                        qh[rt][dt / 2][(dt & 1) * 2 + e] = p;
+                        ql[rt][dt / 2][(dt & 1) * 2 + e] = pack2<false>(u - h2f(p & 0xffff), w - h2f(p >> 16));
                     }
             }
         }
@@ -540,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
             }
             // The chunk's tiles are in LDS: loaded by its waves, or decoded now.
             if constexpr (kTurned) {
-                decode();
+                decode(c & (S::kBufs - 1));
             } else {
                 wait_vmem();
             }
@@ -562,8 +585,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     unit_ids(c + 2);
                 }
             }
-            const uint32_t kb = k_at + (kTurned ? 0 : (c & 1) * 2 * S::kTile);
-            const uint32_t vb = v_at + (kTurned ? 2 * S::kTile : ((c & 1) * 2 + 1) * S::kTile);
+            const uint32_t kb = k_at + (c & (S::kBufs - 1)) * S::kTiles * S::kTile;
+            const uint32_t vb = v_at + ((c & (S::kBufs - 1)) * S::kTiles + S::kTiles - 1) * S::kTile;
+            const auto& tsc = tscs[c & (S::kBufs - 1)];
 
             const auto values = [&](int st, int dt) {
                 const uint32_t p = (vb ^ (dt * 32)) + st * 32 * kRow;
@@ -659,23 +683,51 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                 const int tk = wt * T + st * 32 + gq * 4;  // this lane's tokens: tk + 16 ns + 0..3
                 f4 x[RT][2];
 #pragma unroll
-                for (int ns = 0; ns < 2; ++ns) {
+                for (int rt = 0; rt < RT; ++rt) x[rt][0] = x[rt][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                // K's operands are on their way before the products that take them, V's
+                // before the softmax: left to the scheduler each product waited for its
+                // own load.  (Independent sums next to each other: a product's result
+                // is ready for the next of its own sum some products later.)
+                u4 va[D / 16];
+                if constexpr (kTurned) {
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) x[rt][ns] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int ns = 0; ns < 2; ++ns) {
+                        u4 k0[KK], k1[KK];
 #pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-                        const u4 k0 = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + ns * 16 * kRow);
-                        if constexpr (kTurned) {
-                            const u4 k1 = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                x[rt][ns] = mfma<false>(k1, qh[rt][kk], x[rt][ns]);
-                                x[rt][ns] = mfma<false>(k0, ql[rt][kk], x[rt][ns]);
-                            }
+                        for (int kk = 0; kk < KK; ++kk) {
+                            k0[kk] = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + ns * 16 * kRow);
+                            k1[kk] = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
                         }
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<BF>(k0, qh[rt][kk], x[rt][ns]);
+                        for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k0[kk], ql[rt][kk], x[rt][ns]);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k1[kk], qh[rt][kk], x[rt][ns]);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k0[kk], qh[rt][kk], x[rt][ns]);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
+                } else {
+                    u4 k0[KK][2];
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                        for (int ns = 0; ns < 2; ++ns)
+                            k0[kk][ns] = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + ns * 16 * kRow);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                        for (int ns = 0; ns < 2; ++ns)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<BF>(k0[kk][ns], qh[rt][kk], x[rt][ns]);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt) va[dt] = values(st, dt);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 // Logits in units of log2 (dense pages: the factor enters below);
                 // compressed pages: K's scale per token.
@@ -761,14 +813,17 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     weights(std::false_type{});
                 else
                     weights(std::true_type{});
+                if constexpr (kTurned) {  // (registers for V only now)
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt) va[dt] = values(st, dt);
+                }
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt) {
-                    const u4 v = values(st, dt);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(v, pw[rt], o[rt][dt]);
+                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(va[dt], pw[rt], o[rt][dt]);
                 }
             }
-            if (kTurned && WR > 1) __syncthreads();  // the tiles are decoded again
+            if (kTurned && WR > 1 && S::kBufs == 1) __syncthreads();  // the tiles are decoded again
         }
 
         // A row's sum over its four lanes.
@@ -785,18 +840,21 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
             }
             l[rt] = lane_xor_reduce<16>(l[rt], [](float u, float w) { return u + w; });
             l[rt] = lane_xor_reduce<32>(l[rt], [](float u, float w) { return u + w; });
-            if constexpr (kTurned) {
-                // Rotated back (linear: before any merge): value dt * 16 + gq * 4 + r.
+            if (kTurned && whole) {
+                // Rotated back (the merge does it for pieces): value dt * 16 + gq * 4 + r.
                 const float sh = ((h & 1) ? -inv : inv) * (1.0f / kAlphaV);
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt) {
                     f4 y = o[rt][dt];
-                    f4 z = {y[0] + y[1], y[0] - y[1], y[2] + y[3], y[2] - y[3]};
+                    const f4 z = {y[0] + y[1], y[0] - y[1], y[2] + y[3], y[2] - y[3]};
                     y = f4{z[0] + z[2], z[1] + z[3], z[0] - z[2], z[1] - z[3]};
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        y[r] = butterfly<16>(y[r], lane);
-                        y[r] = butterfly<32>(y[r], lane);
+                    for (int r = 0; r < 4; r += 2) {
+                        float u = y[r], w = y[r + 1];
+                        butterfly2<16>(u, w);
+                        butterfly2<32>(u, w);
+                        y[r] = u;
+                        y[r + 1] = w;
                     }
                     o[rt][dt] = y;
                 }
@@ -882,10 +940,10 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
 }
 
 // Merge of the items that were cut: WAVES waves per query row, D / 4 lanes per
-// piece of it.
-template <bool BF, int D, int WAVES>
+// piece of it; compressed pages' sums are rotated back here.
+template <bool BF, bool TURNED, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
-                                                         const float* __restrict__ ws) {
+                                                         const float* __restrict__ ws, float inv) {
     constexpr int kLanes = D / 4, kSides = 64 * WAVES / kLanes, kRows = 4 / WAVES, kDeep = 4;
     __shared__ float2 sml[kRows][kSides];
     __shared__ f4 so[kRows][kSides][kLanes];
@@ -944,9 +1002,25 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
         __syncthreads();  // (one row per workgroup: all of it is here)
     else
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (side) return;
-    for (int k = 1; k < min(kSides, w1 - w0 + 1); ++k) add(sml[mine][k].x, sml[mine][k].y, so[mine][k][d]);
+    if (side * kLanes >= 64) return;
+    for (int k = 0; k < min(kSides, w1 - w0 + 1); ++k)
+        if (k != side) add(sml[mine][k].x, sml[mine][k].y, so[mine][k][d]);
     y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    if constexpr (TURNED) {  // value d * 4 + r; every side of the wave holds the row
+        const float sh = ((h & 1) ? -inv : inv) * (1.0f / kAlphaV);
+        const f4 z = {y[0] + y[1], y[0] - y[1], y[2] + y[3], y[2] - y[3]};
+        y = f4{z[0] + z[2], z[1] + z[3], z[0] - z[2], z[1] - z[3]};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            y[r] = butterfly<1>(y[r], lane);
+            y[r] = butterfly<2>(y[r], lane);
+            y[r] = butterfly<4>(y[r], lane);
+            y[r] = butterfly<8>(y[r], lane);
+            if (D == 128) y[r] = butterfly<16>(y[r], lane);
+        }
+        y *= f4{sh, -sh, sh, -sh};
+    }
+    if (side) return;
     *reinterpret_cast<u2*>(a.out + (size_t)flat * D + d * 4) =
         u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
 }
@@ -979,9 +1053,11 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     if (!cut) return;
     const unsigned rows = (unsigned)(a.tokens * a.hq);
     if (rows >= 8u * num_cus())  // enough rows to fill the CUs with a wave each
-        hipLaunchKernelGGL((tree_merge_kernel<S::BF, D, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, a, t, ws);
+        hipLaunchKernelGGL((tree_merge_kernel<S::BF, S::kTurned, D, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, a, t, ws,
+                           inv_sqrt_d(D));
     else
-        hipLaunchKernelGGL((tree_merge_kernel<S::BF, D, 4>), dim3(rows), dim3(256), 0, stream, a, t, ws);
+        hipLaunchKernelGGL((tree_merge_kernel<S::BF, S::kTurned, D, 4>), dim3(rows), dim3(256), 0, stream, a, t, ws,
+                           inv_sqrt_d(D));
     check_launch("tree_attention_merge_kernel");
 }
 
@@ -992,7 +1068,8 @@ void launch_format(const TreeArgs& a, hipStream_t stream) {
     if (rows <= 16) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
     if (rows <= 32) return launch_shape<FMT, D, 2, 1, 4>(a, stream);
     if (rows <= 64) return launch_shape<FMT, D, 2, 2, 4>(a, stream);
-    return launch_shape<FMT, D, 2, 4, 4>(a, stream);
+    if (rows <= 128) return launch_shape<FMT, D, 2, 4, 4>(a, stream);
+    return launch_shape<FMT, D, 2, 8, 8>(a, stream);
 }
 
 void launch_tree(int fmt, const TreeArgs& a, hipStream_t stream) {
