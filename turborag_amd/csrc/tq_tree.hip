@@ -39,6 +39,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) u4 lds_u4;
@@ -240,8 +241,27 @@ __device__ __forceinline__ void wait_vmem() { asm volatile("s_waitcnt vmcnt(0)" 
 
 struct DecodeTables {
     uint32_t v[256];  // code byte -> fp16 pair of alpha V4 (low nibble first)
-    uint2 k[256];     // turbo_mse: fp16 pairs of V4, hi and lo; turbo_prod: fp32 pair of K3
+    // turbo_mse: fp16 pairs of V4, hi and lo; turbo_prod: fp32 pair of K3, the
+    // last bit 1 where the residual is subtracted.
+    uint2 k[256];
 };
+// Two table entries of turbo_prod's K and the row's residual RMS -> their
+// values level +- re as fp16 pairs, hi and lo = fp16(value - hi).
+__device__ __forceinline__ uint2 split_k3(uint2 e, float re) {
+    uint32_t s0, s1;  // 1.0, negative where the last bit is 1
+    asm("v_lshl_or_b32 %0, %1, 31, 1.0" : "=v"(s0) : "v"(e.x));
+    asm("v_lshl_or_b32 %0, %1, 31, 1.0" : "=v"(s1) : "v"(e.y));
+    const float x = fmaf(__uint_as_float(s0), re, __uint_as_float(e.x));
+    const float y = fmaf(__uint_as_float(s1), re, __uint_as_float(e.y));
+    const uint32_t hi = pack2<false>(x, y);
+    uint32_t lo;
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\t"
+        "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=&v"(lo)
+        : "v"(hi), "v"(x), "v"(y));
+    return make_uint2(hi, lo);
+}
+
 struct alignas(16) TokenScales {
     float k[128], v[128], lv[128];  // of a chunk's tokens; lv = max(log2 |v|, -25)
 };
@@ -279,6 +299,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
     const int vrow = 4 * gq + (i >> 2);
     const uint32_t v_at = mem0 + (wt * T + vrow) * kRow + ((((i >> 1) & 1) ^ swz(vrow)) * 16) + (i & 1) * 8;
 
+    SeqBlock sb;
+    int total;
+    sb = load_seqs(a, tl, 0, 0, lane, total);
     if (kTurned && tid < 256) {
       if constexpr (kTurned) {
         const int lo = tid & 15, hi = tid >> 4;
@@ -288,14 +311,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
             const uint32_t h = pack2<false>(x, y);
             tab.k[tid] = make_uint2(h, pack2<false>(x - h2f(h & 0xffff), y - h2f(h >> 16)));
         } else {
-            tab.k[tid] = make_uint2(__float_as_uint(pick(kK3, lo & 7)), __float_as_uint(pick(kK3, hi & 7)));
+            const auto entry = [](int n) {
+                return (__float_as_uint(pick(kK3, n & 7)) & ~1u) | (n & 8 ? 0u : 1u);
+            };
+            tab.k[tid] = make_uint2(entry(lo), entry(hi));
         }
       }
     }
 
-    SeqBlock sb;
-    int total;
-    sb = load_seqs(a, tl, 0, 0, lane, total);
     for (int f = 64; f < a.seqs; f += 64) (void)load_seqs(a, tl, f, total, lane, total);
     const Plan plan = make_plan(a, tl, total);
     const int all = plan.total * g.H;
@@ -314,17 +337,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
         const int32_t* __restrict__ table = a.tables + (size_t)pc.s * a.max_blocks;
         __syncthreads();  // the last piece's LDS is free (and the tables are written)
 
-        // This lane's query rows.
-        int row[RT];
-        size_t qo[RT];
-        const int32_t* mrow[RT];
+        // This lane's query rows: their tokens (the last row's past the item's end).
+        int tok[RT];
+        const auto row_of = [&](int rt) { return pc.tile * M + (wr * RT + rt) * 16 + i; };
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            row[rt] = pc.tile * M + (wr * RT + rt) * 16 + i;
-            const int rr = min(row[rt], R - 1), tok = rr / a.group;
-            qo[rt] = ((size_t)(pc.row0 + tok) * a.hq + h * a.group + (rr - tok * a.group)) * D;
-            mrow[rt] = a.mask + (size_t)(pc.row0 + tok) * a.mask_words;
-        }
+        for (int rt = 0; rt < RT; ++rt) tok[rt] = min(row_of(rt), R - 1) / a.group;
+        const auto row_at = [&](int row, int token) {
+            return ((size_t)(pc.row0 + token) * a.hq + h * a.group + (row - token * a.group)) * D;
+        };
         const auto token_of = [&](int c) { return c * C + wt * T + (lane & (T - 1)); };
         const auto page_of = [&](int t, int& tib) {
             const int tc = max(min(t, pc.end - 1), 0);
@@ -394,50 +414,47 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                         tsc.lv[wt * T + r] = fmaxf(log2_hw(fabsf(v)), -25.0f);
                     }
                     uint8_t* to = mem + buf * S::kTiles * S::kTile + (wt * T + r) * kRow;
-                    const uint32_t re = FMT == kProd ? __float_as_uint(h2f(kr[k])) : 0u;
-                    u4 hi[kUnit / 4], lo[kUnit / 4];
-#pragma unroll
-                    for (int q = 0; q < kUnit / 4; ++q) {  // a code dword: 8 values
-                        u4 v;
+                    const float re = FMT == kProd ? h2f(kr[k]) : 0.0f;
+                    // A code dword (8 values) at a time; the next one's table entries are
+                    // on their way meanwhile (each lookup waited for its own otherwise).
+                    uint2 ke[2][4];
+                    uint32_t ve[2][4];
+                    const auto look_up = [&](int q) {
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
-                            const uint32_t kb = kc[k][q] >> (8 * b) & 255, vb = vc[k][q] >> (8 * b) & 255;
-                            v[b] = tab.v[vb];
-                            const uint2 e = tab.k[kb];
+                            ke[q & 1][b] = tab.k[kc[k][q] >> (8 * b) & 255];
+                            ve[q & 1][b] = tab.v[vc[k][q] >> (8 * b) & 255];
+                        }
+                    };
+                    look_up(0);
+#pragma unroll
+                    for (int q = 0; q < kUnit / 4; ++q) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (q + 1 < kUnit / 4) look_up(q + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                        u4 v, hi, lo;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint2 e = ke[q & 1][b];
+                            v[b] = ve[q & 1][b];
                             if constexpr (FMT == kMse) {
-                                hi[q][b] = e.x;
-                                lo[q][b] = e.y;
-                            } else {  // level + (sign ? re : -re)
-                                const float x = __uint_as_float(e.x) +
-                                                __uint_as_float(re ^ ((~kb & 8u) << 28));
-                                const float y = __uint_as_float(e.y) +
-                                                __uint_as_float(re ^ ((~kb & 128u) << 24));
-                                hi[q][b] = pack2<false>(x, y);
-                                lo[q][b] = pack2<false>(x - h2f(hi[q][b] & 0xffff), y - h2f(hi[q][b] >> 16));
+                                hi[b] = e.x;
+                                lo[b] = e.y;
+                            } else {  // level + (sign ? re : -re), 2^-24 of the level off
+                                const uint2 w = split_k3(e, re);
+                                hi[b] = w.x;
+                                lo[b] = w.y;
                             }
                         }
                         const int piece = ((part * (kUnit / 4) + q) ^ swz(r)) * 16;
                         *reinterpret_cast<u4*>(to + 2 * S::kTile + piece) = v;
-                    }
-                    if constexpr (kUnit == 16) {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            const int q = p >> 1, b = (p & 1) * 2, piece = ((part * 4 + p) ^ swz(r)) * 16;
-                            *reinterpret_cast<u4*>(to + piece) =
-                                u4{hi[q][b], hi[q][b + 1], hi[q + 2][b], hi[q + 2][b + 1]};
-                            *reinterpret_cast<u4*>(to + S::kTile + piece) =
-                                u4{lo[q][b], lo[q][b + 1], lo[q + 2][b], lo[q + 2][b + 1]};
+                        for (int b = 0; b < 4; b += 2) {
+                            const int f = part * (kUnit / 2) + q * 2 + b / 2;  // dims 4f..4f + 3
+                            const int kp = (((f >> 3) * 4 + (f & 3)) ^ swz(r)) * 16 + (f >> 2 & 1) * 8;
+                            *reinterpret_cast<u2*>(to + kp) = u2{hi[b], hi[b + 1]};
+                            *reinterpret_cast<u2*>(to + S::kTile + kp) = u2{lo[b], lo[b + 1]};
                         }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < kUnit / 4; ++q)
-#pragma unroll
-                            for (int b = 0; b < 4; b += 2) {
-                                const int f = part * (kUnit / 2) + q * 2 + b / 2;  // dims 4f..4f + 3
-                                const int piece = (((f >> 3) * 4 + (f & 3)) ^ swz(r)) * 16 + (f >> 2 & 1) * 8;
-                                *reinterpret_cast<u2*>(to + piece) = u2{hi[q][b], hi[q][b + 1]};
-                                *reinterpret_cast<u2*>(to + S::kTile + piece) = u2{lo[q][b], lo[q][b + 1]};
-                            }
                     }
                 }
             }
@@ -469,16 +486,28 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
         };
 
         unit_ids(c0);
-        // Query operands.
+        // Query operands; the first chunk is on its way before they are prepared.
         constexpr int KK = D / 32;
         u4 qh[RT][KK], ql[kTurned ? RT : 1][KK];
         float qs[RT];
+        u4 raws[RT][KK];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            u4 raw[KK];
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                raw[kk] = *reinterpret_cast<const u4*>(a.query + qo[rt] + kk * 32 + gq * 8);
+                raws[rt][kk] = *reinterpret_cast<const u4*>(a.query + row_at(min(row_of(rt), R - 1), tok[rt]) +
+                                                            kk * 32 + gq * 8);
+        stage(c0, id);
+        fetch(c0);
+        int next = id, next2 = id2;
+        if (c0 + 1 < c1) {
+            next = table[page_of(token_of(c0 + 1), tib)];
+            if (kPair) next2 = table[page_of(token_of(c0 + 1) + (wt ? -T : T), tib)];
+            unit_ids(c0 + 1);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const u4(&raw)[KK] = raws[rt];
             qs[rt] = scale;
             if constexpr (!kTurned) {
 #pragma unroll
@@ -541,14 +570,6 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
             for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        stage(c0, id);
-        fetch(c0);
-        int next = id, next2 = id2;
-        if (c0 + 1 < c1) {
-            next = table[page_of(token_of(c0 + 1), tib)];
-            if (kPair) next2 = table[page_of(token_of(c0 + 1) + (wt ? -T : T), tib)];
-            unit_ids(c0 + 1);
-        }
         for (int c = c0; c < c1; ++c) {
             const int tb0 = c * C + wt * T;  // the wave's first token
             constexpr uint64_t kAll = T == 64 ? ~0ull : (1ull << (T & 63)) - 1;
@@ -605,10 +626,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     see[rt] = live;
                     if (j0 + T > 0) {  // (words before the drafted tokens: the prefix)
                         const int w0 = j0 >> 5;
+                        const int32_t* mrow = a.mask + (size_t)(pc.row0 + tok[rt]) * a.mask_words;
                         uint32_t w[3];
 #pragma unroll
                         for (int k = 0; k < 3; ++k)
-                            w[k] = w0 + k < 0 ? ~0u : w0 + k < a.mask_words ? (uint32_t)mrow[rt][w0 + k] : 0u;
+                            w[k] = w0 + k < 0 ? ~0u : w0 + k < a.mask_words ? (uint32_t)mrow[w0 + k] : 0u;
                         const int sh = j0 & 31;
                         const uint32_t b0 = (uint32_t)(((uint64_t)w[1] << 32 | w[0]) >> sh);
                         const uint32_t b1 = (uint32_t)(((uint64_t)w[2] << 32 | w[1]) >> sh);
@@ -691,25 +713,18 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                 u4 va[D / 16];
                 if constexpr (kTurned) {
 #pragma unroll
-                    for (int ns = 0; ns < 2; ++ns) {
-                        u4 k0[KK], k1[KK];
+                    for (int ns = 0; ns < 2; ++ns)
 #pragma unroll
                         for (int kk = 0; kk < KK; ++kk) {
-                            k0[kk] = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + ns * 16 * kRow);
-                            k1[kk] = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
+                            const u4 k0 = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + ns * 16 * kRow);
+                            const u4 k1 = *(lds_u4*)(uintptr_t)((ks_at ^ (kk * 64)) + S::kTile + ns * 16 * kRow);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k0, ql[rt][kk], x[rt][ns]);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k1, qh[rt][kk], x[rt][ns]);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k0, qh[rt][kk], x[rt][ns]);
                         }
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k0[kk], ql[rt][kk], x[rt][ns]);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k1[kk], qh[rt][kk], x[rt][ns]);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) x[rt][ns] = mfma<false>(k0[kk], qh[rt][kk], x[rt][ns]);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
                 } else {
                     u4 k0[KK][2];
 #pragma unroll
@@ -729,8 +744,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     for (int dt = 0; dt < D / 16; ++dt) va[dt] = values(st, dt);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                // Logits in units of log2 (dense pages: the factor enters below);
-                // compressed pages: K's scale per token.
+                // Compressed pages: K's scale per token.  (The row's factor to a logit in
+                // units of log2, above zero, enters below.)
                 if constexpr (kTurned) {
 #pragma unroll
                     for (int ns = 0; ns < 2; ++ns) {
@@ -738,7 +753,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[rt][ns][r] *= sk[r] * qs[rt];
+                            for (int r = 0; r < 4; ++r) x[rt][ns][r] *= sk[r];
                     }
                 }
                 uint32_t sees[RT];
@@ -767,7 +782,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            top[rt] = fmaxf(top[rt], kTurned ? x[rt][ns][r] + lv[r] : x[rt][ns][r]);
+                            top[rt] = fmaxf(top[rt], kTurned ? fmaf(x[rt][ns][r], qs[rt], lv[r]) : x[rt][ns][r]);
                 }
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -795,8 +810,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                             float p[4], sum = 0.0f;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                p[r] = exp2_hw(kTurned ? x[rt][ns][r] + ref[rt]
-                                                       : fmaf(x[rt][ns][r], scale, ref[rt]));
+                                p[r] = exp2_hw(fmaf(x[rt][ns][r], kTurned ? qs[rt] : scale, ref[rt]));
                                 sum += p[r];
                                 if constexpr (kTurned) {
                                     p[r] *= sv[r];  // (not 0 * NaN where the row sees nothing)
@@ -872,27 +886,33 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     o[rt][dt] *= f4{sh, -sh, sh, -sh};
             }
         }
+        // (what follows is computed here, not kept over the chunks in registers
+        // that then overflow to memory)
+        int etid = tid;
+        asm volatile("" : "+v"(etid));
+        const int ei = etid & 15, eg = (etid >> 4) & 3;
         const int piece = 2 * blockIdx.x + (first ? 0 : 1);
         float* po = ws + (size_t)piece * M * D;
         float2* pm = reinterpret_cast<float2*>(ws + (size_t)2 * tl.groups * M * D) + (size_t)piece * M;
         if constexpr (WT == 1) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                if (row[rt] >= R) continue;
+                const int row = pc.tile * M + (wr * RT + rt) * 16 + ei;
+                if (row >= R) continue;
                 if (whole) {
                     const float f = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
 #pragma unroll
                     for (int dt = 0; dt < D / 16; ++dt) {
                         const f4 y = o[rt][dt] * f;
-                        *reinterpret_cast<u2*>(a.out + qo[rt] + dt * 16 + gq * 4) =
+                        *reinterpret_cast<u2*>(a.out + row_at(row, row / a.group) + dt * 16 + eg * 4) =
                             u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
                     }
                 } else {
-                    const int r = (wr * RT + rt) * 16 + i;
+                    const int r = (wr * RT + rt) * 16 + ei;
 #pragma unroll
                     for (int dt = 0; dt < D / 16; ++dt)
-                        *reinterpret_cast<f4*>(po + r * D + dt * 16 + gq * 4) = o[rt][dt];
-                    if (gq == 0) pm[r] = make_float2(m[rt], l[rt]);
+                        *reinterpret_cast<f4*>(po + r * D + dt * 16 + eg * 4) = o[rt][dt];
+                    if (eg == 0) pm[r] = make_float2(m[rt], l[rt]);
                 }
             }
         } else {
@@ -900,15 +920,15 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
             float* mo = reinterpret_cast<float*>(mem);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const int r = (wr * RT + rt) * 16 + i;
-                if (gq == 0) ml[wt][r] = make_float2(m[rt], l[rt]);
+                const int r = (wr * RT + rt) * 16 + ei;
+                if (eg == 0) ml[wt][r] = make_float2(m[rt], l[rt]);
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt)
-                    *reinterpret_cast<f4*>(mo + (wt * M + r) * (D + 4) + dt * 16 + gq * 4) = o[rt][dt];
+                    *reinterpret_cast<f4*>(mo + (wt * M + r) * (D + 4) + dt * 16 + eg * 4) = o[rt][dt];
             }
             __syncthreads();
 #pragma unroll 2
-            for (int u = tid; u < M * (D / 4); u += 64 * NW) {
+            for (int u = etid; u < M * (D / 4); u += 64 * NW) {
                 const int r = u / (D / 4), d = u % (D / 4) * 4, rr = pc.tile * M + r;
                 if (rr >= R) break;
                 float mm = -INFINITY, lsum = 0.0f;
@@ -924,8 +944,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                     y += *reinterpret_cast<const f4*>(mo + (w * M + r) * (D + 4) + d) * (e.x == -INFINITY ? 1.0f : f);
                 }
                 if (whole) {
-                    const int tok = rr / a.group;
-                    const size_t to = ((size_t)(pc.row0 + tok) * a.hq + h * a.group + (rr - tok * a.group)) * D + d;
+                    const size_t to = row_at(rr, rr / a.group) + d;
                     y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
                     *reinterpret_cast<u2*>(a.out + to) = u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
                 } else {
