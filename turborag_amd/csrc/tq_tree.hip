@@ -119,8 +119,12 @@ __device__ __forceinline__ float butterfly(float v, int lane) {
 // tile), and workgroup w takes the chunks [w per, (w + 1) per) of that line:
 // the same work for every workgroup, whatever the lengths, which only the
 // device knows.  A piece is a workgroup's part of an item; only its first and
-// its last piece can be cut.
+// its last piece can be cut.  Every item begins with kLead chunks of no tokens:
+// beginning a piece costs about as much as they do, so a workgroup with an item's
+// beginning inside gets as many chunks less (32 ragged sequences, turbo_prod:
+// the last workgroup had ended 10 us after the median one).
 // ---------------------------------------------------------------------------
+constexpr int kLead = 2;
 struct Tiling {
     int m_log, c_log;  // log2 of M, C
     int groups;        // workgroups of the split launch
@@ -134,7 +138,7 @@ struct Plan {
 struct SeqBlock {
     int first;
     int row0, rows, L, end;  // first token row, drafted tokens, prefix length, kv end
-    int chunks, tiles;
+    int chunks, tiles;  // (chunks of an item, kLead among them)
     int before;  // chunks of the head's items before this sequence
 };
 
@@ -148,7 +152,7 @@ __device__ __forceinline__ SeqBlock load_seqs(const TreeArgs& a, const Tiling& g
     b.rows = first + lane < a.seqs ? max(min(r1, a.tokens) - b.row0, 0) : 0;
     b.L = max(L, 0);
     b.end = (int)min((long long)b.L + b.rows, (long long)a.max_kv);
-    b.chunks = max((b.end + (1 << g.c_log) - 1) >> g.c_log, 1);
+    b.chunks = max((b.end + (1 << g.c_log) - 1) >> g.c_log, 1) + kLead;
     b.tiles = (b.rows * a.group + (1 << g.m_log) - 1) >> g.m_log;
     const int cost = b.tiles * b.chunks;
     int up = cost;
@@ -173,7 +177,7 @@ __device__ __forceinline__ Plan make_plan(const TreeArgs& a, const Tiling& g, in
 // A piece, the same in every lane.
 struct Piece {
     int h, s, row0, rows, L, end;
-    int tile, chunk, chunks;  // first chunk of the piece; chunks of its item
+    int tile, chunk, chunks;  // place in the item (from kLead on: chunks of tokens); its chunks
 };
 __device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, const Plan& p, int at,
                                         int lane, SeqBlock& b) {
@@ -218,6 +222,8 @@ template <int FMT, int D, int RT, int WR, int NW>
 struct Shape {
     static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
     static constexpr int WT = NW / WR;
+    // Workgroups of a CU (registers and LDS hold so many).
+    static constexpr int kPerCu = kTurned && RT == 1 && WR == 4 ? 3 : 8 / NW;
     static constexpr int T = WR >= 4 ? 64 : 32, C = T * WT, M = 16 * RT * WR;
     static constexpr int kRow = 2 * D, kTile = C * kRow;
     // Buffers of a chunk's tiles (K, V; compressed pages K hi, K lo, V, one buffer
@@ -271,7 +277,7 @@ struct Nothing {};
 #endif
 
 template <int FMT, int D, int RT, int WR, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a, const Tiling tl,
+__global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 4)) void tree_split_kernel(const TreeArgs a, const Tiling tl,
                                                             float* __restrict__ ws, float scale,
                                                             float inv) {
     using S = Shape<FMT, D, RT, WR, NW>;
@@ -331,8 +337,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
     bool first = true;
     for (int at = (int)min(begin, (long long)all); at < stop;) {
         const Piece pc = locate(a, tl, plan, at, lane, sb);
-        const int c0 = pc.chunk, c1 = min(pc.chunk + (stop - at), pc.chunks);
-        const bool whole = c1 - c0 == pc.chunks;
+        const int upto = min(pc.chunk + (stop - at), pc.chunks);
+        const int c0 = max(pc.chunk - kLead, 0), c1 = upto - kLead;
+        at += upto - pc.chunk;
+        if (c1 <= c0) break;  // (the next workgroup has the item's tokens)
+        const bool whole = c1 - c0 == pc.chunks - kLead;
         const int R = pc.rows * a.group, h = pc.h;
         const int32_t* __restrict__ table = a.tables + (size_t)pc.s * a.max_blocks;
         __syncthreads();  // the last piece's LDS is free (and the tables are written)
@@ -953,7 +962,6 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_split_kernel(const TreeArgs a
                 }
             }
         }
-        at += c1 - c0;
         first = false;
     }
 }
@@ -986,7 +994,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
     const int rr = (tok - row0) * a.group + (qh - h * a.group);
     const int tile = rr >> tl.m_log, r = rr & ((1 << tl.m_log) - 1);
     const int from = h * total + before + tile * chunks;
-    const int w0 = from / p.per, w1 = (from + chunks - 1) / p.per;
+    const int w0 = (from + kLead) / p.per, w1 = (from + chunks - 1) / p.per;
     if (w0 == w1 || w1 >= tl.groups) return;  // whole: written by the split kernel
     const size_t M = (size_t)1 << tl.m_log;
     const float2* pm = reinterpret_cast<const float2*>(ws + (size_t)2 * tl.groups * M * D);
@@ -1007,7 +1015,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
             const int u = min(w + k * kSides, w1);
-            const size_t q = ((size_t)2 * u + (u == w0 && from != u * p.per ? 1 : 0)) * M + r;
+            const size_t q = ((size_t)2 * u + (u == w0 && from > u * p.per ? 1 : 0)) * M + r;
             e[k] = pm[q];
             v[k] = *reinterpret_cast<const f4*>(ws + q * D + d * 4);
         }
@@ -1053,16 +1061,16 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     t.c_log = log2i(S::C);
     t.least = std::max(1, 128 / S::C);
     // The line's length is known to the device only; here its bound.
-    const long long chunks = std::max<long long>(1, ((long long)a.max_kv + S::C - 1) / S::C);
+    const long long chunks = std::max<long long>(1, ((long long)a.max_kv + S::C - 1) / S::C) + kLead;
     const long long items =
         (((long long)a.tokens * a.group) / S::M + std::min(a.seqs, a.tokens)) * a.g.H;
     if (items * chunks >= (1LL << 31) - (1 << 24))
         throw Error("tree_attention: too many (row tile, token chunk) pairs (2^31)");
     t.groups = (int)std::max<long long>(
-        1, std::min<long long>((long long)num_cus() * (8 / NW), (items * chunks + t.least - 1) / t.least));
+        1, std::min<long long>((long long)num_cus() * S::kPerCu, (items * chunks + t.least - 1) / t.least));
     constexpr size_t kPiece = (size_t)S::M * (D + 2) * sizeof(float);
     float* ws = nullptr;
-    const bool cut = chunks > 1;  // an item of one chunk is never cut
+    const bool cut = chunks > 1 + kLead;  // an item of one chunk is never cut
     if (cut)
         ws = static_cast<float*>(Scratch{}.get(stream, 2 * (size_t)t.groups * kPiece, "tree attention",
                                                4 * (size_t)num_cus() * 128 * (D + 2) * sizeof(float)));
@@ -1086,7 +1094,7 @@ void launch_format(const TreeArgs& a, hipStream_t stream) {
     const long long rows = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
     if (rows <= 16) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
     if (rows <= 32) return launch_shape<FMT, D, 2, 1, 4>(a, stream);
-    if (rows <= 64) return launch_shape<FMT, D, 2, 2, 4>(a, stream);
+    if (rows <= 64) return launch_shape<FMT, D, (FMT >= kProd ? 1 : 2), (FMT >= kProd ? 4 : 2), 4>(a, stream);
     if (rows <= 128) return launch_shape<FMT, D, 2, 4, 4>(a, stream);
     return launch_shape<FMT, D, 2, 8, 8>(a, stream);
 }
