@@ -128,7 +128,6 @@ constexpr int kLead = 2;
 struct Tiling {
     int m_log, c_log;  // log2 of M, C
     int groups;        // workgroups of the split launch
-    int least;         // fewest chunks a workgroup takes
 };
 struct Plan {
     int total;  // chunks of one head's items
@@ -170,7 +169,7 @@ __device__ __forceinline__ Plan make_plan(const TreeArgs& a, const Tiling& g, in
     Plan p;
     p.total = total;
     const long long all = (long long)total * a.g.H;
-    p.per = max((int)((all + g.groups - 1) / g.groups), g.least);
+    p.per = max((int)((all + g.groups - 1) / g.groups), 1);
     return p;
 }
 
@@ -223,7 +222,7 @@ struct Shape {
     static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
     static constexpr int WT = NW / WR;
     // Workgroups of a CU (registers and LDS hold so many).
-    static constexpr int kPerCu = kTurned && RT == 1 && WR == 4 ? 3 : 8 / NW;
+    static constexpr int kPerCu = kTurned && RT == 1 && WR == 4 ? 3 : WR == 1 && D == 128 ? 1 : 8 / NW;
     static constexpr int T = WR >= 4 ? 64 : 32, C = T * WT, M = 16 * RT * WR;
     static constexpr int kRow = 2 * D, kTile = C * kRow;
     // Buffers of a chunk's tiles (K, V; compressed pages K hi, K lo, V, one buffer
@@ -277,7 +276,7 @@ struct Nothing {};
 #endif
 
 template <int FMT, int D, int RT, int WR, int NW>
-__global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 4)) void tree_split_kernel(const TreeArgs a, const Tiling tl,
+__global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW + 3) / 4)) void tree_split_kernel(const TreeArgs a, const Tiling tl,
                                                             float* __restrict__ ws, float scale,
                                                             float inv) {
     using S = Shape<FMT, D, RT, WR, NW>;
@@ -407,8 +406,6 @@ __global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 
                 }
             }
         };
-        // K's values lie in the order of the query's operand: 16-byte piece
-        // 4 kk + gq of a row holds dims 32 kk + 4 gq + 0..3 and 16 more.
         const auto decode = [&](int buf) {
             if constexpr (kTurned) {
                 auto& tsc = tscs[buf];
@@ -456,14 +453,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 
                             }
                         }
                         const int piece = ((part * (kUnit / 4) + q) ^ swz(r)) * 16;
+                        *reinterpret_cast<u4*>(to + piece) = hi;
+                        *reinterpret_cast<u4*>(to + S::kTile + piece) = lo;
                         *reinterpret_cast<u4*>(to + 2 * S::kTile + piece) = v;
-#pragma unroll
-                        for (int b = 0; b < 4; b += 2) {
-                            const int f = part * (kUnit / 2) + q * 2 + b / 2;  // dims 4f..4f + 3
-                            const int kp = (((f >> 3) * 4 + (f & 3)) ^ swz(r)) * 16 + (f >> 2 & 1) * 8;
-                            *reinterpret_cast<u2*>(to + kp) = u2{hi[b], hi[b + 1]};
-                            *reinterpret_cast<u2*>(to + S::kTile + kp) = u2{lo[b], lo[b + 1]};
-                        }
                     }
                 }
             }
@@ -522,17 +514,21 @@ __global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) qh[rt][kk] = raw[kk];
             } else {
-                // q's rotation H (q s) as a product: row dt * 16 + i of the operand
-                // holds (-1)^(popcount(row & d) + d + h) at d = 32 kk + 8 gq + e, i.e.
-                // one pattern of e per lane, negated by parity of row >> 3 & d >> 3.
-                uint32_t sg[4];
+                // q's rotation H (q s) as a product.  Row i of tile dt is dim 32 (dt / 2)
+                // + 8 (i / 4) + 4 (dt % 2) + i % 4, so that a lane's results of tiles 2 kk
+                // and 2 kk + 1 are the operand's dims 32 kk + 8 gq + 0..7; it holds
+                // (-1)^(popcount(row & d) + d + h) at d = 32 kk + 8 gq + e: one pattern of e
+                // for even and one for odd dt per lane, negated by kk and dt alone.
+                uint32_t sg[2][4];
+                const int par = h ^ __popc((i >> 2) & gq);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const uint32_t par = (uint32_t)(h ^ ((i >> 3) & gq & 1)) & 1;
-                    const uint32_t s0 = (__popc(i & 7 & e) ^ par) & 1, s1 = (__popc(i & 7 & (e + 1)) ^ par ^ 1) & 1;
-                    sg[e / 2] = 0x3c003c00u | s0 << 15 | s1 << 31;
-                }
-                const uint32_t odd_rows = (gq & 2) ? 0x80008000u : 0u;
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const uint32_t s0 = (__popc((4 * k + (i & 3)) & e) ^ par) & 1;
+                        const uint32_t s1 = (__popc((4 * k + (i & 3)) & (e + 1)) ^ par ^ 1) & 1;
+                        sg[k][e / 2] = 0x3c003c00u | s0 << 15 | s1 << 31;
+                    }
                 f4 x[D / 16];
                 float top = 0.0f;
 #pragma unroll
@@ -540,10 +536,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 
                     x[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int kk = 0; kk < KK; ++kk) {
-                        const uint32_t flip = ((dt & 1) ? odd_rows : 0u) ^
-                                              (__builtin_popcount((dt >> 1) & kk) & 1 ? 0x80008000u : 0u);
-                        x[dt] = mfma<false>(u4{sg[0] ^ flip, sg[1] ^ flip, sg[2] ^ flip, sg[3] ^ flip}, raw[kk],
-                                            x[dt]);
+                        const uint32_t flip = __builtin_popcount((dt >> 1) & kk) & 1 ? 0x80008000u : 0u;
+                        const uint32_t(&p)[4] = sg[dt & 1];
+                        x[dt] = mfma<false>(u4{p[0] ^ flip, p[1] ^ flip, p[2] ^ flip, p[3] ^ flip}, raw[kk], x[dt]);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(x[dt][r]));
@@ -936,10 +931,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 
                     *reinterpret_cast<f4*>(mo + (wt * M + r) * (D + 4) + dt * 16 + eg * 4) = o[rt][dt];
             }
             __syncthreads();
-#pragma unroll 2
-            for (int u = etid; u < M * (D / 4); u += 64 * NW) {
+#pragma unroll
+            for (int k = 0; k < M * (D / 4) / (64 * NW); ++k) {
+                const int u = etid + k * 64 * NW;
                 const int r = u / (D / 4), d = u % (D / 4) * 4, rr = pc.tile * M + r;
-                if (rr >= R) break;
                 float mm = -INFINITY, lsum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WT; ++w) mm = fmaxf(mm, ml[w][r].x);
@@ -947,16 +942,17 @@ __global__ __launch_bounds__(64 * NW, (Shape<FMT, D, RT, WR, NW>::kPerCu * NW / 
 #pragma unroll
                 for (int w = 0; w < WT; ++w) {
                     const float2 e = ml[w][r];
-                    const float f = e.x == -INFINITY ? 0.0f : exp2_hw(e.x - mm);
                     // (an empty part holds zeros, but for a NaN logit)
-                    lsum += e.x == -INFINITY ? e.y : e.y * f;
-                    y += *reinterpret_cast<const f4*>(mo + (w * M + r) * (D + 4) + d) * (e.x == -INFINITY ? 1.0f : f);
+                    const float f = e.x == -INFINITY ? 1.0f : exp2_hw(e.x - mm);
+                    lsum += e.y * f;
+                    y += *reinterpret_cast<const f4*>(mo + (w * M + r) * (D + 4) + d) * f;
                 }
                 if (whole) {
-                    const size_t to = row_at(rr, rr / a.group) + d;
                     y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
-                    *reinterpret_cast<u2*>(a.out + to) = u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
-                } else {
+                    if (rr < R)
+                        *reinterpret_cast<u2*>(a.out + row_at(rr, rr / a.group) + d) =
+                            u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
+                } else if (rr < R) {
                     *reinterpret_cast<f4*>(po + r * D + d) = y;
                     if (d == 0) pm[r] = make_float2(mm, lsum);
                 }
@@ -1059,7 +1055,6 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     Tiling t;
     t.m_log = log2i(S::M);
     t.c_log = log2i(S::C);
-    t.least = std::max(1, 128 / S::C);
     // The line's length is known to the device only; here its bound.
     const long long chunks = std::max<long long>(1, ((long long)a.max_kv + S::C - 1) / S::C) + kLead;
     const long long items =
@@ -1067,7 +1062,7 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     if (items * chunks >= (1LL << 31) - (1 << 24))
         throw Error("tree_attention: too many (row tile, token chunk) pairs (2^31)");
     t.groups = (int)std::max<long long>(
-        1, std::min<long long>((long long)num_cus() * S::kPerCu, (items * chunks + t.least - 1) / t.least));
+        1, std::min<long long>((long long)num_cus() * S::kPerCu, items * chunks));
     constexpr size_t kPiece = (size_t)S::M * (D + 2) * sizeof(float);
     float* ws = nullptr;
     const bool cut = chunks > 1 + kLead;  // an item of one chunk is never cut
@@ -1088,13 +1083,23 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     check_launch("tree_attention_merge_kernel");
 }
 
-// Query rows per tile: the fewest that hold an average sequence's rows.
+// Query rows per tile: those of an average sequence (a tile of more rows decodes
+// or loads a chunk once for all of them; fewer rows leave its products empty).
 template <int FMT, int D>
 void launch_format(const TreeArgs& a, hipStream_t stream) {
+    constexpr bool kTurned = FMT == kProd || FMT == kMse;
     const long long rows = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
-    if (rows <= 16) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
-    if (rows <= 32) return launch_shape<FMT, D, 2, 1, 4>(a, stream);
-    if (rows <= 64) return launch_shape<FMT, D, (FMT >= kProd ? 1 : 2), (FMT >= kProd ? 4 : 2), 4>(a, stream);
+    // Few tokens: waves that each have their own, without a barrier, have the
+    // shortest way (12 sequences of up to 6,001 tokens, turbo_mse at head_dim 64:
+    // 10.2 against 11.4 us; 4 of up to 2,000, fp16: 7.0 against 8.0).  Many: more
+    // waves per CU sharing them (16 of up to 16,384: fp16 38.9 -> 34.0, turbo_prod
+    // 49 -> 42.5 us).
+    if (rows <= 16 && (long long)a.seqs * a.max_kv * a.g.H <= 1024LL * num_cus())
+        return launch_shape<FMT, D, 1, 1, 4>(a, stream);
+    if (rows <= 32) return launch_shape<FMT, D, 1, 2, 4>(a, stream);
+    // (compressed pages: 16 rows a wave leave registers for a third workgroup of
+    // the CU, 51 -> 46 us for 32 sequences of up to 8,192 tokens)
+    if (rows <= 64) return launch_shape<FMT, D, kTurned ? 1 : 2, kTurned ? 4 : 2, 4>(a, stream);
     if (rows <= 128) return launch_shape<FMT, D, 2, 4, 4>(a, stream);
     return launch_shape<FMT, D, 2, 8, 8>(a, stream);
 }
