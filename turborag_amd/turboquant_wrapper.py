@@ -358,6 +358,10 @@ class TurboQuantWrapper:
                 fn = getattr(self._fast, name)
                 fn.argtypes = [c_void_p if a in _DATA_POINTERS else a for a in argtypes]
                 fn.restype = restype
+        self._tree = {"dense": self._fast.tq_launch_dense_tree_attention,
+                      "turbo_prod": self._fast.tq_launch_turbo_prod_tree_attention,
+                      "turbo_mse": self._fast.tq_launch_turbo_mse_tree_attention}
+        self._rope_configs: dict[tuple, TQRopeConfig] = {}
 
     def _bind_symbols(self) -> None:
         for name, (argtypes, restype) in SIGNATURES.items():
@@ -719,55 +723,84 @@ class TurboQuantWrapper:
     # ── a speculative step: norm + rotation, append, tree attention ──── #
 
     @staticmethod
-    def _token_rows(scheme, op, name, t, dtype, tokens, heads, dim):
-        """(pointer, token stride) of [tokens, heads, dim] rows: dims and heads
-        contiguous, any distance between tokens (a view of a fused projection)."""
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{scheme} {op}: {name} must be a GPU tensor")
-        if t.dtype is not dtype:
-            raise ValueError(f"{scheme} {op}: {name} must be {dtype}, got {t.dtype}")
-        if t.shape != (tokens, heads, dim):
-            raise ValueError(f"{scheme} {op}: {name} must be [{tokens}, {heads}, {dim}], got "
-                             f"{list(t.shape)}")
-        s0, s1, s2 = t.stride()
-        if tokens and (s2 != 1 or (s1 != dim and heads > 1)
-                       or (tokens > 1 and s0 < heads * dim)):
-            raise ValueError(f"{scheme} {op}: {name} must have contiguous heads and distinct tokens")
-        return t.data_ptr(), s0
+    def _fit(dev: int, wants, dtype=None, rows=()) -> bool:
+        """Every (tensor, dtype, elements) of wants is on GPU dev, contiguous and
+        large enough; every (tensor, [tokens, heads, dim]) of rows is on it, of
+        `dtype`, with contiguous dims and heads and any distance between tokens (a
+        view of a fused projection)."""
+        try:
+            for t, shape in rows:
+                if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+                    return False
+                if not t.is_contiguous():
+                    (tokens, heads, dim), (s0, s1, s2) = shape, t.stride()
+                    if s2 != 1 or (s1 != dim and heads > 1) or (s0 < heads * dim and tokens > 1):
+                        return False
+            for t, kind, numel in wants:
+                if (t.dtype is not kind or t.get_device() != dev or t.numel() < numel
+                        or not t.is_contiguous()):
+                    return False
+        except AttributeError:
+            return False
+        return True
 
-    @staticmethod
-    def _on_current_device(scheme, op, *tensors):
-        """A launch runs on the current device: every tensor must live there."""
-        dev = torch.cuda.current_device()
-        for t in tensors:
-            if t is not None and t.get_device() != dev:
-                raise ValueError(f"{scheme} {op}: a tensor on GPU {t.get_device()}, the current "
-                                 f"device is {dev}")
+    def _refuse(self, scheme, op, dev, wants=None, rows=None) -> None:
+        """Raises the ValueError of the first tensor that does not fit (wants: name ->
+        (tensor, dtype, elements); rows: name -> (tensor, dtype, shape))."""
+        for name, (t, dtype, shape) in (rows or {}).items():
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise ValueError(f"{scheme} {op}: {name} must be a GPU tensor")
+            if t.dtype != dtype:
+                raise ValueError(f"{scheme} {op}: {name} must be {dtype}, got {t.dtype}")
+            if t.shape != shape:
+                raise ValueError(f"{scheme} {op}: {name} must be {list(shape)}, got {list(t.shape)}")
+            if not self._fit(t.get_device(), (), dtype, ((t, shape),)):
+                raise ValueError(f"{scheme} {op}: {name} must have contiguous heads and distinct "
+                                 f"tokens")
+        self._check(scheme, op, **(wants or {}))
+        for name, (t, *_) in {**(rows or {}), **(wants or {})}.items():
+            if t.get_device() != dev:
+                raise ValueError(f"{scheme} {op}: {name} is on GPU {t.get_device()}, another tensor "
+                                 f"on GPU {dev}")
+        raise ValueError(f"{scheme} {op}: the current device is not the tensors', GPU {dev}")
 
-    def _rope_args(self, scheme, op, key, positions, cos_sin, cfg, q_heads, q_weight, k_weight, eps,
-                   interleaved):
-        """(TQRopeConfig, weight pointers) after the checks both rotation entries share."""
-        if not isinstance(key, torch.Tensor) or key.dtype not in _DTYPES:
-            raise ValueError(f"{scheme} {op}: key must be a float16 or bfloat16 tensor")
-        if key.dim() != 3:
-            raise ValueError(f"{scheme} {op}: key must be [num_tokens, num_kv_heads, head_dim]")
-        N, D = key.shape[0], cfg.head_dim
-        if not isinstance(cos_sin, torch.Tensor) or cos_sin.dim() != 2:
-            raise ValueError(f"{scheme} {op}: cos_sin must be [max_position, rot_dim]")
-        if not (_ready(positions, torch.int32, N) and _ready(cos_sin, torch.float32, 0)):
-            self._check(scheme, op, positions=(positions, torch.int32, N),
-                        cos_sin=(cos_sin, torch.float32, 0))
-        qw = kw = None
+    def _rope(self, scheme, op, query, key, value, positions, cos_sin, out_query, out_key, slots,
+              page_pool, cfg, q_weight, k_weight, eps, interleaved):
+        """The rotation entries' checks; (TQRopeConfig, tokens)."""
+        try:
+            (N, _, _), (max_position, rot_dim) = key.shape, cos_sin.shape
+            Hq = 1 if query is None else query.shape[1]
+            dtype, dev = key.dtype, key.get_device()
+        except (AttributeError, IndexError, ValueError):
+            raise ValueError(f"{scheme} {op}: query and key must be tensors of 3 dimensions, cos_sin "
+                             f"of 2") from None
+        if dtype not in _DTYPES:
+            raise ValueError(f"{scheme} {op}: key must be float16 or bfloat16, got {dtype}")
+        D = cfg.head_dim
+        keys = (N, cfg.num_kv_heads, D)
+        rows = [(key, keys), (out_key if slots is None else value, keys)]
+        if query is not None:
+            rows += (query, (N, Hq, D)), (out_query, (N, Hq, D))
+        wants = [(positions, torch.int32, N), (cos_sin, torch.float32, 0)]
         if q_weight is not None:
-            if not _ready(q_weight, key.dtype, D):
-                self._check(scheme, op, q_weight=(q_weight, key.dtype, D))
-            qw = q_weight.data_ptr()
+            wants.append((q_weight, dtype, D))
         if k_weight is not None:
-            if not _ready(k_weight, key.dtype, D):
-                self._check(scheme, op, k_weight=(k_weight, key.dtype, D))
-            kw = k_weight.data_ptr()
-        rows, rot = cos_sin.shape
-        return TQRopeConfig(_DTYPES[key.dtype], q_heads, rot, bool(interleaved), rows, eps), qw, kw
+            wants.append((k_weight, dtype, D))
+        if slots is not None:
+            wants += (slots, torch.int32, N), (page_pool, torch.uint8, 0)
+        if not self._fit(dev, wants, dtype, rows) or dev < 0 or dev != torch.cuda.current_device():
+            names = ["positions", "cos_sin"] + ["q_weight"] * (q_weight is not None) + [
+                "k_weight"] * (k_weight is not None) + ["slot_mapping", "page_pool"] * (slots is not None)
+            row_names = ("key", "out_key" if slots is None else "value", "query", "out_query")
+            self._refuse(scheme, op, dev, dict(zip(names, wants)),
+                         {n: (t, dtype, shape) for n, (t, shape) in zip(row_names, rows)})
+        kind = (dtype, Hq, rot_dim, bool(interleaved), max_position, eps)
+        rope = self._rope_configs.get(kind)
+        if rope is None:
+            if len(self._rope_configs) >= 64:
+                self._rope_configs.clear()
+            rope = self._rope_configs[kind] = TQRopeConfig(_DTYPES[dtype], *kind[1:])
+        return rope, N
 
     def qk_norm_rope(self, query, key, positions, cos_sin, out_query, out_key, cfg, q_weight=None,
                      k_weight=None, eps: float = 1e-6, interleaved: bool = False,
@@ -777,27 +810,20 @@ class TurboQuantWrapper:
         allowed) at the tokens' positions, into out_query and out_key (which may
         be the inputs).  cos_sin: rope_table's; its width is the rotated part of
         a head.  A token at a position outside the table is skipped."""
-        op = "qk_norm_rope"
-        if not isinstance(query, torch.Tensor) or query.dim() != 3:
-            raise ValueError(f"rope {op}: query must be [num_tokens, num_q_heads, head_dim]")
-        N, Hq, _ = query.shape
-        H, D = cfg.num_kv_heads, cfg.head_dim
-        rope, qw, kw = self._rope_args("rope", op, key, positions, cos_sin, cfg, Hq, q_weight,
-                                       k_weight, eps, interleaved)
-        dtype, rows = key.dtype, self._token_rows
-        q, qs = rows("rope", op, "query", query, dtype, N, Hq, D)
-        k, ks = rows("rope", op, "key", key, dtype, N, H, D)
-        oq, oqs = rows("rope", op, "out_query", out_query, dtype, N, Hq, D)
-        ok, oks = rows("rope", op, "out_key", out_key, dtype, N, H, D)
-        self._on_current_device("rope", op, query, key, positions, cos_sin, out_query, out_key,
-                                q_weight, k_weight)
+        if query is None:
+            raise ValueError("rope qk_norm_rope: query must be a tensor of 3 dimensions")
+        rope, N = self._rope("rope", "qk_norm_rope", query, key, None, positions, cos_sin, out_query,
+                             out_key, None, None, cfg, q_weight, k_weight, eps, interleaved)
         if N == 0:
             return
         rc = self._fast.tq_launch_qk_norm_rope(
-            q, qs, k, ks, qw, kw, cos_sin.data_ptr(), positions.data_ptr(), oq, oqs, ok, oks,
-            ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
+            query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
+            None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), cos_sin.data_ptr(),
+            positions.data_ptr(), out_query.data_ptr(), out_query.stride(0), out_key.data_ptr(),
+            out_key.stride(0), ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
         if rc != 0:
-            self._kernel_raise(rc, "rope", op)
+            self._kernel_raise(rc, "rope", "qk_norm_rope")
 
     def dense_rope_append(self, query, key, value, positions, slot_mapping, cos_sin, out_query,
                           page_pool, layout, cfg, q_weight=None, k_weight=None, eps: float = 1e-6,
@@ -805,35 +831,25 @@ class TurboQuantWrapper:
         """qk_norm_rope with the rotated keys, and the values as they are, written
         into the dense pages named by slot_mapping (pages of key's dtype); query
         and out_query may both be None.  A negative slot stores nothing."""
-        op = "rope_append"
         if (query is None) != (out_query is None):
-            raise ValueError(f"dense {op}: query and out_query go together")
-        if query is not None and (not isinstance(query, torch.Tensor) or query.dim() != 3):
-            raise ValueError(f"dense {op}: query must be [num_tokens, num_q_heads, head_dim]")
-        H, D = cfg.num_kv_heads, cfg.head_dim
-        Hq = query.shape[1] if query is not None else 1
-        rope, qw, kw = self._rope_args("dense", op, key, positions, cos_sin, cfg, Hq, q_weight,
-                                       k_weight, eps, interleaved)
-        N, dtype, rows = key.shape[0], key.dtype, self._token_rows
-        if not (_ready(slot_mapping, torch.int32, N) and _ready(page_pool, torch.uint8, 0)):
-            self._check("dense", op, slot_mapping=(slot_mapping, torch.int32, N),
-                        page_pool=(page_pool, torch.uint8, 0))
-        q, qs, oq, oqs = None, 0, None, 0
-        if query is not None:
-            q, qs = rows("dense", op, "query", query, dtype, N, Hq, D)
-            oq, oqs = rows("dense", op, "out_query", out_query, dtype, N, Hq, D)
-        k, ks = rows("dense", op, "key", key, dtype, N, H, D)
-        v, vs = rows("dense", op, "value", value, dtype, N, H, D)
-        self._on_current_device("dense", op, key, query, value, positions, slot_mapping, cos_sin,
-                                out_query, page_pool, q_weight, k_weight)
+            raise ValueError("dense rope_append: query and out_query go together")
+        if slot_mapping is None:
+            raise ValueError("dense rope_append: slot_mapping must be a GPU tensor")
+        rope, N = self._rope("dense", "rope_append", query, key, value, positions, cos_sin, out_query,
+                             None, slot_mapping, page_pool, cfg, q_weight, k_weight, eps, interleaved)
         if N == 0:
             return
+        q = qs = oq = oqs = 0
+        if query is not None:
+            q, qs, oq, oqs = query.data_ptr(), query.stride(0), out_query.data_ptr(), out_query.stride(0)
         rc = self._fast.tq_launch_dense_rope_append_kv(
-            q, qs, k, ks, v, vs, qw, kw, cos_sin.data_ptr(), positions.data_ptr(),
-            slot_mapping.data_ptr(), page_pool.data_ptr(), oq, oqs, ctypes.byref(layout),
-            ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
+            q, qs, key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
+            None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), cos_sin.data_ptr(),
+            positions.data_ptr(), slot_mapping.data_ptr(), page_pool.data_ptr(), oq, oqs,
+            ctypes.byref(layout), ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
         if rc != 0:
-            self._kernel_raise(rc, "dense", op)
+            self._kernel_raise(rc, "dense", "rope_append")
 
     def tree_attn_output(self, scheme: str, query, page_pool, block_tables, row_start, prefix_len,
                          tree_mask, output, layout, cfg, max_kv_len: int, stream: int = 0) -> None:
@@ -847,42 +863,37 @@ class TurboQuantWrapper:
         j % 32 of tree_mask[r, j // 32] is set (tree_mask_from_parents).
         block_tables [num_seqs, max_blocks] int32 page ids."""
         op = "tree_attn_output"
-        if scheme not in ("dense", "turbo_prod", "turbo_mse"):
+        fn = self._tree.get(scheme)
+        if fn is None:
             raise ValueError(f"{scheme} {op}: no such scheme")
-        D = cfg.head_dim
-        if not isinstance(query, torch.Tensor) or query.dim() != 3 or query.shape[2] != D:
-            raise ValueError(f"{scheme} {op}: query must be [num_tokens, num_q_heads, {D}]")
-        if query.dtype not in (_DTYPES if scheme == "dense" else (torch.float16,)):
-            raise ValueError(f"{scheme} {op}: query must not be {query.dtype}")
-        for name, t in (("block_tables", block_tables), ("tree_mask", tree_mask)):
-            if not isinstance(t, torch.Tensor) or t.dim() != 2:
-                raise ValueError(f"{scheme} {op}: {name} must have two dimensions")
-        N, Hq = query.shape[:2]
-        S = block_tables.shape[0]
-        if tree_mask.shape[0] < N:
-            raise ValueError(f"{scheme} {op}: tree_mask has {tree_mask.shape[0]} rows, needs {N}")
-        want = ((query, query.dtype, N * Hq * D), (page_pool, torch.uint8, 0),
-                (block_tables, torch.int32, 0), (row_start, torch.int32, S + 1),
-                (prefix_len, torch.int32, S), (tree_mask, torch.int32, 0),
-                (output, query.dtype, N * Hq * D))
-        if not all(_ready(*w) for w in want):
-            self._check(scheme, op, **dict(zip(("query", "page_pool", "block_tables", "row_start",
-                                                "prefix_len", "tree_mask", "output"), want)))
-        self._on_current_device(scheme, op, query, page_pool, block_tables, row_start, prefix_len,
-                                tree_mask, output)
+        for name, t, dims in (("query", query, 3), ("block_tables", block_tables, 2),
+                              ("tree_mask", tree_mask, 2)):
+            if not isinstance(t, torch.Tensor) or t.dim() != dims:
+                raise ValueError(f"{scheme} {op}: {name} must be a tensor of {dims} dimensions")
+        N, Hq, D = query.shape
+        S, blocks = block_tables.shape
+        mask_rows, words = tree_mask.shape
+        dtype = query.dtype
+        if D != cfg.head_dim:
+            raise ValueError(f"{scheme} {op}: query must be [num_tokens, num_q_heads, {cfg.head_dim}]")
+        if dtype is not torch.float16 and (scheme != "dense" or dtype is not torch.bfloat16):
+            raise ValueError(f"{scheme} {op}: query must not be {dtype}")
+        if mask_rows < N:
+            raise ValueError(f"{scheme} {op}: tree_mask has {mask_rows} rows, needs {N}")
+        dev = query.get_device()
+        wants = ((query, dtype, 0), (page_pool, torch.uint8, 0), (block_tables, torch.int32, 0),
+                 (row_start, torch.int32, S + 1), (prefix_len, torch.int32, S),
+                 (tree_mask, torch.int32, 0), (output, dtype, N * Hq * D))
+        if not self._fit(dev, wants) or dev < 0 or dev != torch.cuda.current_device():
+            self._refuse(scheme, op, dev, dict(zip(("query", "page_pool", "block_tables", "row_start",
+                                                    "prefix_len", "tree_mask", "output"), wants)))
         if N == 0 or S == 0:
             return
-        args = [query.data_ptr(), page_pool.data_ptr(), block_tables.data_ptr(),
-                block_tables.shape[1], row_start.data_ptr(), prefix_len.data_ptr(),
-                tree_mask.data_ptr(), tree_mask.shape[1], output.data_ptr(), ctypes.byref(layout),
-                ctypes.byref(cfg)]
-        tail = [Hq, S, N, max_kv_len, self._stream(stream)]
-        if scheme == "dense":
-            rc = self._fast.tq_launch_dense_tree_attention(*args, _DTYPES[query.dtype], *tail)
-        elif scheme == "turbo_prod":
-            rc = self._fast.tq_launch_turbo_prod_tree_attention(*args, *tail)
-        else:
-            rc = self._fast.tq_launch_turbo_mse_tree_attention(*args, *tail)
+        kind = (_DTYPES[dtype],) if scheme == "dense" else ()
+        rc = fn(query.data_ptr(), page_pool.data_ptr(), block_tables.data_ptr(), blocks,
+                row_start.data_ptr(), prefix_len.data_ptr(), tree_mask.data_ptr(), words,
+                output.data_ptr(), ctypes.byref(layout), ctypes.byref(cfg), *kind, Hq, S, N,
+                max_kv_len, self._stream(stream))
         if rc != 0:
             self._kernel_raise(rc, scheme, op)
 
