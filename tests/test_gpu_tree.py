@@ -159,6 +159,15 @@ def test_many_sequences(tq, cuda, scheme, dtype):
     Problem(tq, scheme, dtype, lens, widths, 4, 2, 64, seed=4, extra_rows=3).check(cuda)
 
 
+@pytest.mark.parametrize("seqs,H,longest", [(65, 3, 400), (700, 1, 300), (4300, 1, 40), (9000, 2, 9)])
+def test_very_many_sequences(tq, cuda, seqs, H, longest):
+    """From one sequence more than a wave has lanes to more than 64 blocks of 64, whole runs of them
+    empty."""
+    lens = [(37 * s + s * s // 7) % longest for s in range(seqs)]
+    widths = [0 if s // 100 % 4 == 2 else (s * 5 // 3) % 3 for s in range(seqs)]
+    Problem(tq, "dense", FP16, lens, widths, H * 2, H, 64, B=32, seed=4, extra_rows=2).check(cuda)
+
+
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)
 def test_rows_that_attend_nothing(tq, cuda, scheme, dtype):
     p = Problem(tq, scheme, dtype, [0, 0, 40], [3, 2, 2], 8, 2, 128, seed=5, extra_rows=5)

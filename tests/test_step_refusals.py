@@ -128,6 +128,16 @@ def test_tree_geometry_refused(tq):
             assert "head_dim must be 64 or 128" in _message(tq)
         assert _call_tree(tq, scheme, pool=FAKE + 1) == -2
         assert _call_tree(tq, scheme, seqs=0) == 0 and _call_tree(tq, scheme, n=0) == 0
+        cfg = _cfg(tq)  # a region that ends past the page
+        layout = {"dense": tq.make_dense_layout_for, "turbo_prod": tq.make_layout_for,
+                  "turbo_mse": tq.make_mse_layout_for}[scheme](cfg)
+        name = {"dense": "v_offset", "turbo_prod": "v4_codes_offset", "turbo_mse": "v_norms_offset"}[scheme]
+        setattr(layout, name, int(layout.page_size_bytes) - 16)
+        assert _call_tree(tq, scheme, cfg=cfg, layout=layout) == -2
+        assert "past the page" in _message(tq)
+        if scheme == "dense":
+            assert _call_append(tq, layout=layout) == -2
+            assert "past the page" in _message(tq)
     assert _call_tree(tq, "dense", pool=FAKE + 8) == -2
     assert _call_tree(tq, "dense", dtype=2) == -2
     cfg = _cfg(tq)

@@ -363,6 +363,9 @@ extern "C" int tq_launch_dense_rope_append_kv(
         const int H = cfg->num_kv_heads, D = cfg->head_dim, Hq = query ? rope->num_q_heads : 0;
         tq::RopeArgs a{};
         a.g = tq::dense_geom(*cfg, *layout);
+        for (const uint64_t off : {a.g.k_off, a.g.v_off})
+            if (off > a.g.page_size || layout->k_bytes > a.g.page_size - off)
+                throw tq::Error("dense_rope_append_kv: layout does not match cfg (a region ends past the page)");
         if (reinterpret_cast<uintptr_t>(page_pool) & 3)
             throw tq::Error("dense_rope_append_kv: page_pool must be 4-byte aligned");
         if (query) {

@@ -141,8 +141,7 @@ struct SeqBlock {
     int before;  // chunks of the head's items before this sequence
 };
 
-__device__ __forceinline__ SeqBlock load_seqs(const TreeArgs& a, const Tiling& g, int first,
-                                              int before, int lane, int& after) {
+__device__ __forceinline__ SeqBlock read_seqs(const TreeArgs& a, const Tiling& g, int first, int lane) {
     SeqBlock b;
     b.first = first;
     const int s = min(first + lane, a.seqs - 1);
@@ -153,16 +152,53 @@ __device__ __forceinline__ SeqBlock load_seqs(const TreeArgs& a, const Tiling& g
     b.end = (int)min((long long)b.L + b.rows, (long long)a.max_kv);
     b.chunks = max((b.end + (1 << g.c_log) - 1) >> g.c_log, 1) + kLead;
     b.tiles = (b.rows * a.group + (1 << g.m_log) - 1) >> g.m_log;
-    const int cost = b.tiles * b.chunks;
-    int up = cost;
+    b.before = 0;
+    return b;
+}
+__device__ __forceinline__ int sum_up(int v, int lane) {  // over the lanes up to this one
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-        const int u = __shfl_up(up, m, 64);
-        up += lane >= m ? u : 0;
+        const int u = __shfl_up(v, m, 64);
+        v += lane >= m ? u : 0;
     }
+    return v;
+}
+__device__ __forceinline__ int sum_all(int v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+__device__ __forceinline__ SeqBlock load_seqs(const TreeArgs& a, const Tiling& g, int first,
+                                              int before, int lane, int& after) {
+    SeqBlock b = read_seqs(a, g, first, lane);
+    const int cost = b.tiles * b.chunks, up = sum_up(cost, lane);
     b.before = before + up - cost;
     after = before + __builtin_amdgcn_readlane(up, 63);
     return b;
+}
+// More than 64 sequences: lane k's chunks of the blocks of 64 from k span to
+// (k + 1) span, so that a place is found from one sum over lanes and at most
+// span blocks.  Returns the chunks of all.
+__device__ __forceinline__ int span_of(int seqs) { return (seqs + 4095) / 4096; }
+__device__ __forceinline__ int block_sums(const TreeArgs& a, const Tiling& g, int lane, int& mine) {
+    const int span = span_of(a.seqs);
+    int total = 0;
+    mine = 0;
+    for (int f = 0; f < a.seqs; f += 256) {  // (four blocks' loads at a time)
+        int cost[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const SeqBlock b = read_seqs(a, g, f + k * 64, lane);
+            cost[k] = b.tiles * b.chunks;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int sum = __builtin_amdgcn_readfirstlane(sum_all(cost[k]));
+            if ((f / 64 + k) / span == lane) mine += sum;
+            total += sum;
+        }
+    }
+    return total;
 }
 
 __device__ __forceinline__ Plan make_plan(const TreeArgs& a, const Tiling& g, int total) {
@@ -179,18 +215,17 @@ struct Piece {
     int tile, chunk, chunks;  // place in the item (from kLead on: chunks of tokens); its chunks
 };
 __device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, const Plan& p, int at,
-                                        int lane, SeqBlock& b) {
+                                        int lane, int mine, SeqBlock& b) {
     Piece o;
     o.h = at / p.total;
     const int x = at - o.h * p.total;
     if (a.seqs > 64) {
-        int after;
-        if (__builtin_amdgcn_readlane(b.before, 0) > x)  // the next head: from the start
-            b = load_seqs(a, g, 0, 0, lane, after);
-        while (true) {
-            after = __builtin_amdgcn_readlane(b.before + b.tiles * b.chunks, 63);
-            if (x < after || b.first + 64 >= a.seqs) break;
-            b = load_seqs(a, g, b.first + 64, after, lane, after);
+        int after = __builtin_amdgcn_readlane(b.before + b.tiles * b.chunks, 63);
+        if (b.first < 0 || x < __builtin_amdgcn_readlane(b.before, 0) || x >= after) {
+            const int step = 64 * span_of(a.seqs), from = sum_up(mine, lane) - mine;
+            const int k = max(__popcll(__ballot(from <= x && lane * step < a.seqs)) - 1, 0);
+            b = load_seqs(a, g, k * step, __builtin_amdgcn_readlane(from, k), lane, after);
+            while (x >= after && b.first + 64 < a.seqs) b = load_seqs(a, g, b.first + 64, after, lane, after);
         }
     }
     // The last sequence that begins at or before x: one without work begins
@@ -237,10 +272,15 @@ struct Shape {
 
 constexpr float kAlphaV = 1.5982153f;  // alpha V4[c] is fp16-exact to 9.2e-5 for every c
 
-// 16 bytes per lane from p straight into LDS at byte `lds` + 16 lane.
+// 16 bytes per lane from p straight into LDS at byte `lds` (the same in every
+// lane) + 16 lane.  In asm, because the compiler waits for loads of its own kind
+// before any LDS read that follows; wait_vmem() is the wait.  (m0 is nobody
+// else's here: nothing that the compiler emits for these kernels takes it.)
 __device__ __forceinline__ void load_to_lds(const uint8_t* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p)
-                 : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                     __builtin_amdgcn_readfirstlane(lds)),
+                 "v"(p)
+                 : "memory");
 }
 __device__ __forceinline__ void wait_vmem() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -305,8 +345,13 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
     const uint32_t v_at = mem0 + (wt * T + vrow) * kRow + ((((i >> 1) & 1) ^ swz(vrow)) * 16) + (i & 1) * 8;
 
     SeqBlock sb;
-    int total;
-    sb = load_seqs(a, tl, 0, 0, lane, total);
+    int total, mine = 0;
+    if (a.seqs <= 64) {
+        sb = load_seqs(a, tl, 0, 0, lane, total);
+    } else {
+        sb = SeqBlock{-1, 0, 0, 0, 0, 0, 0, 0};
+        total = block_sums(a, tl, lane, mine);
+    }
     if (kTurned && tid < 256) {
       if constexpr (kTurned) {
         const int lo = tid & 15, hi = tid >> 4;
@@ -324,7 +369,6 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
       }
     }
 
-    for (int f = 64; f < a.seqs; f += 64) (void)load_seqs(a, tl, f, total, lane, total);
     const Plan plan = make_plan(a, tl, total);
     const int all = plan.total * g.H;
     const long long begin = (long long)blockIdx.x * plan.per;
@@ -335,7 +379,7 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
 
     bool first = true;
     for (int at = (int)min(begin, (long long)all); at < stop;) {
-        const Piece pc = locate(a, tl, plan, at, lane, sb);
+        const Piece pc = locate(a, tl, plan, at, lane, mine, sb);
         const int upto = min(pc.chunk + (stop - at), pc.chunks);
         const int c0 = max(pc.chunk - kLead, 0), c1 = upto - kLead;
         at += upto - pc.chunk;
@@ -975,15 +1019,34 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
     if (flat >= a.tokens * a.hq) return;
     const int tok = flat / a.hq, qh = flat - tok * a.hq, h = qh / a.group;
     int total = 0, row0 = -1, before = 0, chunks = 1;
-    for (int f = 0; f < a.seqs; f += 64) {
-        const SeqBlock b = load_seqs(a, tl, f, total, lane, total);
+    const auto look = [&](const SeqBlock& b) {
         const uint64_t hit = __ballot(b.row0 <= tok && tok < b.row0 + b.rows);
-        if (hit && row0 < 0) {
-            const int k = __ffsll((unsigned long long)hit) - 1;
-            row0 = __builtin_amdgcn_readlane(b.row0, k);
-            before = __builtin_amdgcn_readlane(b.before, k);
-            chunks = __builtin_amdgcn_readlane(b.chunks, k);
+        if (!hit || row0 >= 0) return;
+        const int k = __ffsll((unsigned long long)hit) - 1;
+        row0 = __builtin_amdgcn_readlane(b.row0, k);
+        before = __builtin_amdgcn_readlane(b.before, k);
+        chunks = __builtin_amdgcn_readlane(b.chunks, k);
+    };
+    if (a.seqs <= 64) {
+        look(load_seqs(a, tl, 0, 0, lane, total));
+    } else {
+        int mine;
+        const int all = block_sums(a, tl, lane, mine);
+        // the last block whose first row is this token's or before it (sequences
+        // without rows begin where the next one does)
+        int from = 0;
+        for (int f = 0; f < a.seqs; f += 4096) {
+            const int s = f + lane * 64;
+            const uint64_t low = __ballot(s < a.seqs && a.row_start[min(s, a.seqs - 1)] <= tok);
+            if (low) from = f + (63 - __clzll((unsigned long long)low)) * 64;
         }
+        const int step = 64 * span_of(a.seqs), k = from / step;
+        total = __builtin_amdgcn_readlane(sum_up(mine, lane) - mine, k);
+        for (int f = k * step; f <= from; f += 64) {
+            const SeqBlock b = load_seqs(a, tl, f, total, lane, total);
+            if (f == from) look(b);
+        }
+        total = all;
     }
     if (row0 < 0) return;  // behind the last sequence
     const Plan p = make_plan(a, tl, total);
@@ -1064,11 +1127,10 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     t.groups = (int)std::max<long long>(
         1, std::min<long long>((long long)num_cus() * S::kPerCu, items * chunks));
     constexpr size_t kPiece = (size_t)S::M * (D + 2) * sizeof(float);
-    float* ws = nullptr;
     const bool cut = chunks > 1 + kLead;  // an item of one chunk is never cut
-    if (cut)
-        ws = static_cast<float*>(Scratch{}.get(stream, 2 * (size_t)t.groups * kPiece, "tree attention",
-                                               4 * (size_t)num_cus() * 128 * (D + 2) * sizeof(float)));
+    // (room for every later call of this head_dim: 131,072 partial rows)
+    float* ws = static_cast<float*>(Scratch{}.get(stream, cut ? 2 * (size_t)t.groups * kPiece : 0, "tree attention",
+                                                  4 * (size_t)num_cus() * 128 * (D + 2) * sizeof(float)));
     hipLaunchKernelGGL((tree_split_kernel<FMT, D, RT, WR, NW>), dim3(t.groups), dim3(64 * NW), 0, stream, a, t,
                        ws, 1.44269504f * inv_sqrt_d(D), inv_sqrt_d(D));
     check_launch("tree_attention_kernel");
@@ -1158,6 +1220,14 @@ int tree_entry(const char* name, int fmt, Geom&& geom, const void* query, const 
             throw Error(w + "max_kv_len must be in [0, 2^30] and fit in max_blocks_per_seq pages");
         if ((long long)tokens * hq >= (1LL << 26))
             throw Error(w + "num_tokens * num_q_heads must be < 2^26");
+        const uint64_t cells = (uint64_t)g.block_size * g.H;
+        const auto outside = [&](uint64_t off, uint64_t size) {
+            return off > g.page_size || cells * size > g.page_size - off;
+        };
+        if (outside(g.kc_off, g.code_stride) || outside(g.vc_off, g.code_stride) ||
+            (fmt > kBf16 && (outside(g.ks_off, 2) || outside(g.vs_off, 2) ||
+                             (fmt == kProd && outside(g.kres_off, 2)))))
+            throw Error(w + "layout does not match cfg (a region ends past the page)");
         const uint64_t al = fmt <= kBf16 ? 16 : 2;
         if (!aligned(pool, al) || !aligned(g.page_size | g.kc_off | g.vc_off, al) ||
             !aligned(g.ks_off | g.kres_off | g.vs_off, 2))
