@@ -155,23 +155,21 @@ __device__ __forceinline__ SeqBlock read_seqs(const TreeArgs& a, const Tiling& g
     b.before = 0;
     return b;
 }
-__device__ __forceinline__ int sum_up(int v, int lane) {  // over the lanes up to this one
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int u = __shfl_up(v, m, 64);
-        v += lane >= m ? u : 0;
-    }
-    return v;
-}
-__device__ __forceinline__ int sum_all(int v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+// Sums over the lanes up to this one: within rows of 16 by shifts, then the
+// rows' last lanes broadcast to the rows behind (every lane active).
+__device__ __forceinline__ int sum_up(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2, 3
     return v;
 }
 __device__ __forceinline__ SeqBlock load_seqs(const TreeArgs& a, const Tiling& g, int first,
                                               int before, int lane, int& after) {
     SeqBlock b = read_seqs(a, g, first, lane);
-    const int cost = b.tiles * b.chunks, up = sum_up(cost, lane);
+    const int cost = b.tiles * b.chunks, up = sum_up(cost);
     b.before = before + up - cost;
     after = before + __builtin_amdgcn_readlane(up, 63);
     return b;
@@ -193,7 +191,7 @@ __device__ __forceinline__ int block_sums(const TreeArgs& a, const Tiling& g, in
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int sum = __builtin_amdgcn_readfirstlane(sum_all(cost[k]));
+            const int sum = __builtin_amdgcn_readlane(sum_up(cost[k]), 63);
             if ((f / 64 + k) / span == lane) mine += sum;
             total += sum;
         }
@@ -222,7 +220,7 @@ __device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, cons
     if (a.seqs > 64) {
         int after = __builtin_amdgcn_readlane(b.before + b.tiles * b.chunks, 63);
         if (b.first < 0 || x < __builtin_amdgcn_readlane(b.before, 0) || x >= after) {
-            const int step = 64 * span_of(a.seqs), from = sum_up(mine, lane) - mine;
+            const int step = 64 * span_of(a.seqs), from = sum_up(mine) - mine;
             const int k = max(__popcll(__ballot(from <= x && lane * step < a.seqs)) - 1, 0);
             b = load_seqs(a, g, k * step, __builtin_amdgcn_readlane(from, k), lane, after);
             while (x >= after && b.first + 64 < a.seqs) b = load_seqs(a, g, b.first + 64, after, lane, after);
@@ -311,9 +309,6 @@ struct alignas(16) TokenScales {
     float k[128], v[128], lv[128];  // of a chunk's tokens; lv = max(log2 |v|, -25)
 };
 struct Nothing {};
-#ifndef TQ_SUB_UNROLL
-#define TQ_SUB_UNROLL 1
-#endif
 
 template <int FMT, int D, int RT, int WR, int NW>
 __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW + 3) / 4)) void tree_split_kernel(const TreeArgs a, const Tiling tl,
@@ -747,7 +742,7 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
             }
 
             // 32 tokens at a time: a row's logits, their weights, the values.
-#pragma unroll TQ_SUB_UNROLL
+#pragma unroll 1
             for (int st = 0; st < T / 32; ++st) {
                 const uint32_t ks_at = kb + st * 32 * kRow;
                 const int tk = wt * T + st * 32 + gq * 4;  // this lane's tokens: tk + 16 ns + 0..3
@@ -1041,7 +1036,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
             if (low) from = f + (63 - __clzll((unsigned long long)low)) * 64;
         }
         const int step = 64 * span_of(a.seqs), k = from / step;
-        total = __builtin_amdgcn_readlane(sum_up(mine, lane) - mine, k);
+        total = __builtin_amdgcn_readlane(sum_up(mine) - mine, k);
         for (int f = k * step; f <= from; f += 64) {
             const SeqBlock b = load_seqs(a, tl, f, total, lane, total);
             if (f == from) look(b);
