@@ -325,6 +325,29 @@ def test_offsets_past_32_bits(tq, cuda):
     assert torch.equal(p.out.cpu().double(), want)
 
 
+@pytest.mark.parametrize("scheme", ["turbo_prod", "turbo_mse"])
+def test_chain_equals_the_paged_step(tq, cuda, scheme):
+    """Trees without branches over a PagedBatch's pages: its own causal step's outputs, both within
+    1e-3 of their row's largest value of the exact ones."""
+    from turborag_amd.batched import PagedBatch
+    b = PagedBatch(tq, scheme, [1500, 37, 300], [3, 8, 5], seed=560, device=cuda)
+    b.append_new_tokens(seed=920)
+    rows, row_seq, row_len = b.decode_rows(seed=921)
+    tables = b.block_tables()
+    want = torch.zeros_like(rows)
+    b.attention(rows, row_seq, row_len, tables, want)
+    # [8 GQA rows of a token, kv heads, D] -> [tokens, query heads, D]
+    query = rows.view(16, 8, 2, 128).transpose(1, 2).reshape(16, 16, 128).contiguous()
+    mask = torch.cat([tree_mask_from_parents(range(-1, w - 1)) for w in b.widths]).to(cuda)
+    out = torch.zeros_like(query)
+    b.tree_attention(query, *b.tree_rows(), mask, tables, out)
+    got = out.view(16, 2, 8, 128).transpose(1, 2).reshape(rows.shape).double()
+    want = want.double()
+    err = ((got - want).abs().amax(-1) / want.abs().amax(-1)).max()
+    assert float(err) < 2e-3
+    b.close()
+
+
 def test_one_step_of_the_three(tq, cuda):
     """Norm, rotation and append of a tree's tokens, then their attention, as a step runs them; and
     the same over turbo_prod pages by rotation and pack."""

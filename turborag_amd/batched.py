@@ -12,7 +12,8 @@ rows of new token j attending L_s + j + 1 tokens (causal over the new
 tokens).  The reference does the same work with one pack call per sequence
 and one fused_attention_output call per sequence and position, each with a
 per-token slot map (tq_backend/turboquant_wrapper.py; the C5 serving
-configuration).
+configuration).  The new tokens may also form trees (``tree_attention``): a
+row then attends the prefix and the new tokens of its mask, not all before it.
 """
 from __future__ import annotations
 
@@ -129,6 +130,21 @@ class PagedBatch:
         self.tq.paged_attn_output(self.scheme, query, self.pool, block_tables, row_seq, row_len,
                                   out, self.layout, self.cfg,
                                   max(L + w for L, w in zip(self.lens, self.widths)), stream)
+
+    def tree_rows(self):
+        """The sequences' new tokens as trees of drafted tokens: (row_start,
+        prefix_len) of tree_attention."""
+        start = np.concatenate([[0], np.cumsum(self.widths)])
+        return (torch.tensor(start, dtype=torch.int32, device=self.dev),
+                torch.tensor(self.lens, dtype=torch.int32, device=self.dev))
+
+    def tree_attention(self, query, row_start, prefix_len, tree_mask, block_tables, out,
+                       stream: int = 0) -> None:
+        """Attention of the appended tokens as trees: query / out [sum of widths,
+        query heads, D], tree_mask their bits (tree_mask_from_parents)."""
+        self.tq.tree_attn_output(self.scheme, query, self.pool, block_tables, row_start, prefix_len,
+                                 tree_mask, out, self.layout, self.cfg,
+                                 max(L + w for L, w in zip(self.lens, self.widths)), stream)
 
     def close(self) -> None:
         self.table.close()
