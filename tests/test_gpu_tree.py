@@ -190,12 +190,17 @@ def test_bits_past_the_drafted_tokens(tq, cuda, scheme, dtype):
     p.check(cuda)
 
 
+# Heads and widths for every number of rows per tile: 7, 18, 54, 72 and 288 rows a sequence.
+TILES = [([6, 8], 2, 2), ([6, 30], 2, 2), ([6, 30], 6, 2), ([6, 30], 8, 2), ([6, 30], 32, 2)]
+
+
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("widths,Hq,H", TILES)
 @pytest.mark.parametrize("D", [64, 128])
-def test_non_finite_values_that_a_row_does_not_see(tq, cuda, scheme, dtype, value, D):
+def test_non_finite_values_that_a_row_does_not_see(tq, cuda, scheme, dtype, value, widths, Hq, H, D):
     """Behind the last token, in another branch of the tree, and on pages of other sequences."""
-    p = Problem(tq, scheme, dtype, [90, 200], [6, 30], 8, 2, D, seed=7)
+    p = Problem(tq, scheme, dtype, [90, 200], widths, Hq, H, D, seed=7)
     for s in (0, 1):
         n = p.lens[s] + p.widths[s]
         for t in range(n, -(-n // 16) * 16):
@@ -205,17 +210,36 @@ def test_non_finite_values_that_a_row_does_not_see(tq, cuda, scheme, dtype, valu
         p.fill_token(s, p.lens[s] + 2, value)
     p.check(cuda)
     # Drafted token 4 of the second sequence: rows that see it are not finite, the others right.
-    r = int(p.row_start[1])
-    sees = (p.mask[r:r + 30, 0] >> 4 & 1).bool()
+    r, w = int(p.row_start[1]), widths[1]
+    sees = (p.mask[r:r + w, 0] >> 4 & 1).bool()
     sees[3], p.mask[r + 3, 0] = False, p.mask[r + 3, 0] & ~(1 << 4)
-    clean, _, _ = p.expect()
-    _, tol, _ = p.expect()
+    clean, tol, _ = p.expect()
     p.fill_token(1, p.lens[1] + 4, value, "v")
     got = p.run(cuda)
-    assert not torch.isfinite(got[r:r + 30][sees]).any()
+    assert not torch.isfinite(got[r:r + w][sees]).any()
     rest = torch.ones(got.shape[0], dtype=torch.bool)
-    rest[r:r + 30] = ~sees
+    rest[r:r + w] = ~sees
     assert ((got - clean).abs()[rest] <= tol[rest]).all()
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("widths,Hq,H", TILES)
+@pytest.mark.parametrize("L", [65, 97, 129, 230])
+def test_non_finite_values_of_the_prefix(tq, cuda, scheme, dtype, widths, Hq, H, L):
+    """In a chunk whose other half holds the drafted tokens or ends the sequence: every row of the
+    sequence sees them, no other's does."""
+    p = Problem(tq, scheme, dtype, [L, 50], widths, Hq, H, 128, seed=17)
+    clean, tol, _ = p.expect()
+    for t in (L - 60, L - 2):
+        q = Problem(tq, scheme, dtype, [L, 50], widths, Hq, H, 128, seed=17)
+        q.fill_token(0, t, float("inf"), "v")
+        got = q.run(cuda)
+        w = widths[0]
+        if scheme == "dense":  # one token of +infinity, all others finite: the sum is +infinity
+            assert (got[:w] == float("inf")).all()
+        else:
+            assert not torch.isfinite(got[:w]).any()
+        assert ((got - clean).abs()[w:] <= tol[w:]).all()
 
 
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)

@@ -662,11 +662,12 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
             };
             // The tokens that each row sees.
             uint64_t see[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) see[rt] = live;
             if (!plain) {
                 const int j0 = tb0 - pc.L;
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    see[rt] = live;
                     if (j0 + T > 0) {  // (words before the drafted tokens: the prefix)
                         const int w0 = j0 >> 5;
                         const int32_t* mrow = a.mask + (size_t)(pc.row0 + tok[rt]) * a.mask_words;
