@@ -6,6 +6,23 @@
 //   out = sum_t softmax_t(<q, k_t> / sqrt(D)) v_t.
 // Compressed pages hold k and v rotated (an orthogonal transform), so q is
 // rotated the same way, and the output rotated back.
+//
+// One pass over a sequence's tokens for up to 256 query rows (drafted tokens x
+// query heads of a kv head), with a running reference and sum per row; the
+// sequences' tokens are one line of work cut into equal parts, one per
+// workgroup, and what was cut is merged by a second launch.  Measured (MI355X,
+// 16 query heads on 2 kv heads, head_dim 128; kernels alone):
+//  - dense bf16, 32 sequences of 1,024 to 32,768 tokens, 4 to 8 drafted tokens
+//    each, 556 MB: 111 + 8 us, the split at 5.0 TB/s where a copy of 1 GiB runs
+//    at 5.2: bound by HBM;
+//  - dense fp16, 64 drafted tokens over 32,768: 37 + 9 us, 470 TFLOP/s of the split
+//    (an 8,192^3 product of the library's: 1,300): the softmax's VALU instructions,
+//    ~280 per wave and 64 tokens beside 64 matrix instructions, and the waits of
+//    two waves per SIMD;
+//  - the same over turbo_prod: 58 + 9 us: twice the matrix instructions (K and q as
+//    fp16 pairs) and the decode (~100 VALU instructions per wave and chunk);
+//  - one sequence of 1,143 tokens, 5 drafted: 8.6 + 4.5 us, latency: lengths -> page
+//    ids -> rows -> products -> partial sums, then the merge's launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -242,13 +259,18 @@ __device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, cons
 }
 
 // ---------------------------------------------------------------------------
-// The split kernel: four waves, WR of them side by side over the tile's rows
-// (16 RT each), 4 / WR over a chunk's tokens (T each).  Both products run
+// The split kernel: NW waves, WR of them side by side over the tile's rows
+// (16 RT each), NW / WR over a chunk's tokens (T each).  Both products run
 // transposed: S' = K Q' has a query row per lane column and four tokens in a
 // lane's registers, so a row's softmax is in-lane but for two lane swaps, and
 // the registers are the B operand of O' = V' P' as they are (the k-order of a
 // 32-token step is 4 (l / 16) + 0..3 of either 16 tokens; V' is read from its
 // token rows in that order by transposing LDS loads).
+//
+// Weights are rounded to the pages' 16-bit type for their product with V (fp16
+// for compressed pages), as far as the output's own rounding; logits, sums and
+// references are fp32.  RT = 2: a K or V operand read from LDS serves two
+// products; one row tile per wave reads as many bytes as LDS gives.
 // ---------------------------------------------------------------------------
 template <int FMT, int D, int RT, int WR, int NW>
 struct Shape {
@@ -311,9 +333,8 @@ struct alignas(16) TokenScales {
 struct Nothing {};
 
 template <int FMT, int D, int RT, int WR, int NW>
-__global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW + 3) / 4)) void tree_split_kernel(const TreeArgs a, const Tiling tl,
-                                                            float* __restrict__ ws, float scale,
-                                                            float inv) {
+__global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW + 3) / 4))
+void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws, float scale, float inv) {
     using S = Shape<FMT, D, RT, WR, NW>;
     constexpr bool BF = S::BF, kTurned = S::kTurned;
     constexpr int T = S::T, C = S::C, M = S::M, WT = S::WT, kRow = S::kRow;
@@ -347,21 +368,19 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
         sb = SeqBlock{-1, 0, 0, 0, 0, 0, 0, 0};
         total = block_sums(a, tl, lane, mine);
     }
-    if (kTurned && tid < 256) {
-      if constexpr (kTurned) {
-        const int lo = tid & 15, hi = tid >> 4;
-        tab.v[tid] = pack2<false>(kAlphaV * pick(kV4, lo), kAlphaV * pick(kV4, hi));
+    if constexpr (kTurned) {
+        const int lo = tid & 15, hi = tid >> 4 & 15;  // (the second 256 threads write the same)
+        tab.v[tid & 255] = pack2<false>(kAlphaV * pick(kV4, lo), kAlphaV * pick(kV4, hi));
         if constexpr (FMT == kMse) {
             const float x = pick(kV4, lo), y = pick(kV4, hi);
             const uint32_t h = pack2<false>(x, y);
-            tab.k[tid] = make_uint2(h, pack2<false>(x - h2f(h & 0xffff), y - h2f(h >> 16)));
+            tab.k[tid & 255] = make_uint2(h, pack2<false>(x - h2f(h & 0xffff), y - h2f(h >> 16)));
         } else {
             const auto entry = [](int n) {
                 return (__float_as_uint(pick(kK3, n & 7)) & ~1u) | (n & 8 ? 0u : 1u);
             };
-            tab.k[tid] = make_uint2(entry(lo), entry(hi));
+            tab.k[tid & 255] = make_uint2(entry(lo), entry(hi));
         }
-      }
     }
 
     const Plan plan = make_plan(a, tl, total);
@@ -1003,7 +1022,9 @@ __global__ __launch_bounds__(64 * NW, ((Shape<FMT, D, RT, WR, NW>::kPerCu * NW +
 }
 
 // Merge of the items that were cut: WAVES waves per query row, D / 4 lanes per
-// piece of it; compressed pages' sums are rotated back here.
+// piece of it; compressed pages' sums are rotated back here.  A wave per row where
+// there are rows for every SIMD (3,072 rows of up to 16 pieces 12.0 -> 7.4 us),
+// else four (1,024 rows of 64 pieces, 34 MB: 13.8 -> 6.6 us).
 template <bool BF, bool TURNED, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
                                                          const float* __restrict__ ws, float inv) {
