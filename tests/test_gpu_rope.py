@@ -267,6 +267,24 @@ def test_zero_rows_and_empty_calls(tq, cuda):
     assert (oq == 1).all()
 
 
+def test_more_threads_than_one_grid_line(tq, cuda):
+    """71 million rows by the general kernel: 4.6e9 lanes, past the 2^32 of a grid's x."""
+    N, n, D = 1 << 22, 100, 128
+    table, cfg = rope_table(5000, 64), _cfg(tq, 1, D)
+    parts, w, pos = _inputs(n, 16, 1, D, BF16, seed=21)
+    q = torch.zeros(N, 16, D, dtype=BF16, device=cuda)
+    k = torch.zeros(N, 1, D, dtype=BF16, device=cuda)
+    whole = torch.zeros(N, dtype=torch.int32, device=cuda)
+    for at in (0, N // 2, N - n):
+        q[at:at + n], k[at:at + n], whole[at:at + n] = parts[0].to(cuda), parts[1].to(cuda), pos.to(cuda)
+    tq.qk_norm_rope(q, k, whole, table.to(cuda), q, k, cfg, _gpu(w[0], cuda), _gpu(w[1], cuda))
+    for at in (0, N // 2, N - n):
+        _close(q[at:at + n], norm_rope(parts[0], w[0], pos, table, False, 1e-6), f"query {at}")
+        _close(k[at:at + n], norm_rope(parts[1], w[1], pos, table, False, 1e-6), f"key {at}")
+    del q, k
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("N", [3, 3000])
 def test_stream_and_capture(tq, cuda, N):
     """On a stream of its own and in a graph, replayed over changed inputs."""

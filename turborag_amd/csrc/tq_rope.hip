@@ -22,6 +22,15 @@ using namespace dev;
 
 constexpr int kBlock = 256;
 
+// Workgroups lie in lines of at most kLine along y: a grid has less than 2^32
+// threads in x, and rows of eight million workgroups or more are 17 GB of heads.
+constexpr unsigned kLine = 1u << 23;
+__device__ __forceinline__ unsigned block_of() { return blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 grid_of(long long blocks) {
+    const unsigned x = (unsigned)std::min<long long>(blocks, kLine);
+    return dim3(x, (unsigned)((blocks + x - 1) / x));
+}
+
 struct RopeArgs {
     const uint16_t *q, *k, *v;   // q null: keys and values only; v null: no append
     const uint16_t *qw, *kw;     // norm weights or null
@@ -86,7 +95,7 @@ template <bool BF>
 __global__ __launch_bounds__(kBlock) void rope_pairs_kernel(const RopeArgs a, int interleaved) {
     const int D = a.g.D, L = D / 2, half = a.rot / 2;
     const int i = threadIdx.x & (L - 1);
-    const long long row = (long long)blockIdx.x * (kBlock / L) + threadIdx.x / L;
+    const long long row = (long long)block_of() * (kBlock / L) + threadIdx.x / L;
     const long long all = (long long)a.n * a.rows;
     const bool valid = row < all;
     const long long rr = valid ? row : all - 1;
@@ -165,7 +174,7 @@ template <bool BF, int D, bool INTER>
 __global__ __launch_bounds__(kBlock) void rope_rows_kernel(const RopeArgs a) {
     constexpr int L = D / 16;
     const int j = threadIdx.x & (L - 1);
-    const int job = blockIdx.x * (kBlock / L) + threadIdx.x / L;
+    const int job = block_of() * (kBlock / L) + threadIdx.x / L;
     const int row = min(job, a.n * a.rows - 1);
     const int t = row / a.rows;
     const int pos = a.pos[t], slot = a.v ? a.slots[t] : 0;
@@ -231,8 +240,8 @@ bool rows_ok(const RopeArgs& a) {
 template <bool BF, int D, bool INTER>
 void launch_rows(const RopeArgs& a, hipStream_t stream) {
     constexpr int per = kBlock / (D / 16);
-    const unsigned blocks = ((unsigned)a.n * a.rows + per - 1) / per;
-    hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER>), dim3(blocks), dim3(kBlock), 0, stream, a);
+    const dim3 grid = grid_of(((long long)a.n * a.rows + per - 1) / per);
+    hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER>), grid, dim3(kBlock), 0, stream, a);
 }
 
 void launch_rope(const RopeArgs& a, bool bf16, bool interleaved, hipStream_t stream) {
@@ -252,7 +261,7 @@ void launch_rope(const RopeArgs& a, bool bf16, bool interleaved, hipStream_t str
     }
     const int per = kBlock / (a.g.D / 2);
     const long long rows = (long long)a.n * a.rows;
-    const dim3 grid((unsigned)((rows + per - 1) / per));
+    const dim3 grid = grid_of((rows + per - 1) / per);
     if (bf16)
         hipLaunchKernelGGL(rope_pairs_kernel<true>, grid, dim3(kBlock), 0, stream, a, (int)interleaved);
     else
