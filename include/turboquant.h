@@ -474,8 +474,9 @@ typedef struct TQRopeConfig {
  * An output may be its own input (same pointer and stride); otherwise outputs
  * overlap neither inputs nor each other.  A token whose position is outside
  * [0, max_position) is skipped: its outputs stay as they were.  num_tokens 0
- * does nothing.  Any head_dim a power of two in [2, 128]; fastest with head_dim
- * 64 or 128 = rot_dim and 16-byte aligned pointers and strides. */
+ * does nothing; num_tokens * (num_q_heads + 2 H) < 2^30.  Any head_dim a power
+ * of two in [2, 128]; fastest with head_dim 64 or 128 = rot_dim and 16-byte
+ * aligned pointers and strides. */
 int tq_launch_qk_norm_rope(const void* query, int64_t query_stride, const void* key,
                            int64_t key_stride, const void* q_weight, const void* k_weight,
                            const float* cos_sin, const int32_t* positions, void* out_query,
@@ -519,8 +520,8 @@ int tq_launch_dense_rope_append_kv(const void* query, int64_t query_stride, cons
  * aligned for dense pages, 2-byte aligned for compressed ones; query and output
  * 16-byte aligned.  The dense entry takes fp16 or bf16 (dtype, TQ_DTYPE_*, of
  * query, pages and output), the others fp16.  num_seqs or num_tokens 0 does
- * nothing.  Split-K partials in the per-stream workspace, as the other
- * attention entries (tq_workspace_release). */
+ * nothing; num_tokens * num_q_heads <= 2^26 - 4.  Split-K partials in the
+ * per-stream workspace, as the other attention entries (tq_workspace_release). */
 int tq_launch_dense_tree_attention(const void* query, const uint8_t* page_pool,
                                    const int32_t* block_tables, int max_blocks_per_seq,
                                    const int32_t* row_start, const int32_t* prefix_len,

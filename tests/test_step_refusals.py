@@ -121,6 +121,13 @@ def test_tree_refused(tq, scheme, bad, word):
     assert word in _message(tq)
 
 
+@pytest.mark.parametrize("scheme", ["dense", "turbo_prod", "turbo_mse"])
+def test_tree_rows_at_the_limit_refused(tq, scheme):
+    """2^26 - 2 rows: the merge's grid would have 2^32 threads."""
+    assert _call_tree(tq, scheme, hq=2, n=(1 << 25) - 1) == -2
+    assert "2^26 - 4" in _message(tq)
+
+
 def test_tree_geometry_refused(tq):
     for scheme in ("dense", "turbo_prod", "turbo_mse"):
         for D in (2, 32):

@@ -1023,8 +1023,8 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
 
 // Merge of the items that were cut: WAVES waves per query row, D / 4 lanes per
 // piece of it; compressed pages' sums are rotated back here.  A wave per row where
-// there are rows for every SIMD (3,072 rows of up to 16 pieces 12.0 -> 7.4 us),
-// else four (1,024 rows of 64 pieces, 34 MB: 13.8 -> 6.6 us).
+// there are rows for every SIMD (32 sequences of 6 drafted tokens, up to 16 pieces
+// per row: 12.0 -> 7.4 us), else four (1,024 rows of 64 pieces, 34 MB: 13.8 -> 6.6 us).
 template <bool BF, bool TURNED, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
                                                          const float* __restrict__ ws, float inv) {
@@ -1235,8 +1235,8 @@ int tree_entry(const char* name, int fmt, Geom&& geom, const void* query, const 
             throw Error(w + "max_blocks_per_seq and mask_words must be > 0");
         if (max_kv < 0 || max_kv > (1 << 30) || (long long)max_blocks * g.block_size < max_kv)
             throw Error(w + "max_kv_len must be in [0, 2^30] and fit in max_blocks_per_seq pages");
-        if ((long long)tokens * hq >= (1LL << 26))
-            throw Error(w + "num_tokens * num_q_heads must be < 2^26");
+        if ((long long)tokens * hq > (1LL << 26) - 4)  // (the merge's grid: 2^32 threads less 256)
+            throw Error(w + "num_tokens * num_q_heads must be at most 2^26 - 4");
         const uint64_t cells = (uint64_t)g.block_size * g.H;
         const auto outside = [&](uint64_t off, uint64_t size) {
             return off > g.page_size || cells * size > g.page_size - off;
