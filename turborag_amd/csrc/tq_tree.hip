@@ -16,11 +16,14 @@
 //    each, 556 MB: 111 + 8 us, the split at 5.0 TB/s where a copy of 1 GiB runs
 //    at 5.2: bound by HBM;
 //  - dense fp16, 64 drafted tokens over 32,768: 37 + 9 us, 470 TFLOP/s of the split
-//    (an 8,192^3 product of the library's: 1,300): the softmax's VALU instructions,
-//    ~280 per wave and 64 tokens beside 64 matrix instructions, and the waits of
-//    two waves per SIMD;
-//  - the same over turbo_prod: 58 + 9 us: twice the matrix instructions (K and q as
-//    fp16 pairs) and the decode (~100 VALU instructions per wave and chunk);
+//    (an 8,192^3 product of the library's: 1,300).  Of a workgroup's 63,000 cycles
+//    5,170 are for each of nine chunks (two waves per SIMD: ~2,050 of matrix
+//    instructions and ~2,900 of the softmax's vector instructions), 10,400 for the
+//    chain lengths -> page ids -> rows, 6,100 for the partial sums, 33 MB in all;
+//  - the same over turbo_prod: 58 + 9 us, 10,300 cycles a chunk: twice the matrix
+//    instructions (K and q as fp16 pairs), as many LDS cycles, and the decode (~100
+//    vector instructions per wave and chunk);
+//  - turbo_prod, 32 sequences of 300 to 8,192 tokens: 43 + 8 us, the same;
 //  - one sequence of 1,143 tokens, 5 drafted: 8.6 + 4.5 us, latency: lengths -> page
 //    ids -> rows -> products -> partial sums, then the merge's launch.
 #include <hip/hip_runtime.h>
