@@ -349,6 +349,39 @@ def test_offsets_past_32_bits(tq, cuda):
     assert torch.equal(p.out.cpu().double(), want)
 
 
+def test_host_threads_on_one_stream(tq, cuda):
+    """Two trees and a slot-mapped attention from three threads on one stream, whose workspace they
+    share: every call gives what it gives alone."""
+    from concurrent.futures import ThreadPoolExecutor
+    trees = [Problem(tq, "dense", FP16, [3000, 900], [5, 9], 16, 2, 128, seed=31),
+             Problem(tq, "turbo_prod", FP16, [2500], [40], 16, 2, 128, seed=32)]
+    for p in trees:
+        p.run(cuda)
+    p = trees[1]
+    N = 2000
+    slots = (p.tables[0, torch.arange(N) // 16] * 16 + torch.arange(N) % 16).int().to(cuda)
+    query = torch.randn(8, 2, 128, generator=torch.Generator().manual_seed(33)).half().to(cuda)
+
+    def tree(p, out):
+        tq.tree_attn_output(p.scheme, *p.gpu, out, p.layout, p.cfg, p.max_kv)
+
+    def slot_mapped(_, out):
+        tq.fused_attn_output(query, p.gpu[1], slots, out, p.layout, p.cfg, 8, N)
+
+    work = [(tree, trees[0], trees[0].out), (tree, trees[1], trees[1].out),
+            (slot_mapped, None, torch.zeros_like(query))]
+    slot_mapped(None, work[2][2])
+    outs = [[torch.zeros_like(w[2]) for _ in range(80)] for w in work]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(3) as pool:
+        for f in [pool.submit(lambda w, mine: [w[0](w[1], o) for o in mine], w, mine)
+                  for w, mine in zip(work, outs)]:
+            f.result()
+    torch.cuda.synchronize()
+    for w, mine in zip(work, outs):
+        assert all(torch.equal(o, w[2]) for o in mine)
+
+
 @pytest.mark.parametrize("scheme", ["turbo_prod", "turbo_mse"])
 def test_chain_equals_the_paged_step(tq, cuda, scheme):
     """Trees without branches over a PagedBatch's pages: its own causal step's outputs, both within

@@ -3559,6 +3559,7 @@ void launch_attention(Scheme s, const uint16_t* query, const uint8_t* pool, cons
                       hipStream_t stream, const Scratch& scratch) {
     const int rows = num_queries * g.H;
     if (rows <= 0) return;
+    const WorkspaceTurn turn(stream);
     const float inv = inv_sqrt_d(g.D);
     const bool prod = s == Scheme::Prod;
     const char* split_name = prod ? "turbo_prod_fused_attn_split" : "turbo_mse_fused_attn_split";
@@ -3605,6 +3606,7 @@ void launch_paged_attention(Scheme s, const uint16_t* query, const uint8_t* pool
                             int num_rows, int max_kv_len, hipStream_t stream) {
     const int rows = num_rows * g.H;
     if (rows <= 0) return;
+    const WorkspaceTurn turn(stream);
     const bool prod = s == Scheme::Prod;
     // Bytes from a page's start that a cell's loads reach (the matrix-core
     // kernel addresses them as 32-bit offsets, and masked tokens read a spare

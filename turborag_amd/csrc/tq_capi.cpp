@@ -420,6 +420,15 @@ void release_all(bool keep_captured = false) {
 }
 }  // namespace
 
+// (Streams that share one of the 64 take turns too.)
+WorkspaceTurn::WorkspaceTurn(hipStream_t stream) {
+    static std::mutex turns[64];
+    std::mutex& m = turns[(reinterpret_cast<uintptr_t>(stream) >> 4) * 0x9E3779B97F4A7C15ull >> 58];
+    m.lock();
+    turn_ = &m;
+}
+WorkspaceTurn::~WorkspaceTurn() { static_cast<std::mutex*>(turn_)->unlock(); }
+
 void* workspace(hipStream_t stream, size_t bytes, size_t want) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) throw Error("hipGetDevice failed");

@@ -85,6 +85,19 @@ struct Scratch {
     void hold(size_t bytes, const char* what) const;
     void* get(hipStream_t stream, size_t bytes, const char* what, size_t want = 0) const;
 };
+// Held from workspace() to the last launch that reads it.  Two host threads that
+// call on one stream share its buffer: one's kernels must not get between the
+// other's, nor may it replace a buffer that the other has but not yet used.
+class WorkspaceTurn {
+public:
+    explicit WorkspaceTurn(hipStream_t stream);
+    ~WorkspaceTurn();
+    WorkspaceTurn(const WorkspaceTurn&) = delete;
+    WorkspaceTurn& operator=(const WorkspaceTurn&) = delete;
+
+private:
+    void* turn_;
+};
 // Synchronizes the devices and frees every cached workspace (tq_workspace_release).
 void release_workspaces();
 

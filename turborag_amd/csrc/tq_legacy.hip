@@ -540,6 +540,7 @@ void launch_qjl_attention(const uint16_t* query, const uint8_t* pool, const int3
                           hipStream_t stream) {
     const int rows = num_queries * g.H;
     if (rows <= 0) return;
+    const WorkspaceTurn turn(stream);
     if (launch_qjl_mfma_attention(query, pool, slots, output, g, num_queries, num_kv_tokens,
                                   stream))
         return;

@@ -1158,6 +1158,7 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
         1, std::min<long long>((long long)num_cus() * S::kPerCu, items * chunks));
     constexpr size_t kPiece = (size_t)S::M * (D + 2) * sizeof(float);
     const bool cut = chunks > 1 + kLead;  // an item of one chunk is never cut
+    const WorkspaceTurn turn(stream);
     // (room for every later call of this head_dim: 131,072 partial rows)
     float* ws = static_cast<float*>(Scratch{}.get(stream, cut ? 2 * (size_t)t.groups * kPiece : 0, "tree attention",
                                                   4 * (size_t)num_cus() * 128 * (D + 2) * sizeof(float)));
