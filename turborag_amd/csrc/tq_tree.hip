@@ -286,7 +286,7 @@ struct Shape {
     // Buffers of a chunk's tiles (K, V; compressed pages K hi, K lo, V, one buffer
     // where other workgroups of the CU work while it is filled).
     static constexpr int kBufs = kTurned && WR < 8 ? 1 : 2, kTiles = kTurned ? 3 : 2;
-    static constexpr int kMerge = WT > 1 ? WT * M * (D + 4) * 4 : 0;
+    static constexpr int kMerge = WT > 1 ? WT * M * D * 4 : 0;
     static constexpr int kLds = kBufs * kTiles * kTile > kMerge ? kBufs * kTiles * kTile : kMerge;
     // Bytes of codes that a lane decodes at a time, how many of them, lanes per token.
     static constexpr int kLane = T * (D / 2) / (WR * 64), kUnit = kLane < 16 ? kLane : 16;
@@ -969,65 +969,70 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
         const int ei = etid & 15, eg = (etid >> 4) & 3;
         const int piece = 2 * blockIdx.x + (first ? 0 : 1);
         float* po = ws + (size_t)piece * M * D;
+        constexpr int DW = D / 16 / WT;
+        const auto merge_at = [&](int w, int rt, int dt) {
+            return ((((w * WR + wr) * RT + rt) * (D / 16) + dt) * 64 + (etid & 63)) * 16;
+        };
         float2* pm = reinterpret_cast<float2*>(ws + (size_t)2 * tl.groups * M * D) + (size_t)piece * M;
-        if constexpr (WT == 1) {
+        if constexpr (WT > 1) {
+            // The token groups' parts of a row on one reference; each group then adds up
+            // and stores its share of the values, DW of the D / 16 tiles.  (Values lie as
+            // the lanes hold them.  Added up row by row, each value with its groups' factors,
+            // this took 8.5 us where it takes 8.1: 5 drafted tokens over 1,143, fp16.)
+            if (eg == 0) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int row = pc.tile * M + (wr * RT + rt) * 16 + ei;
-                if (row >= R) continue;
-                if (whole) {
-                    const float f = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
-#pragma unroll
-                    for (int dt = 0; dt < D / 16; ++dt) {
-                        const f4 y = o[rt][dt] * f;
-                        *reinterpret_cast<u2*>(a.out + row_at(row, row / a.group) + dt * 16 + eg * 4) =
-                            u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
-                    }
-                } else {
-                    const int r = (wr * RT + rt) * 16 + ei;
-#pragma unroll
-                    for (int dt = 0; dt < D / 16; ++dt)
-                        *reinterpret_cast<f4*>(po + r * D + dt * 16 + eg * 4) = o[rt][dt];
-                    if (eg == 0) pm[r] = make_float2(m[rt], l[rt]);
-                }
+                for (int rt = 0; rt < RT; ++rt) ml[wt][(wr * RT + rt) * 16 + ei] = make_float2(m[rt], l[rt]);
             }
-        } else {
             __syncthreads();  // every wave is done with the tiles
-            float* mo = reinterpret_cast<float*>(mem);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const int r = (wr * RT + rt) * 16 + ei;
-                if (eg == 0) ml[wt][r] = make_float2(m[rt], l[rt]);
+                float mm = -INFINITY, lsum = 0.0f;
+                float2 e[WT];
+#pragma unroll
+                for (int w = 0; w < WT; ++w) {
+                    e[w] = ml[w][(wr * RT + rt) * 16 + ei];
+                    mm = fmaxf(mm, e[w].x);
+                }
+                // (an empty part holds zeros, but for a NaN logit)
+                const auto part = [&](float x) { return x == -INFINITY ? 1.0f : exp2_hw(x - mm); };
+#pragma unroll
+                for (int w = 0; w < WT; ++w) lsum += e[w].y * part(e[w].x);
+                const float f = part(m[rt]);
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt)
-                    *reinterpret_cast<f4*>(mo + (wt * M + r) * (D + 4) + dt * 16 + eg * 4) = o[rt][dt];
+                    *reinterpret_cast<f4*>(mem + merge_at(wt, rt, dt)) = o[rt][dt] * f;
+                m[rt] = mm;
+                l[rt] = lsum;
             }
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < M * (D / 4) / (64 * NW); ++k) {
-                const int u = etid + k * 64 * NW;
-                const int r = u / (D / 4), d = u % (D / 4) * 4, rr = pc.tile * M + r;
-                float mm = -INFINITY, lsum = 0.0f;
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int w = 0; w < WT; ++w) mm = fmaxf(mm, ml[w][r].x);
-                f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int dd = 0; dd < DW; ++dd) {
+                    f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 0; w < WT; ++w) {
-                    const float2 e = ml[w][r];
-                    // (an empty part holds zeros, but for a NaN logit)
-                    const float f = e.x == -INFINITY ? 1.0f : exp2_hw(e.x - mm);
-                    lsum += e.y * f;
-                    y += *reinterpret_cast<const f4*>(mo + (w * M + r) * (D + 4) + d) * f;
+                    for (int w = 0; w < WT; ++w)
+                        y += *reinterpret_cast<const f4*>(mem + merge_at(w, rt, wt * DW + dd));
+                    o[rt][dd] = y;
                 }
-                if (whole) {
-                    y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
-                    if (rr < R)
-                        *reinterpret_cast<u2*>(a.out + row_at(rr, rr / a.group) + d) =
-                            u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
-                } else if (rr < R) {
-                    *reinterpret_cast<f4*>(po + r * D + d) = y;
-                    if (d == 0) pm[r] = make_float2(mm, lsum);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = (wr * RT + rt) * 16 + ei, row = pc.tile * M + r;
+            if (row >= R) continue;
+            const int d0 = wt * DW * 16 + eg * 4;
+            if (whole) {
+                const float f = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
+                uint16_t* to = a.out + row_at(row, row / a.group) + d0;
+#pragma unroll
+                for (int dd = 0; dd < DW; ++dd) {
+                    const f4 y = o[rt][dd] * f;
+                    *reinterpret_cast<u2*>(to + dd * 16) = u2{pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3])};
                 }
+            } else {
+#pragma unroll
+                for (int dd = 0; dd < DW; ++dd) *reinterpret_cast<f4*>(po + r * D + d0 + dd * 16) = o[rt][dd];
+                if (wt == 0 && eg == 0) pm[r] = make_float2(m[rt], l[rt]);
             }
         }
         first = false;
