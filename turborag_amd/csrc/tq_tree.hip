@@ -1187,13 +1187,22 @@ template <int FMT, int D>
 void launch_format(const TreeArgs& a, hipStream_t stream) {
     constexpr bool kTurned = FMT == kProd || FMT == kMse;
     const long long rows = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
-    // Few tokens: waves that each have their own, without a barrier, have the
-    // shortest way (12 sequences of up to 6,001 tokens, turbo_mse at head_dim 64:
-    // 10.2 against 11.4 us; 4 of up to 2,000, fp16: 7.0 against 8.0).  Many: more
-    // waves per CU sharing them (16 of up to 16,384: fp16 38.9 -> 34.0, turbo_prod
-    // 49 -> 42.5 us).
-    if (rows <= 16 && (long long)a.seqs * a.max_kv * a.g.H <= 1024LL * num_cus())
-        return launch_shape<FMT, D, 1, 1, 4>(a, stream);
+    // Few tokens: tiles of 16 rows, whose waves each have tokens of their own without a
+    // barrier, have the shortest way (12 sequences of up to 6,001 tokens, turbo_mse at
+    // head_dim 64: 10.2 against 11.4 us; 4 of up to 2,000, fp16: 7.0 against 8.0), and
+    // so many workgroups more that also larger trees gain, although every tile loads
+    // or decodes the tokens again.  Split and merge, one row tile against these:
+    //   one sequence of 2,048, rows of 8, 16, 32 tokens: fp16 13.6 -> 11.6, 15.4 -> 13.0,
+    //     20.4 -> 15.1 us; turbo_prod 15.1 -> 13.7, 17.9 -> 16.6, 22.9 -> 19.6;
+    //   8,192: fp16 8 tokens 17 -> 16.3, 16 tokens 24.3 -> 18.2, 32 tokens 27.4 -> 27.6;
+    //     3 tokens (two tiles) 12.7 -> 13.2, 2,048 11.2 -> 10.7;
+    //   4 sequences of up to 2,000, turbo_prod: 3 tokens 12.9 -> 13.4, 8 16.2 -> 16.6,
+    //     16 20.3 -> 19.8.
+    // Many tokens: more waves per CU sharing them (16 of up to 16,384: fp16 38.9 ->
+    // 34.0, turbo_prod 49 -> 42.5 us).
+    const long long tiles = (rows + 15) / 16, work = tiles * a.seqs * a.max_kv * a.g.H;
+    const long long most = tiles == 1 ? 1024 : std::min<long long>(640, (kTurned ? 8 : 20) * tiles * tiles);
+    if (work <= most * num_cus()) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
     if (rows <= 32) return launch_shape<FMT, D, 1, 2, 4>(a, stream);
     // (compressed pages: 16 rows a wave leave registers for a third workgroup of
     // the CU, 51 -> 46 us for 32 sequences of up to 8,192 tokens)
