@@ -18,6 +18,8 @@ SCHEMES = [("dense", FP16), ("dense", BF16), ("turbo_prod", FP16), ("turbo_mse",
 class Problem:
     """Sequences with prefixes `lens` and `widths` drafted tokens in shuffled pages, on the CPU."""
 
+    room = 0  # tokens that max_kv_len and the block tables hold beyond the longest sequence
+
     def __init__(self, tq, scheme, dtype, lens, widths, Hq, H, D, B=16, seed=0, words=None,
                  kv_scale=1.0, q_scale=1.0, extra_rows=0, extra_blocks=0):
         g = torch.Generator().manual_seed(seed)
@@ -30,6 +32,7 @@ class Problem:
         total = [n + w for n, w in zip(lens, widths)]
         counts = [(n + B - 1) // B for n in total]
         S, P = len(lens), sum(counts) + 1
+        extra_blocks += min(self.room // B, 4_000_000 // max(S, 1))
         order = torch.randperm(P, generator=g).int()
         self.tables = torch.full((S, max(max(counts, default=0), 1) + extra_blocks), -1,
                                  dtype=torch.int32)
@@ -61,7 +64,7 @@ class Problem:
             r = int(self.row_start[s])
             self.mask[r:r + w, :m.shape[1]] = m[:, :words]
         self.query = (torch.randn(N, Hq, D, generator=g) * q_scale).to(dtype)
-        self.max_kv = max(total, default=0)
+        self.max_kv = self.tables.shape[1] * B if self.room else max(total, default=0)
         self.lens, self.widths = lens, widths
 
     def cell_bytes(self, s, t):
@@ -118,6 +121,13 @@ class Problem:
         return got
 
 
+@pytest.fixture(params=[0, 300_000], ids=["", "room"], autouse=True)
+def room(request, monkeypatch):
+    """Tiles are chosen by max_kv_len: small trees run in the large ones too where it says that the
+    cache may hold far more."""
+    monkeypatch.setattr(Problem, "room", request.param)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)
 @pytest.mark.parametrize("lens,widths,Hq,H,B", [
@@ -149,6 +159,14 @@ def test_long_prefixes(tq, cuda, scheme, dtype, D, lens, widths, Hq, H):
     """Sequences split over workgroups and merged."""
     print(f"[tree long] {scheme} {dtype} {lens=} {widths=} {D=}", flush=True)
     Problem(tq, scheme, dtype, lens, widths, Hq, H, D, seed=3).check(cuda)
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("D,lens,widths", [(128, [33000], [3]), (128, [17000, 16000], [3, 4]),
+                                           (64, [45000], [3]), (64, [34000], [7])])
+def test_few_rows_of_many_pieces(tq, cuda, scheme, dtype, D, lens, widths):
+    """Rows whose sums come from more than a hundred workgroups."""
+    Problem(tq, scheme, dtype, lens, widths, 16, 2, D, seed=43).check(cuda)
 
 
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)

@@ -1042,11 +1042,15 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
 // Merge of the items that were cut: WAVES waves per query row, D / 4 lanes per
 // piece of it; compressed pages' sums are rotated back here.  A wave per row where
 // there are rows for every SIMD (32 sequences of 6 drafted tokens, up to 16 pieces
-// per row: 12.0 -> 7.4 us), else four (1,024 rows of 64 pieces, 34 MB: 13.8 -> 6.6 us).
+// per row: 12.0 -> 7.4 us), else four (1,024 rows of 64 pieces, 34 MB: 13.8 -> 6.6 us),
+// or sixteen where rows are few and four waves would take four or more rounds of
+// loads (48 rows of 256 pieces 8.9 -> 7.5 us, 128 of 128 8.9 -> 7.8, 128 of 192 under
+// turbo_prod 12.0 -> 9.1; 256 rows of 131 pieces 8.1 -> 8.4).
+constexpr int merge_threads(int waves) { return waves > 4 ? 64 * waves : 256; }
 template <bool BF, bool TURNED, int D, int WAVES>
-__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
+__global__ __launch_bounds__(merge_threads(WAVES)) void tree_merge_kernel(const TreeArgs a, const Tiling tl,
                                                          const float* __restrict__ ws, float inv) {
-    constexpr int kLanes = D / 4, kSides = 64 * WAVES / kLanes, kRows = 4 / WAVES, kDeep = 4;
+    constexpr int kLanes = D / 4, kSides = 64 * WAVES / kLanes, kRows = merge_threads(WAVES) / (64 * WAVES), kDeep = 4;
     __shared__ float2 sml[kRows][kSides];
     __shared__ f4 so[kRows][kSides][kLanes];
     const int lane = threadIdx.x & 63, mine = threadIdx.x / (64 * WAVES);
@@ -1124,8 +1128,20 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, const
     else
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (side * kLanes >= 64) return;
-    for (int k = 0; k < min(kSides, w1 - w0 + 1); ++k)
-        if (k != side) add(sml[mine][k].x, sml[mine][k].y, so[mine][k][d]);
+    const int sides = min(kSides, w1 - w0 + 1);
+    for (int s = 0; s < sides; s += 8) {
+        float2 e[8];
+        f4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int u = min(s + k, sides - 1);
+            e[k] = sml[mine][u];
+            v[k] = so[mine][u][d];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (s + k < sides && s + k != side) add(e[k].x, e[k].y, v[k]);
+    }
     y *= lsum == 0.0f ? 0.0f : 1.0f / lsum;
     if constexpr (TURNED) {  // value d * 4 + r; every side of the wave holds the row
         const float sh = ((h & 1) ? -inv : inv) * (1.0f / kAlphaV);
@@ -1172,12 +1188,19 @@ void launch_shape(const TreeArgs& a, hipStream_t stream) {
     check_launch("tree_attention_kernel");
     if (!cut) return;
     const unsigned rows = (unsigned)(a.tokens * a.hq);
-    if (rows >= 8u * num_cus())  // enough rows to fill the CUs with a wave each
-        hipLaunchKernelGGL((tree_merge_kernel<S::BF, S::kTurned, D, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, a, t, ws,
-                           inv_sqrt_d(D));
+    const auto merge = [&](auto waves) {
+        constexpr int W = decltype(waves)::value, per = merge_threads(W) / (64 * W);
+        hipLaunchKernelGGL((tree_merge_kernel<S::BF, S::kTurned, D, W>), dim3((rows + per - 1) / per),
+                           dim3(merge_threads(W)), 0, stream, a, t, ws, inv_sqrt_d(D));
+    };
+    // Waves per row: see tree_merge_kernel.  (Pieces of an item, of average length.)
+    const long long pieces = std::min<long long>(chunks, t.groups / items);
+    if (rows >= 8u * num_cus())
+        merge(std::integral_constant<int, 1>{});
+    else if (rows < (unsigned)num_cus() && pieces * (D / 4) >= 4 * 1024)
+        merge(std::integral_constant<int, 16>{});
     else
-        hipLaunchKernelGGL((tree_merge_kernel<S::BF, S::kTurned, D, 4>), dim3(rows), dim3(256), 0, stream, a, t, ws,
-                           inv_sqrt_d(D));
+        merge(std::integral_constant<int, 4>{});
     check_launch("tree_attention_merge_kernel");
 }
 
