@@ -24,7 +24,7 @@
 //    instructions (K and q as fp16 pairs), as many LDS cycles, and the decode (~100
 //    vector instructions per wave and chunk);
 //  - turbo_prod, 32 sequences of 300 to 8,192 tokens: 43 + 8 us, the same;
-//  - one sequence of 1,143 tokens, 5 drafted: 8.6 + 4.5 us, latency: lengths -> page
+//  - one sequence of 1,143 tokens, 5 drafted: 6.6 + 4.3 us, latency: lengths -> page
 //    ids -> rows -> products -> partial sums, then the merge's launch.
 #include <hip/hip_runtime.h>
 
