@@ -341,11 +341,15 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
     using S = Shape<FMT, D, RT, WR, NW>;
     constexpr bool BF = S::BF, kTurned = S::kTurned;
     constexpr int T = S::T, C = S::C, M = S::M, WT = S::WT, kRow = S::kRow;
-    // The reference of a row's weights follows its running maximum once that is
-    // kSlack above it (rescaling the sums of 16 rows at every new maximum of one
-    // of them took a quarter of the instructions).  Weights are 2^kOff at the
-    // reference: at most 2^15 in fp16, where small ones stay normal.
-    constexpr float kSlack = 4.0f, kOff = BF ? 0.0f : 11.0f;
+    // Weights are 2^(logit - m).  The reference m lies kOff below the running
+    // maximum when it is set, and is set again once the maximum is kOff + kSlack
+    // above it (rescaling the sums of 16 rows at every new maximum of one of them
+    // took a quarter of the instructions): weights are at most 2^15 in fp16, where
+    // small ones stay normal.  The product logit = x scale is rounded with the
+    // difference, so a weight's exponent is off by up to half an ulp of m, which for
+    // logits from kHuge on (an ulp of 1/2) counts in whole powers of two: those
+    // are rounded first, and their m is the maximum itself.
+    constexpr float kSlack = 4.0f, kOff = BF ? 0.0f : 11.0f, kHuge = 4194304.0f;
     __shared__ __attribute__((aligned(1024))) uint8_t mem[S::kLds];
     __shared__ float2 ml[WT][M];
     __shared__ typename std::conditional<kTurned, DecodeTables, Nothing>::type tab;
@@ -847,7 +851,7 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
                 // Running maximum.  Compressed pages: of logit + log2 |V's scale|, so
                 // that the weights times their scales, what PV takes, are at most 2^15
                 // whatever the scales are (-25: scales of zero take part too).
-                float top[RT], ref[RT];
+                float top[RT], ref[RT], to_log[RT];  // (x to_log: the logit)
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) top[rt] = -INFINITY;
 #pragma unroll
@@ -865,15 +869,34 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
                     float t = kTurned ? top[rt] : top[rt] * scale;
                     t = lane_xor_reduce<16>(t, [](float u, float w) { return fmaxf(u, w); });
                     t = lane_xor_reduce<32>(t, [](float u, float w) { return fmaxf(u, w); });
-                    if (__ballot(t > m[rt] + kSlack)) {
-                        const float mn = t > m[rt] + kSlack ? t : m[rt];
-                        const float f = t > m[rt] + kSlack ? exp2_hw(m[rt] - mn) : 1.0f;
+                    to_log[rt] = kTurned ? qs[rt] : scale;
+                    if (__ballot(t > m[rt] + (kOff + kSlack) || fabsf(t) >= kHuge)) {
+                        const bool huge = fabsf(t) >= kHuge;
+                        if (__ballot(huge)) {
+                            // (V's scale is lost in the sum t; without it a weight is at
+                            // most 1, its product with a scale at most 65,504)
+                            float y = -INFINITY;
+#pragma unroll
+                            for (int ns = 0; ns < 2; ++ns)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    x[rt][ns][r] *= huge ? to_log[rt] : 1.0f;
+                                    y = fmaxf(y, x[rt][ns][r]);
+                                }
+                            y = lane_xor_reduce<16>(y, [](float u, float w) { return fmaxf(u, w); });
+                            y = lane_xor_reduce<32>(y, [](float u, float w) { return fmaxf(u, w); });
+                            t = huge ? y : t;
+                            to_log[rt] = huge ? 1.0f : to_log[rt];
+                        }
+                        const bool up = t > m[rt] + (huge ? 0.0f : kOff + kSlack);
+                        const float mn = up ? t - (huge ? 0.0f : kOff) : m[rt];
+                        const float f = up ? exp2_hw(m[rt] - mn) : 1.0f;
                         m[rt] = mn;
                         l[rt] *= f;
 #pragma unroll
                         for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
                     }
-                    ref[rt] = kOff - (m[rt] == -INFINITY ? 0.0f : m[rt]);
+                    ref[rt] = m[rt] == -INFINITY ? 0.0f : -m[rt];
                 }
                 u4 pw[RT];
                 const auto weights = [&](auto masked) {
@@ -886,7 +909,7 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
                             float p[4], sum = 0.0f;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                p[r] = exp2_hw(fmaf(x[rt][ns][r], kTurned ? qs[rt] : scale, ref[rt]));
+                                p[r] = exp2_hw(fmaf(x[rt][ns][r], to_log[rt], ref[rt]));
                                 sum += p[r];
                                 if constexpr (kTurned) {
                                     p[r] *= sv[r];  // (not 0 * NaN where the row sees nothing)
