@@ -101,11 +101,13 @@ def cell_rows(scheme, dtype, pool, layout, cfg, ids, t):
             V4.double()[nibbles(layout.v_codes_offset)] * scale(layout.v_norms_offset))
 
 
-def tree_attention(scheme, query, pool, tables, row_start, prefix, mask, layout, cfg, max_kv):
+def tree_attention(scheme, query, pool, tables, row_start, prefix, mask, layout, cfg, max_kv,
+                   weight=None):
     """(output, tolerance, rows written) float64 [N, Hq, D] of CPU tensors.
 
-    Roundings: weights to the pages' 16-bit type (half a step of fp16 or bf16,
-    2 U32 of their exponential's argument and sum apart), the output once.  A
+    Roundings: weights (`weight` of each; by default to the pages' 16-bit type,
+    half a step of fp16 or bf16; 2 U32 of their exponential's argument and sum
+    apart), the output once.  A
     logit is a sum of D products in fp32: D + 4 roundings of at most sum |q k|,
     and the argument's own 2.  Compressed pages: q and k as fp16 pairs (2^-21 of
     each product together), V's levels within 2^-13 of the codebook, and the
@@ -118,6 +120,8 @@ def tree_attention(scheme, query, pool, tables, row_start, prefix, mask, layout,
     written = torch.zeros(N, dtype=torch.bool)
     turned = scheme != "dense"
     had = hadamard(D)
+    if weight is None:
+        weight = unit(query.dtype)
     for s in range(prefix.numel()):
         r0, r1, L = int(row_start[s]), int(row_start[s + 1]), int(prefix[s])
         n = r1 - r0
@@ -159,7 +163,7 @@ def tree_attention(scheme, query, pool, tables, row_start, prefix, mask, layout,
                    else torch.zeros(n * G, 1)) * dl
             # (weights and their sum each move by arg; 64 U32 the sums' own roundings, which
             # grow with the logarithm of the tokens: chunks, lanes and waves are summed apart)
-            e = big * (unit(query.dtype) + 2 * arg + 64 * U32 + (2.0 ** -13 if turned else 0.0))
+            e = big * (weight + 2 * arg + 64 * U32 + (2.0 ** -13 if turned else 0.0))
             # fp16 weights are multiples of 2^-24 where they are subnormal, so half of that off; a
             # row's largest weight is 2^11 or more: 2^-25 / 2^11 of it each
             if query.dtype == torch.float16:

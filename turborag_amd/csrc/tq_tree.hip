@@ -92,6 +92,21 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
+// What pack2's result hi leaves of a and b, packed likewise.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2_rest(uint32_t hi, float a, float b) {
+    if constexpr (BF) {
+        return pack2<BF>(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+    } else {
+        uint32_t lo;
+        asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\t"
+            "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+            : "=&v"(lo)
+            : "v"(hi), "v"(a), "v"(b));
+        return lo;
+    }
+}
+
 // All ones in the halves of x that are infinite or NaN.
 template <bool BF>
 __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
@@ -270,9 +285,12 @@ __device__ __forceinline__ Piece locate(const TreeArgs& a, const Tiling& g, cons
 // 32-token step is 4 (l / 16) + 0..3 of either 16 tokens; V' is read from its
 // token rows in that order by transposing LDS loads).
 //
-// Weights are rounded to the pages' 16-bit type for their product with V (fp16
-// for compressed pages), as far as the output's own rounding; logits, sums and
-// references are fp32.  RT = 2: a K or V operand read from LDS serves two
+// Weights enter their product with V in two parts of the pages' 16-bit type (fp16
+// for compressed pages): ~22 bits (bf16: 16) as in the other attention kernels.
+// One part alone, rounded as far as the output is, left flat rows 1.4 times the
+// error of fp32 weights; the second costs 64 drafted tokens over 32,768 43.1 ->
+// 49.5 us (fp16), 61.4 -> 64.4 (turbo_prod), 32 sequences 115.8 -> 118.2 (bf16), 46.7
+// -> 48.9 (turbo_prod).  Logits, sums and references are fp32.  RT = 2: a K or V operand read from LDS serves two
 // products; one row tile per wave reads as many bytes as LDS gives.
 // ---------------------------------------------------------------------------
 template <int FMT, int D, int RT, int WR, int NW>
@@ -322,12 +340,7 @@ __device__ __forceinline__ uint2 split_k3(uint2 e, float re) {
     const float x = fmaf(__uint_as_float(s0), re, __uint_as_float(e.x));
     const float y = fmaf(__uint_as_float(s1), re, __uint_as_float(e.y));
     const uint32_t hi = pack2<false>(x, y);
-    uint32_t lo;
-    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-        : "=&v"(lo)
-        : "v"(hi), "v"(x), "v"(y));
-    return make_uint2(hi, lo);
+    return make_uint2(hi, pack2_rest<false>(hi, x, y));
 }
 
 struct alignas(16) TokenScales {
@@ -639,17 +652,18 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
             for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
+        bool search = false;  // every chunk's values for infinities (see its end)
         for (int c = c0; c < c1; ++c) {
             const int tb0 = c * C + wt * T;  // the wave's first token
             constexpr uint64_t kAll = T == 64 ? ~0ull : (1ull << (T & 63)) - 1;
             const uint64_t live = __ballot(readable(token_of(c), id)) & kAll;
-            const bool plain = live == kAll && tb0 + T <= pc.L;
+            const bool plain = !search && live == kAll && tb0 + T <= pc.L;
             // (the same in every wave: two token groups know each other's tokens)
             bool plain_all = plain;
             if constexpr (WR > 1 && WT > 1) {
                 static_assert(WT == 2, "two token groups");
                 const uint64_t other = __ballot(readable(token_of(c) + (wt ? -T : T), id2)) & kAll;
-                plain_all = live == kAll && other == kAll && c * C + C <= pc.L;
+                plain_all = !search && live == kAll && other == kAll && c * C + C <= pc.L;
             }
             // The chunk's tiles are in LDS: loaded by its waves, or decoded now.  (A
             // wave's issue priority: products before softmax before decode, so that a
@@ -898,7 +912,7 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
                     }
                     ref[rt] = m[rt] == -INFINITY ? 0.0f : -m[rt];
                 }
-                u4 pw[RT];
+                u4 pw[RT], pl[RT];
                 const auto weights = [&](auto masked) {
 #pragma unroll
                     for (int ns = 0; ns < 2; ++ns) {
@@ -917,8 +931,12 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
                                 }
                             }
                             l[rt] += sum;
-                            pw[rt][ns * 2] = pack2<BF>(p[0], p[1]);
-                            pw[rt][ns * 2 + 1] = pack2<BF>(p[2], p[3]);
+#pragma unroll
+                            for (int r = 0; r < 4; r += 2) {
+                                const uint32_t hi = pack2<BF>(p[r], p[r + 1]);
+                                pw[rt][ns * 2 + r / 2] = hi;
+                                pl[rt][ns * 2 + r / 2] = pack2_rest<BF>(hi, p[r], p[r + 1]);
+                            }
                         }
                     }
                 };
@@ -931,12 +949,49 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
                     for (int dt = 0; dt < D / 16; ++dt) va[dt] = values(st, dt);
                 }
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) {
+                for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(va[dt], pl[rt], o[rt][dt]);
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma<BF>(va[dt], pw[rt], o[rt][dt]);
-                }
             }
             if (kTurned && WR > 1 && S::kBufs == 1) __syncthreads();  // the tiles are decoded again
+            // Infinite times a weight's low part, or times a weight that is zero, may
+            // be NaN where the sum is infinite.  Sums that are not finite at the end
+            // begin again, with every chunk searched.
+            if constexpr (!kTurned) {
+                if (c + 1 == c1 && !search) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int dt = 0; dt < D / 16; ++dt)
+                            sum += (o[rt][dt][0] + o[rt][dt][1]) + (o[rt][dt][2] + o[rt][dt][3]);
+                    const bool odd = !(fabsf(sum) < INFINITY);
+                    if (WR > 1 ? __syncthreads_or(odd) : __ballot(odd) != 0) {
+                        search = true;
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            m[rt] = -INFINITY;
+                            l[rt] = 0.0f;
+#pragma unroll
+                            for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                        }
+                        id = table[page_of(token_of(c0), tib)];
+                        if (kPair) id2 = table[page_of(token_of(c0) + (wt ? -T : T), tib)];
+                        stage(c0, id);
+                        next = id;
+                        next2 = id2;
+                        if (c0 + 1 < c1) {
+                            next = table[page_of(token_of(c0 + 1), tib)];
+                            if (kPair) next2 = table[page_of(token_of(c0 + 1) + (wt ? -T : T), tib)];
+                        }
+                        c = c0 - 1;
+                    }
+                }
+            }
         }
 
         // A row's sum over its four lanes.
