@@ -315,13 +315,12 @@ constexpr float kAlphaV = 1.5982153f;  // alpha V4[c] is fp16-exact to 9.2e-5 fo
 
 // 16 bytes per lane from p straight into LDS at byte `lds` (the same in every
 // lane) + 16 lane.  In asm, because the compiler waits for loads of its own kind
-// before any LDS read that follows; wait_vmem() is the wait.  (m0 is nobody
-// else's here: nothing that the compiler emits for these kernels takes it.)
+// before any LDS read that follows; wait_vmem() is the wait.
 __device__ __forceinline__ void load_to_lds(const uint8_t* p, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
                      __builtin_amdgcn_readfirstlane(lds)),
                  "v"(p)
-                 : "memory");
+                 : "m0", "memory");
 }
 __device__ __forceinline__ void wait_vmem() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
