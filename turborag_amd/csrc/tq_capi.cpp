@@ -340,18 +340,36 @@ void reap_retired() {
     }
 }
 
+// The turns (WorkspaceTurn); streams that share one of them take turns too.
+// Taken before g_ws_mu.
+constexpr unsigned kTurns = 64;
+std::mutex g_turns[kTurns];
+unsigned turn_of(hipStream_t stream) {
+    return (unsigned)((reinterpret_cast<uintptr_t>(stream) >> 4) * 0x9E3779B97F4A7C15ull >> 58);
+}
+
 // Evicts the least recently used cached buffer that no captured graph
-// references and whose stream is not being captured (none: the cache grows).
+// references, whose stream is not being captured and that no other thread has
+// but not yet launched on, i.e. whose turn (held by the caller: `mine`) is free
+// (none: the cache grows).
 // Its stream idle: freed now.  Still running work: retired behind an event
 // recorded on that stream.  A stream the runtime no longer knows (destroyed):
 // parked, freed only by tq_workspace_release, since it cannot be ordered
 // behind that stream's last kernels.  Lock held.
-void evict_lru() {
+void evict_lru(unsigned mine) {
+    std::vector<decltype(g_ws)::iterator> order;
+    for (auto it = g_ws.begin(); it != g_ws.end(); ++it)
+        if (!it->second.captured) order.push_back(it);
+    std::sort(order.begin(), order.end(),
+              [](auto a, auto b) { return a->second.last_use < b->second.last_use; });
     auto victim = g_ws.end();
-    for (auto it = g_ws.begin(); it != g_ws.end(); ++it) {
-        if (it->second.captured) continue;
-        if (victim != g_ws.end() && it->second.last_use >= victim->second.last_use) continue;
+    std::unique_lock<std::mutex> turn;
+    for (auto it : order) {
+        const unsigned t = turn_of(it->first.second);
+        if (t != mine) turn = std::unique_lock<std::mutex>(g_turns[t], std::try_to_lock);
+        if (t != mine && !turn.owns_lock()) continue;
         victim = it;
+        break;
     }
     if (victim == g_ws.end()) return;
     const int dev = victim->first.first;
@@ -420,14 +438,8 @@ void release_all(bool keep_captured = false) {
 }
 }  // namespace
 
-// (Streams that share one of the 64 take turns too.)
-WorkspaceTurn::WorkspaceTurn(hipStream_t stream) {
-    static std::mutex turns[64];
-    std::mutex& m = turns[(reinterpret_cast<uintptr_t>(stream) >> 4) * 0x9E3779B97F4A7C15ull >> 58];
-    m.lock();
-    turn_ = &m;
-}
-WorkspaceTurn::~WorkspaceTurn() { static_cast<std::mutex*>(turn_)->unlock(); }
+WorkspaceTurn::WorkspaceTurn(hipStream_t stream) : turn_(turn_of(stream)) { g_turns[turn_].lock(); }
+WorkspaceTurn::~WorkspaceTurn() { g_turns[turn_].unlock(); }
 
 void* workspace(hipStream_t stream, size_t bytes, size_t want) {
     int dev = 0;
@@ -448,7 +460,7 @@ void* workspace(hipStream_t stream, size_t bytes, size_t want) {
     }
     if (!cap) {
         reap_retired();
-        if (it == g_ws.end() && g_ws.size() >= kMaxStreams) evict_lru();
+        if (it == g_ws.end() && g_ws.size() >= kMaxStreams) evict_lru(turn_of(stream));
     }
     WsBuf& b = g_ws[{dev, stream}];
     size_t n = std::max({need, b.n * 2, size_t(1) << 20});
@@ -501,6 +513,10 @@ void* Scratch::get(hipStream_t stream, size_t bytes, const char* what, size_t wa
 }
 
 void release_workspaces() {
+    // Every turn: no thread has a buffer that it has not yet launched on.
+    std::vector<std::unique_lock<std::mutex>> turns;
+    turns.reserve(kTurns);
+    for (std::mutex& m : g_turns) turns.emplace_back(m);
     std::lock_guard<std::mutex> lock(g_ws_mu);
     release_all();
 }

@@ -87,7 +87,9 @@ struct Scratch {
 };
 // Held from workspace() to the last launch that reads it.  Two host threads that
 // call on one stream share its buffer: one's kernels must not get between the
-// other's, nor may it replace a buffer that the other has but not yet used.
+// other's, nor may it replace a buffer that the other has but not yet used.  A
+// buffer whose turn is held is neither evicted nor released.  Every caller of
+// workspace() holds its stream's turn.
 class WorkspaceTurn {
 public:
     explicit WorkspaceTurn(hipStream_t stream);
@@ -96,7 +98,7 @@ public:
     WorkspaceTurn& operator=(const WorkspaceTurn&) = delete;
 
 private:
-    void* turn_;
+    unsigned turn_;
 };
 // Synchronizes the devices and frees every cached workspace (tq_workspace_release).
 void release_workspaces();
