@@ -31,6 +31,6 @@ def turns(tmp_path_factory):
     return out
 
 
-@pytest.mark.parametrize("what", ["release", "evict"])
+@pytest.mark.parametrize("what", ["release", "evict", "threads"])
 def test_a_buffer_in_hand_stays(turns, what):
     assert "ok" in _run(turns, what, timeout=60)

@@ -15,6 +15,7 @@
 #include <map>
 #include <mutex>
 #include <new>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -303,6 +304,7 @@ struct WsBuf {
     size_t n = 0;
     bool captured = false;  // handed out during a stream capture
     uint64_t last_use = 0;  // handout tick (eviction order)
+    hipEvent_t done = nullptr;  // hipStreamPerThread: behind its thread's last call
 };
 uint64_t g_ws_tick = 0;
 struct Retired {
@@ -311,7 +313,24 @@ struct Retired {
     int dev;
 };
 std::mutex g_ws_mu;
-std::map<std::pair<int, hipStream_t>, WsBuf> g_ws;
+// hipStreamPerThread names another stream in every host thread, so its buffers
+// belong to a thread each (0: any other stream).  Another thread can neither query
+// that stream nor record on it: its own thread records an event as it ends its turn.
+struct WsKey {
+    int dev;
+    hipStream_t stream;
+    uint64_t thread;
+    bool operator<(const WsKey& o) const {
+        return std::tie(dev, stream, thread) < std::tie(o.dev, o.stream, o.thread);
+    }
+};
+uint64_t thread_of(hipStream_t s) {
+    if (s != hipStreamPerThread) return 0;
+    static std::atomic<uint64_t> threads{0};
+    thread_local const uint64_t id = ++threads;
+    return id;
+}
+std::map<WsKey, WsBuf> g_ws;
 std::vector<Retired> g_retired;
 constexpr size_t kMaxStreams = 64;
 
@@ -344,9 +363,10 @@ void reap_retired() {
 // Taken before g_ws_mu.
 constexpr unsigned kTurns = 64;
 std::mutex g_turns[kTurns];
-unsigned turn_of(hipStream_t stream) {
-    return (unsigned)((reinterpret_cast<uintptr_t>(stream) >> 4) * 0x9E3779B97F4A7C15ull >> 58);
+unsigned turn_of(hipStream_t stream, uint64_t thread) {
+    return (unsigned)(((reinterpret_cast<uintptr_t>(stream) >> 4) + thread) * 0x9E3779B97F4A7C15ull >> 58);
 }
+unsigned turn_of(hipStream_t stream) { return turn_of(stream, thread_of(stream)); }
 
 // Evicts the least recently used cached buffer that no captured graph
 // references, whose stream is not being captured and that no other thread has
@@ -365,15 +385,21 @@ void evict_lru(unsigned mine) {
     auto victim = g_ws.end();
     std::unique_lock<std::mutex> turn;
     for (auto it : order) {
-        const unsigned t = turn_of(it->first.second);
+        const unsigned t = turn_of(it->first.stream, it->first.thread);
         if (t != mine) turn = std::unique_lock<std::mutex>(g_turns[t], std::try_to_lock);
         if (t != mine && !turn.owns_lock()) continue;
         victim = it;
         break;
     }
     if (victim == g_ws.end()) return;
-    const int dev = victim->first.first;
-    const hipStream_t s = victim->first.second;
+    const int dev = victim->first.dev;
+    const hipStream_t s = victim->first.stream;
+    Retired r{victim->second.p, victim->second.done, dev};
+    if (victim->first.thread) {  // (no event: parked)
+        g_retired.push_back(r);
+        g_ws.erase(victim);
+        return;
+    }
     int cur = 0;
     (void)hipGetDevice(&cur);
     (void)hipSetDevice(dev);
@@ -381,7 +407,6 @@ void evict_lru(unsigned mine) {
         (void)hipSetDevice(cur);
         return;
     }
-    Retired r{victim->second.p, nullptr, dev};
     const hipError_t q = hipStreamQuery(s);
     if (q == hipSuccess) {
         (void)hipFree(r.p);
@@ -403,7 +428,7 @@ void evict_lru(unsigned mine) {
 // (with keep_captured, those a captured graph references stay).  Lock held.
 void release_all(bool keep_captured = false) {
     std::vector<int> devs;
-    for (const auto& kv : g_ws) devs.push_back(kv.first.first);
+    for (const auto& kv : g_ws) devs.push_back(kv.first.dev);
     for (const auto& r : g_retired) devs.push_back(r.dev);
     std::sort(devs.begin(), devs.end());
     devs.erase(std::unique(devs.begin(), devs.end()), devs.end());
@@ -417,8 +442,9 @@ void release_all(bool keep_captured = false) {
             ++it;
             continue;
         }
-        (void)hipSetDevice(it->first.first);
+        (void)hipSetDevice(it->first.dev);
         (void)hipFree(it->second.p);
+        if (it->second.done) (void)hipEventDestroy(it->second.done);
         it = g_ws.erase(it);
     }
     for (size_t k = 0; k < g_retired.size();) {
@@ -438,14 +464,34 @@ void release_all(bool keep_captured = false) {
 }
 }  // namespace
 
-WorkspaceTurn::WorkspaceTurn(hipStream_t stream) : turn_(turn_of(stream)) { g_turns[turn_].lock(); }
-WorkspaceTurn::~WorkspaceTurn() { g_turns[turn_].unlock(); }
+WorkspaceTurn::WorkspaceTurn(hipStream_t stream) : stream_(stream), turn_(turn_of(stream)) {
+    g_turns[turn_].lock();
+}
+WorkspaceTurn::~WorkspaceTurn() {
+    if (stream_ == hipStreamPerThread) {
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        std::lock_guard<std::mutex> lock(g_ws_mu);
+        const auto it = g_ws.find({dev, stream_, thread_of(stream_)});
+        if (it != g_ws.end() && !capturing(stream_)) {
+            WsBuf& b = it->second;
+            if ((!b.done && hipEventCreateWithFlags(&b.done, hipEventDisableTiming) != hipSuccess) ||
+                hipEventRecord(b.done, stream_) != hipSuccess) {
+                (void)hipGetLastError();
+                if (b.done) (void)hipEventDestroy(b.done);
+                b.done = nullptr;
+            }
+        }
+    }
+    g_turns[turn_].unlock();
+}
 
 void* workspace(hipStream_t stream, size_t bytes, size_t want) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) throw Error("hipGetDevice failed");
     std::lock_guard<std::mutex> lock(g_ws_mu);
-    auto it = g_ws.find({dev, stream});
+    const WsKey key{dev, stream, thread_of(stream)};
+    auto it = g_ws.find(key);
     if (bytes == 0 && it != g_ws.end() && it->second.n >= want) {  // nothing to hand out or make
         it->second.last_use = ++g_ws_tick;
         return it->second.p;
@@ -462,7 +508,7 @@ void* workspace(hipStream_t stream, size_t bytes, size_t want) {
         reap_retired();
         if (it == g_ws.end() && g_ws.size() >= kMaxStreams) evict_lru(turn_of(stream));
     }
-    WsBuf& b = g_ws[{dev, stream}];
+    WsBuf& b = g_ws[key];
     size_t n = std::max({need, b.n * 2, size_t(1) << 20});
     void* p = nullptr;
     bool ok = hipMalloc(&p, n) == hipSuccess;

@@ -69,7 +69,8 @@ float inv_sqrt_d(int D);
 // (the reference's TQ_CHECK_LAUNCH, include/tq_cuda_check.h:18-24).
 void check_launch(const char* what);
 
-// Per-(device, stream) scratch for split-K partials.  Grows; an outgrown
+// Per-(device, stream) scratch for split-K partials (hipStreamPerThread: of each
+// host thread).  Grows; an outgrown
 // buffer is freed once the stream's earlier kernels have finished.  Outside a
 // stream capture the buffer is made to hold `want` bytes too (null only for 0
 // bytes): a capture cannot allocate, so a call leaves room for the calls like it
@@ -98,6 +99,7 @@ public:
     WorkspaceTurn& operator=(const WorkspaceTurn&) = delete;
 
 private:
+    hipStream_t stream_;
     unsigned turn_;
 };
 // Synchronizes the devices and frees every cached workspace (tq_workspace_release).
