@@ -37,8 +37,8 @@ def plan(p: Problem) -> Plan:
     G, S, turned = Hq // H, len(p.lens), p.scheme != "dense"
     rows = -(-N * G // S)
     tiles = -(-rows // 16)
-    most = 1024 if tiles == 1 else min(640, (8 if turned else 20) * tiles * tiles)
-    if tiles * S * p.max_kv * H <= most * cus:
+    most = 1024 if not turned or D == 64 or tiles == 1 else 0 if tiles == 2 else 640
+    if (D == 64 and tiles == 1) or tiles * S * p.max_kv * H <= most * cus:
         RT, WR, NW = 1, 1, 4
     elif rows <= 32:
         RT, WR, NW = 1, 2, 4

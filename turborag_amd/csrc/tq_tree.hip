@@ -1287,22 +1287,29 @@ template <int FMT, int D>
 void launch_format(const TreeArgs& a, hipStream_t stream) {
     constexpr bool kTurned = FMT == kProd || FMT == kMse;
     const long long rows = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
-    // Few tokens: tiles of 16 rows, whose waves each have tokens of their own without a
-    // barrier, have the shortest way (12 sequences of up to 6,001 tokens, turbo_mse at
-    // head_dim 64: 10.2 against 11.4 us; 4 of up to 2,000, fp16: 7.0 against 8.0), and
-    // so many workgroups more that also larger trees gain, although every tile loads
-    // or decodes the tokens again.  Split and merge, one row tile against these:
-    //   one sequence of 2,048, rows of 8, 16, 32 tokens: fp16 13.6 -> 11.6, 15.4 -> 13.0,
-    //     20.4 -> 15.1 us; turbo_prod 15.1 -> 13.7, 17.9 -> 16.6, 22.9 -> 19.6;
-    //   8,192: fp16 8 tokens 17 -> 16.3, 16 tokens 24.3 -> 18.2, 32 tokens 27.4 -> 27.6;
-    //     3 tokens (two tiles) 12.7 -> 13.2, 2,048 11.2 -> 10.7;
-    //   4 sequences of up to 2,000, turbo_prod: 3 tokens 12.9 -> 13.4, 8 16.2 -> 16.6,
-    //     16 20.3 -> 19.8.
-    // Many tokens: more waves per CU sharing them (16 of up to 16,384: fp16 38.9 ->
-    // 34.0, turbo_prod 49 -> 42.5 us).
+    // Tiles of 16 rows: each wave has tokens of its own, so no barrier, the shortest way
+    // from a sequence's length to its sums.  Split + merge in us, these against the tiles
+    // below (16 query heads on 2 kv heads, head_dim 128 unless said):
+    //  - up to 16 rows, where the others are half empty, at head_dim 64: 32 sequences of up
+    //    to 16,384 tokens fp16 38.4 / 40.5, turbo_prod 37.4 / 52.4, turbo_mse 34.3 / 48.8;
+    //  - the same at head_dim 128 while a CU's share of tokens is small (tokens x tiles x kv
+    //    heads per CU in brackets): 8 of up to 8,192 17.2 / 18.5, 20.2 / 21.6, 19.4 / 20.1
+    //    (512), 8 of up to 16,384 22.3 / 23.9, 29.7 / 30.6, 27.9 / 28.0 (1,024); beyond, level
+    //    (16: 39.4 / 39.4, 45.1 / 44.7, 42.1 / 40.4; 2,047), and a sequence of far more rows
+    //    than the others has half the tiles;
+    //  - more rows load or decode the tokens once per tile, which the shorter way outweighs
+    //    while that share is small.  fp16: 8 drafted tokens over 2,048 12.1 / 15.0 (64), 32
+    //    over 6,500 24.2 / 29.7 (816), 4 x 8 over 8,000 21.5 / 22.8 (1,001), 16 x 3-4 over
+    //    8,192 33.7 / 24.8 (2,046).  head_dim 64: 4 x 8 over 8,000 17.8 / 19.0 fp16, 19.2 /
+    //    21.6 turbo_prod, 18.4 / 21.4 turbo_mse (1,001);
+    //  - compressed pages at head_dim 128, whose decode is the longest, sooner: turbo_prod
+    //    32 over 2,048 19.8 / 23.1 (260), 16 over 8,192 26.6 / 27.8 (513), 32 over 6,500
+    //    33.4 / 32.0 (816), 32 over 8,192 39.8 / 34.0 (1,028); turbo_mse 25.0 / 27.6 (513), 31.2 /
+    //    31.7 (816).  Two tiles, which one of 32 rows holds without loss: 4 x 2-3 over 2,000
+    //    13.7 / 13.1, 8 over 2,048 of 32 / 8 heads 17.4 / 16.7.
     const long long tiles = (rows + 15) / 16, work = tiles * a.seqs * a.max_kv * a.g.H;
-    const long long most = tiles == 1 ? 1024 : std::min<long long>(640, (kTurned ? 8 : 20) * tiles * tiles);
-    if (work <= most * num_cus()) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
+    const long long most = !kTurned || D == 64 || tiles == 1 ? 1024 : tiles == 2 ? 0 : 640;
+    if ((D == 64 && tiles == 1) || work <= most * num_cus()) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
     if (rows <= 32) return launch_shape<FMT, D, 1, 2, 4>(a, stream);
     // (compressed pages: 16 rows a wave leave registers for a third workgroup of
     // the CU, 51 -> 46 us for 32 sequences of up to 8,192 tokens)
