@@ -513,7 +513,8 @@ int tq_launch_dense_rope_append_kv(const void* query, int64_t query_stride, cons
  * own bit says so.  Tokens past 32 * mask_words drafted ones have no bit.  Rows
  * that attend nothing get 0; rows past row_start[num_seqs] stay as they were.
  * max_kv_len >= every prefix_len[s] + n_s sizes the launch (tokens past it are
- * not attended) and must fit in max_blocks_per_seq pages.  A token whose page
+ * not attended) and must fit in max_blocks_per_seq pages; the kernel is chosen
+ * for sequences near it, so a bound far above them costs time.  A token whose page
  * id is negative is not attended; other page ids are valid.  Masked and unused
  * tokens never reach a row, whatever their pages hold (NaN, infinities).
  * head_dim 64 or 128; page_pool, the page size and the regions' offsets 16-byte

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kBlock) void rope_pairs_kernel(const RopeArgs a, in
 // One row per lane group: a table row is as many bytes as two rows of heads,
 // but a token's rows find it in the caches; two, four and five rows per group
 // with the table row in registers took 66 to 69 us against 66 for the append
-// of 32,768 tokens of 16/2 heads (352 MB: 5.3 TB/s, as a copy of 1 GiB runs),
+// of 32,768 tokens of 16/2 heads (352 MB: 5.3 TB/s; a copy of 1 GiB runs at 5.2),
 // and 3.7 to 4.7 against 3.4 for 1,143 tokens of 14/2 heads at head_dim 64.
 // ---------------------------------------------------------------------------
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));

@@ -13,18 +13,18 @@
 // workgroup, and what was cut is merged by a second launch.  Measured (MI355X,
 // 16 query heads on 2 kv heads, head_dim 128; kernels alone):
 //  - dense bf16, 32 sequences of 1,024 to 32,768 tokens, 4 to 8 drafted tokens
-//    each, 556 MB: 111 + 8 us, the split at 5.0 TB/s where a copy of 1 GiB runs
-//    at 5.2: bound by HBM;
-//  - dense fp16, 64 drafted tokens over 32,768: 37 + 9 us, 470 TFLOP/s of the split
-//    (an 8,192^3 product of the library's: 1,300).  Of a workgroup's 63,000 cycles
-//    5,170 are for each of nine chunks (two waves per SIMD: ~2,050 of matrix
-//    instructions and ~2,900 of the softmax's vector instructions), 10,400 for the
-//    chain lengths -> page ids -> rows, 6,100 for the partial sums, 33 MB in all;
-//  - the same over turbo_prod: 58 + 9 us, 10,300 cycles a chunk: twice the matrix
-//    instructions (K and q as fp16 pairs), as many LDS cycles, and the decode (~100
-//    vector instructions per wave and chunk);
-//  - turbo_prod, 32 sequences of 300 to 8,192 tokens: 43 + 8 us, the same;
-//  - one sequence of 1,143 tokens, 5 drafted: 6.6 + 4.3 us, latency: lengths -> page
+//    each, 556 MB: a call 118 us, 4.7 TB/s where a copy of 1 GiB runs at 5.2: bound
+//    by HBM;
+//  - dense fp16, 64 drafted tokens over 32,768: 46 + 9 us, 375 TFLOP/s of the split
+//    (an 8,192^3 product of the library's: 1,300).  Of a workgroup's 77,000 cycles
+//    6,800 are for each of nine chunks (two waves per SIMD: ~3,100 of matrix
+//    instructions, the rest the softmax's vector instructions), 9,500 for the chain
+//    lengths -> page ids -> rows, 4,500 for the partial sums, 33 MB in all;
+//  - the same over turbo_prod: 65 + 9 us, 10,900 cycles a chunk: more matrix
+//    instructions (K and q as fp16 pairs), LDS cycles, and the decode (~100 vector
+//    instructions per wave and chunk);
+//  - turbo_prod, 32 sequences of 300 to 8,192 tokens: 46 + 8 us, the same;
+//  - one sequence of 1,143 tokens, 5 drafted: 7.2 + 4.2 us, latency: lengths -> page
 //    ids -> rows -> products -> partial sums, then the merge's launch.
 #include <hip/hip_runtime.h>
 
@@ -357,7 +357,7 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
     // maximum when it is set, and is set again once the maximum is kOff + kSlack
     // above it (rescaling the sums of 16 rows at every new maximum of one of them
     // took a quarter of the instructions): weights are at most 2^15 in fp16, where
-    // small ones stay normal.  The product logit = x scale is rounded with the
+    // small ones stay normal and those below 2^-25, 2^-36 of the largest, are lost.  The product logit = x scale is rounded with the
     // difference, so a weight's exponent is off by up to half an ulp of m, which for
     // logits from kHuge on (an ulp of 1/2) counts in whole powers of two: those
     // are rounded first, and their m is the maximum itself.
@@ -666,7 +666,7 @@ void tree_split_kernel(const TreeArgs a, const Tiling tl, float* __restrict__ ws
             }
             // The chunk's tiles are in LDS: loaded by its waves, or decoded now.  (A
             // wave's issue priority: products before softmax before decode, so that a
-            // SIMD's waves take turns at matrix and vector instructions: 46.1 -> 43.4 us
+            // SIMD's waves take turns at matrix and vector instructions: 48.2 -> 45.7 us
             // for 32 sequences of up to 8,192 tokens, turbo_prod.  Two waves per SIMD
             // on dense pages gained nothing from it.)
             if constexpr (kTurned) {
@@ -1311,8 +1311,9 @@ void launch_format(const TreeArgs& a, hipStream_t stream) {
     const long long most = !kTurned || D == 64 || tiles == 1 ? 1024 : tiles == 2 ? 0 : 640;
     if ((D == 64 && tiles == 1) || work <= most * num_cus()) return launch_shape<FMT, D, 1, 1, 4>(a, stream);
     if (rows <= 32) return launch_shape<FMT, D, 1, 2, 4>(a, stream);
-    // (compressed pages: 16 rows a wave leave registers for a third workgroup of
-    // the CU, 51 -> 46 us for 32 sequences of up to 8,192 tokens)
+    // (compressed pages: 16 rows a wave leave registers, but for five at head_dim 128
+    // that spill, for a third workgroup of the CU: 48.6 -> 45.7 us for 32 sequences of
+    // up to 8,192 tokens)
     if (rows <= 64) return launch_shape<FMT, D, kTurned ? 1 : 2, kTurned ? 4 : 2, 4>(a, stream);
     if (rows <= 128) return launch_shape<FMT, D, 2, 4, 4>(a, stream);
     return launch_shape<FMT, D, 2, 8, 8>(a, stream);
