@@ -144,7 +144,12 @@ std::vector<hipStream_t> others(hipStream_t s, int n) {
                 const tq::WorkspaceTurn t(stream(1000 + k));
                 got[k] = true;
             });
-        nap(200);
+        const auto count = [&] {
+            int c = 0;
+            for (auto& g : got) c += g ? 1 : 0;
+            return c;
+        };
+        for (int ms = 0; ms < 20000 && count() < n; ++ms) nap(1);
         for (int k = 0; k < n + 40 && (int)out.size() < n; ++k)
             if (got[k]) out.push_back(stream(1000 + k));
     }
