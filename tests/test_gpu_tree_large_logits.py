@@ -166,3 +166,22 @@ def test_equal_logits_share(tq, cuda, monkeypatch, widths, Hq, H, room, dtype, a
                 # weights that count is below 2^-18
                 tol = size * (unit(dtype) + 2.0 ** -18 + 64 * U32) + unit(dtype) * ref.abs() + tiny(dtype)
                 assert ((got[r0 + j, i] - ref).abs() <= tol).all(), (s, j, i)
+
+
+@pytest.mark.parametrize("scheme,dtype", [("dense", FP16), ("dense", BF16), ("turbo_prod", FP16),
+                                          ("turbo_mse", FP16)])
+@pytest.mark.parametrize("widths,Hq,H,room", TILES)
+def test_rows_of_all_sizes(tq, cuda, monkeypatch, widths, Hq, H, room, scheme, dtype):
+    """Rows of one tile with logits from 1e-3 to 1e8: each as exact as it is among its like."""
+    monkeypatch.setattr(Problem, "room", room)
+    p = Problem(tq, scheme, dtype, [1070, 300, 0], [widths, max(widths - 2, 1), 1], Hq, H, 128, seed=64,
+                kv_scale=2e3)
+    g = torch.Generator().manual_seed(65)
+    size = 10.0 ** (-6 + 10 * torch.rand(*p.query.shape[:2], 1, generator=g))
+    p.query = (p.query.float() * size).to(dtype)
+    if scheme == "dense":
+        dense_values(p, 1.0)
+    else:
+        value_scales(p, -3, 3)
+    check(p, cuda, least=0.0)
+    p.check(cuda)
