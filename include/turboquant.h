@@ -345,6 +345,10 @@ int tq_block_table_blocks(const TQBlockTable* t, int32_t seq_id, int32_t* out_bl
 /* Releases every page of seq_id back to the allocator (no reference
  * counterpart: the reference never frees a sequence). */
 int tq_block_table_free_sequence(TQBlockTable* t, int32_t seq_id);
+/* Cuts seq_id to its first num_tokens tokens (at most those it has) and gives
+ * the pages behind them back, the last one first (no reference counterpart: its
+ * sequences never shrink). */
+int tq_block_table_truncate(TQBlockTable* t, int32_t seq_id, int num_tokens);
 
 /* ---------------------------------------------------------------------- */
 /* Kernels the reference compiles but never exports (superset of its ABI): */
@@ -499,6 +503,37 @@ int tq_launch_dense_rope_append_kv(const void* query, int64_t query_stride, cons
                                    const TQDensePageLayout* layout, const TQRopeConfig* rope,
                                    const TQConfig* cfg, int num_tokens, void* stream);
 
+/* Positions with several axes, as the tokens of images and video have them
+ * (time, height, width): every pair of a head's rotated dims turns by the
+ * position on its own axis. */
+typedef struct TQRopeAxes {
+    int num_axes;     /* 1 .. 4                                                       */
+    uint8_t axis[64]; /* of pair i < rot_dim / 2, less than num_axes; others not read */
+} TQRopeAxes;
+
+/* tq_launch_qk_norm_rope with several axes: axis x's position of token t is
+ * positions[x * axis_stride + t] (axis_stride >= num_tokens where num_axes > 1),
+ * and pair i turns by the angle in cos_sin's column i at its axis's position.
+ * (The column is the pair's among all: a table whose frequencies begin again with
+ * every axis has them in its columns.)  A token with a position outside
+ * [0, max_position) on any axis is skipped.  With equal positions on all axes the
+ * outputs are those of the entry without axes, bit for bit. */
+int tq_launch_qk_norm_rope_axes(const void* query, int64_t query_stride, const void* key,
+                                int64_t key_stride, const void* q_weight, const void* k_weight,
+                                const float* cos_sin, const int32_t* positions, int64_t axis_stride,
+                                void* out_query, int64_t out_query_stride, void* out_key,
+                                int64_t out_key_stride, const TQRopeAxes* axes,
+                                const TQRopeConfig* rope, const TQConfig* cfg, int num_tokens,
+                                void* stream);
+/* tq_launch_dense_rope_append_kv with several axes, likewise. */
+int tq_launch_dense_rope_axes_append_kv(
+    const void* query, int64_t query_stride, const void* key, int64_t key_stride, const void* value,
+    int64_t value_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
+    const int32_t* positions, int64_t axis_stride, const int32_t* slot_mapping, uint8_t* page_pool,
+    void* out_query, int64_t out_query_stride, const TQDensePageLayout* layout,
+    const TQRopeAxes* axes, const TQRopeConfig* rope, const TQConfig* cfg, int num_tokens,
+    void* stream);
+
 /* Attention of drafted token trees over a paged cache: softmax(q k^T /
  * sqrt(D)) v.  query / output [num_tokens, num_q_heads, D]; query head i reads
  * kv head i / (num_q_heads / H) (num_q_heads a multiple of H).  Sequence s
@@ -544,6 +579,99 @@ int tq_launch_turbo_mse_tree_attention(const uint16_t* query, const uint8_t* pag
                                        const TQTurbomsePageLayout* layout, const TQConfig* cfg,
                                        int num_q_heads, int num_seqs, int num_tokens,
                                        int max_kv_len, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Eviction from a paged cache by accumulated attention weight (superset of  */
+/* the reference ABI, whose caches only grow): the softmax weights that       */
+/* query rows give to every cached token, summed into scores; the tokens that */
+/* a budget keeps; their cells moved to the front.  Inference only.           */
+/* ---------------------------------------------------------------------- */
+
+/* Scores: fp32 [num_seqs][H][score_stride], token t of sequence s and kv head h
+ * at (s * H + h) * score_stride + t.  For every token t below a sequence's end,
+ *   scores_out = decay * scores_in + sum of softmax_t(q k^T / sqrt(D))
+ * over the sequence's rows and the query heads of h (query head i: kv head
+ * i / (num_q_heads / H)); tokens behind the end stay as they were.  query
+ * [num_tokens, num_q_heads, D]; sequence s owns the rows row_start[s] ..
+ * row_start[s + 1] - 1 (row_start: num_seqs + 1 non-decreasing values from 0),
+ * n_s of them.  causal != 0: row j of a sequence attends its first prefix_len[s]
+ * + j + 1 tokens (its own among them; a decode step's new tokens, or the last
+ * tokens of a prompt), and the end is prefix_len[s] + n_s; otherwise every row
+ * attends the first prefix_len[s] tokens, which is the end.  Nothing past
+ * max_kv_len (>= every end; <= score_stride) is attended or written.  A
+ * sequence without rows gets decay * scores_in.  scores_in may be NULL or decay
+ * 0 (nothing is read and added), and may be scores_out; otherwise they do not
+ * overlap.  decay is in [0, 1].  Pages as in the paged entries; a token whose
+ * page id is negative has weight 0.  What a row does not attend never reaches
+ * it, whatever its page holds; a NaN or +infinity among a row's logits makes the
+ * row's weights NaN.  A sum is taken in the same order in every call of the same
+ * sizes: no atomics.  head_dim 64 or 128; alignments and dtype as in the tree
+ * attention entries.  num_seqs 0 does nothing; num_tokens * num_q_heads <= 2^26;
+ * ceil(max_kv_len / 128) times that, or times num_seqs * H, at most 2^30.  Keeps
+ * the rows' statistics (and, for up to 32 rows per sequence and kv head, their
+ * logits, up to 256 MB) in the per-stream workspace, as the attention entries: a
+ * capture needs an earlier call with the same sizes. */
+int tq_launch_dense_attention_weights(
+    const void* query, const uint8_t* page_pool, const int32_t* block_tables,
+    int max_blocks_per_seq, const int32_t* row_start, const int32_t* prefix_len, int causal,
+    const float* scores_in, float* scores_out, int64_t score_stride, float decay,
+    const TQDensePageLayout* layout, const TQConfig* cfg, int dtype, int num_q_heads, int num_seqs,
+    int num_tokens, int max_kv_len, void* stream);
+int tq_launch_turbo_prod_attention_weights(
+    const uint16_t* query, const uint8_t* page_pool, const int32_t* block_tables,
+    int max_blocks_per_seq, const int32_t* row_start, const int32_t* prefix_len, int causal,
+    const float* scores_in, float* scores_out, int64_t score_stride, float decay,
+    const TQTurboProdPageLayout* layout, const TQConfig* cfg, int num_q_heads, int num_seqs,
+    int num_tokens, int max_kv_len, void* stream);
+int tq_launch_turbo_mse_attention_weights(
+    const uint16_t* query, const uint8_t* page_pool, const int32_t* block_tables,
+    int max_blocks_per_seq, const int32_t* row_start, const int32_t* prefix_len, int causal,
+    const float* scores_in, float* scores_out, int64_t score_stride, float decay,
+    const TQTurbomsePageLayout* layout, const TQConfig* cfg, int num_q_heads, int num_seqs,
+    int num_tokens, int max_kv_len, void* stream);
+
+/* The tokens that a budget keeps, for every sequence and kv head: all
+ * kv_len[s] tokens (cut to [0, max_kv_len]) if they are at most `budget`;
+ * otherwise the first `sink`, the last `recent` and, of those between, the ones
+ * with the highest scores up to `budget` in all.  Of equal scores the lower
+ * tokens are kept; NaN ranks below every number, -0 equals 0.  kept
+ * [num_seqs][num_kv_heads][budget]: their places in rising order, then -1.
+ * new_len [num_seqs] (or NULL): their number.  out_scores (or NULL): the kept
+ * tokens' scores in kept's order and 0 behind them up to max_kv_len, out_stride
+ * elements from one head's to the next; it may be scores (with score_stride),
+ * otherwise they do not overlap.  sink + recent <= budget; num_seqs *
+ * num_kv_heads < 2^22. */
+int tq_launch_select_kv(const float* scores, int64_t score_stride, const int32_t* kv_len,
+                        int num_seqs, int num_kv_heads, int max_kv_len, int budget, int sink,
+                        int recent, int32_t* kept, int32_t* new_len, float* out_scores,
+                        int64_t out_stride, void* stream);
+
+/* Moves the cells (keys, values, scales) of kept tokens to the front: for every
+ * sequence s, kv head h and j < budget with kept[(s * H + h) * budget + j] = t >=
+ * 0, the cell of token t and head h becomes that of token j.  out_block_tables
+ * NULL: in place; kept rises strictly in j, so t >= j (a place that does not
+ * rise above j is not moved), and no page belongs to two sequences.  Otherwise
+ * token j lies in the pages of out_block_tables [num_seqs][out_max_blocks_per_seq],
+ * all of them different from those of block_tables, which keep what they hold
+ * (they may be shared).  Tokens past a table's end, and those whose page id is
+ * negative on either side, are not moved.  Cells behind the kept ones stay as
+ * they were.  Bytes are copied as they are.  head_dim 64 or 128; alignments as in
+ * the tree attention entries.  In place, flags in the per-stream workspace. */
+int tq_launch_dense_compact_kv(uint8_t* page_pool, const int32_t* block_tables,
+                               int max_blocks_per_seq, const int32_t* kept, int budget,
+                               const int32_t* out_block_tables, int out_max_blocks_per_seq,
+                               const TQDensePageLayout* layout, const TQConfig* cfg, int num_seqs,
+                               void* stream);
+int tq_launch_turbo_prod_compact_kv(uint8_t* page_pool, const int32_t* block_tables,
+                                    int max_blocks_per_seq, const int32_t* kept, int budget,
+                                    const int32_t* out_block_tables, int out_max_blocks_per_seq,
+                                    const TQTurboProdPageLayout* layout, const TQConfig* cfg,
+                                    int num_seqs, void* stream);
+int tq_launch_turbo_mse_compact_kv(uint8_t* page_pool, const int32_t* block_tables,
+                                   int max_blocks_per_seq, const int32_t* kept, int budget,
+                                   const int32_t* out_block_tables, int out_max_blocks_per_seq,
+                                   const TQTurbomsePageLayout* layout, const TQConfig* cfg,
+                                   int num_seqs, void* stream);
 
 /* ---------------------------------------------------------------------- */
 /* On-disk CAG store (superset of the reference ABI).  The reference reads  */

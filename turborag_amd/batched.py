@@ -14,6 +14,8 @@ and one fused_attention_output call per sequence and position, each with a
 per-token slot map (tq_backend/turboquant_wrapper.py; the C5 serving
 configuration).  The new tokens may also form trees (``tree_attention``): a
 row then attends the prefix and the new tokens of its mask, not all before it.
+``add_weights`` and ``evict`` keep the caches to a budget: the scores that the
+steps' attention weights add up to choose the tokens that stay.
 """
 from __future__ import annotations
 
@@ -145,6 +147,38 @@ class PagedBatch:
         self.tq.tree_attn_output(self.scheme, query, self.pool, block_tables, row_start, prefix_len,
                                  tree_mask, out, self.layout, self.cfg,
                                  max(L + w for L, w in zip(self.lens, self.widths)), stream)
+
+    # ── eviction ───────────────────────────────────────────────────── #
+
+    def add_weights(self, query, row_start, prefix_len, block_tables, scores, decay: float = 1.0,
+                    stream: int = 0) -> None:
+        """Adds the weights that the appended tokens' rows (tree_rows, query
+        [sum of widths, query heads, D]) give to every cached token up to their own
+        to scores [S, H, tokens]."""
+        self.tq.attn_weights(self.scheme, query, self.pool, block_tables, row_start, prefix_len, scores,
+                             self.layout, self.cfg, max(L + w for L, w in zip(self.lens, self.widths)),
+                             scores_in=scores, decay=decay, stream=stream)
+
+    def evict(self, scores, budget: int, block_tables, sink: int = 4, recent: int = 32, new_widths=None,
+              stream: int = 0) -> list[int]:
+        """Cuts every sequence to at most `budget` tokens (its first `sink`, last
+        `recent` and highest scores): cells and scores are moved to the front, and
+        the pages behind go back to the allocator.  The sequences' tokens are those
+        that their block tables hold; new_widths: the new tokens of the next step.
+        Returns their lengths.  Positions go on from the tokens ever appended, not
+        from what is left."""
+        held = [self.table.num_tokens(s) for s in range(self.S)]
+        kept = torch.empty(self.S, self.H, budget, dtype=torch.int32, device=self.dev)
+        lens = torch.tensor(held, dtype=torch.int32, device=self.dev)
+        self.tq.select_kv(scores, lens, kept, sink=sink, recent=recent, out_scores=scores, stream=stream)
+        self.tq.compact_kv(self.scheme, self.pool, block_tables, kept, self.layout, self.cfg,
+                           stream=stream)
+        self.lens = [min(n, budget) for n in held]
+        for s, n in enumerate(self.lens):
+            self.table.truncate(s, n)
+        if new_widths is not None:
+            self.widths = [int(x) for x in new_widths]
+        return list(self.lens)
 
     def close(self) -> None:
         self.table.close()

@@ -182,3 +182,20 @@ extern "C" int tq_block_table_free_sequence(TQBlockTable* t, int32_t seq_id) {
     t->seqs.erase(it);
     return 0;
 }
+
+extern "C" int tq_block_table_truncate(TQBlockTable* t, int32_t seq_id, int num_tokens) {
+    if (!t) return -1;
+    std::lock_guard<std::mutex> lock(t->mu);
+    auto it = t->seqs.find(seq_id);
+    if (it == t->seqs.end()) return fail("tq_block_table: unknown sequence");
+    TQBlockTable::Seq& s = it->second;
+    if (num_tokens < 0 || num_tokens > s.num_tokens)
+        return fail("tq_block_table_truncate: num_tokens must be in [0, the sequence's tokens]");
+    const size_t keep = ((size_t)num_tokens + t->block_size - 1) / t->block_size;
+    while (s.blocks.size() > keep) {
+        tq_allocator_free_block(t->alloc, s.blocks.back());
+        s.blocks.pop_back();
+    }
+    s.num_tokens = num_tokens;
+    return 0;
+}

@@ -1,5 +1,6 @@
 // tq_rope.hip — per-head RMS norm and position rotation of queries and keys,
-// and the same with the append of keys and values to dense pages.
+// and the same with the append of keys and values to dense pages; positions with
+// one axis, or with several (time, height, width), each turning pairs of its own.
 //
 // Mathematics, per (token, head) row x of D values, in fp32 with one rounding
 // at the end:
@@ -43,7 +44,34 @@ struct RopeArgs {
     int n, hq, rows;             // tokens, query heads worked on, rows per token
     int rot, max_position;
     float eps;
+    // Several axes: axis x's position of token t is pos[x * pos_stride + t], and pair i's
+    // axis the two bits 2 (i % 32) of axis_bits[i / 32].
+    int axes;
+    int64_t pos_stride;
+    uint64_t axis_bits[2];
 };
+constexpr int kMaxAxes = 4;
+__device__ __forceinline__ int axis_of(const RopeArgs& a, int pair) {
+    return (int)(a.axis_bits[pair >> 5] >> (2 * (pair & 31))) & 3;
+}
+// The token's positions (axes that do not exist: the first one's); whether all lie in the table.
+struct Positions {
+    int p[kMaxAxes];
+    bool inside;
+    __device__ __forceinline__ int of(int axis) const {
+        const int lo = axis & 1 ? p[1] : p[0], hi = axis & 1 ? p[3] : p[2];
+        return axis & 2 ? hi : lo;
+    }
+};
+__device__ __forceinline__ Positions positions_of(const RopeArgs& a, int t) {
+    Positions o;
+    o.inside = true;
+#pragma unroll
+    for (int x = 0; x < kMaxAxes; ++x) o.p[x] = a.pos[(x < a.axes ? x : 0) * a.pos_stride + t];
+#pragma unroll
+    for (int x = 0; x < kMaxAxes; ++x) o.inside = o.inside && o.p[x] >= 0 && o.p[x] < a.max_position;
+    return o;
+}
 
 template <bool BF>
 __device__ __forceinline__ float to_float(uint16_t x) {
@@ -91,7 +119,7 @@ __device__ __forceinline__ Row row_of(const RopeArgs& a, int t, int r, int slot)
 // Any head_dim, rotated part and alignment: D/2 lanes per row, two values per
 // lane.  Lane i < rot/2 holds pair i, the others two values that pass.
 // ---------------------------------------------------------------------------
-template <bool BF>
+template <bool BF, bool AXES>
 __global__ __launch_bounds__(kBlock) void rope_pairs_kernel(const RopeArgs a, int interleaved) {
     const int D = a.g.D, L = D / 2, half = a.rot / 2;
     const int i = threadIdx.x & (L - 1);
@@ -100,8 +128,16 @@ __global__ __launch_bounds__(kBlock) void rope_pairs_kernel(const RopeArgs a, in
     const bool valid = row < all;
     const long long rr = valid ? row : all - 1;
     const int t = (int)(rr / a.rows), r = (int)(rr - (long long)t * a.rows);
-    const int pos = a.pos[t];
-    const bool inside = pos >= 0 && pos < a.max_position;
+    int pos;
+    bool inside;
+    if constexpr (AXES) {
+        const Positions p = positions_of(a, t);
+        pos = p.of(i < half ? axis_of(a, i) : 0);
+        inside = p.inside;
+    } else {
+        pos = a.pos[t];
+        inside = pos >= 0 && pos < a.max_position;
+    }
     const Row o = row_of(a, t, r, a.v ? a.slots[t] : 0);
     const bool turned = i < half;
     const int e0 = !turned || interleaved ? 2 * i : i;
@@ -170,25 +206,47 @@ __device__ __forceinline__ u4 pack8(const float* y) {
     return w;
 }
 
-template <bool BF, int D, bool INTER>
+// Axes of a lane's eight pairs: one for all tokens and pairs, one per lane (blocks of
+// whole eights), or one per pair.
+constexpr int kOneAxis = 0, kLaneAxis = 1, kPairAxis = 2;
+
+template <bool BF, int D, bool INTER, int AXES>
 __global__ __launch_bounds__(kBlock) void rope_rows_kernel(const RopeArgs a) {
     constexpr int L = D / 16;
     const int j = threadIdx.x & (L - 1);
     const int job = block_of() * (kBlock / L) + threadIdx.x / L;
     const int row = min(job, a.n * a.rows - 1);
     const int t = row / a.rows;
-    const int pos = a.pos[t], slot = a.v ? a.slots[t] : 0;
+    Positions ps;
+    if constexpr (AXES == kOneAxis) {
+        ps.p[0] = a.pos[t];
+        ps.inside = ps.p[0] >= 0 && ps.p[0] < a.max_position;
+    } else {
+        ps = positions_of(a, t);
+    }
+    const int slot = a.v ? a.slots[t] : 0;
     const Row o = row_of(a, t, row - t * a.rows, slot);
     const int at0 = INTER ? 16 * j : 8 * j, at1 = INTER ? 16 * j + 8 : D / 2 + 8 * j;
     u4 w0 = *reinterpret_cast<const u4*>(o.src + at0), w1 = *reinterpret_cast<const u4*>(o.src + at1);
-    const bool live = job == row && pos >= 0 && pos < a.max_position && o.dst;
+    const bool live = job == row && ps.inside && o.dst;
     if (o.what != 2) {  // (the same for a row's lanes)
-        const float* tr = a.table + (size_t)(live ? pos : 0) * D + 8 * j;
         float c[8], s[8], y[16];
+        if constexpr (AXES == kPairAxis) {
+            const uint32_t bits = (uint32_t)(a.axis_bits[j >> 2] >> (16 * (j & 3)));
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(tr + e);
-            *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(tr + D / 2 + e);
+            for (int e = 0; e < 8; ++e) {
+                const float* tr = a.table + (size_t)(live ? ps.of(bits >> (2 * e)) : 0) * D + 8 * j + e;
+                c[e] = tr[0];
+                s[e] = tr[D / 2];
+            }
+        } else {
+            const int pos = AXES == kOneAxis ? ps.p[0] : ps.of(axis_of(a, 8 * j));
+            const float* tr = a.table + (size_t)(live ? pos : 0) * D + 8 * j;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(tr + e);
+                *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(tr + D / 2 + e);
+            }
         }
         unpack8<BF>(w0, y);
         unpack8<BF>(w1, y + 8);
@@ -241,7 +299,16 @@ template <bool BF, int D, bool INTER>
 void launch_rows(const RopeArgs& a, hipStream_t stream) {
     constexpr int per = kBlock / (D / 16);
     const dim3 grid = grid_of(((long long)a.n * a.rows + per - 1) / per);
-    hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER>), grid, dim3(kBlock), 0, stream, a);
+    const auto go = [&](auto axes) {
+        hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER, decltype(axes)::value>), grid, dim3(kBlock), 0, stream, a);
+    };
+    if (a.axes == 1) return go(std::integral_constant<int, kOneAxis>{});
+    // a field of eight pairs' axes (16 bits) is eight times its first one
+    for (int i = 0; i < D / 2; i += 8) {
+        const unsigned f = (unsigned)(a.axis_bits[i >> 5] >> (2 * (i & 31))) & 0xffff;
+        if (f != (f & 3) * 0x5555u) return go(std::integral_constant<int, kPairAxis>{});
+    }
+    go(std::integral_constant<int, kLaneAxis>{});
 }
 
 void launch_rope(const RopeArgs& a, bool bf16, bool interleaved, hipStream_t stream) {
@@ -262,10 +329,14 @@ void launch_rope(const RopeArgs& a, bool bf16, bool interleaved, hipStream_t str
     const int per = kBlock / (a.g.D / 2);
     const long long rows = (long long)a.n * a.rows;
     const dim3 grid = grid_of((rows + per - 1) / per);
+    const auto go = [&](auto bf, auto axes) {
+        hipLaunchKernelGGL((rope_pairs_kernel<decltype(bf)::value, decltype(axes)::value>), grid, dim3(kBlock), 0,
+                           stream, a, (int)interleaved);
+    };
     if (bf16)
-        hipLaunchKernelGGL(rope_pairs_kernel<true>, grid, dim3(kBlock), 0, stream, a, (int)interleaved);
+        a.axes == 1 ? go(std::true_type{}, std::false_type{}) : go(std::true_type{}, std::true_type{});
     else
-        hipLaunchKernelGGL(rope_pairs_kernel<false>, grid, dim3(kBlock), 0, stream, a, (int)interleaved);
+        a.axes == 1 ? go(std::false_type{}, std::false_type{}) : go(std::false_type{}, std::true_type{});
     check_launch(what);
 }
 
@@ -296,6 +367,23 @@ void check_rows(const char* what, const char* name, const void* p, int64_t strid
         throw Error(std::string(what) + ": " + name + " token stride must be at least heads * head_dim");
 }
 
+// Takes the axes over (null: one axis).
+void set_axes(const char* what, RopeArgs& a, const TQRopeAxes* axes, int64_t pos_stride) {
+    a.axes = 1;
+    if (!axes) return;
+    if (axes->num_axes < 1 || axes->num_axes > kMaxAxes)
+        throw Error(std::string(what) + ": num_axes must be in [1, 4]");
+    for (int i = 0; i < a.rot / 2; ++i) {
+        if (axes->axis[i] >= axes->num_axes)
+            throw Error(std::string(what) + ": a pair's axis must be less than num_axes");
+        a.axis_bits[i >> 5] |= (uint64_t)axes->axis[i] << (2 * (i & 31));
+    }
+    if (axes->num_axes > 1 && (pos_stride < a.n || pos_stride >= (int64_t(1) << 40)))
+        throw Error(std::string(what) + ": axis_stride must be at least num_tokens");
+    a.axes = axes->num_axes;
+    a.pos_stride = pos_stride;
+}
+
 template <class F>
 int rope_entry(void* stream, F&& f) {
     try {
@@ -311,26 +399,20 @@ int rope_entry(void* stream, F&& f) {
     }
 }
 
-}  // namespace
-}  // namespace tq
-
-extern "C" int tq_launch_qk_norm_rope(const void* query, int64_t query_stride, const void* key,
-                                      int64_t key_stride, const void* q_weight,
-                                      const void* k_weight, const float* cos_sin,
-                                      const int32_t* positions, void* out_query,
-                                      int64_t out_query_stride, void* out_key,
-                                      int64_t out_key_stride, const TQRopeConfig* rope,
-                                      const TQConfig* cfg, int num_tokens, void* stream) {
+int norm_rope_entry(const char* what, const void* query, int64_t query_stride, const void* key,
+                    int64_t key_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
+                    const int32_t* positions, int64_t axis_stride, void* out_query, int64_t out_query_stride,
+                    void* out_key, int64_t out_key_stride, const TQRopeAxes* axes, const TQRopeConfig* rope,
+                    const TQConfig* cfg, int num_tokens, void* stream) {
     if (!query || !key || !cos_sin || !positions || !out_query || !out_key || !rope || !cfg) return -1;
-    return tq::rope_entry(stream, [&] {
-        const char* what = "qk_norm_rope";
-        tq::check_rope(what, *rope, *cfg, num_tokens);
+    return rope_entry(stream, [&] {
+        check_rope(what, *rope, *cfg, num_tokens);
         const int H = cfg->num_kv_heads, D = cfg->head_dim, Hq = rope->num_q_heads;
-        tq::check_rows(what, "query", query, query_stride, Hq, D, num_tokens);
-        tq::check_rows(what, "key", key, key_stride, H, D, num_tokens);
-        tq::check_rows(what, "out_query", out_query, out_query_stride, Hq, D, num_tokens);
-        tq::check_rows(what, "out_key", out_key, out_key_stride, H, D, num_tokens);
-        tq::RopeArgs a{};
+        check_rows(what, "query", query, query_stride, Hq, D, num_tokens);
+        check_rows(what, "key", key, key_stride, H, D, num_tokens);
+        check_rows(what, "out_query", out_query, out_query_stride, Hq, D, num_tokens);
+        check_rows(what, "out_key", out_key, out_key_stride, H, D, num_tokens);
+        RopeArgs a{};
         a.q = static_cast<const uint16_t*>(query);
         a.k = static_cast<const uint16_t*>(key);
         a.qw = static_cast<const uint16_t*>(q_weight);
@@ -352,37 +434,36 @@ extern "C" int tq_launch_qk_norm_rope(const void* query, int64_t query_stride, c
         a.rot = rope->rot_dim;
         a.max_position = rope->max_position;
         a.eps = rope->eps;
-        tq::launch_rope(a, rope->dtype == TQ_DTYPE_BF16, rope->interleaved != 0,
-                        static_cast<hipStream_t>(stream));
+        set_axes(what, a, axes, axis_stride);
+        launch_rope(a, rope->dtype == TQ_DTYPE_BF16, rope->interleaved != 0, static_cast<hipStream_t>(stream));
     });
 }
 
-extern "C" int tq_launch_dense_rope_append_kv(
-    const void* query, int64_t query_stride, const void* key, int64_t key_stride, const void* value,
-    int64_t value_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
-    const int32_t* positions, const int32_t* slot_mapping, uint8_t* page_pool, void* out_query,
-    int64_t out_query_stride, const TQDensePageLayout* layout, const TQRopeConfig* rope,
-    const TQConfig* cfg, int num_tokens, void* stream) {
+int rope_append_entry(const std::string& what, const void* query, int64_t query_stride, const void* key,
+                      int64_t key_stride, const void* value, int64_t value_stride, const void* q_weight,
+                      const void* k_weight, const float* cos_sin, const int32_t* positions,
+                      int64_t axis_stride, const int32_t* slot_mapping, uint8_t* page_pool, void* out_query,
+                      int64_t out_query_stride, const TQDensePageLayout* layout, const TQRopeAxes* axes,
+                      const TQRopeConfig* rope, const TQConfig* cfg, int num_tokens, void* stream) {
     if (!key || !value || !cos_sin || !positions || !slot_mapping || !page_pool || !layout || !rope ||
         !cfg || !query != !out_query)
         return -1;
-    return tq::rope_entry(stream, [&] {
-        const char* what = "dense_rope_append_kv";
-        tq::check_rope(what, *rope, *cfg, num_tokens);
+    return rope_entry(stream, [&] {
+        const char* w = what.c_str();
+        check_rope(w, *rope, *cfg, num_tokens);
         const int H = cfg->num_kv_heads, D = cfg->head_dim, Hq = query ? rope->num_q_heads : 0;
-        tq::RopeArgs a{};
-        a.g = tq::dense_geom(*cfg, *layout);
+        RopeArgs a{};
+        a.g = dense_geom(*cfg, *layout);
         for (const uint64_t off : {a.g.k_off, a.g.v_off})
             if (off > a.g.page_size || layout->k_bytes > a.g.page_size - off)
-                throw tq::Error("dense_rope_append_kv: layout does not match cfg (a region ends past the page)");
-        if (reinterpret_cast<uintptr_t>(page_pool) & 3)
-            throw tq::Error("dense_rope_append_kv: page_pool must be 4-byte aligned");
+                throw Error(what + ": layout does not match cfg (a region ends past the page)");
+        if (reinterpret_cast<uintptr_t>(page_pool) & 3) throw Error(what + ": page_pool must be 4-byte aligned");
         if (query) {
-            tq::check_rows(what, "query", query, query_stride, Hq, D, num_tokens);
-            tq::check_rows(what, "out_query", out_query, out_query_stride, Hq, D, num_tokens);
+            check_rows(w, "query", query, query_stride, Hq, D, num_tokens);
+            check_rows(w, "out_query", out_query, out_query_stride, Hq, D, num_tokens);
         }
-        tq::check_rows(what, "key", key, key_stride, H, D, num_tokens);
-        tq::check_rows(what, "value", value, value_stride, H, D, num_tokens);
+        check_rows(w, "key", key, key_stride, H, D, num_tokens);
+        check_rows(w, "value", value, value_stride, H, D, num_tokens);
         a.q = static_cast<const uint16_t*>(query);
         a.k = static_cast<const uint16_t*>(key);
         a.v = static_cast<const uint16_t*>(value);
@@ -403,7 +484,58 @@ extern "C" int tq_launch_dense_rope_append_kv(
         a.rot = rope->rot_dim;
         a.max_position = rope->max_position;
         a.eps = rope->eps;
-        tq::launch_rope(a, rope->dtype == TQ_DTYPE_BF16, rope->interleaved != 0,
-                        static_cast<hipStream_t>(stream));
+        set_axes(w, a, axes, axis_stride);
+        launch_rope(a, rope->dtype == TQ_DTYPE_BF16, rope->interleaved != 0, static_cast<hipStream_t>(stream));
     });
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int tq_launch_qk_norm_rope(const void* query, int64_t query_stride, const void* key,
+                                      int64_t key_stride, const void* q_weight,
+                                      const void* k_weight, const float* cos_sin,
+                                      const int32_t* positions, void* out_query,
+                                      int64_t out_query_stride, void* out_key,
+                                      int64_t out_key_stride, const TQRopeConfig* rope,
+                                      const TQConfig* cfg, int num_tokens, void* stream) {
+    return tq::norm_rope_entry("qk_norm_rope", query, query_stride, key, key_stride, q_weight, k_weight, cos_sin,
+                               positions, 0, out_query, out_query_stride, out_key, out_key_stride, nullptr, rope,
+                               cfg, num_tokens, stream);
+}
+
+extern "C" int tq_launch_qk_norm_rope_axes(const void* query, int64_t query_stride, const void* key,
+                                           int64_t key_stride, const void* q_weight, const void* k_weight,
+                                           const float* cos_sin, const int32_t* positions, int64_t axis_stride,
+                                           void* out_query, int64_t out_query_stride, void* out_key,
+                                           int64_t out_key_stride, const TQRopeAxes* axes,
+                                           const TQRopeConfig* rope, const TQConfig* cfg, int num_tokens,
+                                           void* stream) {
+    if (!axes) return -1;
+    return tq::norm_rope_entry("qk_norm_rope_axes", query, query_stride, key, key_stride, q_weight, k_weight,
+                               cos_sin, positions, axis_stride, out_query, out_query_stride, out_key,
+                               out_key_stride, axes, rope, cfg, num_tokens, stream);
+}
+
+extern "C" int tq_launch_dense_rope_append_kv(
+    const void* query, int64_t query_stride, const void* key, int64_t key_stride, const void* value,
+    int64_t value_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
+    const int32_t* positions, const int32_t* slot_mapping, uint8_t* page_pool, void* out_query,
+    int64_t out_query_stride, const TQDensePageLayout* layout, const TQRopeConfig* rope,
+    const TQConfig* cfg, int num_tokens, void* stream) {
+    return tq::rope_append_entry("dense_rope_append_kv", query, query_stride, key, key_stride, value, value_stride,
+                                 q_weight, k_weight, cos_sin, positions, 0, slot_mapping, page_pool, out_query,
+                                 out_query_stride, layout, nullptr, rope, cfg, num_tokens, stream);
+}
+
+extern "C" int tq_launch_dense_rope_axes_append_kv(
+    const void* query, int64_t query_stride, const void* key, int64_t key_stride, const void* value,
+    int64_t value_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
+    const int32_t* positions, int64_t axis_stride, const int32_t* slot_mapping, uint8_t* page_pool,
+    void* out_query, int64_t out_query_stride, const TQDensePageLayout* layout, const TQRopeAxes* axes,
+    const TQRopeConfig* rope, const TQConfig* cfg, int num_tokens, void* stream) {
+    if (!axes) return -1;
+    return tq::rope_append_entry("dense_rope_axes_append_kv", query, query_stride, key, key_stride, value,
+                                 value_stride, q_weight, k_weight, cos_sin, positions, axis_stride, slot_mapping,
+                                 page_pool, out_query, out_query_stride, layout, axes, rope, cfg, num_tokens, stream);
 }

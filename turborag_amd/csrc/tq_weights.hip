@@ -1,0 +1,737 @@
+// tq_weights.hip — softmax weights of query rows on the tokens of paged caches,
+// summed over a kv head's rows: what an eviction by accumulated attention goes by.
+//
+//   out[s][h][t] = decay in[s][h][t] + sum over rows r of 2^(x_rt - M_r) / l_r,
+//   x_rt = log2(e) <q_r, k_t> / sqrt(D), M_r = max over t, l_r = sum of 2^(x_rt - M_r).
+//
+// No value is read.  A weight needs its row's M and l, so the tokens are gone over
+// twice: the first launch takes K's products with the rows and leaves each chunk's
+// (max, sum) of every row; the last one forms the weights and adds them up over the
+// rows, always in the same order and without atomics.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "tq_device.h"
+
+namespace tq {
+namespace {
+
+using namespace dev;
+
+// What the pages hold.
+constexpr int kFp16 = 0, kBf16 = 1, kProd = 2, kMse = 3;
+
+struct WeightArgs {
+    const uint16_t* query;
+    const uint8_t* pool;
+    const int32_t *tables, *row_start, *prefix;
+    const float* in;  // null: nothing is added to
+    float* out;
+    int64_t stride;  // of in and out, from one head's scores to the next
+    float decay;
+    PageGeom g;  // dense pages: kc_off and code_stride of fp16/bf16 rows
+    int max_blocks, hq, group, seqs, tokens, max_kv, causal;  // group: query heads per kv head
+    // The workspace.  A row's index is that of its query: token * hq + query head.
+    int chunks;             // of every sequence
+    float* logits;          // [rows][logit_stride]: x, or null
+    int64_t logit_stride;
+    float2* part;           // [chunks][rows]: (max, sum) of a chunk
+    float2* stat;           // [rows]: (M, 1 / l)
+    const uint16_t* turned;  // [rows][2 D]: q rotated, hi and lo (compressed pages)
+    const float* turned_scale;  // [rows]
+};
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// C += A B, A [16 x 32] by rows, B [32 x 16] by columns: lane l holds row
+// (column) l % 16, k = 8 (l / 16) + 0..7; of C column l % 16, rows
+// 4 (l / 16) + 0..3.
+template <bool BF>
+__device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0,
+                                                       0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0,
+                                                      0);
+}
+
+// A sequence's rows and tokens, as far as the call's bounds allow.
+struct Seq {
+    int row0, rows, L, end;  // first token row, token rows, prefix, tokens that some row may see
+};
+__device__ __forceinline__ Seq seq_of(const WeightArgs& a, int s) {
+    Seq q;
+    q.row0 = min(max(a.row_start[s], 0), a.tokens);
+    q.rows = max(min(a.row_start[s + 1], a.tokens) - q.row0, 0);
+    q.L = min(max(a.prefix[s], 0), a.max_kv);
+    q.end = min(q.L + (a.causal ? q.rows : 0), a.max_kv);
+    return q;
+}
+
+// ---------------------------------------------------------------------------
+// Codes -> fp16 operands.  A code's fp16 value is looked up byte by byte: v_perm_b32
+// takes four bytes by four selectors out of an 8-entry table in two registers (no LDS:
+// four lookups an instruction).  The eight codes of a dword come out as dims 0 2 | 4 6 |
+// 1 3 | 5 7, the order that the rotated queries are stored in.
+// ---------------------------------------------------------------------------
+struct Bytes8 {
+    uint32_t a, b;  // entries 0..3, 4..7
+};
+struct Halves8 {
+    Bytes8 lo, hi;  // low and high bytes of eight fp16 values
+};
+constexpr uint16_t half_bits(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+constexpr float half_rest(float x) { return x - (float)(_Float16)x; }
+template <class F>
+constexpr Halves8 halves8(F f) {
+    Halves8 r{};
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t v = half_bits(f(k));
+        (k < 4 ? r.lo.a : r.lo.b) |= (v & 255) << (8 * (k & 3));
+        (k < 4 ? r.hi.a : r.hi.b) |= (v >> 8) << (8 * (k & 3));
+    }
+    return r;
+}
+constexpr float k3_at(int k) { return kK3[k]; }
+constexpr float k3_rest(int k) { return half_rest(kK3[k]); }
+constexpr float v4_at(int k) { return kV4[8 + k]; }  // the upper half: V4[15 - c] = -V4[c]
+constexpr float v4_rest(int k) { return half_rest(kV4[8 + k]); }
+constexpr bool v4_symmetric() {
+    for (int k = 0; k < 8; ++k)
+        if (kV4[7 - k] != -kV4[8 + k]) return false;
+    return true;
+}
+static_assert(v4_symmetric(), "a code's value is +- that of its mirror");
+
+__device__ __forceinline__ uint32_t look(const Bytes8& t, uint32_t sel) {
+    return __builtin_amdgcn_perm(t.b, t.a, sel);
+}
+// Byte planes -> fp16 pairs of bytes 0 1 and 2 3.
+__device__ __forceinline__ uint32_t pair01(uint32_t hi, uint32_t lo) {
+    return __builtin_amdgcn_perm(hi, lo, 0x05010400u);
+}
+__device__ __forceinline__ uint32_t pair23(uint32_t hi, uint32_t lo) {
+    return __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+}
+
+// turbo_prod: K3 level in two fp16 parts, and the residual's sign as +-1.
+struct KeyParts {
+    u4 hi, lo, sign;
+};
+template <int FMT>
+__device__ __forceinline__ KeyParts decode8(uint32_t w) {
+    KeyParts r;
+    if constexpr (FMT == kProd) {
+        constexpr Halves8 H = halves8(k3_at), R = halves8(k3_rest);
+        const uint32_t e = w & 0x07070707u, o = w >> 4 & 0x07070707u;
+        const uint32_t eh = look(H.hi, e), el = look(H.lo, e), oh = look(H.hi, o), ol = look(H.lo, o);
+        r.hi = u4{pair01(eh, el), pair23(eh, el), pair01(oh, ol), pair23(oh, ol)};
+        const uint32_t fh = look(R.hi, e), fl = look(R.lo, e), ph = look(R.hi, o), pl = look(R.lo, o);
+        r.lo = u4{pair01(fh, fl), pair23(fh, fl), pair01(ph, pl), pair23(ph, pl)};
+        // (bit 3 set: added; 0xbc00 is -1)
+        const uint32_t se = (w << 4 & 0x80808080u) ^ 0xbcbcbcbcu, so = (w & 0x80808080u) ^ 0xbcbcbcbcu;
+        const auto wide01 = [](uint32_t p) { return __builtin_amdgcn_perm(p, p, 0x010c000cu); };
+        const auto wide23 = [](uint32_t p) { return __builtin_amdgcn_perm(p, p, 0x030c020cu); };
+        r.sign = u4{wide01(se), wide23(se), wide01(so), wide23(so)};
+    } else {
+        constexpr Halves8 H = halves8(v4_at), R = halves8(v4_rest);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t n = (k ? w >> 4 : w) & 0x0f0f0f0fu;
+            const uint32_t below = ~n & 0x08080808u, minus = below << 4;
+            const uint32_t m = (n ^ (below - (below >> 3))) & 0x07070707u;  // of the upper half
+            const uint32_t hh = look(H.hi, m) | minus, hl = look(H.lo, m);
+            const uint32_t rh = look(R.hi, m) ^ minus, rl = look(R.lo, m);
+            r.hi[2 * k] = pair01(hh, hl);
+            r.hi[2 * k + 1] = pair23(hh, hl);
+            r.lo[2 * k] = pair01(rh, rl);
+            r.lo[2 * k + 1] = pair23(rh, rl);
+        }
+    }
+    return r;
+}
+
+// ---------------------------------------------------------------------------
+// Queries of compressed pages: q's rotation H (q s) in two fp16 parts, brought by a
+// power of two to a largest value in [2^13, 2^14) (22 bits of it are kept and no row
+// leaves fp16's range); D / 8 lanes a row, eight dims each.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(256) void turn_queries_kernel(const uint16_t* __restrict__ query, int hq, int group,
+                                                           int rows, uint16_t* __restrict__ turned,
+                                                           float* __restrict__ turned_scale, float scale) {
+    constexpr int L = D / 8;
+    const int j = threadIdx.x % L, at = blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int row = min(at, rows - 1), h = row % hq / group;
+    const u4 raw = *reinterpret_cast<const u4*>(query + (size_t)row * D + 8 * j);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = h2f(raw[e / 2] >> (16 * (e & 1)) & 0xffff) * sign_of(e, h);
+#pragma unroll
+    for (int m = 1; m < 8; m <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (!(e & m)) {
+                const float u = x[e], v = x[e | m];
+                x[e] = u + v;
+                x[e | m] = u - v;
+            }
+#pragma unroll
+    for (int m = 1; m < L; m <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float o = xor_lane(x[e], m);
+            x[e] = j & m ? o - x[e] : x[e] + o;
+        }
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+    top = max_lanes<L>(top);
+    const int ex = (int)(__float_as_uint(top) >> 23) - 127;
+    const int sh = top > 0.0f && ex < 128 ? 13 - max(ex, -100) : 0;
+    const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+    if (at != row) return;
+    u4 hi, lo;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {  // dims 0 2 | 4 6 | 1 3 | 5 7
+        const int d = (p & 1) * 4 + (p >> 1);
+        const float u = x[d] * up, v = x[d + 2] * up;
+        hi[p] = f2h2(u, v);
+        lo[p] = f2h2(u - h2f(hi[p] & 0xffff), v - h2f(hi[p] >> 16));
+    }
+    *reinterpret_cast<u4*>(turned + (size_t)row * 2 * D + 8 * j) = hi;
+    *reinterpret_cast<u4*>(turned + (size_t)row * 2 * D + D + 8 * j) = lo;
+    if (j == 0) turned_scale[row] = scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+}
+
+// ---------------------------------------------------------------------------
+// The passes over K.  A workgroup has one kv head and a chunk of C tokens of one
+// sequence, T of them a wave; K's operands stay in registers while the rows go by
+// in tiles of 16.  The products run transposed (K Q'): a query row is a lane column,
+// so its maximum and sum are in-lane but for two lane swaps, and a token's sum over
+// the rows is in-lane over the tiles, across 16 lanes once at the end.
+//   kStats: (max, sum) of the chunk for every row;  kStore: x too;
+//   kSum: the weights, summed over the rows.
+// ---------------------------------------------------------------------------
+constexpr int kStats = 0, kStore = 1, kSum = 2;
+constexpr int kRowBlock = 256;  // rows whose statistics lie in LDS at a time
+
+// Tokens of a wave: 16 TT.  (Compressed pages: three operands a token tile.)
+template <int FMT>
+constexpr int kTT = FMT == kProd || FMT == kMse ? 2 : 4;
+
+template <int FMT, int D, int MODE>
+__global__ __launch_bounds__(256) void weights_kernel(const WeightArgs a, float scale) {
+    constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
+    constexpr int TT = kTT<FMT>, T = 16 * TT, C = 4 * T, KK = D / 32;
+    __shared__ float2 ml[MODE == kSum ? 1 : 4][MODE == kSum ? 1 : kRowBlock];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, gq = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PageGeom& g = a.g;
+
+    // Eight chunks in turn, then the same ones of the next head: the workgroups of one
+    // chunk run on one XCD, whose L2 then holds the lines that the heads share.
+    const unsigned b = blockIdx.y * gridDim.x + blockIdx.x, eight = b / 8;
+    const int h = (int)(eight % (unsigned)g.H);
+    const long long sc = (long long)(eight / (unsigned)g.H) * 8 + b % 8;
+    if (sc >= (long long)a.seqs * a.chunks) return;
+    const int s = (int)(sc / a.chunks), c = (int)(sc - (long long)s * a.chunks);
+    const Seq q = seq_of(a, s);
+    if (c * C >= q.end) return;
+    const int R = q.rows * a.group, t0 = c * C + wv * T;
+    if (R == 0) {  // (no row and, without any in the call, no query)
+        const int64_t at = ((int64_t)s * g.H + h) * a.stride;
+        if (MODE == kSum)
+            for (int t = c * C + tid; t < min(c * C + C, q.end); t += 256)
+                a.out[at + t] = a.in ? a.decay * a.in[at + t] : 0.0f;
+        return;
+    }
+
+    // K's rows: lane (i, gq) has token i of each tile.
+    const uint64_t dummy = (uint64_t)(reinterpret_cast<uintptr_t>(a.query) - reinterpret_cast<uintptr_t>(a.pool));
+    const int32_t* __restrict__ table = a.tables + (size_t)s * a.max_blocks;
+    int id[TT], tib[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int t = min(t0 + tt * 16 + i, q.end - 1);
+        const int pg = g.bs_shift >= 0 ? t >> g.bs_shift : t / g.block_size;
+        tib[tt] = t - pg * g.block_size;
+        id[tt] = table[pg];
+    }
+    u4 k[TT][KK];                  // dense: operands
+    typedef uint32_t code_t __attribute__((ext_vector_type(KK), aligned(2)));
+    code_t code[TT];               // compressed: a quarter of a token's codes
+    uint32_t scales[TT];           // its RMS, its residual's RMS above
+    uint32_t live[TT];             // tokens of the tile that can be read (bits)
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const bool ok = t0 + tt * 16 + i < q.end && id[tt] >= 0;
+        live[tt] = (uint32_t)__ballot(ok) & 0xffffu;
+        const uint64_t page = (uint64_t)max(id[tt], 0) * g.page_size;
+        const uint64_t cell = (uint64_t)(tib[tt] * g.H + h);
+        if constexpr (!kTurned) {
+            const uint8_t* p = a.pool + (ok ? page + g.kc_off + cell * (2 * D) : dummy) + gq * 16;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) k[tt][kk] = *reinterpret_cast<const u4*>(p + kk * 64);
+        } else {
+            code[tt] = *reinterpret_cast<const code_t*>(
+                a.pool + (ok ? page + g.kc_off + cell * (D / 2) : dummy) + gq * (D / 8));
+            scales[tt] = ld_u16(a.pool + (ok ? page + g.ks_off + cell * 2 : dummy));
+            if (FMT == kProd) scales[tt] |= (uint32_t)ld_u16(a.pool + (ok ? page + g.kres_off + cell * 2 : dummy)) << 16;
+        }
+    }
+    KeyParts kp[kTurned ? TT : 1][KK];
+    float ks[kTurned ? TT : 1][4], kr[kTurned ? TT : 1][4];  // of the tokens 4 gq + 0..3
+    if constexpr (kTurned) {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) kp[tt][kk] = decode8<FMT>(code[tt][kk]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t w = (uint32_t)__shfl((int)scales[tt], 4 * gq + r, 64);
+                ks[tt][r] = h2f(w & 0xffff);
+                kr[tt][r] = FMT == kProd ? h2f(w >> 16) : 0.0f;
+            }
+        }
+    }
+    // Every row sees every token of the wave.
+    uint32_t all = 0xffffu;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) all &= live[tt];
+    const bool plain = all == 0xffffu && t0 + T <= q.L;
+
+    float acc[TT][4];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[tt][r] = 0.0f;
+
+    for (int rb = 0; rb < R; rb += kRowBlock) {
+        const int upto = min(R, rb + kRowBlock);
+        for (int r0 = rb; r0 < upto; r0 += 16) {
+            const int row = min(r0 + i, R - 1), tok = row / a.group;
+            const size_t nat = (size_t)(q.row0 + tok) * a.hq + h * a.group + (row - tok * a.group);
+            f4 x[TT], y[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) x[tt] = y[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            float row_scale = scale;
+            if constexpr (!kTurned) {
+                u4 qf[KK];
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+                    qf[kk] = *reinterpret_cast<const u4*>(a.query + nat * D + kk * 32 + gq * 8);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<BF>(k[tt][kk], qf[kk], x[tt]);
+            } else {
+                u4 qh[KK], ql[KK];
+                const uint16_t* p = a.turned + nat * 2 * D + gq * (D / 4);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    qh[kk] = *reinterpret_cast<const u4*>(p + kk * 8);
+                    ql[kk] = *reinterpret_cast<const u4*>(p + D + kk * 8);
+                }
+                row_scale = a.turned_scale[nat];
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, qh[kk], x[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+                        if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, qh[kk], y[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, ql[kk], x[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+                        if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, ql[kk], y[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].lo, qh[kk], x[tt]);
+                }
+            }
+            // x in powers of two; what the row does not see: -infinity.
+            const int limit = min(q.L + (a.causal ? tok + 1 : 0), a.max_kv);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = x[tt][r];
+                    if constexpr (kTurned) {
+                        if (FMT == kProd) v = fmaf(kr[tt][r], y[tt][r], v);
+                        v *= ks[tt][r];
+                    }
+                    x[tt][r] = v * row_scale;
+                }
+            if (!plain) {
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int t = tt * 16 + 4 * gq + r;
+                        if (t0 + t >= limit || !(live[tt] >> (4 * gq + r) & 1)) x[tt][r] = -INFINITY;
+                    }
+            }
+            if constexpr (MODE == kSum) {
+                float2 st = a.stat[nat];
+                if (r0 + i >= R) st = make_float2(INFINITY, 0.0f);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[tt][r] = fmaf(exp2_hw(x[tt][r] - st.x), st.y, acc[tt][r]);
+            } else {
+                float m = -INFINITY;
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) m = fmaxf(m, x[tt][r]);
+                const auto larger = [](float u, float w) { return fmaxf(u, w); };
+                m = lane_xor_reduce<32>(lane_xor_reduce<16>(m, larger), larger);
+                const float ref = m == -INFINITY ? 0.0f : m;
+                float l = 0.0f;
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) l += exp2_hw(x[tt][r] - ref);
+                const auto sum = [](float u, float w) { return u + w; };
+                l = lane_xor_reduce<32>(lane_xor_reduce<16>(l, sum), sum);
+                if (gq == 0) ml[wv][r0 - rb + i] = make_float2(m, l);
+                if constexpr (MODE == kStore) {
+                    if (r0 + i < R) {
+                        float* to = a.logits + (int64_t)nat * a.logit_stride + t0 + 4 * gq;
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f4*>(to + tt * 16) = x[tt];
+                    }
+                }
+            }
+        }
+        if constexpr (MODE != kSum) {
+            __syncthreads();
+            for (int r = rb + tid; r < upto; r += 256) {
+                const int tok = r / a.group;
+                const size_t nat = (size_t)(q.row0 + tok) * a.hq + h * a.group + (r - tok * a.group);
+                float m = -INFINITY, l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][r - rb].x);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float2 e = ml[w][r - rb];
+                    l += e.x == -INFINITY ? e.y : e.y * exp2_hw(e.x - m);
+                }
+                a.part[(size_t)c * ((size_t)a.tokens * a.hq) + nat] = make_float2(m, l);
+            }
+            __syncthreads();
+        }
+    }
+    if constexpr (MODE == kSum) {
+        const int64_t at = ((int64_t)s * g.H + h) * a.stride;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            float mine = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float w = sum_lanes<16>(acc[tt][r]);
+                mine = i == r ? w : mine;
+            }
+            const int t = t0 + tt * 16 + 4 * gq + i;
+            if (i < 4 && t < q.end) a.out[at + t] = a.in ? fmaf(a.decay, a.in[at + t], mine) : mine;
+        }
+    }
+}
+
+// (max, sum) of a part added to a row's.
+__device__ __forceinline__ void add_part(float& m, float& l, float2 e) {
+    const float n = fmaxf(m, e.x);
+    l = (m == -INFINITY ? l : l * exp2_hw(m - n)) + (e.x == -INFINITY ? e.y : e.y * exp2_hw(e.x - n));
+    m = n;
+}
+// A row's (M, 1 / l); one that sees nothing gives every token 2^-infinity * 0.
+__device__ __forceinline__ float2 row_stat(float m, float l) {
+    return l == 0.0f ? make_float2(INFINITY, 0.0f) : make_float2(m, 1.0f / l);
+}
+
+// The last sequence that begins at or before token row `tok` (those without rows begin
+// where the next one does); a wave together.
+__device__ __forceinline__ int find_seq(const WeightArgs& a, int tok, int lane) {
+    int lo = 0, span = a.seqs;
+    while (span > 1) {
+        const int step = (span + 63) / 64, at = lane * step;
+        const uint64_t low = __ballot(at < span && a.row_start[lo + min(at, span - 1)] <= tok);
+        const int k = max(63 - __clzll((unsigned long long)(low | 1)), 0);
+        lo += k * step;
+        span = min(step, span - k * step);
+    }
+    return lo;
+}
+
+// Chunks -> rows, 16 rows a workgroup and 16 parts of the chunks.  A wave holds rows of up
+// to 16 tokens, which may belong to several sequences.
+template <int FMT>
+__global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
+    constexpr int C = 64 * kTT<FMT>;
+    __shared__ float2 ml[16][16];
+    const int lane = threadIdx.x & 63, i = threadIdx.x & 15, p = threadIdx.x >> 4;
+    const size_t rows = (size_t)a.tokens * a.hq, row = (size_t)blockIdx.x * 16 + i;
+    const int first = (int)((size_t)blockIdx.x * 16 / a.hq), last = (int)(min((size_t)blockIdx.x * 16 + 15, rows - 1) / a.hq);
+    const int tok = (int)(min(row, rows - 1) / a.hq);
+    int n = 0;
+    for (int t = first; t <= last; ++t) {
+        const int s = find_seq(a, t, lane);
+        const Seq q = seq_of(a, s);
+        if (t == tok && t >= q.row0 && t < q.row0 + q.rows) n = (q.end + C - 1) / C;
+    }
+    float m = -INFINITY, l = 0.0f;
+    if (row < rows)
+        for (int c = p; c < n; c += 16) add_part(m, l, a.part[(size_t)c * rows + row]);
+    ml[p][i] = make_float2(m, l);
+    __syncthreads();
+    if (p || row >= rows) return;
+    for (int k = 1; k < 16; ++k) add_part(m, l, ml[k][i]);
+    a.stat[row] = row_stat(m, l);
+}
+
+// The weights of stored x: 1,024 tokens of one kv head a workgroup.
+constexpr int kSumTokens = 1024;
+template <int FMT>
+__global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
+    constexpr int C = 64 * kTT<FMT>;
+    __shared__ float2 st[16];
+    const int tid = threadIdx.x, i = tid & 15, p = tid >> 4;
+    const int blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
+    const unsigned b = blockIdx.y * gridDim.x + blockIdx.x;
+    const int sh = (int)(b / (unsigned)blocks), blk = (int)(b % (unsigned)blocks);
+    const int s = sh / a.g.H, h = sh - s * a.g.H;
+    if (s >= a.seqs) return;
+    const Seq q = seq_of(a, s);
+    if (blk * kSumTokens >= q.end) return;
+    const int R = q.rows * a.group, n = (q.end + C - 1) / C, t = blk * kSumTokens + tid * 4;
+    const size_t rows = (size_t)a.tokens * a.hq;
+    const bool inside = t < n * C;  // (x is there up to the end of the last chunk)
+    f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r0 = 0; r0 < R; r0 += 16) {
+        const int upto = min(16, R - r0);
+        const auto nat_of = [&](int r) {
+            const int tok = r / a.group;
+            return (size_t)(q.row0 + tok) * a.hq + h * a.group + (r - tok * a.group);
+        };
+        // statistics: 16 lanes a row
+        if (r0) __syncthreads();
+        float m = -INFINITY, l = 0.0f;
+        if (p < upto) {
+            const size_t nat = nat_of(r0 + p);
+            for (int c = i; c < n; c += 16) add_part(m, l, a.part[(size_t)c * rows + nat]);
+        }
+#pragma unroll
+        for (int k = 1; k < 16; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
+        if (i == 0 && p < upto) st[p] = row_stat(m, l);
+        __syncthreads();
+        if (inside)
+            for (int r = 0; r < upto; ++r) {
+                const f4 x = *reinterpret_cast<const f4*>(a.logits + (int64_t)nat_of(r0 + r) * a.logit_stride + t);
+                const float2 e = st[r];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = fmaf(exp2_hw(x[k] - e.x), e.y, acc[k]);
+            }
+    }
+    const int64_t at = (int64_t)sh * a.stride + t;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (t + k < q.end) a.out[at + k] = a.in ? fmaf(a.decay, a.in[at + k], acc[k]) : acc[k];
+}
+
+dim3 grid_of(long long blocks) {
+    const unsigned x = (unsigned)std::min<long long>(blocks, 1 << 23);
+    return dim3(x, (unsigned)((blocks + x - 1) / x));
+}
+
+template <int FMT, int D>
+void launch_format(WeightArgs a, hipStream_t stream) {
+    constexpr bool kTurned = FMT == kProd || FMT == kMse;
+    constexpr int C = 64 * kTT<FMT>;
+    const size_t rows = (size_t)a.tokens * a.hq;
+    a.chunks = (a.max_kv + C - 1) / C;
+    a.logit_stride = (int64_t)a.chunks * C;
+    // x is stored where that moves fewer bytes than K's second reading.
+    const long long per_seq = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
+    const bool store = per_seq <= 32 && rows * (size_t)a.logit_stride * 4 <= (size_t(256) << 20);
+    const auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+    const size_t parts = up((size_t)a.chunks * rows * sizeof(float2));
+    const size_t second = store ? up(rows * (size_t)a.logit_stride * 4) : up(rows * sizeof(float2));
+    const size_t turned = kTurned ? up(rows * 4 * D) : 0, scales = kTurned ? up(rows * 4) : 0;
+    const WorkspaceTurn turn(stream);
+    uint8_t* ws = static_cast<uint8_t*>(Scratch{}.get(stream, parts + second + turned + scales, "attention weights"));
+    a.part = reinterpret_cast<float2*>(ws);
+    a.logits = reinterpret_cast<float*>(ws + parts);
+    a.stat = reinterpret_cast<float2*>(ws + parts);
+    a.turned = reinterpret_cast<uint16_t*>(ws + parts + second);
+    a.turned_scale = reinterpret_cast<float*>(ws + parts + second + turned);
+    const float scale = 1.44269504f * inv_sqrt_d(D);
+    if (kTurned && rows) {
+        constexpr int per = 256 / (D / 8);
+        hipLaunchKernelGGL(turn_queries_kernel<D>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a.query,
+                           a.hq, a.group, (int)rows, const_cast<uint16_t*>(a.turned),
+                           const_cast<float*>(a.turned_scale), scale * inv_sqrt_d(D));
+        check_launch("attention_weights_turn_kernel");
+    }
+    const dim3 grid = grid_of(((long long)a.seqs * a.chunks + 7) / 8 * 8 * a.g.H);
+    if (store) {
+        if (rows) hipLaunchKernelGGL((weights_kernel<FMT, D, kStore>), grid, dim3(256), 0, stream, a, scale);
+        check_launch("attention_weights_kernel");
+        const long long blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
+        hipLaunchKernelGGL(weights_sum_kernel<FMT>, grid_of(blocks * a.seqs * a.g.H), dim3(256), 0, stream, a);
+        check_launch("attention_weights_sum_kernel");
+        return;
+    }
+    hipLaunchKernelGGL((weights_kernel<FMT, D, kStats>), grid, dim3(256), 0, stream, a, scale);
+    check_launch("attention_weights_kernel");
+    hipLaunchKernelGGL(weights_rows_kernel<FMT>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, a);
+    check_launch("attention_weights_rows_kernel");
+    hipLaunchKernelGGL((weights_kernel<FMT, D, kSum>), grid, dim3(256), 0, stream, a, scale);
+    check_launch("attention_weights_sum_kernel");
+}
+
+bool aligned(uint64_t v, uint64_t a) { return (v & (a - 1)) == 0; }
+bool aligned(const void* p, uint64_t a) { return aligned(reinterpret_cast<uintptr_t>(p), a); }
+
+PageGeom dense_rows(const TQConfig& cfg, const TQDensePageLayout& l) {
+    const DenseGeom d = dense_geom(cfg, l);
+    PageGeom g{};
+    g.page_size = d.page_size;
+    g.kc_off = d.k_off;
+    g.vc_off = d.v_off;
+    g.code_stride = 2 * d.D;
+    g.H = d.H;
+    g.D = d.D;
+    g.block_size = d.block_size;
+    g.bs_shift = (d.block_size & (d.block_size - 1)) == 0 ? __builtin_ctz(d.block_size) : -1;
+    return g;
+}
+
+template <class Geom>
+int weights_entry(const char* name, int fmt, Geom&& geom, const void* query, const uint8_t* pool,
+                  const int32_t* tables, int max_blocks, const int32_t* row_start, const int32_t* prefix,
+                  int causal, const float* in, float* out, int64_t stride, float decay, int hq, int seqs,
+                  int tokens, int max_kv, void* stream) {
+    if ((!query && tokens) || !pool || !tables || !row_start || !prefix || !out) return -1;
+    try {
+        const std::string w = std::string(name) + ": ";
+        WeightArgs a{};
+        a.g = geom();
+        const PageGeom& g = a.g;
+        if (g.D != 64 && g.D != 128) throw Error(w + "head_dim must be 64 or 128");
+        if (hq <= 0 || hq % g.H || hq > 65535)
+            throw Error(w + "num_q_heads must be a multiple of num_kv_heads, at most 65535");
+        if (seqs < 0 || tokens < 0) throw Error(w + "num_seqs and num_tokens must be >= 0");
+        if (max_blocks <= 0) throw Error(w + "max_blocks_per_seq must be > 0");
+        if (max_kv < 0 || max_kv > (1 << 30) || (long long)max_blocks * g.block_size < max_kv)
+            throw Error(w + "max_kv_len must be in [0, 2^30] and fit in max_blocks_per_seq pages");
+        if (stride < max_kv || stride >= (int64_t(1) << 40))
+            throw Error(w + "score_stride must be at least max_kv_len");
+        if (!(decay >= 0.0f) || decay > 1.0f) throw Error(w + "decay must be in [0, 1]");
+        if ((long long)tokens * hq > (1LL << 26)) throw Error(w + "num_tokens * num_q_heads must be at most 2^26");
+        const long long chunks = (max_kv + 127) / 128;
+        if (chunks * std::max<long long>((long long)tokens * hq, (long long)seqs * g.H) > (1LL << 30))
+            throw Error(w + "too many (row, 128 tokens) or (sequence, kv head, 128 tokens) pairs (2^30)");
+        const uint64_t cells = (uint64_t)g.block_size * g.H;
+        const auto outside = [&](uint64_t off, uint64_t size) {
+            return off > g.page_size || cells * size > g.page_size - off;
+        };
+        if (outside(g.kc_off, g.code_stride) ||
+            (fmt > kBf16 && (outside(g.ks_off, 2) || (fmt == kProd && outside(g.kres_off, 2)))))
+            throw Error(w + "layout does not match cfg (a region ends past the page)");
+        const uint64_t al = fmt <= kBf16 ? 16 : 2;
+        if (!aligned(pool, al) || !aligned(g.page_size | g.kc_off, al) || !aligned(g.ks_off | g.kres_off, 2))
+            throw Error(w + (al == 16 ? "page_pool, page size and offsets must be 16-byte aligned"
+                                      : "page_pool, page size and offsets must be 2-byte aligned"));
+        if (!aligned(query, 16)) throw Error(w + "query must be 16-byte aligned");
+        if (!aligned(in, 4) || !aligned(out, 4)) throw Error(w + "scores must be 4-byte aligned");
+        if (seqs == 0 || max_kv == 0) return 0;
+        a.query = static_cast<const uint16_t*>(query);
+        a.pool = pool;
+        a.tables = tables;
+        a.row_start = row_start;
+        a.prefix = prefix;
+        a.in = decay == 0.0f ? nullptr : in;
+        a.out = out;
+        a.stride = stride;
+        a.decay = decay;
+        a.max_blocks = max_blocks;
+        a.hq = hq;
+        a.group = hq / g.H;
+        a.seqs = seqs;
+        a.tokens = tokens;
+        a.max_kv = max_kv;
+        a.causal = causal != 0;
+        const hipStream_t st = static_cast<hipStream_t>(stream);
+        const auto go = [&](auto f) {
+            constexpr int F = decltype(f)::value;
+            g.D == 128 ? launch_format<F, 128>(a, st) : launch_format<F, 64>(a, st);
+        };
+        switch (fmt) {
+            case kFp16: go(std::integral_constant<int, kFp16>{}); break;
+            case kBf16: go(std::integral_constant<int, kBf16>{}); break;
+            case kProd: go(std::integral_constant<int, kProd>{}); break;
+            default: go(std::integral_constant<int, kMse>{});
+        }
+        debug_sync(stream);
+        return 0;
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return -2;
+    } catch (...) {
+        set_last_error("unknown error");
+        return -2;
+    }
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int tq_launch_dense_attention_weights(
+    const void* query, const uint8_t* page_pool, const int32_t* block_tables, int max_blocks_per_seq,
+    const int32_t* row_start, const int32_t* prefix_len, int causal, const float* scores_in, float* scores_out,
+    int64_t score_stride, float decay, const TQDensePageLayout* layout, const TQConfig* cfg, int dtype,
+    int num_q_heads, int num_seqs, int num_tokens, int max_kv_len, void* stream) {
+    if (!layout || !cfg) return -1;
+    return tq::weights_entry(
+        "dense_attention_weights", dtype == TQ_DTYPE_BF16 ? tq::kBf16 : tq::kFp16,
+        [&] {
+            if (dtype != TQ_DTYPE_FP16 && dtype != TQ_DTYPE_BF16)
+                throw tq::Error("dense_attention_weights: dtype must be TQ_DTYPE_FP16 or TQ_DTYPE_BF16");
+            return tq::dense_rows(*cfg, *layout);
+        },
+        query, page_pool, block_tables, max_blocks_per_seq, row_start, prefix_len, causal, scores_in, scores_out,
+        score_stride, decay, num_q_heads, num_seqs, num_tokens, max_kv_len, stream);
+}
+
+extern "C" int tq_launch_turbo_prod_attention_weights(
+    const uint16_t* query, const uint8_t* page_pool, const int32_t* block_tables, int max_blocks_per_seq,
+    const int32_t* row_start, const int32_t* prefix_len, int causal, const float* scores_in, float* scores_out,
+    int64_t score_stride, float decay, const TQTurboProdPageLayout* layout, const TQConfig* cfg,
+    int num_q_heads, int num_seqs, int num_tokens, int max_kv_len, void* stream) {
+    if (!layout || !cfg) return -1;
+    return tq::weights_entry(
+        "turbo_prod_attention_weights", tq::kProd, [&] { return tq::prod_geom(*cfg, *layout); }, query, page_pool,
+        block_tables, max_blocks_per_seq, row_start, prefix_len, causal, scores_in, scores_out, score_stride, decay,
+        num_q_heads, num_seqs, num_tokens, max_kv_len, stream);
+}
+
+extern "C" int tq_launch_turbo_mse_attention_weights(
+    const uint16_t* query, const uint8_t* page_pool, const int32_t* block_tables, int max_blocks_per_seq,
+    const int32_t* row_start, const int32_t* prefix_len, int causal, const float* scores_in, float* scores_out,
+    int64_t score_stride, float decay, const TQTurbomsePageLayout* layout, const TQConfig* cfg, int num_q_heads,
+    int num_seqs, int num_tokens, int max_kv_len, void* stream) {
+    if (!layout || !cfg) return -1;
+    return tq::weights_entry(
+        "turbo_mse_attention_weights", tq::kMse, [&] { return tq::mse_geom(*cfg, *layout); }, query, page_pool,
+        block_tables, max_blocks_per_seq, row_start, prefix_len, causal, scores_in, scores_out, score_stride, decay,
+        num_q_heads, num_seqs, num_tokens, max_kv_len, stream);
+}

@@ -108,6 +108,12 @@ class TQRopeConfig(ctypes.Structure):
     ]
 
 
+class TQRopeAxes(ctypes.Structure):
+    """include/turboquant.h: the axes of several-axis positions (rope_axes makes one)."""
+
+    _fields_ = [("num_axes", c_int), ("axis", ctypes.c_uint8 * 64)]
+
+
 class TQStoreFormat(ctypes.Structure):
     """Format record of the on-disk store (.bin footer, .meta keys)."""
 
@@ -126,6 +132,8 @@ class TQStoreFormat(ctypes.Structure):
 # Every exported symbol and its ctypes signature (argtypes, restype).
 _P = POINTER
 _I64 = ctypes.c_int64
+_LAYOUTS = {"dense": TQDensePageLayout, "turbo_prod": TQTurboProdPageLayout,
+            "turbo_mse": TQTurbomsePageLayout}
 SIGNATURES: dict[str, tuple[list, object]] = {
     "tq_last_error": ([], ctypes.c_char_p),
     "tq_workspace_release": ([], c_int),
@@ -210,6 +218,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "tq_block_table_num_tokens": ([c_void_p, c_int32, _P(c_int)], c_int),
     "tq_block_table_blocks": ([c_void_p, c_int32, _P(c_int32), c_int, _P(c_int)], c_int),
     "tq_block_table_free_sequence": ([c_void_p, c_int32], c_int),
+    "tq_block_table_truncate": ([c_void_p, c_int32, c_int], c_int),
     # the reference's unexported kernels: QJL-1b, legacy INT4, dense, SDPA reference
     "tq_make_qjl_layout": ([_P(TQConfig), _P(TQQJLPageLayout)], c_int),
     "tq_launch_qjl_pack_kv": ([c_void_p, c_void_p, _P(c_int32), _P(c_uint8), _P(TQQJLPageLayout),
@@ -251,6 +260,28 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                                             _P(c_int32), _P(c_int32), _P(c_int32), c_int,
                                             c_void_p, _P(TQTurbomsePageLayout), _P(TQConfig),
                                             c_int, c_int, c_int, c_int, c_void_p], c_int),
+    # positions with several axes
+    "tq_launch_qk_norm_rope_axes": ([c_void_p, _I64, c_void_p, _I64, c_void_p, c_void_p,
+                                     _P(c_float), _P(c_int32), _I64, c_void_p, _I64, c_void_p,
+                                     _I64, _P(TQRopeAxes), _P(TQRopeConfig), _P(TQConfig), c_int,
+                                     c_void_p], c_int),
+    "tq_launch_dense_rope_axes_append_kv": ([c_void_p, _I64, c_void_p, _I64, c_void_p, _I64,
+                                             c_void_p, c_void_p, _P(c_float), _P(c_int32), _I64,
+                                             _P(c_int32), _P(c_uint8), c_void_p, _I64,
+                                             _P(TQDensePageLayout), _P(TQRopeAxes),
+                                             _P(TQRopeConfig), _P(TQConfig), c_int, c_void_p],
+                                            c_int),
+    # eviction: attention weights, selection, compaction
+    **{f"tq_launch_{scheme}_attention_weights": (
+        [c_void_p, _P(c_uint8), _P(c_int32), c_int, _P(c_int32), _P(c_int32), c_int, _P(c_float),
+         _P(c_float), _I64, c_float, _P(layout), _P(TQConfig)]
+        + [c_int] * (5 if scheme == "dense" else 4) + [c_void_p], c_int)
+       for scheme, layout in _LAYOUTS.items()},
+    "tq_launch_select_kv": ([_P(c_float), _I64, _P(c_int32), c_int, c_int, c_int, c_int, c_int, c_int,
+                             _P(c_int32), _P(c_int32), _P(c_float), _I64, c_void_p], c_int),
+    **{f"tq_launch_{scheme}_compact_kv": (
+        [_P(c_uint8), _P(c_int32), c_int, _P(c_int32), c_int, _P(c_int32), c_int, _P(layout),
+         _P(TQConfig), c_int, c_void_p], c_int) for scheme, layout in _LAYOUTS.items()},
     # on-disk store (tq_backend/cag_store.py formats)
     "tq_store_sha256_hex": ([c_void_p, c_size_t, ctypes.c_char_p], c_int),
     "tq_store_key": ([ctypes.c_char_p, c_int, ctypes.c_char_p, ctypes.c_char_p, c_size_t], c_int),
@@ -302,6 +333,25 @@ def rope_table(max_position: int, rot_dim: int, base: float = 10000.0, inv_freq=
             raise ValueError(f"rope_table: inv_freq must hold {rot_dim // 2} values")
     a = torch.arange(max_position, dtype=torch.float64)[:, None] * f
     return torch.cat([a.cos(), a.sin()], 1).to(device=device, dtype=torch.float32)
+
+
+def rope_axes(sections, in_turn: bool = False) -> TQRopeAxes:
+    """The axes of qk_norm_rope and dense_rope_append: sections[x] pairs of a
+    head's dims turn by the position on axis x (their sum is half of the rotated
+    part).  The pairs lie in blocks, an axis behind the other, or (in_turn) are
+    dealt in turn to the axes that have some left."""
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= 4 or min(left) < 0 or not 1 <= sum(left) <= 64:
+        raise ValueError("rope_axes: 1 to 4 sections of together 1 to 64 pairs")
+    if in_turn:
+        most = max(left)
+        pairs = [x for k in range(most) for x, n in enumerate(left) if k < n]
+    else:
+        pairs = [x for x, n in enumerate(left) for _ in range(n)]
+    axes = TQRopeAxes(num_axes=len(left))
+    axes.axis[:len(pairs)] = pairs
+    axes.pairs = len(pairs)
+    return axes
 
 
 def tree_mask_from_parents(parents) -> torch.Tensor:
@@ -361,6 +411,8 @@ class TurboQuantWrapper:
         self._tree = {"dense": self._fast.tq_launch_dense_tree_attention,
                       "turbo_prod": self._fast.tq_launch_turbo_prod_tree_attention,
                       "turbo_mse": self._fast.tq_launch_turbo_mse_tree_attention}
+        self._weights = {n: getattr(self._fast, f"tq_launch_{n}_attention_weights") for n in _LAYOUTS}
+        self._compact = {n: getattr(self._fast, f"tq_launch_{n}_compact_kv") for n in _LAYOUTS}
         self._rope_configs: dict[tuple, TQRopeConfig] = {}
 
     def _bind_symbols(self) -> None:
@@ -765,7 +817,7 @@ class TurboQuantWrapper:
         raise ValueError(f"{scheme} {op}: the current device is not the tensors', GPU {dev}")
 
     def _rope(self, scheme, op, query, key, value, positions, cos_sin, out_query, out_key, slots,
-              page_pool, cfg, q_weight, k_weight, eps, interleaved):
+              page_pool, cfg, q_weight, k_weight, eps, interleaved, axes=None):
         """The rotation entries' checks; (TQRopeConfig, tokens)."""
         try:
             (N, _, _), (max_position, rot_dim) = key.shape, cos_sin.shape
@@ -782,6 +834,15 @@ class TurboQuantWrapper:
         if query is not None:
             rows += (query, (N, Hq, D)), (out_query, (N, Hq, D))
         wants = [(positions, torch.int32, N), (cos_sin, torch.float32, 0)]
+        if axes is not None:
+            try:
+                fits = positions.shape == (axes.num_axes, N) and 2 * axes.pairs == rot_dim
+            except AttributeError:
+                fits = False
+            if not fits:
+                raise ValueError(f"{scheme} {op}: positions must be [axes, {N}], and axes rope_axes's of "
+                                 f"{rot_dim // 2} pairs")
+            wants[0] = (positions, torch.int32, 0)
         if q_weight is not None:
             wants.append((q_weight, dtype, D))
         if k_weight is not None:
@@ -804,30 +865,41 @@ class TurboQuantWrapper:
 
     def qk_norm_rope(self, query, key, positions, cos_sin, out_query, out_key, cfg, q_weight=None,
                      k_weight=None, eps: float = 1e-6, interleaved: bool = False,
-                     stream: int = 0) -> None:
+                     stream: int = 0, axes: TQRopeAxes | None = None) -> None:
         """Per-head RMS norm (where a weight [D] is given) and rotation of query
         [N, Hq, D] and key [N, H, D] (fp16 or bf16; views of a fused projection
         allowed) at the tokens' positions, into out_query and out_key (which may
         be the inputs).  cos_sin: rope_table's; its width is the rotated part of
-        a head.  A token at a position outside the table is skipped."""
+        a head.  A token at a position outside the table is skipped.  With axes
+        (rope_axes's) positions is [axes, N], and every pair of dims turns by the
+        position on its axis."""
         if query is None:
             raise ValueError("rope qk_norm_rope: query must be a tensor of 3 dimensions")
         rope, N = self._rope("rope", "qk_norm_rope", query, key, None, positions, cos_sin, out_query,
-                             out_key, None, None, cfg, q_weight, k_weight, eps, interleaved)
+                             out_key, None, None, cfg, q_weight, k_weight, eps, interleaved, axes)
         if N == 0:
             return
-        rc = self._fast.tq_launch_qk_norm_rope(
-            query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
-            None if q_weight is None else q_weight.data_ptr(),
-            None if k_weight is None else k_weight.data_ptr(), cos_sin.data_ptr(),
-            positions.data_ptr(), out_query.data_ptr(), out_query.stride(0), out_key.data_ptr(),
-            out_key.stride(0), ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
+        qw = None if q_weight is None else q_weight.data_ptr()
+        kw = None if k_weight is None else k_weight.data_ptr()
+        if axes is None:
+            rc = self._fast.tq_launch_qk_norm_rope(
+                query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0), qw, kw,
+                cos_sin.data_ptr(), positions.data_ptr(), out_query.data_ptr(), out_query.stride(0),
+                out_key.data_ptr(), out_key.stride(0), ctypes.byref(rope), ctypes.byref(cfg), N,
+                self._stream(stream))
+        else:
+            rc = self._fast.tq_launch_qk_norm_rope_axes(
+                query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0), qw, kw,
+                cos_sin.data_ptr(), positions.data_ptr(), N, out_query.data_ptr(),
+                out_query.stride(0), out_key.data_ptr(), out_key.stride(0), ctypes.byref(axes),
+                ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
         if rc != 0:
             self._kernel_raise(rc, "rope", "qk_norm_rope")
 
     def dense_rope_append(self, query, key, value, positions, slot_mapping, cos_sin, out_query,
                           page_pool, layout, cfg, q_weight=None, k_weight=None, eps: float = 1e-6,
-                          interleaved: bool = False, stream: int = 0) -> None:
+                          interleaved: bool = False, stream: int = 0,
+                          axes: TQRopeAxes | None = None) -> None:
         """qk_norm_rope with the rotated keys, and the values as they are, written
         into the dense pages named by slot_mapping (pages of key's dtype); query
         and out_query may both be None.  A negative slot stores nothing."""
@@ -836,18 +908,27 @@ class TurboQuantWrapper:
         if slot_mapping is None:
             raise ValueError("dense rope_append: slot_mapping must be a GPU tensor")
         rope, N = self._rope("dense", "rope_append", query, key, value, positions, cos_sin, out_query,
-                             None, slot_mapping, page_pool, cfg, q_weight, k_weight, eps, interleaved)
+                             None, slot_mapping, page_pool, cfg, q_weight, k_weight, eps, interleaved,
+                             axes)
         if N == 0:
             return
         q = qs = oq = oqs = 0
         if query is not None:
             q, qs, oq, oqs = query.data_ptr(), query.stride(0), out_query.data_ptr(), out_query.stride(0)
-        rc = self._fast.tq_launch_dense_rope_append_kv(
-            q, qs, key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
-            None if q_weight is None else q_weight.data_ptr(),
-            None if k_weight is None else k_weight.data_ptr(), cos_sin.data_ptr(),
-            positions.data_ptr(), slot_mapping.data_ptr(), page_pool.data_ptr(), oq, oqs,
-            ctypes.byref(layout), ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
+        qw = None if q_weight is None else q_weight.data_ptr()
+        kw = None if k_weight is None else k_weight.data_ptr()
+        if axes is None:
+            rc = self._fast.tq_launch_dense_rope_append_kv(
+                q, qs, key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), qw, kw,
+                cos_sin.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
+                page_pool.data_ptr(), oq, oqs, ctypes.byref(layout), ctypes.byref(rope),
+                ctypes.byref(cfg), N, self._stream(stream))
+        else:
+            rc = self._fast.tq_launch_dense_rope_axes_append_kv(
+                q, qs, key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), qw, kw,
+                cos_sin.data_ptr(), positions.data_ptr(), N, slot_mapping.data_ptr(),
+                page_pool.data_ptr(), oq, oqs, ctypes.byref(layout), ctypes.byref(axes),
+                ctypes.byref(rope), ctypes.byref(cfg), N, self._stream(stream))
         if rc != 0:
             self._kernel_raise(rc, "dense", "rope_append")
 
@@ -894,6 +975,137 @@ class TurboQuantWrapper:
                 row_start.data_ptr(), prefix_len.data_ptr(), tree_mask.data_ptr(), words,
                 output.data_ptr(), ctypes.byref(layout), ctypes.byref(cfg), *kind, Hq, S, N,
                 max_kv_len, self._stream(stream))
+        if rc != 0:
+            self._kernel_raise(rc, scheme, op)
+
+    # ── eviction: attention weights, selection, compaction ──────────── #
+
+    def attn_weights(self, scheme: str, query, page_pool, block_tables, row_start, prefix_len, scores,
+                     layout, cfg, max_kv_len: int, causal: bool = True, scores_in=None,
+                     decay: float = 1.0, stream: int = 0) -> None:
+        """What the rows' softmax weights on every cached token add up to, over a kv
+        head's query rows: scores = decay * scores_in + the sum (scores_in None: the
+        sum; it may be scores).
+
+        scheme, query [num_tokens, Hq, D], block_tables, row_start and prefix_len as
+        in tree_attn_output; scores (and scores_in) [num_seqs, H, >= max_kv_len] fp32,
+        rows contiguous in their last dimension.  causal: row j of a sequence attends
+        its first prefix_len + j + 1 tokens, otherwise the first prefix_len.  Tokens
+        past what the last row attends keep their scores."""
+        op = "attn_weights"
+        fn = self._weights.get(scheme)
+        if fn is None:
+            raise ValueError(f"{scheme} {op}: no such scheme")
+        for name, t, dims in (("query", query, 3), ("block_tables", block_tables, 2), ("scores", scores, 3)):
+            if not isinstance(t, torch.Tensor) or t.dim() != dims:
+                raise ValueError(f"{scheme} {op}: {name} must be a tensor of {dims} dimensions")
+        N, Hq, D = query.shape
+        S, blocks = block_tables.shape
+        dtype, H = query.dtype, cfg.num_kv_heads
+        if D != cfg.head_dim:
+            raise ValueError(f"{scheme} {op}: query must be [num_tokens, num_q_heads, {cfg.head_dim}]")
+        if dtype is not torch.float16 and (scheme != "dense" or dtype is not torch.bfloat16):
+            raise ValueError(f"{scheme} {op}: query must not be {dtype}")
+        if scores.shape[:2] != (S, H):
+            raise ValueError(f"{scheme} {op}: scores must be [{S}, {H}, max_kv_len], got "
+                             f"{list(scores.shape)}")
+        if scores_in is not None and (not isinstance(scores_in, torch.Tensor)
+                                      or scores_in.shape != scores.shape):
+            raise ValueError(f"{scheme} {op}: scores_in must be of scores' shape")
+        dev = query.get_device()
+        wants = [(query, dtype, 0), (page_pool, torch.uint8, 0), (block_tables, torch.int32, 0),
+                 (row_start, torch.int32, S + 1), (prefix_len, torch.int32, S),
+                 (scores, torch.float32, 0)]
+        if scores_in is not None:
+            wants.append((scores_in, torch.float32, 0))
+        if not self._fit(dev, wants) or dev < 0 or dev != torch.cuda.current_device():
+            self._refuse(scheme, op, dev, dict(zip(("query", "page_pool", "block_tables", "row_start",
+                                                    "prefix_len", "scores", "scores_in"), wants)))
+        if S == 0:
+            return
+        kind = (_DTYPES[dtype],) if scheme == "dense" else ()
+        rc = fn(query.data_ptr(), page_pool.data_ptr(), block_tables.data_ptr(), blocks,
+                row_start.data_ptr(), prefix_len.data_ptr(), causal,
+                None if scores_in is None else scores_in.data_ptr(), scores.data_ptr(),
+                scores.shape[2], decay, ctypes.byref(layout), ctypes.byref(cfg), *kind, Hq, S, N,
+                max_kv_len, self._stream(stream))
+        if rc != 0:
+            self._kernel_raise(rc, scheme, op)
+
+    def select_kv(self, scores, kv_len, kept, new_len=None, sink: int = 0, recent: int = 0,
+                  out_scores=None, stream: int = 0) -> None:
+        """The tokens that a budget keeps of every sequence and kv head: the first
+        `sink`, the last `recent` and the highest scores of the others.
+
+        scores [num_seqs, H, max_kv_len] fp32, kv_len [num_seqs] int32; kept
+        [num_seqs, H, budget] int32 gets their places in rising order, then -1;
+        new_len [num_seqs] int32 their number; out_scores (scores' shape, or scores
+        itself) their scores, then 0."""
+        op = "select_kv"
+        for name, t in (("scores", scores), ("kept", kept)):
+            if not isinstance(t, torch.Tensor) or t.dim() != 3:
+                raise ValueError(f"evict {op}: {name} must be a tensor of 3 dimensions")
+        S, H, T = scores.shape
+        budget = kept.shape[2]
+        if kept.shape[:2] != (S, H):
+            raise ValueError(f"evict {op}: kept must be [{S}, {H}, budget], got {list(kept.shape)}")
+        if out_scores is not None and (not isinstance(out_scores, torch.Tensor)
+                                       or out_scores.shape != scores.shape):
+            raise ValueError(f"evict {op}: out_scores must be of scores' shape")
+        dev = scores.get_device()
+        wants = {"scores": (scores, torch.float32, 0), "kv_len": (kv_len, torch.int32, S),
+                 "kept": (kept, torch.int32, 0)}
+        if new_len is not None:
+            wants["new_len"] = (new_len, torch.int32, S)
+        if out_scores is not None:
+            wants["out_scores"] = (out_scores, torch.float32, 0)
+        if not self._fit(dev, wants.values()) or dev < 0 or dev != torch.cuda.current_device():
+            self._refuse("evict", op, dev, wants)
+        if S == 0:
+            return
+        rc = self._fast.tq_launch_select_kv(
+            scores.data_ptr(), T, kv_len.data_ptr(), S, H, T, budget, sink, recent, kept.data_ptr(),
+            None if new_len is None else new_len.data_ptr(),
+            None if out_scores is None else out_scores.data_ptr(), T, self._stream(stream))
+        if rc != 0:
+            self._kernel_raise(rc, "evict", op)
+
+    def compact_kv(self, scheme: str, page_pool, block_tables, kept, layout, cfg,
+                   out_block_tables=None, stream: int = 0) -> None:
+        """Moves the kept tokens' cells (select_kv's kept [num_seqs, H, budget]) to the
+        front of their sequences: in place, or (out_block_tables [num_seqs, blocks])
+        into other pages, the originals staying as they are."""
+        op = "compact_kv"
+        fn = self._compact.get(scheme)
+        if fn is None:
+            raise ValueError(f"{scheme} {op}: no such scheme")
+        for name, t, dims in (("block_tables", block_tables, 2), ("kept", kept, 3),
+                              ("out_block_tables", out_block_tables, 2)):
+            if (t is not None or dims == 3) and (not isinstance(t, torch.Tensor) or t.dim() != dims):
+                raise ValueError(f"{scheme} {op}: {name} must be a tensor of {dims} dimensions")
+        if block_tables is None:
+            raise ValueError(f"{scheme} {op}: block_tables must be a tensor of 2 dimensions")
+        S, blocks = block_tables.shape
+        if kept.shape[:2] != (S, cfg.num_kv_heads):
+            raise ValueError(f"{scheme} {op}: kept must be [{S}, {cfg.num_kv_heads}, budget], got "
+                             f"{list(kept.shape)}")
+        if out_block_tables is not None and out_block_tables.shape[0] != S:
+            raise ValueError(f"{scheme} {op}: out_block_tables must be [{S}, blocks], got "
+                             f"{list(out_block_tables.shape)}")
+        dev = kept.get_device()
+        wants = {"page_pool": (page_pool, torch.uint8, 0), "block_tables": (block_tables, torch.int32, 0),
+                 "kept": (kept, torch.int32, 0)}
+        if out_block_tables is not None:
+            wants["out_block_tables"] = (out_block_tables, torch.int32, 0)
+        if not self._fit(dev, wants.values()) or dev < 0 or dev != torch.cuda.current_device():
+            self._refuse(scheme, op, dev, wants)
+        if S == 0:
+            return
+        out, out_blocks = None, 0
+        if out_block_tables is not None:
+            out, out_blocks = out_block_tables.data_ptr(), out_block_tables.shape[1]
+        rc = fn(page_pool.data_ptr(), block_tables.data_ptr(), blocks, kept.data_ptr(), kept.shape[2],
+                out, out_blocks, ctypes.byref(layout), ctypes.byref(cfg), S, self._stream(stream))
         if rc != 0:
             self._kernel_raise(rc, scheme, op)
 
@@ -1148,6 +1360,13 @@ class BlockTable:
         rc = self._tq.lib.tq_block_table_free_sequence(self.handle, seq_id)
         if rc != 0:
             raise KeyError(seq_id)
+
+    def truncate(self, seq_id: int, num_tokens: int) -> None:
+        """Cuts a sequence to its first num_tokens tokens; the pages behind go back."""
+        rc = self._tq.lib.tq_block_table_truncate(self.handle, seq_id, num_tokens)
+        if rc != 0:
+            self.num_tokens(seq_id)  # KeyError: no such sequence
+            raise ValueError(self._tq._last_cuda_error())
 
     def close(self) -> None:
         if self.handle:
