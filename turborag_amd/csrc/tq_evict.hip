@@ -14,9 +14,12 @@ using namespace dev;
 
 // ---------------------------------------------------------------------------
 // Selection.  One workgroup per (sequence, kv head): a radix search of the lowest kept
-// score over the bits of an order-preserving key, three digits of 11, 11 and 10 bits,
-// counted in LDS; then the kept tokens in order, their places from counts of each wave's
-// stretch of tokens.  4 bytes a token and pass: bound by the latency of the passes.
+// score over the bits of an order-preserving key, digits of 10, 11 and 11 bits counted
+// in LDS, which ends as soon as all tokens of the digit are kept; then the kept tokens
+// in order, from a bit per token in LDS, whose words' counts are summed up over the
+// threads.  A lane has kDeep tokens in registers, a tile of the workgroup; a row of one
+// tile is read once for its keys.
+// 4 bytes a token: bound by the latency of the steps, one after the other.
 // ---------------------------------------------------------------------------
 struct SelectArgs {
     const float* scores;
@@ -27,18 +30,41 @@ struct SelectArgs {
     int heads, max_kv, budget, sink, recent;
 };
 
-// Larger scores have larger keys; -0 is 0, NaN is below everything.
+// Larger scores have larger keys; -0 is 0, NaN is below everything.  Keys lie between
+// those of tokens that are none (0) and of tokens that stay whatever their score (~0).
+constexpr uint32_t kNoToken = 0u, kStays = ~0u;
 __device__ __forceinline__ uint32_t key_of(float f) {
-    const uint32_t u = __float_as_uint(f == 0.0f ? 0.0f : f);
-    return f != f ? 0u : u >> 31 ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(f + 0.0f);
+    return f != f ? 1u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 
-constexpr int kWaves = 16, kThreads = 64 * kWaves, kBins = 2048;
+// f(0), f(1), ..., as constants.
+template <int N, int K = 0, class F>
+__device__ __forceinline__ void for_each_lane(F&& f) {
+    if constexpr (K < N) {
+        f(std::integral_constant<int, K>{});
+        for_each_lane<N, K + 1>(f);
+    }
+}
+// The wave's mask m into lane K of `to`.  (The wait states between a vector instruction's
+// scalar result and the next one that reads it, which the compiler does not see here.)
+template <int K>
+__device__ __forceinline__ void into_lane(uint2& to, uint64_t m) {
+    asm("s_nop 3\n\tv_writelane_b32 %0, %2, %4\n\tv_writelane_b32 %1, %3, %4"
+        : "+v"(to.x), "+v"(to.y)
+        : "s"((uint32_t)m), "s"((uint32_t)(m >> 32)), "n"(K));
+}
 
-__global__ __launch_bounds__(kThreads) void select_kv_kernel(const SelectArgs a) {
-    __shared__ uint32_t bins[kBins];
-    __shared__ uint32_t above[kWaves], found[2];
-    __shared__ int2 counts[kWaves];
+// The first digit's counters lie in COPIES side by side, a lane's by its number: scores of
+// a softmax have few exponents, and lanes that count at one address or bank take turns.
+template <int WAVES, int COPIES, int kDeep>
+__global__ __launch_bounds__(64 * WAVES) void select_kv_kernel(const SelectArgs a) {
+    constexpr int kThreads = 64 * WAVES, kTile = kThreads * kDeep;
+    static_assert(COPIES >= 4 && 1024 * COPIES >= 2048, "counters");
+    __shared__ __attribute__((aligned(16))) uint32_t bins[1024 * COPIES];
+    __shared__ uint32_t above[WAVES], found[3];
+    __shared__ uint2 marks[2][kTile / 64];  // kept for certain; with the lowest kept key
+    __shared__ int2 counts[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t row = blockIdx.x;
     const int s = (int)(row / a.heads), B = a.budget;
@@ -47,117 +73,204 @@ __global__ __launch_bounds__(kThreads) void select_kv_kernel(const SelectArgs a)
     int32_t* kept = a.kept + row * B;
     float* out = a.out ? a.out + row * a.out_stride : nullptr;
     if (a.new_len && row == (int64_t)s * a.heads && tid == 0) a.new_len[s] = n;
-    for (int j = n + tid; j < B; j += kThreads) kept[j] = -1;
 
     if (L <= B) {
-        for (int j = tid; j < L; j += kThreads) kept[j] = j;
+        for (int j = tid; j < B; j += kThreads) kept[j] = j < L ? j : -1;
         if (out && out != x)
             for (int j = tid; j < L; j += kThreads) out[j] = x[j];
-    } else {
-        // [lo, hi): the tokens that their scores decide on.
-        const int lo = a.sink, hi = L - a.recent;
-        uint32_t want = (uint32_t)(B - a.sink - a.recent), prefix = 0;
-        int shift = 32;
-        if (want) {
-            for (int pass = 0; pass < 3; ++pass) {
-                const int bits = pass < 2 ? 11 : 10, from = shift;
-                shift -= bits;
-                const uint32_t top = (1u << bits) - 1;
-                for (int k = tid; k < kBins; k += kThreads) bins[k] = 0;
-                __syncthreads();
-                for (int t = lo + tid; t < hi; t += kThreads) {
-                    const uint32_t key = key_of(x[t]);
-                    if (from == 32 || key >> from == prefix) atomicAdd(&bins[key >> shift & top], 1u);
-                }
-                __syncthreads();
-                // The digit at which the tokens from the top reach `want`: a wave has 128
-                // bins, a lane two of them (from the top).
-                const int d1 = kBins - 1 - 2 * tid, d0 = d1 - 1;
-                const uint32_t n1 = bins[d1], n0 = bins[d0];
-                uint32_t up = n1 + n0;
+        if (out)
+            for (int j = n + tid; j < a.max_kv; j += kThreads) out[j] = 0.0f;
+        return;
+    }
+    const auto clear_rest = [&] {  // (four at a time; the row may begin at any float)
+        typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+        for (int j = n + 4 * tid; j < a.max_kv; j += 4 * kThreads) {
+            if (j + 4 <= a.max_kv)
+                *reinterpret_cast<f4u*>(out + j) = f4u{0.0f, 0.0f, 0.0f, 0.0f};
+            else
+                for (int k = j; k < a.max_kv; ++k) out[k] = 0.0f;
+        }
+    };
+    const bool in_place = out == x;
+    if (out && !in_place) clear_rest();
+    // [lo, hi): the tokens that their scores decide on.
+    const int lo = a.sink, hi = L - a.recent, tiles = (L + kTile - 1) / kTile;
+    constexpr int per = 64 * kDeep;  // a wave's tokens of a tile, in a row, lane by lane
+    uint32_t keys[kDeep];
+    const auto load = [&](int tile) __attribute__((always_inline)) {
+        const int t0 = tile * kTile + wv * per + lane, end = min(tile * kTile + (wv + 1) * per, L);
 #pragma unroll
-                for (int m = 1; m < 64; m <<= 1) {
-                    const uint32_t o = __shfl_up(up, m, 64);
-                    if (lane >= m) up += o;
-                }
-                if (lane == 63) above[wv] = up;
-                __syncthreads();
-                uint32_t before = up - n1 - n0;
-                for (int w = 0; w < wv; ++w) before += above[w];
-                if (before < want && before + n1 >= want) {
-                    found[0] = (uint32_t)d1;
-                    found[1] = want - before;
-                } else if (before + n1 < want && before + n1 + n0 >= want) {
-                    found[0] = (uint32_t)d0;
-                    found[1] = want - before - n1;
-                }
-                __syncthreads();
-                prefix = prefix << bits | found[0];
-                want = found[1];
-                __syncthreads();
+        for (int k = 0; k < kDeep; ++k) keys[k] = __float_as_uint(x[min(t0 + k * 64, L - 1)]);
+        const int w0 = tile * kTile + wv * per;  // (the same in every lane)
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) {
+            keys[k] = key_of(__uint_as_float(keys[k]));
+            if (w0 + k * 64 < lo || w0 + k * 64 + 64 > min(hi, end)) {
+                const int t = t0 + k * 64;
+                keys[k] = t >= end ? kNoToken : t < lo || t >= hi ? kStays : keys[k];
             }
         }
-        // prefix: the lowest kept key; `want` tokens with it are kept, the first ones.
-        const bool none = a.sink + a.recent == B;
-        const int per = ((L + kWaves - 1) / kWaves + 63) & ~63, t0 = min(wv * per, L), t1 = min(t0 + per, L);
-        const auto look = [&](int t, bool& sure, bool& tie) {
-            const bool in = t < t1;
-            const uint32_t key = in ? key_of(x[t]) : 0u;
-            const bool mid = t >= lo && t < hi;
-            sure = in && (!mid || (!none && key > prefix));
-            tie = in && mid && !none && key == prefix;
-        };
-        int sure_n = 0, tie_n = 0;
-        for (int t = t0; t < t1; t += 64) {
-            bool sure, tie;
-            look(t + lane, sure, tie);
-            sure_n += __popcll(__ballot(sure));
-            tie_n += __popcll(__ballot(tie));
-        }
-        if (lane == 0) counts[wv] = make_int2(sure_n, tie_n);
+    };
+    // f(key, k) of the wave's tokens of the tile.
+    const auto each = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) f(keys[k], k);
+    };
+    load(0);
+
+    uint32_t want = (uint32_t)(B - a.sink - a.recent), prefix = 0;
+    int shift = 32;
+    bool ties = false;  // of the tokens with the prefix only the first `want` are kept
+    const auto digit = [&](auto first, auto width) __attribute__((always_inline)) {
+        constexpr bool kFirst = decltype(first)::value;
+        constexpr int kBits = decltype(width)::value, kBins = 1 << kBits, kMine = kBins / kThreads;
+        constexpr int kCopies = kFirst ? COPIES : 1;
+        const int from = shift;
+        shift -= kBits;
+        for (int k = tid * 4; k < kBins * kCopies; k += kThreads * 4)
+            *reinterpret_cast<uint4*>(bins + k) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        int at = 0, ties = 0;  // kept tokens and ties before the wave's
-        for (int w = 0; w < wv; ++w) {
-            at += counts[w].x;
-            ties += counts[w].y;
+        // The first digit counts every lane's keys: kStays alone has the highest one (an
+        // infinity's is one less), and kNoToken's are subtracted from the lowest.  Later, none
+        // but counted keys have the prefix, unless it is 0.
+        const bool checked = prefix == 0;
+        for (int tile = 0; tile < tiles; ++tile) {
+            if (tiles > 1 && (!kFirst || tile)) load(tile);
+            each([&](uint32_t key, int) {
+                if (kFirst || (key >> (from & 31) == prefix && (!checked || key != kNoToken)))
+                    atomicAdd(&bins[(key >> shift & (kBins - 1)) * kCopies + (lane & (kCopies - 1))], 1u);
+            });
         }
-        at += min(ties, (int)want);
-        const uint64_t below = (1ull << lane) - 1;
-        for (int t = t0; t < t1; t += 64) {
-            bool sure, tie;
-            look(t + lane, sure, tie);
-            const uint64_t tm = __ballot(tie);
-            const bool keep = sure || (tie && ties + __popcll(tm & below) < (int)want);
-            const uint64_t km = __ballot(keep);
-            if (keep) kept[at + __popcll(km & below)] = t + lane;
-            at += __popcll(km);
-            ties += __popcll(tm);
+        __syncthreads();
+        // The digit at which the tokens from the top reach `want`: kMine bins a thread,
+        // from the top down.
+        uint32_t mine[kMine], sum = 0;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) {
+            const int d = kBins - 1 - (tid * kMine + e);
+            if constexpr (kFirst) {
+                mine[e] = 0;
+#pragma unroll
+                for (int k = 0; k < COPIES; k += 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(bins + d * COPIES + ((k + 4 * tid) & (COPIES - 1)));
+                    mine[e] += w.x + w.y + w.z + w.w;
+                }
+                if (d == kBins - 1) mine[e] = 0;
+                if (d == 0) mine[e] -= (uint32_t)(tiles * kTile - L);
+            } else {
+                mine[e] = bins[d];
+            }
+            sum += mine[e];
         }
-        if (out) {
-            // In order, so that in place no score is overwritten before it is read: place j
-            // takes the score of a token at j or behind it.
-            __threadfence_block();
-            __syncthreads();
-            constexpr int kDeep = 4;
-            for (int j0 = 0; j0 < n; j0 += kDeep * kThreads) {
-                float v[kDeep];
+        uint32_t up = sum;
 #pragma unroll
-                for (int k = 0; k < kDeep; ++k) {
-                    const int j = j0 + k * kThreads + tid;
-                    v[k] = j < n ? x[kept[j]] : 0.0f;
-                }
-                __syncthreads();
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint32_t o = __shfl_up(up, m, 64);
+            if (lane >= m) up += o;
+        }
+        if (lane == 63) above[wv] = up;
+        __syncthreads();
+        uint32_t before = up - sum;
 #pragma unroll
-                for (int k = 0; k < kDeep; ++k) {
-                    const int j = j0 + k * kThreads + tid;
-                    if (j < n) out[j] = v[k];
+        for (int w = 0; w < WAVES; ++w) before += w < wv ? above[w] : 0u;
+        if (before < want && before + sum >= want) {
+#pragma unroll
+            for (int e = 0; e < kMine; ++e) {
+                if (before < want && before + mine[e] >= want) {
+                    found[0] = (uint32_t)(kBins - 1 - (tid * kMine + e));
+                    found[1] = want - before;
+                    found[2] = mine[e];
                 }
+                before += mine[e];
             }
         }
+        __syncthreads();
+        prefix = prefix << kBits | found[0];
+        want = found[1];
+        ties = found[2] != want;
+        if (ties) __syncthreads();  // (found is written again)
+    };
+    if (want) {
+        digit(std::true_type{}, std::integral_constant<int, 10>{});
+        for (int k = 0; k < 2 && ties; ++k) digit(std::false_type{}, std::integral_constant<int, 11>{});
+    }
+    // Kept: keys from `sure` on and, of those from `tie` on, the first `want`.
+    const bool none = a.sink + a.recent == B;
+    const uint32_t tie = none ? kStays : max(prefix << shift, 1u);
+    const uint32_t sure = none ? kStays : ties ? (prefix + 1u) << shift : tie;
+    int at = 0, equal = 0;  // kept tokens and equal ones of the tiles so far
+    for (int tile = 0; tile < tiles; ++tile) {
+        if (tiles > 1) load(tile);
+        uint2 certain = {0, 0}, same = {0, 0};  // lane k: the bits of the wave's tokens 64 k ..
+        for_each_lane<kDeep>([&](auto k) { into_lane<k.value>(certain, __ballot(keys[k.value] >= sure)); });
+        if (sure != tie)
+            for_each_lane<kDeep>(
+                [&](auto k) { into_lane<k.value>(same, __ballot(keys[k.value] - tie < sure - tie)); });
+        if (lane < kDeep) {
+            marks[0][wv * kDeep + lane] = certain;
+            marks[1][wv * kDeep + lane] = same;
+        }
+        __syncthreads();
+        // A thread has 32 tokens of the tile, which lie in a row.
+        constexpr int kWords = kTile / 32;
+        static_assert(kWords <= kThreads, "a word per thread");
+        uint32_t keep = 0, ties_of = 0;
+        if (tid < kWords) {
+            keep = reinterpret_cast<const uint32_t*>(marks[0])[tid];
+            ties_of = reinterpret_cast<const uint32_t*>(marks[1])[tid];
+        }
+        int2 up = make_int2(__popc(keep), __popc(ties_of));
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int ox = __shfl_up(up.x, m, 64), oy = __shfl_up(up.y, m, 64);
+            if (lane >= m) up.x += ox, up.y += oy;
+        }
+        if (lane == 63) counts[wv] = up;
+        __syncthreads();
+        int base = at + up.x - __popc(keep), eq = equal + up.y - __popc(ties_of), next = at, next_eq = equal;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const int2 e = counts[w];
+            base += w < wv ? e.x : 0;
+            eq += w < wv ? e.y : 0;
+            next += e.x;
+            next_eq += e.y;
+        }
+        const int quota = (int)want;  // of the equal ones
+        base += min(eq, quota) - min(equal, quota);
+        while (ties_of && eq < quota) {
+            keep |= ties_of & -ties_of;
+            ties_of &= ties_of - 1;
+            ++eq;
+        }
+        const int t0 = tile * kTile + tid * 32;
+        while (keep) {
+            kept[base++] = t0 + __ffs(keep) - 1;
+            keep &= keep - 1;
+        }
+        at = next + min(next_eq, quota) - min(equal, quota);
+        equal = next_eq;
+        if (tiles > 1) __syncthreads();  // (marks and counts are written again)
     }
     if (out) {
+        // In order: place j takes the score of a token at j or behind it, so in place none is
+        // overwritten before it is read.
+        __threadfence_block();
         __syncthreads();
-        for (int j = n + tid; j < a.max_kv; j += kThreads) out[j] = 0.0f;
+        constexpr int kPlaces = 4;
+        for (int j0 = 0; j0 < n; j0 += kPlaces * kThreads) {
+            float f[kPlaces];
+#pragma unroll
+            for (int k = 0; k < kPlaces; ++k) f[k] = x[kept[min(j0 + k * kThreads + tid, n - 1)]];
+            if (in_place) __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kPlaces; ++k) {
+                const int j = j0 + k * kThreads + tid;
+                if (j < n) out[j] = f[k];
+            }
+            if (in_place) __syncthreads();
+        }
+        if (in_place) clear_rest();
     }
 }
 
@@ -419,8 +532,13 @@ extern "C" int tq_launch_select_kv(const float* scores, int64_t score_stride, co
         if (rows == 0) return;
         const tq::SelectArgs a{scores,  score_stride, out_stride, kv_len, kept, new_len, out_scores,
                                num_kv_heads, max_kv_len, budget, sink, recent};
-        hipLaunchKernelGGL(tq::select_kv_kernel, dim3((unsigned)rows), dim3(tq::kThreads), 0,
-                           static_cast<hipStream_t>(stream), a);
+        const hipStream_t st = static_cast<hipStream_t>(stream);
+        if (max_kv_len <= 2048)
+            hipLaunchKernelGGL((tq::select_kv_kernel<4, 8, 8>), dim3((unsigned)rows), dim3(256), 0, st, a);
+        else if (max_kv_len <= 8192)
+            hipLaunchKernelGGL((tq::select_kv_kernel<16, 32, 8>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+        else
+            hipLaunchKernelGGL((tq::select_kv_kernel<16, 32, 32>), dim3((unsigned)rows), dim3(1024), 0, st, a);
         tq::check_launch("select_kv_kernel");
     });
 }

@@ -206,78 +206,123 @@ __device__ __forceinline__ u4 pack8(const float* y) {
     return w;
 }
 
-// Axes of a lane's eight pairs: one for all tokens and pairs, one per lane (blocks of
-// whole eights), or one per pair.
-constexpr int kOneAxis = 0, kLaneAxis = 1, kPairAxis = 2;
+// Norm (the row's weight, if any) and rotation of a lane's two pieces, by cos and sin of
+// its pairs.
+template <bool BF, int D, bool INTER>
+__device__ __forceinline__ void turn_row(u4& w0, u4& w1, const uint16_t* weight, int at0, int at1, float eps,
+                                         const float* c, const float* s) {
+    constexpr int L = D / 16;
+    float y[16];
+    unpack8<BF>(w0, y);
+    unpack8<BF>(w1, y + 8);
+    if (weight) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ss = fmaf(y[e], y[e], ss);
+        ss += quad_xor<1>(ss);
+        ss += quad_xor<2>(ss);
+        if (L == 8)  // every lane of a quad holds its sum: the row's other quad by mirror
+            ss += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(ss), 0x141, 0xF, 0xF, true));
+        const float n = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+        float w[16];
+        unpack8<BF>(*reinterpret_cast<const u4*>(weight + at0), w);
+        unpack8<BF>(*reinterpret_cast<const u4*>(weight + at1), w + 8);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = y[e] * n * w[e];
+    }
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const int i0 = INTER ? 2 * p : p, i1 = INTER ? 2 * p + 1 : p + 8;
+        const float u = y[i0], v = y[i1];
+        y[i0] = fmaf(u, c[p], -(v * s[p]));
+        y[i1] = fmaf(u, s[p], v * c[p]);
+    }
+    w0 = pack8<BF>(y);
+    w1 = pack8<BF>(y + 8);
+}
 
-template <bool BF, int D, bool INTER, int AXES>
+// AXES: the positions have several axes, and a lane's eight pairs one of them (blocks of
+// whole eights).
+template <bool BF, int D, bool INTER, bool AXES>
 __global__ __launch_bounds__(kBlock) void rope_rows_kernel(const RopeArgs a) {
     constexpr int L = D / 16;
     const int j = threadIdx.x & (L - 1);
     const int job = block_of() * (kBlock / L) + threadIdx.x / L;
     const int row = min(job, a.n * a.rows - 1);
     const int t = row / a.rows;
-    Positions ps;
-    if constexpr (AXES == kOneAxis) {
-        ps.p[0] = a.pos[t];
-        ps.inside = ps.p[0] >= 0 && ps.p[0] < a.max_position;
+    int pos;
+    bool inside;
+    if constexpr (AXES) {
+        const Positions p = positions_of(a, t);
+        pos = p.of(axis_of(a, 8 * j));
+        inside = p.inside;
     } else {
-        ps = positions_of(a, t);
+        pos = a.pos[t];
+        inside = pos >= 0 && pos < a.max_position;
     }
     const int slot = a.v ? a.slots[t] : 0;
     const Row o = row_of(a, t, row - t * a.rows, slot);
     const int at0 = INTER ? 16 * j : 8 * j, at1 = INTER ? 16 * j + 8 : D / 2 + 8 * j;
     u4 w0 = *reinterpret_cast<const u4*>(o.src + at0), w1 = *reinterpret_cast<const u4*>(o.src + at1);
-    const bool live = job == row && ps.inside && o.dst;
+    const bool live = job == row && inside && o.dst;
     if (o.what != 2) {  // (the same for a row's lanes)
-        float c[8], s[8], y[16];
-        if constexpr (AXES == kPairAxis) {
-            const uint32_t bits = (uint32_t)(a.axis_bits[j >> 2] >> (16 * (j & 3)));
+        const float* tr = a.table + (size_t)(live ? pos : 0) * D + 8 * j;
+        float c[8], s[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float* tr = a.table + (size_t)(live ? ps.of(bits >> (2 * e)) : 0) * D + 8 * j + e;
-                c[e] = tr[0];
-                s[e] = tr[D / 2];
-            }
-        } else {
-            const int pos = AXES == kOneAxis ? ps.p[0] : ps.of(axis_of(a, 8 * j));
-            const float* tr = a.table + (size_t)(live ? pos : 0) * D + 8 * j;
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(tr + e);
-                *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(tr + D / 2 + e);
-            }
+        for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(tr + e);
+            *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(tr + D / 2 + e);
         }
-        unpack8<BF>(w0, y);
-        unpack8<BF>(w1, y + 8);
-        if (o.w) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) ss = fmaf(y[e], y[e], ss);
-            ss += quad_xor<1>(ss);
-            ss += quad_xor<2>(ss);
-            if (L == 8)  // every lane of a quad holds its sum: the row's other quad by mirror
-                ss += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(ss), 0x141, 0xF, 0xF, true));
-            const float n = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-            float w[16];
-            unpack8<BF>(*reinterpret_cast<const u4*>(o.w + at0), w);
-            unpack8<BF>(*reinterpret_cast<const u4*>(o.w + at1), w + 8);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = y[e] * n * w[e];
-        }
-#pragma unroll
-        for (int p = 0; p < 8; ++p) {
-            const int i0 = INTER ? 2 * p : p, i1 = INTER ? 2 * p + 1 : p + 8;
-            const float u = y[i0], v = y[i1];
-            y[i0] = fmaf(u, c[p], -(v * s[p]));
-            y[i1] = fmaf(u, s[p], v * c[p]);
-        }
-        w0 = pack8<BF>(y);
-        w1 = pack8<BF>(y + 8);
+        turn_row<BF, D, INTER>(w0, w1, o.w, at0, at1, a.eps, c, s);
     }
     if (live) {
         *reinterpret_cast<u4*>(o.dst + at0) = w0;
         *reinterpret_cast<u4*>(o.dst + at1) = w1;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The same where a lane's pairs have different axes: cos and sin are 16 loads of a value
+// instead of four of four, so a lane group has kTokenRows rows of its token, which share
+// them: the append of 32,768 tokens of 16/2 heads takes 107 us with one row per group, 72
+// with four, 73 with five, and 91 with cos and sin gathered once per token into LDS (where
+// every workgroup waits for them).
+// ---------------------------------------------------------------------------
+constexpr int kTokenRows = 4;
+
+template <bool BF, int D, bool INTER>
+__global__ __launch_bounds__(kBlock) void rope_pair_axes_kernel(const RopeArgs a) {
+    constexpr int L = D / 16;
+    const int j = threadIdx.x & (L - 1), blocks = (a.rows + kTokenRows - 1) / kTokenRows;
+    const int job = block_of() * (kBlock / L) + threadIdx.x / L;
+    // (rows a line of groups apart, so that a wave's loads lie in a row)
+    const int tj = job / blocks, t = min(tj, a.n - 1), r0 = job - tj * blocks;
+    const Positions ps = positions_of(a, t);
+    const int slot = a.v ? a.slots[t] : 0;
+    const int at0 = INTER ? 16 * j : 8 * j, at1 = INTER ? 16 * j + 8 : D / 2 + 8 * j;
+    Row o[kTokenRows];
+    u4 w0[kTokenRows], w1[kTokenRows];
+#pragma unroll
+    for (int k = 0; k < kTokenRows; ++k) {
+        o[k] = row_of(a, t, min(r0 + k * blocks, a.rows - 1), slot);
+        w0[k] = *reinterpret_cast<const u4*>(o[k].src + at0);
+        w1[k] = *reinterpret_cast<const u4*>(o[k].src + at1);
+    }
+    const uint32_t bits = (uint32_t)(a.axis_bits[j >> 2] >> (16 * (j & 3)));
+    float c[8], s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float* tr = a.table + (size_t)(ps.inside ? ps.of(bits >> (2 * e)) : 0) * D + 8 * j + e;
+        c[e] = tr[0];
+        s[e] = tr[D / 2];
+    }
+#pragma unroll
+    for (int k = 0; k < kTokenRows; ++k) {
+        if (o[k].what != 2) turn_row<BF, D, INTER>(w0[k], w1[k], o[k].w, at0, at1, a.eps, c, s);
+        if (tj == t && r0 + k * blocks < a.rows && ps.inside && o[k].dst) {
+            *reinterpret_cast<u4*>(o[k].dst + at0) = w0[k];
+            *reinterpret_cast<u4*>(o[k].dst + at1) = w1[k];
+        }
     }
 }
 
@@ -299,16 +344,20 @@ template <bool BF, int D, bool INTER>
 void launch_rows(const RopeArgs& a, hipStream_t stream) {
     constexpr int per = kBlock / (D / 16);
     const dim3 grid = grid_of(((long long)a.n * a.rows + per - 1) / per);
-    const auto go = [&](auto axes) {
-        hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER, decltype(axes)::value>), grid, dim3(kBlock), 0, stream, a);
-    };
-    if (a.axes == 1) return go(std::integral_constant<int, kOneAxis>{});
-    // a field of eight pairs' axes (16 bits) is eight times its first one
+    if (a.axes == 1) {
+        hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER, false>), grid, dim3(kBlock), 0, stream, a);
+        return;
+    }
+    // a field of eight pairs' axes (16 bits) is 0x5555 times its first one
     for (int i = 0; i < D / 2; i += 8) {
         const unsigned f = (unsigned)(a.axis_bits[i >> 5] >> (2 * (i & 31))) & 0xffff;
-        if (f != (f & 3) * 0x5555u) return go(std::integral_constant<int, kPairAxis>{});
+        if (f == (f & 3) * 0x5555u) continue;
+        const long long jobs = (long long)a.n * ((a.rows + kTokenRows - 1) / kTokenRows);
+        hipLaunchKernelGGL((rope_pair_axes_kernel<BF, D, INTER>), grid_of((jobs + per - 1) / per), dim3(kBlock), 0,
+                           stream, a);
+        return;
     }
-    go(std::integral_constant<int, kLaneAxis>{});
+    hipLaunchKernelGGL((rope_rows_kernel<BF, D, INTER, true>), grid, dim3(kBlock), 0, stream, a);
 }
 
 void launch_rope(const RopeArgs& a, bool bf16, bool interleaved, hipStream_t stream) {

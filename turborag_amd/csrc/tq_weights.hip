@@ -212,29 +212,52 @@ __global__ __launch_bounds__(256) void turn_queries_kernel(const uint16_t* __res
     if (j == 0) turned_scale[row] = scale * __uint_as_float((uint32_t)(127 - sh) << 23);
 }
 
+// (max, sum) of a part added to a row's.
+__device__ __forceinline__ void add_part(float& m, float& l, float2 e) {
+    const float n = fmaxf(m, e.x);
+    l = (m == -INFINITY ? l : l * exp2_hw(m - n)) + (e.x == -INFINITY ? e.y : e.y * exp2_hw(e.x - n));
+    m = n;
+}
+
 // ---------------------------------------------------------------------------
 // The passes over K.  A workgroup has one kv head and a chunk of C tokens of one
-// sequence, T of them a wave; K's operands stay in registers while the rows go by
-// in tiles of 16.  The products run transposed (K Q'): a query row is a lane column,
-// so its maximum and sum are in-lane but for two lane swaps, and a token's sum over
-// the rows is in-lane over the tiles, across 16 lanes once at the end.
+// sequence; 4 groups of its waves have T tokens each at a time, whose K operands stay
+// in registers while the rows go by in tiles of 16, dealt to WR waves; the rows'
+// operands come from LDS, a block of kRowBlock rows at a time.  The products run
+// transposed (K Q'): a query row is a lane column, so its maximum and sum are in-lane
+// but for two lane swaps, and a token's sum over the rows is in-lane over the tiles,
+// across 16 lanes once at the end.
 //   kStats: (max, sum) of the chunk for every row;  kStore: x too;
 //   kSum: the weights, summed over the rows.
 // ---------------------------------------------------------------------------
 constexpr int kStats = 0, kStore = 1, kSum = 2;
-constexpr int kRowBlock = 256;  // rows whose statistics lie in LDS at a time
+constexpr int kChunk = 256;
+// x is exact to half an ulp; its difference from a reference of this size on is taken
+// after x itself is rounded, so that no exponent is above 0 (one of up to half an ulp of
+// the reference otherwise, the same in both passes).
+constexpr float kHuge = 4194304.0f;
 
-// Tokens of a wave: 16 TT.  (Compressed pages: three operands a token tile.)
-template <int FMT>
-constexpr int kTT = FMT == kProd || FMT == kMse ? 2 : 4;
+template <int FMT, int D, int WR, int MODE>
+struct Shape {
+    static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
+    // (compressed pages: three operands a token tile)
+    static constexpr int TT = kTurned ? 2 : 4, T = 16 * TT, kSubs = kChunk / (4 * T);
+    static constexpr int kParts = kTurned ? 2 : 1;  // of a query row
+    static constexpr int kRowBytes = 2 * D;
+    static constexpr int kRowBlock = 32768 / (kParts * kRowBytes);
+    static constexpr int kThreads = 256 * WR;
+};
 
-template <int FMT, int D, int MODE>
-__global__ __launch_bounds__(256) void weights_kernel(const WeightArgs a, float scale) {
-    constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
-    constexpr int TT = kTT<FMT>, T = 16 * TT, C = 4 * T, KK = D / 32;
-    __shared__ float2 ml[MODE == kSum ? 1 : 4][MODE == kSum ? 1 : kRowBlock];
+template <int FMT, int D, int WR, int MODE>
+__global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a, float scale) {
+    using S = Shape<FMT, D, WR, MODE>;
+    constexpr bool kTurned = S::kTurned, BF = S::BF;
+    constexpr int TT = S::TT, T = S::T, KK = D / 32, C = kChunk, kRowBlock = S::kRowBlock;
+    __shared__ __attribute__((aligned(16))) uint8_t rows_mem[32768];
+    __shared__ float row_scales[kTurned ? kRowBlock : 1];
+    __shared__ float2 ml[MODE == kSum ? 1 : 4][kRowBlock];  // kSum: the rows' (M, 1 / l)
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, gq = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wv & 3, wr = wv >> 2;
     const PageGeom& g = a.g;
 
     // Eight chunks in turn, then the same ones of the next head: the workgroups of one
@@ -246,213 +269,280 @@ __global__ __launch_bounds__(256) void weights_kernel(const WeightArgs a, float 
     const int s = (int)(sc / a.chunks), c = (int)(sc - (long long)s * a.chunks);
     const Seq q = seq_of(a, s);
     if (c * C >= q.end) return;
-    const int R = q.rows * a.group, t0 = c * C + wv * T;
+    const int R = q.rows * a.group;
     if (R == 0) {  // (no row and, without any in the call, no query)
         const int64_t at = ((int64_t)s * g.H + h) * a.stride;
         if (MODE == kSum)
-            for (int t = c * C + tid; t < min(c * C + C, q.end); t += 256)
+            for (int t = c * C + tid; t < min(c * C + C, q.end); t += S::kThreads)
                 a.out[at + t] = a.in ? a.decay * a.in[at + t] : 0.0f;
         return;
     }
 
-    // K's rows: lane (i, gq) has token i of each tile.
     const uint64_t dummy = (uint64_t)(reinterpret_cast<uintptr_t>(a.query) - reinterpret_cast<uintptr_t>(a.pool));
     const int32_t* __restrict__ table = a.tables + (size_t)s * a.max_blocks;
+    // K's rows of the wave's T tokens from t0 on: lane (i, gq) has token i of each tile.
     int id[TT], tib[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        const int t = min(t0 + tt * 16 + i, q.end - 1);
-        const int pg = g.bs_shift >= 0 ? t >> g.bs_shift : t / g.block_size;
-        tib[tt] = t - pg * g.block_size;
-        id[tt] = table[pg];
-    }
-    u4 k[TT][KK];                  // dense: operands
+    u4 k[kTurned ? 1 : TT][KK];    // dense: operands
     typedef uint32_t code_t __attribute__((ext_vector_type(KK), aligned(2)));
     code_t code[TT];               // compressed: a quarter of a token's codes
     uint32_t scales[TT];           // its RMS, its residual's RMS above
     uint32_t live[TT];             // tokens of the tile that can be read (bits)
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        const bool ok = t0 + tt * 16 + i < q.end && id[tt] >= 0;
-        live[tt] = (uint32_t)__ballot(ok) & 0xffffu;
-        const uint64_t page = (uint64_t)max(id[tt], 0) * g.page_size;
-        const uint64_t cell = (uint64_t)(tib[tt] * g.H + h);
-        if constexpr (!kTurned) {
-            const uint8_t* p = a.pool + (ok ? page + g.kc_off + cell * (2 * D) : dummy) + gq * 16;
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) k[tt][kk] = *reinterpret_cast<const u4*>(p + kk * 64);
-        } else {
-            code[tt] = *reinterpret_cast<const code_t*>(
-                a.pool + (ok ? page + g.kc_off + cell * (D / 2) : dummy) + gq * (D / 8));
-            scales[tt] = ld_u16(a.pool + (ok ? page + g.ks_off + cell * 2 : dummy));
-            if (FMT == kProd) scales[tt] |= (uint32_t)ld_u16(a.pool + (ok ? page + g.kres_off + cell * 2 : dummy)) << 16;
-        }
-    }
-    KeyParts kp[kTurned ? TT : 1][KK];
-    float ks[kTurned ? TT : 1][4], kr[kTurned ? TT : 1][4];  // of the tokens 4 gq + 0..3
-    if constexpr (kTurned) {
+    const auto pages = [&](int t0) {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
+            const int t = min(t0 + tt * 16 + i, q.end - 1);
+            const int pg = g.bs_shift >= 0 ? t >> g.bs_shift : t / g.block_size;
+            tib[tt] = t - pg * g.block_size;
+            id[tt] = table[pg];
+        }
+    };
+    const auto fetch = [&](int t0) {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) kp[tt][kk] = decode8<FMT>(code[tt][kk]);
+        for (int tt = 0; tt < TT; ++tt) {
+            const bool ok = t0 + tt * 16 + i < q.end && id[tt] >= 0;
+            live[tt] = (uint32_t)__ballot(ok) & 0xffffu;
+            const uint64_t page = (uint64_t)max(id[tt], 0) * g.page_size;
+            const uint64_t cell = (uint64_t)(tib[tt] * g.H + h);
+            if constexpr (!kTurned) {
+                const uint8_t* p = a.pool + (ok ? page + g.kc_off + cell * (2 * D) : dummy) + gq * 16;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t w = (uint32_t)__shfl((int)scales[tt], 4 * gq + r, 64);
-                ks[tt][r] = h2f(w & 0xffff);
-                kr[tt][r] = FMT == kProd ? h2f(w >> 16) : 0.0f;
+                for (int kk = 0; kk < KK; ++kk) k[tt][kk] = *reinterpret_cast<const u4*>(p + kk * 64);
+            } else {
+                code[tt] = *reinterpret_cast<const code_t*>(
+                    a.pool + (ok ? page + g.kc_off + cell * (D / 2) : dummy) + gq * (D / 8));
+                scales[tt] = ld_u16(a.pool + (ok ? page + g.ks_off + cell * 2 : dummy));
+                if (FMT == kProd)
+                    scales[tt] |= (uint32_t)ld_u16(a.pool + (ok ? page + g.kres_off + cell * 2 : dummy)) << 16;
             }
         }
-    }
-    // Every row sees every token of the wave.
-    uint32_t all = 0xffffu;
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) all &= live[tt];
-    const bool plain = all == 0xffffu && t0 + T <= q.L;
+    };
+    const int first = c * C + wt * T;
+    pages(first);
 
-    float acc[TT][4];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[tt][r] = 0.0f;
-
-    for (int rb = 0; rb < R; rb += kRowBlock) {
-        const int upto = min(R, rb + kRowBlock);
-        for (int r0 = rb; r0 < upto; r0 += 16) {
-            const int row = min(r0 + i, R - 1), tok = row / a.group;
-            const size_t nat = (size_t)(q.row0 + tok) * a.hq + h * a.group + (row - tok * a.group);
-            f4 x[TT], y[TT];
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) x[tt] = y[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            float row_scale = scale;
-            if constexpr (!kTurned) {
-                u4 qf[KK];
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-                    qf[kk] = *reinterpret_cast<const u4*>(a.query + nat * D + kk * 32 + gq * 8);
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<BF>(k[tt][kk], qf[kk], x[tt]);
-            } else {
-                u4 qh[KK], ql[KK];
-                const uint16_t* p = a.turned + nat * 2 * D + gq * (D / 4);
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    qh[kk] = *reinterpret_cast<const u4*>(p + kk * 8);
-                    ql[kk] = *reinterpret_cast<const u4*>(p + D + kk * 8);
-                }
-                row_scale = a.turned_scale[nat];
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, qh[kk], x[tt]);
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-                        if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, qh[kk], y[tt]);
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, ql[kk], x[tt]);
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-                        if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, ql[kk], y[tt]);
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].lo, qh[kk], x[tt]);
-                }
+    // The block's rows into LDS, in 16-byte pieces exchanged by an exclusive or with the
+    // row: the 16 rows that a load touches at one column are in different banks.
+    const auto nat_of = [&](int row) {
+        const int tok = row / a.group;
+        return (size_t)(q.row0 + tok) * a.hq + h * a.group + (row - tok * a.group);
+    };
+    const auto swz = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+    const auto stage = [&](int rb, int n) {
+        constexpr int kPieces = S::kRowBytes / 16;
+        if constexpr (!kTurned) {
+            for (int x = tid; x < n * kPieces; x += S::kThreads) {
+                const int r = x / kPieces, p = x % kPieces;
+                const size_t nat = nat_of(min(rb + r, R - 1));
+                *reinterpret_cast<u4*>(rows_mem + r * S::kRowBytes + (p ^ swz(r)) * 16) =
+                    *reinterpret_cast<const u4*>(a.query + nat * D + p * 8);
+                if (MODE == kSum && p == 0) ml[0][r] = rb + r < R ? a.stat[nat] : make_float2(INFINITY, 0.0f);
             }
-            // x in powers of two; what the row does not see: -infinity.
-            const int limit = min(q.L + (a.causal ? tok + 1 : 0), a.max_kv);
+        } else {
+            for (int x = tid; x < n * 2 * kPieces; x += S::kThreads) {
+                const int r = x / (2 * kPieces), y = x % (2 * kPieces), p = y % kPieces, part = y / kPieces;
+                const size_t nat = nat_of(min(rb + r, R - 1));
+                *reinterpret_cast<u4*>(rows_mem + part * 16384 + r * S::kRowBytes + (p ^ swz(r)) * 16) =
+                    *reinterpret_cast<const u4*>(a.turned + nat * 2 * D + part * D + p * 8);
+                if (y == 0) row_scales[r] = a.turned_scale[nat];
+                if (MODE == kSum && y == 0) ml[0][r] = rb + r < R ? a.stat[nat] : make_float2(INFINITY, 0.0f);
+            }
+        }
+    };
+
+    float acc[S::kSubs][TT][4];
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
+    for (int u = 0; u < S::kSubs; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = x[tt][r];
-                    if constexpr (kTurned) {
-                        if (FMT == kProd) v = fmaf(kr[tt][r], y[tt][r], v);
-                        v *= ks[tt][r];
-                    }
-                    x[tt][r] = v * row_scale;
-                }
-            if (!plain) {
+        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+            for (int r = 0; r < 4; ++r) acc[u][tt][r] = 0.0f;
+
+    if (S::kSubs == 1) fetch(first);
+    for (int rb = 0; rb < R; rb += kRowBlock) {
+        const int n = min((R - rb + 15) & ~15, kRowBlock);
+        if (rb) __syncthreads();
+        stage(rb, n);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < S::kSubs; ++u) {
+            const int t0 = first + u * 4 * T;
+            if (S::kSubs > 1) {
+                if (rb || u) pages(t0);
+                fetch(t0);
+            }
+            KeyParts kp[kTurned ? TT : 1][KK];
+            float ks[kTurned ? TT : 1][4], kr[kTurned ? TT : 1][4];  // of the tokens 4 gq + 0..3
+            if constexpr (kTurned) {
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) kp[tt][kk] = decode8<FMT>(code[tt][kk]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int t = tt * 16 + 4 * gq + r;
-                        if (t0 + t >= limit || !(live[tt] >> (4 * gq + r) & 1)) x[tt][r] = -INFINITY;
+                        const uint32_t w = (uint32_t)__shfl((int)scales[tt], 4 * gq + r, 64);
+                        ks[tt][r] = h2f(w & 0xffff);
+                        kr[tt][r] = FMT == kProd ? h2f(w >> 16) : 0.0f;
                     }
+                }
             }
-            if constexpr (MODE == kSum) {
-                float2 st = a.stat[nat];
-                if (r0 + i >= R) st = make_float2(INFINITY, 0.0f);
+            // Every row sees every token of the wave.
+            uint32_t all = 0xffffu;
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+            for (int tt = 0; tt < TT; ++tt) all &= live[tt];
+            const bool plain = all == 0xffffu && t0 + T <= q.L;
+            if (t0 >= q.end && (MODE == kSum || (MODE == kStats && u))) continue;
+
+            for (int r0 = wr * 16; r0 < n; r0 += 16 * WR) {
+                const int row = min(rb + r0 + i, R - 1);
+                const auto operand = [&](int part, int piece) {
+                    return *reinterpret_cast<const u4*>(rows_mem + part * 16384 + (r0 + i) * S::kRowBytes +
+                                                        (piece ^ swz(r0 + i)) * 16);
+                };
+                f4 x[TT], y[TT];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[tt][r] = fmaf(exp2_hw(x[tt][r] - st.x), st.y, acc[tt][r]);
-            } else {
-                float m = -INFINITY;
+                for (int tt = 0; tt < TT; ++tt) x[tt] = y[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                float rs = scale;
+                if constexpr (!kTurned) {
+                    u4 qf[KK];
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+                    for (int kk = 0; kk < KK; ++kk) qf[kk] = operand(0, kk * 4 + gq);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) m = fmaxf(m, x[tt][r]);
-                const auto larger = [](float u, float w) { return fmaxf(u, w); };
-                m = lane_xor_reduce<32>(lane_xor_reduce<16>(m, larger), larger);
-                const float ref = m == -INFINITY ? 0.0f : m;
-                float l = 0.0f;
+                    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<BF>(k[tt][kk], qf[kk], x[tt]);
+                } else {
+                    u4 qh[KK], ql[KK];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) l += exp2_hw(x[tt][r] - ref);
-                const auto sum = [](float u, float w) { return u + w; };
-                l = lane_xor_reduce<32>(lane_xor_reduce<16>(l, sum), sum);
-                if (gq == 0) ml[wv][r0 - rb + i] = make_float2(m, l);
-                if constexpr (MODE == kStore) {
-                    if (r0 + i < R) {
-                        float* to = a.logits + (int64_t)nat * a.logit_stride + t0 + 4 * gq;
+                    for (int kk = 0; kk < KK; ++kk) {
+                        qh[kk] = operand(0, gq * KK + kk);
+                        ql[kk] = operand(1, gq * KK + kk);
+                    }
+                    rs = row_scales[r0 + i];
 #pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f4*>(to + tt * 16) = x[tt];
+                    for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, qh[kk], x[tt]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt)
+                            if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, qh[kk], y[tt]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, ql[kk], x[tt]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt)
+                            if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, ql[kk], y[tt]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].lo, qh[kk], x[tt]);
+                    }
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (FMT == kProd) x[tt][r] = fmaf(kr[tt][r], y[tt][r], x[tt][r]);
+                            x[tt][r] *= ks[tt][r];
+                        }
+                }
+                // x rs: the logit in powers of two.  What the row does not see: -infinity.
+                if (!plain) {
+                    const int limit = min(q.L + (a.causal ? row / a.group + 1 : 0), a.max_kv);
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int t = tt * 16 + 4 * gq + r;
+                            if (t0 + t >= limit || !(live[tt] >> (4 * gq + r) & 1)) x[tt][r] = -INFINITY;
+                        }
+                }
+                const auto rounded = [&] {
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) x[tt] *= rs;
+                    rs = 1.0f;
+                };
+                if constexpr (MODE == kSum) {
+                    const float2 st = ml[0][r0 + i];
+                    if (__ballot(fabsf(st.x) >= kHuge)) rounded();
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
+                } else {
+                    if (MODE == kStore) rounded();
+                    float m = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+#pragma unroll
+                    for (int tt = 1; tt < TT; ++tt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) m = fmaxf(m, x[tt][r]);
+                    const auto larger = [](float u, float w) { return fmaxf(u, w); };
+                    m = lane_xor_reduce<32>(lane_xor_reduce<16>(m, larger), larger) * rs;
+                    if (MODE == kStats && __ballot(fabsf(m) >= kHuge)) rounded();
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) l4[r] += exp2_hw(fmaf(x[tt][r], rs, -ref));
+                    float l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    const auto sum = [](float u, float w) { return u + w; };
+                    l = lane_xor_reduce<32>(lane_xor_reduce<16>(l, sum), sum);
+                    if (gq == 0) {
+                        if (u) {  // (the wave's own entry)
+                            const float2 e = ml[wt][r0 + i];
+                            add_part(m, l, e);
+                        }
+                        ml[wt][r0 + i] = make_float2(m, l);
+                    }
+                    if constexpr (MODE == kStore) {
+                        if (rb + r0 + i < R) {
+                            float* to = a.logits + (int64_t)nat_of(row) * a.logit_stride + t0 + 4 * gq;
+#pragma unroll
+                            for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f4*>(to + tt * 16) = x[tt];
+                        }
                     }
                 }
             }
         }
         if constexpr (MODE != kSum) {
             __syncthreads();
-            for (int r = rb + tid; r < upto; r += 256) {
-                const int tok = r / a.group;
-                const size_t nat = (size_t)(q.row0 + tok) * a.hq + h * a.group + (r - tok * a.group);
+            for (int r = tid; r < min(n, R - rb); r += S::kThreads) {
                 float m = -INFINITY, l = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][r - rb].x);
+                for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][r].x);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const float2 e = ml[w][r - rb];
+                    const float2 e = ml[w][r];
                     l += e.x == -INFINITY ? e.y : e.y * exp2_hw(e.x - m);
                 }
-                a.part[(size_t)c * ((size_t)a.tokens * a.hq) + nat] = make_float2(m, l);
+                a.part[(size_t)c * ((size_t)a.tokens * a.hq) + nat_of(rb + r)] = make_float2(m, l);
             }
-            __syncthreads();
         }
     }
     if constexpr (MODE == kSum) {
+        // Over the lanes' rows, then over the waves that shared them.
+        __syncthreads();
+        float* sums = reinterpret_cast<float*>(rows_mem);  // [WR][C]
         const int64_t at = ((int64_t)s * g.H + h) * a.stride;
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            float mine = 0.0f;
+        for (int u = 0; u < S::kSubs; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float w = sum_lanes<16>(acc[tt][r]);
-                mine = i == r ? w : mine;
+            for (int tt = 0; tt < TT; ++tt) {
+                float mine = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float w = sum_lanes<16>(acc[u][tt][r]);
+                    mine = i == r ? w : mine;
+                }
+                if (i < 4) sums[wr * C + u * 4 * T + wt * T + tt * 16 + 4 * gq + i] = mine;
             }
-            const int t = t0 + tt * 16 + 4 * gq + i;
-            if (i < 4 && t < q.end) a.out[at + t] = a.in ? fmaf(a.decay, a.in[at + t], mine) : mine;
+        __syncthreads();
+        const int t = c * C + tid;
+        if (tid < C && t < q.end) {
+            float w = sums[tid];
+#pragma unroll
+            for (int k2 = 1; k2 < WR; ++k2) w += sums[k2 * C + tid];
+            a.out[at + t] = a.in ? fmaf(a.decay, a.in[at + t], w) : w;
         }
     }
 }
 
-// (max, sum) of a part added to a row's.
-__device__ __forceinline__ void add_part(float& m, float& l, float2 e) {
-    const float n = fmaxf(m, e.x);
-    l = (m == -INFINITY ? l : l * exp2_hw(m - n)) + (e.x == -INFINITY ? e.y : e.y * exp2_hw(e.x - n));
-    m = n;
-}
 // A row's (M, 1 / l); one that sees nothing gives every token 2^-infinity * 0.
 __device__ __forceinline__ float2 row_stat(float m, float l) {
     return l == 0.0f ? make_float2(INFINITY, 0.0f) : make_float2(m, 1.0f / l);
@@ -472,37 +562,36 @@ __device__ __forceinline__ int find_seq(const WeightArgs& a, int tok, int lane) 
     return lo;
 }
 
-// Chunks -> rows, 16 rows a workgroup and 16 parts of the chunks.  A wave holds rows of up
-// to 16 tokens, which may belong to several sequences.
-template <int FMT>
+// Chunks -> rows, 4 rows a workgroup and 64 lines of chunks.
 __global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
-    constexpr int C = 64 * kTT<FMT>;
-    __shared__ float2 ml[16][16];
-    const int lane = threadIdx.x & 63, i = threadIdx.x & 15, p = threadIdx.x >> 4;
-    const size_t rows = (size_t)a.tokens * a.hq, row = (size_t)blockIdx.x * 16 + i;
-    const int first = (int)((size_t)blockIdx.x * 16 / a.hq), last = (int)(min((size_t)blockIdx.x * 16 + 15, rows - 1) / a.hq);
-    const int tok = (int)(min(row, rows - 1) / a.hq);
+    __shared__ float2 ml[4][4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, i = lane & 3, p = threadIdx.x >> 2;
+    const size_t rows = (size_t)a.tokens * a.hq, row0 = (size_t)blockIdx.x * 4, row = min(row0 + i, rows - 1);
+    const int last = (int)(min(row0 + 3, rows - 1) / a.hq), tok = (int)(row / a.hq);
     int n = 0;
-    for (int t = first; t <= last; ++t) {
-        const int s = find_seq(a, t, lane);
-        const Seq q = seq_of(a, s);
-        if (t == tok && t >= q.row0 && t < q.row0 + q.rows) n = (q.end + C - 1) / C;
+    for (int t = (int)(row0 / a.hq); t <= last; ++t) {  // (one token, or a few of few heads)
+        const Seq q = seq_of(a, find_seq(a, t, lane));
+        if (t == tok && t >= q.row0 && t < q.row0 + q.rows) n = (q.end + kChunk - 1) / kChunk;
     }
     float m = -INFINITY, l = 0.0f;
-    if (row < rows)
-        for (int c = p; c < n; c += 16) add_part(m, l, a.part[(size_t)c * rows + row]);
-    ml[p][i] = make_float2(m, l);
+    for (int c = p; c < n; c += 128) {
+        const float2 e0 = a.part[(size_t)c * rows + row], e1 = a.part[(size_t)min(c + 64, n - 1) * rows + row];
+        add_part(m, l, e0);
+        if (c + 64 < n) add_part(m, l, e1);
+    }
+#pragma unroll
+    for (int k = 4; k < 64; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
+    if (lane < 4) ml[wv][i] = make_float2(m, l);
     __syncthreads();
-    if (p || row >= rows) return;
-    for (int k = 1; k < 16; ++k) add_part(m, l, ml[k][i]);
+    if (threadIdx.x >= 4 || row0 + i >= rows) return;
+    for (int k = 1; k < 4; ++k) add_part(m, l, ml[k][i]);
     a.stat[row] = row_stat(m, l);
 }
 
 // The weights of stored x: 1,024 tokens of one kv head a workgroup.
 constexpr int kSumTokens = 1024;
-template <int FMT>
 __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
-    constexpr int C = 64 * kTT<FMT>;
+    constexpr int C = kChunk;
     __shared__ float2 st[16];
     const int tid = threadIdx.x, i = tid & 15, p = tid >> 4;
     const int blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
@@ -555,7 +644,7 @@ dim3 grid_of(long long blocks) {
 template <int FMT, int D>
 void launch_format(WeightArgs a, hipStream_t stream) {
     constexpr bool kTurned = FMT == kProd || FMT == kMse;
-    constexpr int C = 64 * kTT<FMT>;
+    constexpr int C = kChunk;
     const size_t rows = (size_t)a.tokens * a.hq;
     a.chunks = (a.max_kv + C - 1) / C;
     a.logit_stride = (int64_t)a.chunks * C;
@@ -583,18 +672,27 @@ void launch_format(WeightArgs a, hipStream_t stream) {
     }
     const dim3 grid = grid_of(((long long)a.seqs * a.chunks + 7) / 8 * 8 * a.g.H);
     if (store) {
-        if (rows) hipLaunchKernelGGL((weights_kernel<FMT, D, kStore>), grid, dim3(256), 0, stream, a, scale);
+        if (rows) hipLaunchKernelGGL((weights_kernel<FMT, D, 1, kStore>), grid, dim3(256), 0, stream, a, scale);
         check_launch("attention_weights_kernel");
         const long long blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
-        hipLaunchKernelGGL(weights_sum_kernel<FMT>, grid_of(blocks * a.seqs * a.g.H), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(weights_sum_kernel, grid_of(blocks * a.seqs * a.g.H), dim3(256), 0, stream, a);
         check_launch("attention_weights_sum_kernel");
         return;
     }
-    hipLaunchKernelGGL((weights_kernel<FMT, D, kStats>), grid, dim3(256), 0, stream, a, scale);
+    const auto pass = [&](auto mode, auto wr) {
+        constexpr int MODE = decltype(mode)::value, WR = decltype(wr)::value;
+        hipLaunchKernelGGL((weights_kernel<FMT, D, WR, MODE>), grid, dim3(256 * WR), 0, stream, a, scale);
+    };
+    // Two waves share a token's rows where there are few chunks.
+    const bool two = (long long)a.seqs * a.chunks * a.g.H < 4LL * num_cus();
+    const auto both = [&](auto mode) {
+        two ? pass(mode, std::integral_constant<int, 2>{}) : pass(mode, std::integral_constant<int, 1>{});
+    };
+    both(std::integral_constant<int, kStats>{});
     check_launch("attention_weights_kernel");
-    hipLaunchKernelGGL(weights_rows_kernel<FMT>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(weights_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
     check_launch("attention_weights_rows_kernel");
-    hipLaunchKernelGGL((weights_kernel<FMT, D, kSum>), grid, dim3(256), 0, stream, a, scale);
+    both(std::integral_constant<int, kSum>{});
     check_launch("attention_weights_sum_kernel");
 }
 
@@ -637,9 +735,9 @@ int weights_entry(const char* name, int fmt, Geom&& geom, const void* query, con
             throw Error(w + "score_stride must be at least max_kv_len");
         if (!(decay >= 0.0f) || decay > 1.0f) throw Error(w + "decay must be in [0, 1]");
         if ((long long)tokens * hq > (1LL << 26)) throw Error(w + "num_tokens * num_q_heads must be at most 2^26");
-        const long long chunks = (max_kv + 127) / 128;
+        const long long chunks = (max_kv + kChunk - 1) / kChunk;
         if (chunks * std::max<long long>((long long)tokens * hq, (long long)seqs * g.H) > (1LL << 30))
-            throw Error(w + "too many (row, 128 tokens) or (sequence, kv head, 128 tokens) pairs (2^30)");
+            throw Error(w + "too many (row, 256 tokens) or (sequence, kv head, 256 tokens) pairs (2^30)");
         const uint64_t cells = (uint64_t)g.block_size * g.H;
         const auto outside = [&](uint64_t off, uint64_t size) {
             return off > g.page_size || cells * size > g.page_size - off;
