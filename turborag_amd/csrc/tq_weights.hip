@@ -33,8 +33,9 @@ struct WeightArgs {
     float decay;
     PageGeom g;  // dense pages: kc_off and code_stride of fp16/bf16 rows
     int max_blocks, hq, group, seqs, tokens, max_kv, causal;  // group: query heads per kv head
+    uint32_t group_mul, group_shift;  // of the division by it
     // The workspace.  A row's index is that of its query: token * hq + query head.
-    int chunks;             // of every sequence
+    int chunk;              // tokens of a statistic
     float* logits;          // [rows][logit_stride]: x, or null
     int64_t logit_stride;
     float2* part;           // [chunks][rows]: (max, sum) of a chunk
@@ -61,6 +62,12 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0,
                                                       0);
+}
+
+// n / group, n < 2^31: with 2^(shift - 1) < group <= 2^shift and mul = ceil(2^(32 + shift) /
+// group) - 2^32, n (2^32 + mul) / 2^(32 + shift) is n / group and less than 1 / group more.
+__device__ __forceinline__ int over_group(const WeightArgs& a, int n) {
+    return (int)((__umulhi((uint32_t)n, a.group_mul) + (uint32_t)n) >> a.group_shift);
 }
 
 // A sequence's rows and tokens, as far as the call's bounds allow.
@@ -164,14 +171,13 @@ __device__ __forceinline__ KeyParts decode8(uint32_t w) {
 // power of two to a largest value in [2^13, 2^14) (22 bits of it are kept and no row
 // leaves fp16's range); D / 8 lanes a row, eight dims each.
 // ---------------------------------------------------------------------------
+struct Turned {
+    u4 hi, lo;
+    float unscale;  // undoes the power of two
+};
 template <int D>
-__global__ __launch_bounds__(256) void turn_queries_kernel(const uint16_t* __restrict__ query, int hq, int group,
-                                                           int rows, uint16_t* __restrict__ turned,
-                                                           float* __restrict__ turned_scale, float scale) {
+__device__ __forceinline__ Turned turn_query(u4 raw, int h, int j) {
     constexpr int L = D / 8;
-    const int j = threadIdx.x % L, at = blockIdx.x * (256 / L) + threadIdx.x / L;
-    const int row = min(at, rows - 1), h = row % hq / group;
-    const u4 raw = *reinterpret_cast<const u4*>(query + (size_t)row * D + 8 * j);
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = h2f(raw[e / 2] >> (16 * (e & 1)) & 0xffff) * sign_of(e, h);
@@ -198,18 +204,31 @@ __global__ __launch_bounds__(256) void turn_queries_kernel(const uint16_t* __res
     const int ex = (int)(__float_as_uint(top) >> 23) - 127;
     const int sh = top > 0.0f && ex < 128 ? 13 - max(ex, -100) : 0;
     const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-    if (at != row) return;
-    u4 hi, lo;
+    Turned t;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {  // dims 0 2 | 4 6 | 1 3 | 5 7
         const int d = (p & 1) * 4 + (p >> 1);
         const float u = x[d] * up, v = x[d + 2] * up;
-        hi[p] = f2h2(u, v);
-        lo[p] = f2h2(u - h2f(hi[p] & 0xffff), v - h2f(hi[p] >> 16));
+        t.hi[p] = f2h2(u, v);
+        t.lo[p] = f2h2(u - h2f(t.hi[p] & 0xffff), v - h2f(t.hi[p] >> 16));
     }
-    *reinterpret_cast<u4*>(turned + (size_t)row * 2 * D + 8 * j) = hi;
-    *reinterpret_cast<u4*>(turned + (size_t)row * 2 * D + D + 8 * j) = lo;
-    if (j == 0) turned_scale[row] = scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+    t.unscale = __uint_as_float((uint32_t)(127 - sh) << 23);
+    return t;
+}
+// All rows, for the passes that go over more than a few.
+template <int D>
+__global__ __launch_bounds__(256) void turn_queries_kernel(const uint16_t* __restrict__ query, int hq, int group,
+                                                           int rows, uint16_t* __restrict__ turned,
+                                                           float* __restrict__ turned_scale, float scale) {
+    constexpr int L = D / 8;
+    const int j = threadIdx.x % L, at = blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int row = min(at, rows - 1);
+    const u4 raw = *reinterpret_cast<const u4*>(query + (size_t)row * D + 8 * j);
+    const Turned t = turn_query<D>(raw, row % hq / group, j);
+    if (at != row) return;
+    *reinterpret_cast<u4*>(turned + (size_t)row * 2 * D + 8 * j) = t.hi;
+    *reinterpret_cast<u4*>(turned + (size_t)row * 2 * D + D + 8 * j) = t.lo;
+    if (j == 0) turned_scale[row] = scale * t.unscale;
 }
 
 // (max, sum) of a part added to a row's.
@@ -227,37 +246,42 @@ __device__ __forceinline__ void add_part(float& m, float& l, float2 e) {
 // transposed (K Q'): a query row is a lane column, so its maximum and sum are in-lane
 // but for two lane swaps, and a token's sum over the rows is in-lane over the tiles,
 // across 16 lanes once at the end.
-//   kStats: (max, sum) of the chunk for every row;  kStore: x too;
+//   kStats: (max, sum) of the chunk for every row;  kStore, kStoreFew: x too;
 //   kSum: the weights, summed over the rows.
+// kStoreFew (up to 16 rows): small blocks, whose queries it rotates itself.
 // ---------------------------------------------------------------------------
-constexpr int kStats = 0, kStore = 1, kSum = 2;
-constexpr int kChunk = 256;
+#ifndef TURNED_TT
+#define TURNED_TT 2
+#endif
+constexpr int kStats = 0, kStore = 1, kSum = 2, kStoreFew = 3;
 // x is exact to half an ulp; its difference from a reference of this size on is taken
 // after x itself is rounded, so that no exponent is above 0 (one of up to half an ulp of
 // the reference otherwise, the same in both passes).
 constexpr float kHuge = 4194304.0f;
 
-template <int FMT, int D, int WR, int MODE>
+template <int FMT, int D, int WT, int WR, int MODE>
 struct Shape {
     static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
     // (compressed pages: three operands a token tile)
-    static constexpr int TT = kTurned ? 2 : 4, T = 16 * TT, kSubs = kChunk / (4 * T);
+    static constexpr int TT = kTurned ? TURNED_TT : 4, T = 16 * TT, kSubs = kTurned ? 4 / TT : 1, C = T * WT * kSubs;
     static constexpr int kParts = kTurned ? 2 : 1;  // of a query row
     static constexpr int kRowBytes = 2 * D;
-    static constexpr int kRowBlock = 32768 / (kParts * kRowBytes);
-    static constexpr int kThreads = 256 * WR;
+    static constexpr bool kStores = MODE == kStore || MODE == kStoreFew, kTurns = kTurned && MODE == kStoreFew;
+    static constexpr int kPart = MODE == kStoreFew ? 4096 : MODE == kStore && !kTurned ? 8192 : 32768 / kParts;  // bytes of a block's part
+    static constexpr int kRowBlock = kPart / kRowBytes;
+    static constexpr int kThreads = 64 * WT * WR;
 };
 
-template <int FMT, int D, int WR, int MODE>
-__global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a, float scale) {
-    using S = Shape<FMT, D, WR, MODE>;
+template <int FMT, int D, int WT, int WR, int MODE>
+__global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightArgs a, float scale) {
+    using S = Shape<FMT, D, WT, WR, MODE>;
     constexpr bool kTurned = S::kTurned, BF = S::BF;
-    constexpr int TT = S::TT, T = S::T, KK = D / 32, C = kChunk, kRowBlock = S::kRowBlock;
-    __shared__ __attribute__((aligned(16))) uint8_t rows_mem[32768];
+    constexpr int TT = S::TT, T = S::T, KK = D / 32, C = S::C, kRowBlock = S::kRowBlock;
+    __shared__ __attribute__((aligned(16))) uint8_t rows_mem[S::kPart * S::kParts];
     __shared__ float row_scales[kTurned ? kRowBlock : 1];
-    __shared__ float2 ml[MODE == kSum ? 1 : 4][kRowBlock];  // kSum: the rows' (M, 1 / l)
+    __shared__ float2 ml[MODE == kSum ? 1 : WT][kRowBlock];  // kSum: the rows' (M, 1 / l)
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, gq = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wv & 3, wr = wv >> 2;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wv % WT, wr = wv / WT;
     const PageGeom& g = a.g;
 
     // Eight chunks in turn, then the same ones of the next head: the workgroups of one
@@ -265,8 +289,9 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
     const unsigned b = blockIdx.y * gridDim.x + blockIdx.x, eight = b / 8;
     const int h = (int)(eight % (unsigned)g.H);
     const long long sc = (long long)(eight / (unsigned)g.H) * 8 + b % 8;
-    if (sc >= (long long)a.seqs * a.chunks) return;
-    const int s = (int)(sc / a.chunks), c = (int)(sc - (long long)s * a.chunks);
+    const int chunks = (a.max_kv + C - 1) / C;
+    if (sc >= (long long)a.seqs * chunks) return;
+    const int s = (int)(sc / chunks), c = (int)(sc - (long long)s * chunks);
     const Seq q = seq_of(a, s);
     if (c * C >= q.end) return;
     const int R = q.rows * a.group;
@@ -317,36 +342,62 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
         }
     };
     const int first = c * C + wt * T;
-    pages(first);
 
     // The block's rows into LDS, in 16-byte pieces exchanged by an exclusive or with the
-    // row: the 16 rows that a load touches at one column are in different banks.
+    // row: the 16 rows that a load touches at one column are in different banks.  They are
+    // on their way (in registers) while the block before is worked on, the first one
+    // while K is.
     const auto nat_of = [&](int row) {
-        const int tok = row / a.group;
+        const int tok = over_group(a, row);
         return (size_t)(q.row0 + tok) * a.hq + h * a.group + (row - tok * a.group);
     };
     const auto swz = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
-    const auto stage = [&](int rb, int n) {
-        constexpr int kPieces = S::kRowBytes / 16;
-        if constexpr (!kTurned) {
-            for (int x = tid; x < n * kPieces; x += S::kThreads) {
-                const int r = x / kPieces, p = x % kPieces;
-                const size_t nat = nat_of(min(rb + r, R - 1));
-                *reinterpret_cast<u4*>(rows_mem + r * S::kRowBytes + (p ^ swz(r)) * 16) =
-                    *reinterpret_cast<const u4*>(a.query + nat * D + p * 8);
-                if (MODE == kSum && p == 0) ml[0][r] = rb + r < R ? a.stat[nat] : make_float2(INFINITY, 0.0f);
-            }
-        } else {
-            for (int x = tid; x < n * 2 * kPieces; x += S::kThreads) {
-                const int r = x / (2 * kPieces), y = x % (2 * kPieces), p = y % kPieces, part = y / kPieces;
-                const size_t nat = nat_of(min(rb + r, R - 1));
-                *reinterpret_cast<u4*>(rows_mem + part * 16384 + r * S::kRowBytes + (p ^ swz(r)) * 16) =
-                    *reinterpret_cast<const u4*>(a.turned + nat * 2 * D + part * D + p * 8);
-                if (y == 0) row_scales[r] = a.turned_scale[nat];
-                if (MODE == kSum && y == 0) ml[0][r] = rb + r < R ? a.stat[nat] : make_float2(INFINITY, 0.0f);
-            }
+    constexpr int kPieces = S::kRowBytes / 16 * S::kParts, kHold = S::kTurns ? 1 : S::kPart * S::kParts / 16 / S::kThreads;
+    u4 hold[kHold];
+    float2 hold_stat;
+    float hold_scale;
+    const auto take = [&](int rb) {
+        if constexpr (S::kTurns) {  // D / 8 lanes a row
+            static_assert(kRowBlock * (D / 8) == S::kThreads, "a thread per eight dims of a block");
+            hold[0] = *reinterpret_cast<const u4*>(a.query + nat_of(min(rb + tid / (D / 8), R - 1)) * D + tid % (D / 8) * 8);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) {
+            const int x = k * S::kThreads + tid, p = x % kPieces;
+            const size_t nat = nat_of(min(rb + x / kPieces, R - 1));
+            hold[k] = *reinterpret_cast<const u4*>((kTurned ? a.turned : a.query) + nat * (S::kParts * D) + p * 8);
+        }
+        static_assert(kRowBlock <= S::kThreads, "a thread per row of a block");
+        if (kTurned || MODE == kSum) {
+            const size_t nat = nat_of(min(rb + tid, R - 1));
+            if (kTurned) hold_scale = a.turned_scale[nat];
+            if (MODE == kSum) hold_stat = a.stat[nat];
         }
     };
+    const auto put = [&](int rb) {
+        if constexpr (S::kTurns) {
+            const int r = tid / (D / 8), p = tid % (D / 8);
+            const Turned t = turn_query<D>(hold[0], h, p);
+            uint8_t* to = rows_mem + r * S::kRowBytes + (p ^ swz(r)) * 16;
+            *reinterpret_cast<u4*>(to) = t.hi;
+            *reinterpret_cast<u4*>(to + S::kPart) = t.lo;
+            if (p == 0) row_scales[r] = scale * t.unscale;
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) {
+            const int x = k * S::kThreads + tid, r = x / kPieces, y = x % kPieces;
+            const int p = y % (S::kRowBytes / 16), part = y / (S::kRowBytes / 16);
+            *reinterpret_cast<u4*>(rows_mem + part * S::kPart + r * S::kRowBytes + (p ^ swz(r)) * 16) = hold[k];
+        }
+        if (tid < kRowBlock) {
+            if (kTurned) row_scales[tid] = hold_scale;
+            if (MODE == kSum) ml[0][tid] = rb + tid < R ? hold_stat : make_float2(INFINITY, 0.0f);
+        }
+    };
+    take(0);
+    pages(first);
 
     float acc[S::kSubs][TT][4];
 #pragma unroll
@@ -360,11 +411,13 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
     for (int rb = 0; rb < R; rb += kRowBlock) {
         const int n = min((R - rb + 15) & ~15, kRowBlock);
         if (rb) __syncthreads();
-        stage(rb, n);
+        if (kTurned && rb) take(rb);
+        put(rb);
         __syncthreads();
+        if (!kTurned && rb + kRowBlock < R) take(rb + kRowBlock);  // (those have no registers left)
 #pragma unroll
         for (int u = 0; u < S::kSubs; ++u) {
-            const int t0 = first + u * 4 * T;
+            const int t0 = first + u * WT * T;
             if (S::kSubs > 1) {
                 if (rb || u) pages(t0);
                 fetch(t0);
@@ -394,7 +447,7 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
             for (int r0 = wr * 16; r0 < n; r0 += 16 * WR) {
                 const int row = min(rb + r0 + i, R - 1);
                 const auto operand = [&](int part, int piece) {
-                    return *reinterpret_cast<const u4*>(rows_mem + part * 16384 + (r0 + i) * S::kRowBytes +
+                    return *reinterpret_cast<const u4*>(rows_mem + part * S::kPart + (r0 + i) * S::kRowBytes +
                                                         (piece ^ swz(r0 + i)) * 16);
                 };
                 f4 x[TT], y[TT];
@@ -442,7 +495,7 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
                 }
                 // x rs: the logit in powers of two.  What the row does not see: -infinity.
                 if (!plain) {
-                    const int limit = min(q.L + (a.causal ? row / a.group + 1 : 0), a.max_kv);
+                    const int limit = min(q.L + (a.causal ? over_group(a, row) + 1 : 0), a.max_kv);
 #pragma unroll
                     for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
@@ -465,7 +518,7 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
                         for (int r = 0; r < 4; ++r)
                             acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
                 } else {
-                    if (MODE == kStore) rounded();
+                    if (S::kStores) rounded();
                     float m = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
 #pragma unroll
                     for (int tt = 1; tt < TT; ++tt)
@@ -490,7 +543,7 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
                         }
                         ml[wt][r0 + i] = make_float2(m, l);
                     }
-                    if constexpr (MODE == kStore) {
+                    if constexpr (S::kStores) {
                         if (rb + r0 + i < R) {
                             float* to = a.logits + (int64_t)nat_of(row) * a.logit_stride + t0 + 4 * gq;
 #pragma unroll
@@ -505,9 +558,9 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
             for (int r = tid; r < min(n, R - rb); r += S::kThreads) {
                 float m = -INFINITY, l = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][r].x);
+                for (int w = 0; w < WT; ++w) m = fmaxf(m, ml[w][r].x);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+                for (int w = 0; w < WT; ++w) {
                     const float2 e = ml[w][r];
                     l += e.x == -INFINITY ? e.y : e.y * exp2_hw(e.x - m);
                 }
@@ -530,9 +583,10 @@ __global__ __launch_bounds__(256 * WR, 2) void weights_kernel(const WeightArgs a
                     const float w = sum_lanes<16>(acc[u][tt][r]);
                     mine = i == r ? w : mine;
                 }
-                if (i < 4) sums[wr * C + u * 4 * T + wt * T + tt * 16 + 4 * gq + i] = mine;
+                if (i < 4) sums[wr * C + u * WT * T + wt * T + tt * 16 + 4 * gq + i] = mine;
             }
         __syncthreads();
+        static_assert(C <= S::kThreads, "a thread per token");
         const int t = c * C + tid;
         if (tid < C && t < q.end) {
             float w = sums[tid];
@@ -571,7 +625,7 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
     int n = 0;
     for (int t = (int)(row0 / a.hq); t <= last; ++t) {  // (one token, or a few of few heads)
         const Seq q = seq_of(a, find_seq(a, t, lane));
-        if (t == tok && t >= q.row0 && t < q.row0 + q.rows) n = (q.end + kChunk - 1) / kChunk;
+        if (t == tok && t >= q.row0 && t < q.row0 + q.rows) n = (q.end + a.chunk - 1) / a.chunk;
     }
     float m = -INFINITY, l = 0.0f;
     for (int c = p; c < n; c += 128) {
@@ -588,11 +642,11 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
     a.stat[row] = row_stat(m, l);
 }
 
-// The weights of stored x: 1,024 tokens of one kv head a workgroup.
-constexpr int kSumTokens = 1024;
+// The weights of stored x: 1,024 tokens of one kv head a workgroup, four a thread.  Eight
+// rows' x are on their way while the rows' statistics are put together (16 lanes a row).
+constexpr int kSumTokens = 1024, kSumRows = 64;
 __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
-    constexpr int C = kChunk;
-    __shared__ float2 st[16];
+    __shared__ float2 st[kSumRows];
     const int tid = threadIdx.x, i = tid & 15, p = tid >> 4;
     const int blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
     const unsigned b = blockIdx.y * gridDim.x + blockIdx.x;
@@ -601,39 +655,68 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
     if (s >= a.seqs) return;
     const Seq q = seq_of(a, s);
     if (blk * kSumTokens >= q.end) return;
-    const int R = q.rows * a.group, n = (q.end + C - 1) / C, t = blk * kSumTokens + tid * 4;
+    const int C = a.chunk, R = q.rows * a.group, n = (q.end + C - 1) / C, t = blk * kSumTokens + tid * 4;
     const size_t rows = (size_t)a.tokens * a.hq;
-    const bool inside = t < n * C;  // (x is there up to the end of the last chunk)
-    f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int r0 = 0; r0 < R; r0 += 16) {
-        const int upto = min(16, R - r0);
-        const auto nat_of = [&](int r) {
-            const int tok = r / a.group;
-            return (size_t)(q.row0 + tok) * a.hq + h * a.group + (r - tok * a.group);
-        };
-        // statistics: 16 lanes a row
-        if (r0) __syncthreads();
-        float m = -INFINITY, l = 0.0f;
-        if (p < upto) {
-            const size_t nat = nat_of(r0 + p);
-            for (int c = i; c < n; c += 16) add_part(m, l, a.part[(size_t)c * rows + nat]);
-        }
+    // (x is there up to the end of the last chunk)
+    const int at_t = min(t, n * C - 4);
+    const auto nat_of = [&](int r) {
+        const int tok = over_group(a, r);
+        return (size_t)(q.row0 + tok) * a.hq + h * a.group + (r - tok * a.group);
+    };
+    constexpr int kDeep = 8;
+    f4 x[kDeep], acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    const auto load = [&](int r0) {
 #pragma unroll
-        for (int k = 1; k < 16; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
-        if (i == 0 && p < upto) st[p] = row_stat(m, l);
-        __syncthreads();
-        if (inside)
-            for (int r = 0; r < upto; ++r) {
-                const f4 x = *reinterpret_cast<const f4*>(a.logits + (int64_t)nat_of(r0 + r) * a.logit_stride + t);
-                const float2 e = st[r];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] = fmaf(exp2_hw(x[k] - e.x), e.y, acc[k]);
-            }
-    }
+        for (int k = 0; k < kDeep; ++k)
+            x[k] = *reinterpret_cast<const f4*>(a.logits + (int64_t)nat_of(min(r0 + k, R - 1)) * a.logit_stride + at_t);
+    };
+    if (R) load(0);
     const int64_t at = (int64_t)sh * a.stride + t;
+    // (a row of scores may begin at any float)
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+    const bool four = t + 4 <= q.end;
+    f4 before = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.in) {
+        if (four)
+            before = *reinterpret_cast<const f4u*>(a.in + at);
+        else
+            for (int k = 0; t + k < q.end; ++k) before[k] = a.in[at + k];
+    }
+    for (int r0 = 0; r0 < R; r0 += kSumRows) {
+        const int upto = min(kSumRows, R - r0);
+        if (r0) __syncthreads();
+        for (int g0 = 0; g0 < upto; g0 += 16) {
+            float m = -INFINITY, l = 0.0f;
+            const size_t nat = nat_of(min(r0 + g0 + p, R - 1));
+            for (int c = i; c < n; c += 128) {
+                float2 e[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (t + k < q.end) a.out[at + k] = a.in ? fmaf(a.decay, a.in[at + k], acc[k]) : acc[k];
+                for (int k = 0; k < 8; ++k) e[k] = a.part[(size_t)min(c + 16 * k, n - 1) * rows + nat];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + 16 * k < n) add_part(m, l, e[k]);
+            }
+#pragma unroll
+            for (int k = 1; k < 16; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
+            if (i == 0) st[g0 + p] = g0 + p < upto ? row_stat(m, l) : make_float2(INFINITY, 0.0f);
+        }
+        __syncthreads();
+        for (int r = 0; r < upto; r += kDeep) {
+            if (r0 + r) load(r0 + r);
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const float2 e = st[r + k];  // (a row that is none: weights of 0)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) acc[w] = fmaf(exp2_hw(x[k][w] - e.x), e.y, acc[w]);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = a.in ? fmaf(a.decay, before[k], acc[k]) : acc[k];
+    if (four)
+        *reinterpret_cast<f4u*>(a.out + at) = acc;
+    else
+        for (int k = 0; t + k < q.end; ++k) a.out[at + k] = acc[k];
 }
 
 dim3 grid_of(long long blocks) {
@@ -641,20 +724,29 @@ dim3 grid_of(long long blocks) {
     return dim3(x, (unsigned)((blocks + x - 1) / x));
 }
 
+#ifndef STAT_WT
+#define STAT_WT 2
+#define STAT_WR 2
+#define SUM_WT 2
+#define SUM_WR 2
+#endif
+constexpr int kStatWT = STAT_WT, kStatWR = STAT_WR, kSumWT = SUM_WT, kSumWR = SUM_WR, kStatChunk = 64 * kStatWT;
+
 template <int FMT, int D>
 void launch_format(WeightArgs a, hipStream_t stream) {
     constexpr bool kTurned = FMT == kProd || FMT == kMse;
-    constexpr int C = kChunk;
+    constexpr int kStoreMost = kTurned ? 64 : 32;
     const size_t rows = (size_t)a.tokens * a.hq;
-    a.chunks = (a.max_kv + C - 1) / C;
-    a.logit_stride = (int64_t)a.chunks * C;
     // x is stored where that moves fewer bytes than K's second reading.
     const long long per_seq = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
-    const bool store = per_seq <= 32 && rows * (size_t)a.logit_stride * 4 <= (size_t(256) << 20);
+    const size_t padded = ((size_t)a.max_kv + 255) / 256 * 256;
+    const bool store = per_seq <= kStoreMost && rows * padded * 4 <= (size_t(256) << 20), few = store && per_seq <= 16;
+    a.chunk = store || kTurned ? 256 : kStatChunk;
+    a.logit_stride = (int64_t)padded;
     const auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
-    const size_t parts = up((size_t)a.chunks * rows * sizeof(float2));
-    const size_t second = store ? up(rows * (size_t)a.logit_stride * 4) : up(rows * sizeof(float2));
-    const size_t turned = kTurned ? up(rows * 4 * D) : 0, scales = kTurned ? up(rows * 4) : 0;
+    const size_t parts = up(((size_t)a.max_kv + a.chunk - 1) / a.chunk * rows * sizeof(float2));
+    const size_t second = store ? up(rows * padded * 4) : up(rows * sizeof(float2));
+    const size_t turned = kTurned && !few ? up(rows * 4 * D) : 0, scales = kTurned && !few ? up(rows * 4) : 0;
     const WorkspaceTurn turn(stream);
     uint8_t* ws = static_cast<uint8_t*>(Scratch{}.get(stream, parts + second + turned + scales, "attention weights"));
     a.part = reinterpret_cast<float2*>(ws);
@@ -663,37 +755,41 @@ void launch_format(WeightArgs a, hipStream_t stream) {
     a.turned = reinterpret_cast<uint16_t*>(ws + parts + second);
     a.turned_scale = reinterpret_cast<float*>(ws + parts + second + turned);
     const float scale = 1.44269504f * inv_sqrt_d(D);
-    if (kTurned && rows) {
+    if (kTurned && rows && !few) {
         constexpr int per = 256 / (D / 8);
         hipLaunchKernelGGL(turn_queries_kernel<D>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a.query,
                            a.hq, a.group, (int)rows, const_cast<uint16_t*>(a.turned),
                            const_cast<float*>(a.turned_scale), scale * inv_sqrt_d(D));
         check_launch("attention_weights_turn_kernel");
     }
-    const dim3 grid = grid_of(((long long)a.seqs * a.chunks + 7) / 8 * 8 * a.g.H);
+    const auto pass = [&](auto wt, auto wr, auto mode) {
+        constexpr int WT = decltype(wt)::value, WR = decltype(wr)::value, MODE = decltype(mode)::value;
+        using S = Shape<FMT, D, WT, WR, MODE>;
+        const long long chunks = ((long long)a.max_kv + S::C - 1) / S::C;
+        hipLaunchKernelGGL((weights_kernel<FMT, D, WT, WR, MODE>), grid_of((a.seqs * chunks + 7) / 8 * 8 * a.g.H),
+                           dim3(S::kThreads), 0, stream, a, kTurned ? scale * inv_sqrt_d(D) : scale);
+        check_launch(MODE == kSum ? "attention_weights_sum_kernel" : "attention_weights_kernel");
+    };
+    using std::integral_constant;
+    constexpr integral_constant<int, 1> one{};
+    constexpr integral_constant<int, 4> four{};
     if (store) {
-        if (rows) hipLaunchKernelGGL((weights_kernel<FMT, D, 1, kStore>), grid, dim3(256), 0, stream, a, scale);
-        check_launch("attention_weights_kernel");
+        if (rows) few ? pass(four, one, integral_constant<int, kStoreFew>{}) : pass(four, one, integral_constant<int, kStore>{});
         const long long blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
         hipLaunchKernelGGL(weights_sum_kernel, grid_of(blocks * a.seqs * a.g.H), dim3(256), 0, stream, a);
         check_launch("attention_weights_sum_kernel");
         return;
     }
-    const auto pass = [&](auto mode, auto wr) {
-        constexpr int MODE = decltype(mode)::value, WR = decltype(wr)::value;
-        hipLaunchKernelGGL((weights_kernel<FMT, D, WR, MODE>), grid, dim3(256 * WR), 0, stream, a, scale);
-    };
-    // Two waves share a token's rows where there are few chunks.
-    const bool two = (long long)a.seqs * a.chunks * a.g.H < 4LL * num_cus();
-    const auto both = [&](auto mode) {
-        two ? pass(mode, std::integral_constant<int, 2>{}) : pass(mode, std::integral_constant<int, 1>{});
-    };
-    both(std::integral_constant<int, kStats>{});
-    check_launch("attention_weights_kernel");
+    if constexpr (kTurned)
+        pass(four, one, integral_constant<int, kStats>{});
+    else
+        pass(integral_constant<int, kStatWT>{}, integral_constant<int, kStatWR>{}, integral_constant<int, kStats>{});
     hipLaunchKernelGGL(weights_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
     check_launch("attention_weights_rows_kernel");
-    both(std::integral_constant<int, kSum>{});
-    check_launch("attention_weights_sum_kernel");
+    if constexpr (kTurned)
+        pass(four, one, integral_constant<int, kSum>{});
+    else
+        pass(integral_constant<int, kSumWT>{}, integral_constant<int, kSumWR>{}, integral_constant<int, kSum>{});
 }
 
 bool aligned(uint64_t v, uint64_t a) { return (v & (a - 1)) == 0; }
@@ -735,9 +831,9 @@ int weights_entry(const char* name, int fmt, Geom&& geom, const void* query, con
             throw Error(w + "score_stride must be at least max_kv_len");
         if (!(decay >= 0.0f) || decay > 1.0f) throw Error(w + "decay must be in [0, 1]");
         if ((long long)tokens * hq > (1LL << 26)) throw Error(w + "num_tokens * num_q_heads must be at most 2^26");
-        const long long chunks = (max_kv + kChunk - 1) / kChunk;
+        const long long chunks = (max_kv + 127) / 128;
         if (chunks * std::max<long long>((long long)tokens * hq, (long long)seqs * g.H) > (1LL << 30))
-            throw Error(w + "too many (row, 256 tokens) or (sequence, kv head, 256 tokens) pairs (2^30)");
+            throw Error(w + "too many (row, 128 tokens) or (sequence, kv head, 128 tokens) pairs (2^30)");
         const uint64_t cells = (uint64_t)g.block_size * g.H;
         const auto outside = [&](uint64_t off, uint64_t size) {
             return off > g.page_size || cells * size > g.page_size - off;
@@ -764,6 +860,8 @@ int weights_entry(const char* name, int fmt, Geom&& geom, const void* query, con
         a.max_blocks = max_blocks;
         a.hq = hq;
         a.group = hq / g.H;
+        while ((1 << a.group_shift) < a.group) ++a.group_shift;
+        a.group_mul = (uint32_t)(((1ull << 32) * ((1ull << a.group_shift) - a.group) + a.group - 1) / a.group);
         a.seqs = seqs;
         a.tokens = tokens;
         a.max_kv = max_kv;
