@@ -239,6 +239,167 @@ __device__ __forceinline__ void add_part(float& m, float& l, float2 e) {
 }
 
 // ---------------------------------------------------------------------------
+// K of a wave's 16 TT tokens of a sequence: lane (i, gq) has token i of each tile.
+// ---------------------------------------------------------------------------
+template <int FMT, int D, int TT>
+struct Keys {
+    static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
+    static constexpr int KK = D / 32, T = 16 * TT;
+    typedef uint32_t code_t __attribute__((ext_vector_type(KK), aligned(2)));
+    int id[TT], tib[TT];
+    uint32_t live[TT];                  // tokens of the tile that can be read (bits)
+    u4 k[kTurned ? 1 : TT][KK];         // dense: operands
+    code_t code[kTurned ? TT : 1];      // compressed: a quarter of a token's codes
+    uint32_t scales[kTurned ? TT : 1];  // its RMS, its residual's RMS above
+    KeyParts kp[kTurned ? TT : 1][KK];
+    float ks[kTurned ? TT : 1][4], kr[kTurned ? TT : 1][4];  // of the tokens 4 gq + 0..3
+
+    __device__ __forceinline__ void pages(const WeightArgs& a, const int32_t* table, int t0, int end, int i) {
+        const PageGeom& g = a.g;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            const int t = min(t0 + tt * 16 + i, end - 1);
+            const int pg = g.bs_shift >= 0 ? t >> g.bs_shift : t / g.block_size;
+            tib[tt] = t - pg * g.block_size;
+            id[tt] = table[pg];
+        }
+    }
+    // (what cannot be read comes from the query instead)
+    __device__ __forceinline__ void fetch(const WeightArgs& a, int h, int t0, int end, int i, int gq) {
+        const PageGeom& g = a.g;
+        const uint64_t dummy = (uint64_t)(reinterpret_cast<uintptr_t>(a.query) - reinterpret_cast<uintptr_t>(a.pool));
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            const bool ok = t0 + tt * 16 + i < end && id[tt] >= 0;
+            live[tt] = (uint32_t)__ballot(ok) & 0xffffu;
+            const uint64_t page = (uint64_t)max(id[tt], 0) * g.page_size;
+            const uint64_t cell = (uint64_t)(tib[tt] * g.H + h);
+            if constexpr (!kTurned) {
+                const uint8_t* p = a.pool + (ok ? page + g.kc_off + cell * (2 * D) : dummy) + gq * 16;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) k[tt][kk] = *reinterpret_cast<const u4*>(p + kk * 64);
+            } else {
+                code[tt] = *reinterpret_cast<const code_t*>(
+                    a.pool + (ok ? page + g.kc_off + cell * (D / 2) : dummy) + gq * (D / 8));
+                scales[tt] = ld_u16(a.pool + (ok ? page + g.ks_off + cell * 2 : dummy));
+                if (FMT == kProd)
+                    scales[tt] |= (uint32_t)ld_u16(a.pool + (ok ? page + g.kres_off + cell * 2 : dummy)) << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void decode(int gq) {
+        if constexpr (kTurned) {
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) kp[tt][kk] = decode8<FMT>(code[tt][kk]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t w = (uint32_t)__shfl((int)scales[tt], 4 * gq + r, 64);
+                    ks[tt][r] = h2f(w & 0xffff);
+                    kr[tt][r] = FMT == kProd ? h2f(w >> 16) : 0.0f;
+                }
+            }
+        }
+    }
+    // Every row sees all of them whose first L tokens it sees.
+    __device__ __forceinline__ bool plain(int t0, int L) const {
+        uint32_t all = 0xffffu;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) all &= live[tt];
+        return all == 0xffffu && t0 + T <= L;
+    }
+    // Their products with 16 query rows: operand(part, piece) is a row's 16-byte piece.
+    template <class Operand>
+    __device__ __forceinline__ void products(f4 (&x)[TT], int gq, Operand&& operand) const {
+        f4 y[TT];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) x[tt] = y[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (!kTurned) {
+            u4 qf[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) qf[kk] = operand(0, kk * 4 + gq);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<BF>(k[tt][kk], qf[kk], x[tt]);
+        } else {
+            u4 qh[KK], ql[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                qh[kk] = operand(0, gq * KK + kk);
+                ql[kk] = operand(1, gq * KK + kk);
+            }
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, qh[kk], x[tt]);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+                    if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, qh[kk], y[tt]);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, ql[kk], x[tt]);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+                    if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, ql[kk], y[tt]);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].lo, qh[kk], x[tt]);
+            }
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (FMT == kProd) x[tt][r] = fmaf(kr[tt][r], y[tt][r], x[tt][r]);
+                    x[tt][r] *= ks[tt][r];
+                }
+        }
+    }
+    // -infinity for the tokens that a row of so many does not see.
+    __device__ __forceinline__ void mask(f4 (&x)[TT], int t0, int limit, int gq) const {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int t = tt * 16 + 4 * gq + r;
+                if (t0 + t >= limit || !(live[tt] >> (4 * gq + r) & 1)) x[tt][r] = -INFINITY;
+            }
+    }
+};
+
+// Tokens that a row sees.
+__device__ __forceinline__ int limit_of(const WeightArgs& a, const Seq& q, int row) {
+    return min(q.L + (a.causal ? over_group(a, row) + 1 : 0), a.max_kv);
+}
+__device__ __forceinline__ size_t query_row(const WeightArgs& a, const Seq& q, int h, int row) {
+    const int tok = over_group(a, row);
+    return (size_t)(q.row0 + tok) * a.hq + h * a.group + (row - tok * a.group);
+}
+// Rows lie in LDS in 16-byte pieces exchanged by an exclusive or with the row: the 16 rows
+// that a load touches at one column are in different banks.
+template <int D>
+__device__ __forceinline__ int swizzle(int row) {
+    return D == 128 ? row & 15 : (row >> 1) & 7;
+}
+__device__ __forceinline__ float max_of(float u, float w) { return fmaxf(u, w); }
+__device__ __forceinline__ float sum_of(float u, float w) { return u + w; }
+// Over the four lanes that hold a row's tokens.
+__device__ __forceinline__ float row_max(float m) {
+    return lane_xor_reduce<32>(lane_xor_reduce<16>(m, max_of), max_of);
+}
+__device__ __forceinline__ float row_sum(float l) {
+    return lane_xor_reduce<32>(lane_xor_reduce<16>(l, sum_of), sum_of);
+}
+template <int TT>
+__device__ __forceinline__ float largest(const f4 (&x)[TT]) {
+    float m = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+#pragma unroll
+    for (int tt = 1; tt < TT; ++tt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, x[tt][r]);
+    return m;
+}
+
+// ---------------------------------------------------------------------------
 // The passes over K.  A workgroup has one kv head and a chunk of C tokens of one
 // sequence; 4 groups of its waves have T tokens each at a time, whose K operands stay
 // in registers while the rows go by in tiles of 16, dealt to WR waves; the rows'
@@ -250,9 +411,6 @@ __device__ __forceinline__ void add_part(float& m, float& l, float2 e) {
 //   kSum: the weights, summed over the rows.
 // kStoreFew (up to 16 rows): small blocks, whose queries it rotates itself.
 // ---------------------------------------------------------------------------
-#ifndef TURNED_TT
-#define TURNED_TT 2
-#endif
 constexpr int kStats = 0, kStore = 1, kSum = 2, kStoreFew = 3;
 // x is exact to half an ulp; its difference from a reference of this size on is taken
 // after x itself is rounded, so that no exponent is above 0 (one of up to half an ulp of
@@ -261,9 +419,9 @@ constexpr float kHuge = 4194304.0f;
 
 template <int FMT, int D, int WT, int WR, int MODE>
 struct Shape {
-    static constexpr bool kTurned = FMT == kProd || FMT == kMse, BF = FMT == kBf16;
+    static constexpr bool kTurned = FMT == kProd || FMT == kMse;
     // (compressed pages: three operands a token tile)
-    static constexpr int TT = kTurned ? TURNED_TT : 4, T = 16 * TT, kSubs = kTurned ? 4 / TT : 1, C = T * WT * kSubs;
+    static constexpr int TT = kTurned ? 2 : 4, T = 16 * TT, kSubs = kTurned ? 2 : 1, C = T * WT * kSubs;
     static constexpr int kParts = kTurned ? 2 : 1;  // of a query row
     static constexpr int kRowBytes = 2 * D;
     static constexpr bool kStores = MODE == kStore || MODE == kStoreFew, kTurns = kTurned && MODE == kStoreFew;
@@ -275,8 +433,8 @@ struct Shape {
 template <int FMT, int D, int WT, int WR, int MODE>
 __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightArgs a, float scale) {
     using S = Shape<FMT, D, WT, WR, MODE>;
-    constexpr bool kTurned = S::kTurned, BF = S::BF;
-    constexpr int TT = S::TT, T = S::T, KK = D / 32, C = S::C, kRowBlock = S::kRowBlock;
+    constexpr bool kTurned = S::kTurned;
+    constexpr int TT = S::TT, T = S::T, C = S::C, kRowBlock = S::kRowBlock;
     __shared__ __attribute__((aligned(16))) uint8_t rows_mem[S::kPart * S::kParts];
     __shared__ float row_scales[kTurned ? kRowBlock : 1];
     __shared__ float2 ml[MODE == kSum ? 1 : WT][kRowBlock];  // kSum: the rows' (M, 1 / l)
@@ -303,55 +461,14 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
         return;
     }
 
-    const uint64_t dummy = (uint64_t)(reinterpret_cast<uintptr_t>(a.query) - reinterpret_cast<uintptr_t>(a.pool));
     const int32_t* __restrict__ table = a.tables + (size_t)s * a.max_blocks;
-    // K's rows of the wave's T tokens from t0 on: lane (i, gq) has token i of each tile.
-    int id[TT], tib[TT];
-    u4 k[kTurned ? 1 : TT][KK];    // dense: operands
-    typedef uint32_t code_t __attribute__((ext_vector_type(KK), aligned(2)));
-    code_t code[TT];               // compressed: a quarter of a token's codes
-    uint32_t scales[TT];           // its RMS, its residual's RMS above
-    uint32_t live[TT];             // tokens of the tile that can be read (bits)
-    const auto pages = [&](int t0) {
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const int t = min(t0 + tt * 16 + i, q.end - 1);
-            const int pg = g.bs_shift >= 0 ? t >> g.bs_shift : t / g.block_size;
-            tib[tt] = t - pg * g.block_size;
-            id[tt] = table[pg];
-        }
-    };
-    const auto fetch = [&](int t0) {
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const bool ok = t0 + tt * 16 + i < q.end && id[tt] >= 0;
-            live[tt] = (uint32_t)__ballot(ok) & 0xffffu;
-            const uint64_t page = (uint64_t)max(id[tt], 0) * g.page_size;
-            const uint64_t cell = (uint64_t)(tib[tt] * g.H + h);
-            if constexpr (!kTurned) {
-                const uint8_t* p = a.pool + (ok ? page + g.kc_off + cell * (2 * D) : dummy) + gq * 16;
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) k[tt][kk] = *reinterpret_cast<const u4*>(p + kk * 64);
-            } else {
-                code[tt] = *reinterpret_cast<const code_t*>(
-                    a.pool + (ok ? page + g.kc_off + cell * (D / 2) : dummy) + gq * (D / 8));
-                scales[tt] = ld_u16(a.pool + (ok ? page + g.ks_off + cell * 2 : dummy));
-                if (FMT == kProd)
-                    scales[tt] |= (uint32_t)ld_u16(a.pool + (ok ? page + g.kres_off + cell * 2 : dummy)) << 16;
-            }
-        }
-    };
+    Keys<FMT, D, TT> keys;
     const int first = c * C + wt * T;
 
-    // The block's rows into LDS, in 16-byte pieces exchanged by an exclusive or with the
-    // row: the 16 rows that a load touches at one column are in different banks.  They are
-    // on their way (in registers) while the block before is worked on, the first one
-    // while K is.
-    const auto nat_of = [&](int row) {
-        const int tok = over_group(a, row);
-        return (size_t)(q.row0 + tok) * a.hq + h * a.group + (row - tok * a.group);
-    };
-    const auto swz = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+    // The block's rows into LDS: on their way (in registers) while the block before is
+    // worked on, the first one while K is.
+    const auto nat_of = [&](int row) { return query_row(a, q, h, row); };
+    const auto swz = [](int row) { return swizzle<D>(row); };
     constexpr int kPieces = S::kRowBytes / 16 * S::kParts, kHold = S::kTurns ? 1 : S::kPart * S::kParts / 16 / S::kThreads;
     u4 hold[kHold];
     float2 hold_stat;
@@ -397,7 +514,7 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
         }
     };
     take(0);
-    pages(first);
+    keys.pages(a, table, first, q.end, i);
 
     float acc[S::kSubs][TT][4];
 #pragma unroll
@@ -407,7 +524,7 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[u][tt][r] = 0.0f;
 
-    if (S::kSubs == 1) fetch(first);
+    if (S::kSubs == 1) keys.fetch(a, h, first, q.end, i, gq);
     for (int rb = 0; rb < R; rb += kRowBlock) {
         const int n = min((R - rb + 15) & ~15, kRowBlock);
         if (rb) __syncthreads();
@@ -419,29 +536,11 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
         for (int u = 0; u < S::kSubs; ++u) {
             const int t0 = first + u * WT * T;
             if (S::kSubs > 1) {
-                if (rb || u) pages(t0);
-                fetch(t0);
+                if (rb || u) keys.pages(a, table, t0, q.end, i);
+                keys.fetch(a, h, t0, q.end, i, gq);
             }
-            KeyParts kp[kTurned ? TT : 1][KK];
-            float ks[kTurned ? TT : 1][4], kr[kTurned ? TT : 1][4];  // of the tokens 4 gq + 0..3
-            if constexpr (kTurned) {
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt) {
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) kp[tt][kk] = decode8<FMT>(code[tt][kk]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t w = (uint32_t)__shfl((int)scales[tt], 4 * gq + r, 64);
-                        ks[tt][r] = h2f(w & 0xffff);
-                        kr[tt][r] = FMT == kProd ? h2f(w >> 16) : 0.0f;
-                    }
-                }
-            }
-            // Every row sees every token of the wave.
-            uint32_t all = 0xffffu;
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) all &= live[tt];
-            const bool plain = all == 0xffffu && t0 + T <= q.L;
+            keys.decode(gq);
+            const bool plain = keys.plain(t0, q.L);
             if (t0 >= q.end && (MODE == kSum || (MODE == kStats && u))) continue;
 
             for (int r0 = wr * 16; r0 < n; r0 += 16 * WR) {
@@ -450,60 +549,11 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
                     return *reinterpret_cast<const u4*>(rows_mem + part * S::kPart + (r0 + i) * S::kRowBytes +
                                                         (piece ^ swz(r0 + i)) * 16);
                 };
-                f4 x[TT], y[TT];
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt) x[tt] = y[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                float rs = scale;
-                if constexpr (!kTurned) {
-                    u4 qf[KK];
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) qf[kk] = operand(0, kk * 4 + gq);
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<BF>(k[tt][kk], qf[kk], x[tt]);
-                } else {
-                    u4 qh[KK], ql[KK];
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-                        qh[kk] = operand(0, gq * KK + kk);
-                        ql[kk] = operand(1, gq * KK + kk);
-                    }
-                    rs = row_scales[r0 + i];
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, qh[kk], x[tt]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt)
-                            if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, qh[kk], y[tt]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, ql[kk], x[tt]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt)
-                            if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, ql[kk], y[tt]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].lo, qh[kk], x[tt]);
-                    }
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (FMT == kProd) x[tt][r] = fmaf(kr[tt][r], y[tt][r], x[tt][r]);
-                            x[tt][r] *= ks[tt][r];
-                        }
-                }
-                // x rs: the logit in powers of two.  What the row does not see: -infinity.
-                if (!plain) {
-                    const int limit = min(q.L + (a.causal ? over_group(a, row) + 1 : 0), a.max_kv);
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int t = tt * 16 + 4 * gq + r;
-                            if (t0 + t >= limit || !(live[tt] >> (4 * gq + r) & 1)) x[tt][r] = -INFINITY;
-                        }
-                }
+                f4 x[TT];
+                keys.products(x, gq, operand);
+                // x rs: the logit in powers of two.
+                float rs = kTurned ? row_scales[r0 + i] : scale;
+                if (!plain) keys.mask(x, t0, limit_of(a, q, row), gq);
                 const auto rounded = [&] {
 #pragma unroll
                     for (int tt = 0; tt < TT; ++tt) x[tt] *= rs;
@@ -519,13 +569,7 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
                             acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
                 } else {
                     if (S::kStores) rounded();
-                    float m = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
-#pragma unroll
-                    for (int tt = 1; tt < TT; ++tt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) m = fmaxf(m, x[tt][r]);
-                    const auto larger = [](float u, float w) { return fmaxf(u, w); };
-                    m = lane_xor_reduce<32>(lane_xor_reduce<16>(m, larger), larger) * rs;
+                    float m = row_max(largest(x)) * rs;
                     if (MODE == kStats && __ballot(fabsf(m) >= kHuge)) rounded();
                     const float ref = m == -INFINITY ? 0.0f : m;
                     float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -533,9 +577,7 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
                     for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) l4[r] += exp2_hw(fmaf(x[tt][r], rs, -ref));
-                    float l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                    const auto sum = [](float u, float w) { return u + w; };
-                    l = lane_xor_reduce<32>(lane_xor_reduce<16>(l, sum), sum);
+                    float l = row_sum((l4[0] + l4[1]) + (l4[2] + l4[3]));
                     if (gq == 0) {
                         if (u) {  // (the wave's own entry)
                             const float2 e = ml[wt][r0 + i];
@@ -642,33 +684,36 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
     a.stat[row] = row_stat(m, l);
 }
 
-// The weights of stored x: 1,024 tokens of one kv head a workgroup, four a thread.  Eight
-// rows' x are on their way while the rows' statistics are put together (16 lanes a row).
+// The weights of stored x: a workgroup has one kv head and 1,024 / G tokens, four a lane,
+// whose rows its G groups of waves share.  Eight rows' x are on their way while the rows'
+// statistics are put together.
 constexpr int kSumTokens = 1024, kSumRows = 64;
+template <int G>
 __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
+    constexpr int T = kSumTokens / G, kLanes = 256 / G;
     __shared__ float2 st[kSumRows];
-    const int tid = threadIdx.x, i = tid & 15, p = tid >> 4;
-    const int blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
+    __shared__ f4 sums[G > 1 ? G - 1 : 1][kLanes];
+    const int tid = threadIdx.x;
+    const int part = tid % kLanes, grp = __builtin_amdgcn_readfirstlane(tid / kLanes);
+    const int blocks = (a.max_kv + T - 1) / T;
     const unsigned b = blockIdx.y * gridDim.x + blockIdx.x;
     const int sh = (int)(b / (unsigned)blocks), blk = (int)(b % (unsigned)blocks);
     const int s = sh / a.g.H, h = sh - s * a.g.H;
     if (s >= a.seqs) return;
     const Seq q = seq_of(a, s);
-    if (blk * kSumTokens >= q.end) return;
-    const int C = a.chunk, R = q.rows * a.group, n = (q.end + C - 1) / C, t = blk * kSumTokens + tid * 4;
+    if (blk * T >= q.end) return;
+    const int C = a.chunk, R = q.rows * a.group, n = (q.end + C - 1) / C, t = blk * T + part * 4;
     const size_t rows = (size_t)a.tokens * a.hq;
     // (x is there up to the end of the last chunk)
     const int at_t = min(t, n * C - 4);
-    const auto nat_of = [&](int r) {
-        const int tok = over_group(a, r);
-        return (size_t)(q.row0 + tok) * a.hq + h * a.group + (r - tok * a.group);
-    };
-    constexpr int kDeep = 8;
+    const auto nat_of = [&](int r) { return query_row(a, q, h, r); };
+    constexpr int kDeep = 8;  // rows of a group at a time: grp + G k
     f4 x[kDeep], acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const auto load = [&](int r0) {
 #pragma unroll
         for (int k = 0; k < kDeep; ++k)
-            x[k] = *reinterpret_cast<const f4*>(a.logits + (int64_t)nat_of(min(r0 + k, R - 1)) * a.logit_stride + at_t);
+            x[k] = *reinterpret_cast<const f4*>(a.logits + (int64_t)nat_of(min(r0 + grp + G * k, R - 1)) * a.logit_stride +
+                                                at_t);
     };
     if (R) load(0);
     const int64_t at = (int64_t)sh * a.stride + t;
@@ -676,7 +721,7 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
     typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
     const bool four = t + 4 <= q.end;
     f4 before = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (a.in) {
+    if (a.in && grp == 0) {
         if (four)
             before = *reinterpret_cast<const f4u*>(a.in + at);
         else
@@ -685,31 +730,47 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
     for (int r0 = 0; r0 < R; r0 += kSumRows) {
         const int upto = min(kSumRows, R - r0);
         if (r0) __syncthreads();
-        for (int g0 = 0; g0 < upto; g0 += 16) {
+        // (16 lanes a row, or 4 for more rows: all of them at once)
+        const auto statistics = [&](auto lanes) __attribute__((always_inline)) {
+            constexpr int L = decltype(lanes)::value, kRows = 256 / L;
+            const int i = tid % L, p = tid / L;
             float m = -INFINITY, l = 0.0f;
-            const size_t nat = nat_of(min(r0 + g0 + p, R - 1));
-            for (int c = i; c < n; c += 128) {
+            const size_t nat = nat_of(min(r0 + p, R - 1));
+            for (int c = i; c < n; c += 8 * L) {
                 float2 e[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) e[k] = a.part[(size_t)min(c + 16 * k, n - 1) * rows + nat];
+                for (int k = 0; k < 8; ++k) e[k] = a.part[(size_t)min(c + L * k, n - 1) * rows + nat];
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    if (c + 16 * k < n) add_part(m, l, e[k]);
+                    if (c + L * k < n) add_part(m, l, e[k]);
             }
 #pragma unroll
-            for (int k = 1; k < 16; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
-            if (i == 0) st[g0 + p] = g0 + p < upto ? row_stat(m, l) : make_float2(INFINITY, 0.0f);
-        }
+            for (int k = 1; k < L; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
+            // (a row that is none: weights of 0)
+            if (i == 0) st[p] = p < upto ? row_stat(m, l) : make_float2(INFINITY, 0.0f);
+            for (int r = kRows + tid; r < kSumRows; r += 256) st[r] = make_float2(INFINITY, 0.0f);
+        };
+        if (upto <= 16)
+            statistics(std::integral_constant<int, 16>{});
+        else
+            statistics(std::integral_constant<int, 4>{});
         __syncthreads();
-        for (int r = 0; r < upto; r += kDeep) {
+        for (int r = 0; r < upto; r += kDeep * G) {
             if (r0 + r) load(r0 + r);
 #pragma unroll
             for (int k = 0; k < kDeep; ++k) {
-                const float2 e = st[r + k];  // (a row that is none: weights of 0)
+                const float2 e = st[r + grp + G * k];
 #pragma unroll
                 for (int w = 0; w < 4; ++w) acc[w] = fmaf(exp2_hw(x[k][w] - e.x), e.y, acc[w]);
             }
         }
+    }
+    if constexpr (G > 1) {
+        if (grp) sums[grp - 1][part] = acc;
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int k = 0; k < G - 1; ++k) acc += sums[k][part];
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = a.in ? fmaf(a.decay, before[k], acc[k]) : acc[k];
@@ -741,6 +802,7 @@ void launch_format(WeightArgs a, hipStream_t stream) {
     const long long per_seq = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
     const size_t padded = ((size_t)a.max_kv + 255) / 256 * 256;
     const bool store = per_seq <= kStoreMost && rows * padded * 4 <= (size_t(256) << 20), few = store && per_seq <= 16;
+    const float scale = 1.44269504f * inv_sqrt_d(D);
     a.chunk = store || kTurned ? 256 : kStatChunk;
     a.logit_stride = (int64_t)padded;
     const auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
@@ -754,7 +816,6 @@ void launch_format(WeightArgs a, hipStream_t stream) {
     a.stat = reinterpret_cast<float2*>(ws + parts);
     a.turned = reinterpret_cast<uint16_t*>(ws + parts + second);
     a.turned_scale = reinterpret_cast<float*>(ws + parts + second + turned);
-    const float scale = 1.44269504f * inv_sqrt_d(D);
     if (kTurned && rows && !few) {
         constexpr int per = 256 / (D / 8);
         hipLaunchKernelGGL(turn_queries_kernel<D>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a.query,
@@ -775,8 +836,12 @@ void launch_format(WeightArgs a, hipStream_t stream) {
     constexpr integral_constant<int, 4> four{};
     if (store) {
         if (rows) few ? pass(four, one, integral_constant<int, kStoreFew>{}) : pass(four, one, integral_constant<int, kStore>{});
-        const long long blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
-        hipLaunchKernelGGL(weights_sum_kernel, grid_of(blocks * a.seqs * a.g.H), dim3(256), 0, stream, a);
+        const long long heads = (long long)a.seqs * a.g.H, blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
+        if (blocks * heads >= 4LL * num_cus())
+            hipLaunchKernelGGL(weights_sum_kernel<1>, grid_of(blocks * heads), dim3(256), 0, stream, a);
+        else  // few workgroups: smaller ones
+            hipLaunchKernelGGL(weights_sum_kernel<4>, grid_of((a.max_kv + kSumTokens / 4 - 1) / (kSumTokens / 4) * heads),
+                               dim3(256), 0, stream, a);
         check_launch("attention_weights_sum_kernel");
         return;
     }
