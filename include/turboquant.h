@@ -606,11 +606,12 @@ int tq_launch_turbo_mse_tree_attention(const uint16_t* query, const uint8_t* pag
  * it, whatever its page holds; a NaN or +infinity among a row's logits makes the
  * row's weights NaN.  A sum is taken in the same order in every call of the same
  * sizes: no atomics.  head_dim 64 or 128; alignments and dtype as in the tree
- * attention entries.  num_seqs 0 does nothing; num_tokens * num_q_heads <= 2^26;
- * ceil(max_kv_len / 128) times that, or times num_seqs * H, at most 2^30.  Keeps
- * the rows' statistics (and, for up to 32 rows per sequence and kv head, their
- * logits, up to 256 MB) in the per-stream workspace, as the attention entries: a
- * capture needs an earlier call with the same sizes. */
+ * attention entries.  num_seqs 0 does nothing; num_tokens * num_q_heads <= 2^25;
+ * ceil(max_kv_len / 128) times that, or times num_seqs * H, at most 2^30.  The
+ * per-stream workspace holds the rows' statistics (8 bytes for each row and 128
+ * or 256 tokens) and, for up to 32 rows per sequence and kv head (compressed
+ * pages 64), their logits, up to 256 MB: a capture needs an earlier call with the
+ * same sizes on its stream. */
 int tq_launch_dense_attention_weights(
     const void* query, const uint8_t* page_pool, const int32_t* block_tables,
     int max_blocks_per_seq, const int32_t* row_start, const int32_t* prefix_len, int causal,

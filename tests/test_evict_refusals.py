@@ -93,7 +93,7 @@ def test_weights_refused(tq, scheme):
     for bad, word in [
             (dict(hq=15), "num_q_heads"), (dict(hq=0), "num_q_heads"), (dict(hq=1 << 17), "num_q_heads"),
             (dict(seqs=-1), "num_seqs"), (dict(n=-1), "num_tokens"), (dict(blocks=0), "max_blocks"),
-            (dict(kv=129), "max_kv_len"), (dict(kv=-1), "max_kv_len"), (dict(n=1 << 23), "2^26"),
+            (dict(kv=129), "max_kv_len"), (dict(kv=-1), "max_kv_len"), (dict(n=(1 << 21) + 1), "2^25"),
             (dict(stride=99), "score_stride"), (dict(decay=-0.5), "decay"), (dict(decay=math.nan), "decay"),
             (dict(decay=1.5), "decay"), (dict(q=FAKE + 8), "16-byte"), (dict(out=FAKE + 2), "4-byte"),
             (dict(inn=FAKE + 1), "4-byte"), (dict(pool=FAKE + 1), "aligned"),

@@ -95,6 +95,37 @@ def test_select_long(tq, cuda, S, H, T, budget):
     assert torch.equal(out[..., :budget], x.gather(2, want)) and (out[..., budget:] == 0).all()
 
 
+@pytest.mark.parametrize("T", [2047, 2048, 2049, 8192, 8193, 32768, 32769, 65537])
+@pytest.mark.parametrize("kind", ["softmax", "ties", "special"])
+def test_select_widths(tq, cuda, T, kind):
+    """Around the tiles that a workgroup holds, with lengths from one to all of it."""
+    x = _values(kind, (5, 2, T), seed=T)
+    lens, budget, sink, recent = [T, T - 1, T // 2, 1, 700], 600, 3, 50
+    for in_place in (False, True):
+        kept, new, out = _select(tq, cuda, x, lens, budget, sink, recent, in_place)
+        for s, L in enumerate(lens):
+            n = min(L, budget)
+            key = torch.where(x[s, :, :L].isnan(), -INF, x[s, :, :L].double())
+            # (NaN below -infinity: behind every number by a second, stable sort)
+            order = key.sort(dim=-1, descending=True, stable=True).indices
+            nan = x[s, :, :L].isnan().gather(1, order)
+            order = order.gather(1, nan.to(torch.int8).sort(dim=-1, stable=True).indices)
+            rank = torch.empty_like(order).scatter_(1, order, torch.arange(L).expand(2, L))
+            if L > budget:
+                rank[:, :sink] = -1
+                rank[:, L - recent:] = -1
+                mid = torch.arange(sink, L - recent)
+                place = rank[:, mid].argsort(dim=-1, stable=True).argsort(dim=-1, stable=True)
+                rank[:, mid] = place
+                keep = (rank < budget - sink - recent)
+            else:
+                keep = torch.ones(2, L, dtype=torch.bool)
+            want = torch.stack([k.nonzero()[:, 0] for k in keep]).int()
+            assert torch.equal(kept[s, :, :n], want) and (kept[s, :, n:] == -1).all() and new[s] == n
+            assert torch.equal(_bits(out[s, :, :n]), _bits(x[s].gather(1, want.long())))
+            assert (_bits(out[s, :, n:]) == 0).all()
+
+
 # ── compaction ───────────────────────────────────────────────────────────── #
 
 def _kept(S, H, lens, budget, how, seed):
@@ -232,6 +263,47 @@ def test_two_streams_and_graphs(tq, cuda):
             assert torch.equal(pools[k].cpu(), want[k])
         call(0)  # (eager between replays)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+def test_eviction_in_a_graph(tq, cuda, scheme, dtype):
+    """Weights, selection and compaction as one graph on a stream: every replay, with lengths that
+    change between them, has the results of the calls one by one."""
+    p = Problem(tq, scheme, dtype, [900, 400], [4, 4], 16, 2, 128, seed=51)
+    pool, tables, q, start = (x.to(cuda) for x in (p.pool, p.tables, p.query, p.row_start))
+    prefix, lens = torch.zeros(2, dtype=I32, device=cuda), torch.zeros(2, dtype=I32, device=cuda)
+    scores, kept = torch.zeros(2, 2, 904, device=cuda), torch.zeros(2, 2, 128, dtype=I32, device=cuda)
+
+    def step(stream):
+        tq.attn_weights(scheme, q, pool, tables, start, prefix, scores, p.layout, p.cfg, 904, scores_in=scores,
+                        decay=0.5, stream=stream)
+        tq.select_kv(scores, lens, kept, sink=2, recent=10, out_scores=scores, stream=stream)
+        tq.compact_kv(scheme, pool, tables, kept, p.layout, p.cfg, stream=stream)
+
+    def reset(k):
+        pool.copy_(p.pool)
+        scores.copy_(torch.rand(2, 2, 904, generator=torch.Generator().manual_seed(k)))
+        prefix.copy_(torch.tensor([900 - 100 * k, 400 - 7 * k], dtype=I32))
+        lens.copy_(prefix + 4)
+        torch.cuda.synchronize()
+
+    st = torch.cuda.Stream()
+    want = []
+    for k in range(4):
+        reset(k)
+        step(st.cuda_stream)
+        torch.cuda.synchronize()
+        want.append([x.clone() for x in (scores, kept, pool)])
+        assert (kept >= 0).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        step(st.cuda_stream)
+    for k in (2, 0, 3, 1):
+        reset(k)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip((scores, kept, pool), want[k]):
+            assert torch.equal(got, ref)
 
 
 # ── together ─────────────────────────────────────────────────────────────── #

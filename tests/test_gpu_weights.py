@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from oracle.evict_oracle import attention_weights
+from oracle.step_oracle import hadamard, signs
 from test_gpu_tree import SCHEMES, Problem
 
 pytestmark = pytest.mark.gpu
@@ -162,6 +163,56 @@ def test_logit_sizes(tq, cuda, scheme, dtype, width, scale):
     Weights(tq, scheme, dtype, [700, 90], [width] * 2, 16, 2, 128, seed=11, q_scale=scale).check(cuda)
 
 
+@pytest.mark.parametrize("scheme,dtype,q,k", [("dense", FP16, 6e4, 6e4), ("dense", BF16, 1e15, 1e15),
+                                              ("turbo_prod", FP16, 6e4, 3e4), ("turbo_mse", FP16, 6e4, 3e4)])
+@pytest.mark.parametrize("width", [1, 4, 9])
+def test_huge_logits(tq, cuda, scheme, dtype, q, k, width):
+    """Logits of 1e10 (bf16 1e31): two equal largest ones share a row's weight, and the others, many
+    orders of magnitude below, get nothing (turbo_prod's two differ by their residuals: one takes it
+    all).  Only exact operations are left: equal logits are the same sums, their difference from the
+    maximum 0, the weights 1/2 or 1."""
+    w = Weights(tq, scheme, dtype, [300], [width], 16, 2, 128, seed=23, causal=False, before=False)
+    p = w.p
+    p.query[:] = q
+    if scheme == "dense":
+        for t in range(300):
+            p.fill_token(0, t, 1.0, "k")
+        for t in (17, 290):
+            p.fill_token(0, t, k, "k")
+    else:
+        # every token's codes are token 17's, whose product with the rotated query is positive
+        for t in range(300):
+            p.fill_token(0, t, 1e-3, "k")
+        page, H, B, D = int(p.layout.page_size_bytes), 2, 16, 128
+        off = int(p.layout.k4_codes_offset if scheme == "turbo_prod" else p.layout.k_codes_offset)
+        for t in range(300):
+            at = int(p.tables[0, t // B]) * page + off + t % B * H * D // 2
+            p.pool[at:at + H * D // 2] = 0x88 if scheme == "turbo_mse" else 0x44
+        had = hadamard(D)
+        for h in range(H):
+            turned = (torch.full((D,), float(q), dtype=torch.float64) * signs(h, D)) @ had
+            top = int(turned.abs().argmax())
+            # (the rotation of a constant row is one dim: its code is the level of the same sign)
+            code = 15 if turned[top] > 0 else 0
+            for t in range(300):
+                at = int(p.tables[0, t // B]) * page + off + (t % B * H + h) * D // 2 + top // 2
+                old = int(p.pool[at])
+                p.pool[at] = (old & 0xF0) | code if top % 2 == 0 else (old & 0x0F) | code << 4
+        for t in (17, 290):
+            p.fill_token(0, t, k, "k")
+    w.upload(cuda)
+    w.call()
+    torch.cuda.synchronize()
+    got = w.out.cpu()[0, :, :300]
+    want = w.expect()[0][0, :, :300].float()
+    total = 8.0 * width
+    if scheme == "turbo_prod":
+        assert ((want[:, 17] == total) | (want[:, 290] == total)).all()
+    else:
+        assert (want[:, 17] == total / 2).all() and (want[:, 290] == total / 2).all()
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("width", [1, 9])
 def test_equal_logits(tq, cuda, width):
     """A zero query: every token that a row sees gets the same weight."""
@@ -187,6 +238,28 @@ def test_long(tq, cuda, scheme, dtype):
     """Over 40,000 tokens: more chunks than a line of the merge, several workgroups of sums."""
     for width in (1, 6):
         Weights(tq, scheme, dtype, [40001], [width], 8, 1, 64, seed=14, before=False).check(cuda)
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 8, 9])
+def test_rows_per_sequence(tq, cuda, scheme, dtype, width):
+    """8 to 72 rows of a kv head: the row counts at which another way is taken (16, 32, 64)."""
+    Weights(tq, scheme, dtype, [600, 257], [width] * 2, 16, 2, 128, seed=19 + width).check(cuda)
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_uneven_rows(tq, cuda, scheme, dtype, D):
+    """One sequence has far more rows than the average, which chooses the way; others have none."""
+    widths = [1] * 30 + [40] + [0] * 29
+    Weights(tq, scheme, dtype, [70] * 30 + [500] + [70] * 29, widths, 8, 1, D, seed=20).check(cuda)
+    Weights(tq, scheme, dtype, [70] * 3 + [500], [1, 60, 0, 90], 8, 1, D, seed=21).check(cuda)
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+def test_many_sequences(tq, cuda, scheme, dtype):
+    """Workgroups enough for large ones in the sum over stored rows."""
+    Weights(tq, scheme, dtype, [1500] + [20] * 70, [1] * 71, 16, 8, 64, seed=22, before=True).check(cuda)
 
 
 def test_capacity_far_above_the_lengths(tq, cuda):

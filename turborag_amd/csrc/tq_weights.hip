@@ -513,8 +513,10 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
             if (MODE == kSum) ml[0][tid] = rb + tid < R ? hold_stat : make_float2(INFINITY, 0.0f);
         }
     };
-    take(0);
+    // (page ids first: K hangs on them)
     keys.pages(a, table, first, q.end, i);
+    __builtin_amdgcn_sched_barrier(0);
+    take(0);
 
     float acc[S::kSubs][TT][4];
 #pragma unroll
@@ -895,7 +897,7 @@ int weights_entry(const char* name, int fmt, Geom&& geom, const void* query, con
         if (stride < max_kv || stride >= (int64_t(1) << 40))
             throw Error(w + "score_stride must be at least max_kv_len");
         if (!(decay >= 0.0f) || decay > 1.0f) throw Error(w + "decay must be in [0, 1]");
-        if ((long long)tokens * hq > (1LL << 26)) throw Error(w + "num_tokens * num_q_heads must be at most 2^26");
+        if ((long long)tokens * hq > (1LL << 25)) throw Error(w + "num_tokens * num_q_heads must be at most 2^25");
         const long long chunks = (max_kv + 127) / 128;
         if (chunks * std::max<long long>((long long)tokens * hq, (long long)seqs * g.H) > (1LL << 30))
             throw Error(w + "too many (row, 128 tokens) or (sequence, kv head, 128 tokens) pairs (2^30)");
