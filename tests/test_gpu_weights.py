@@ -247,6 +247,20 @@ def test_rows_per_sequence(tq, cuda, scheme, dtype, width):
     Weights(tq, scheme, dtype, [600, 257], [width] * 2, 16, 2, 128, seed=19 + width).check(cuda)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("lens,widths,Hq,H", [
+    ([600], [17], 16, 2),            # 136 rows: several blocks of a chunk, the last a part
+    ([300, 1], [40, 40], 8, 1),      # 320 rows: more than a group of statistics
+    ([40, 0, 500], [1, 90, 33], 8, 1),
+    ([2000], [70], 8, 1),            # 560 rows: too much to store for dense pages
+    ([17000], [10], 8, 1),           # 80 rows of a long sequence: read again, blocks shared
+])
+def test_many_rows(tq, cuda, scheme, dtype, lens, widths, Hq, H, D):
+    """More than 64 rows of a kv head in few chunks: workgroups share a chunk's rows."""
+    Weights(tq, scheme, dtype, lens, widths, Hq, H, D, seed=30 + sum(widths) % 7).check(cuda)
+
+
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)
 @pytest.mark.parametrize("D", [64, 128])
 def test_uneven_rows(tq, cuda, scheme, dtype, D):

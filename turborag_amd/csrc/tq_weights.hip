@@ -36,6 +36,7 @@ struct WeightArgs {
     uint32_t group_mul, group_shift;  // of the division by it
     // The workspace.  A row's index is that of its query: token * hq + query head.
     int chunk;              // tokens of a statistic
+    int row_split;          // workgroups that share a chunk's rows
     float* logits;          // [rows][logit_stride]: x, or null
     int64_t logit_stride;
     float2* part;           // [chunks][rows]: (max, sum) of a chunk
@@ -407,32 +408,38 @@ __device__ __forceinline__ float largest(const f4 (&x)[TT]) {
 // transposed (K Q'): a query row is a lane column, so its maximum and sum are in-lane
 // but for two lane swaps, and a token's sum over the rows is in-lane over the tiles,
 // across 16 lanes once at the end.
-//   kStats: (max, sum) of the chunk for every row;  kStore, kStoreFew: x too;
+//   kStats: (max, sum) of the chunk for every row;  kStore: x too;
 //   kSum: the weights, summed over the rows.
-// kStoreFew (up to 16 rows): small blocks, whose queries it rotates itself.
+// Blocks of few rows (of 16 at head_dim 128): compressed pages' queries are rotated here.
+// kSplits: a.row_split workgroups share a chunk's blocks.
 // ---------------------------------------------------------------------------
-constexpr int kStats = 0, kStore = 1, kSum = 2, kStoreFew = 3;
+constexpr int kStats = 0, kStore = 1, kSum = 2;
+template <int FMT, int D>
+struct Blocks {  // rows of a block
+    static constexpr int kFew = 2048 / D, kSmall = 4096 / D;
+    static constexpr int kLarge = (FMT == kProd || FMT == kMse ? 8192 : 16384) / D;
+};
 // x is exact to half an ulp; its difference from a reference of this size on is taken
 // after x itself is rounded, so that no exponent is above 0 (one of up to half an ulp of
 // the reference otherwise, the same in both passes).
 constexpr float kHuge = 4194304.0f;
 
-template <int FMT, int D, int WT, int WR, int MODE>
+template <int FMT, int D, int WT, int WR, int MODE, int RB>
 struct Shape {
     static constexpr bool kTurned = FMT == kProd || FMT == kMse;
     // (compressed pages: three operands a token tile)
     static constexpr int TT = kTurned ? 2 : 4, T = 16 * TT, kSubs = kTurned ? 2 : 1, C = T * WT * kSubs;
     static constexpr int kParts = kTurned ? 2 : 1;  // of a query row
     static constexpr int kRowBytes = 2 * D;
-    static constexpr bool kStores = MODE == kStore || MODE == kStoreFew, kTurns = kTurned && MODE == kStoreFew;
-    static constexpr int kPart = MODE == kStoreFew ? 4096 : MODE == kStore && !kTurned ? 8192 : 32768 / kParts;  // bytes of a block's part
-    static constexpr int kRowBlock = kPart / kRowBytes;
+    static constexpr bool kTurns = kTurned && MODE == kStore && RB == Blocks<FMT, D>::kFew;
+    static constexpr int kRowBlock = RB, kPart = RB * kRowBytes;  // bytes of a block's part
+    static constexpr bool kSplits = MODE != kSum && RB == Blocks<FMT, D>::kSmall;
     static constexpr int kThreads = 64 * WT * WR;
 };
 
-template <int FMT, int D, int WT, int WR, int MODE>
+template <int FMT, int D, int WT, int WR, int MODE, int RB>
 __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightArgs a, float scale) {
-    using S = Shape<FMT, D, WT, WR, MODE>;
+    using S = Shape<FMT, D, WT, WR, MODE, RB>;
     constexpr bool kTurned = S::kTurned;
     constexpr int TT = S::TT, T = S::T, C = S::C, kRowBlock = S::kRowBlock;
     __shared__ __attribute__((aligned(16))) uint8_t rows_mem[S::kPart * S::kParts];
@@ -444,11 +451,17 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
 
     // Eight chunks in turn, then the same ones of the next head: the workgroups of one
     // chunk run on one XCD, whose L2 then holds the lines that the heads share.
-    const unsigned b = blockIdx.y * gridDim.x + blockIdx.x, eight = b / 8;
+    const int chunks = (a.max_kv + C - 1) / C;
+    unsigned b = blockIdx.y * gridDim.x + blockIdx.x, part_of = 0;
+    if (S::kSplits && a.row_split > 1) {
+        const unsigned whole = ((unsigned)a.seqs * (unsigned)chunks + 7) / 8 * 8 * (unsigned)g.H;
+        part_of = b / whole;
+        b -= part_of * whole;
+    }
+    const unsigned eight = b / 8;
     const int h = (int)(eight % (unsigned)g.H);
     const long long sc = (long long)(eight / (unsigned)g.H) * 8 + b % 8;
-    const int chunks = (a.max_kv + C - 1) / C;
-    if (sc >= (long long)a.seqs * chunks) return;
+    if (sc >= (long long)a.seqs * chunks || (S::kSplits && part_of >= (unsigned)a.row_split)) return;
     const int s = (int)(sc / chunks), c = (int)(sc - (long long)s * chunks);
     const Seq q = seq_of(a, s);
     if (c * C >= q.end) return;
@@ -516,7 +529,9 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
     // (page ids first: K hangs on them)
     keys.pages(a, table, first, q.end, i);
     __builtin_amdgcn_sched_barrier(0);
-    take(0);
+    const int rb0 = S::kSplits ? (int)part_of * kRowBlock : 0, step = S::kSplits ? a.row_split * kRowBlock : kRowBlock;
+    if (S::kSplits && rb0 >= R) return;
+    take(rb0);
 
     float acc[S::kSubs][TT][4];
 #pragma unroll
@@ -527,18 +542,18 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
             for (int r = 0; r < 4; ++r) acc[u][tt][r] = 0.0f;
 
     if (S::kSubs == 1) keys.fetch(a, h, first, q.end, i, gq);
-    for (int rb = 0; rb < R; rb += kRowBlock) {
+    for (int rb = rb0; rb < R; rb += step) {
         const int n = min((R - rb + 15) & ~15, kRowBlock);
-        if (rb) __syncthreads();
-        if (kTurned && rb) take(rb);
+        if (rb != rb0) __syncthreads();
+        if (kTurned && rb != rb0) take(rb);
         put(rb);
         __syncthreads();
-        if (!kTurned && rb + kRowBlock < R) take(rb + kRowBlock);  // (those have no registers left)
+        if (!kTurned && rb + step < R) take(rb + step);  // (those have no registers left)
 #pragma unroll
         for (int u = 0; u < S::kSubs; ++u) {
             const int t0 = first + u * WT * T;
             if (S::kSubs > 1) {
-                if (rb || u) keys.pages(a, table, t0, q.end, i);
+                if (rb != rb0 || u) keys.pages(a, table, t0, q.end, i);
                 keys.fetch(a, h, t0, q.end, i, gq);
             }
             keys.decode(gq);
@@ -570,7 +585,7 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
                         for (int r = 0; r < 4; ++r)
                             acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
                 } else {
-                    if (S::kStores) rounded();
+                    if (MODE == kStore) rounded();
                     float m = row_max(largest(x)) * rs;
                     if (MODE == kStats && __ballot(fabsf(m) >= kHuge)) rounded();
                     const float ref = m == -INFINITY ? 0.0f : m;
@@ -587,7 +602,7 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
                         }
                         ml[wt][r0 + i] = make_float2(m, l);
                     }
-                    if constexpr (S::kStores) {
+                    if constexpr (MODE == kStore) {
                         if (rb + r0 + i < R) {
                             float* to = a.logits + (int64_t)nat_of(row) * a.logit_stride + t0 + 4 * gq;
 #pragma unroll
@@ -686,14 +701,14 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
     a.stat[row] = row_stat(m, l);
 }
 
-// The weights of stored x: a workgroup has one kv head and 1,024 / G tokens, four a lane,
-// whose rows its G groups of waves share.  Eight rows' x are on their way while the rows'
+// The weights of stored x: a workgroup has one kv head and T tokens, four a lane, whose
+// rows its G groups of waves share.  Eight rows' x are on their way while the rows'
 // statistics are put together.
-constexpr int kSumTokens = 1024, kSumRows = 64;
-template <int G>
-__global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
-    constexpr int T = kSumTokens / G, kLanes = 256 / G;
-    __shared__ float2 st[kSumRows];
+constexpr int kSumRows = 64;
+template <int T, int G>
+__global__ __launch_bounds__(T / 4 * G) void weights_sum_kernel(const WeightArgs a) {
+    constexpr int kLanes = T / 4, kThreads = kLanes * G, kGroupRows = G > 4 ? 128 : kSumRows;
+    __shared__ float2 st[kGroupRows];
     __shared__ f4 sums[G > 1 ? G - 1 : 1][kLanes];
     const int tid = threadIdx.x;
     const int part = tid % kLanes, grp = __builtin_amdgcn_readfirstlane(tid / kLanes);
@@ -729,12 +744,12 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
         else
             for (int k = 0; t + k < q.end; ++k) before[k] = a.in[at + k];
     }
-    for (int r0 = 0; r0 < R; r0 += kSumRows) {
-        const int upto = min(kSumRows, R - r0);
+    for (int r0 = 0; r0 < R; r0 += kGroupRows) {
+        const int upto = min(kGroupRows, R - r0);
         if (r0) __syncthreads();
-        // (16 lanes a row, or 4 for more rows: all of them at once)
+        // (16 lanes a row, or fewer for more rows: all of them at once)
         const auto statistics = [&](auto lanes) __attribute__((always_inline)) {
-            constexpr int L = decltype(lanes)::value, kRows = 256 / L;
+            constexpr int L = decltype(lanes)::value, kRows = kThreads / L;
             const int i = tid % L, p = tid / L;
             float m = -INFINITY, l = 0.0f;
             const size_t nat = nat_of(min(r0 + p, R - 1));
@@ -749,13 +764,13 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(const WeightArgs a) {
 #pragma unroll
             for (int k = 1; k < L; k <<= 1) add_part(m, l, make_float2(xor_lane(m, k), xor_lane(l, k)));
             // (a row that is none: weights of 0)
-            if (i == 0) st[p] = p < upto ? row_stat(m, l) : make_float2(INFINITY, 0.0f);
-            for (int r = kRows + tid; r < kSumRows; r += 256) st[r] = make_float2(INFINITY, 0.0f);
+            if (i == 0 && p < kGroupRows) st[p] = p < upto ? row_stat(m, l) : make_float2(INFINITY, 0.0f);
+            for (int r = kRows + tid; r < kGroupRows; r += kThreads) st[r] = make_float2(INFINITY, 0.0f);
         };
-        if (upto <= 16)
+        if (upto <= kThreads / 16)
             statistics(std::integral_constant<int, 16>{});
         else
-            statistics(std::integral_constant<int, 4>{});
+            statistics(std::integral_constant<int, kThreads / kGroupRows>{});
         __syncthreads();
         for (int r = 0; r < upto; r += kDeep * G) {
             if (r0 + r) load(r0 + r);
@@ -787,30 +802,33 @@ dim3 grid_of(long long blocks) {
     return dim3(x, (unsigned)((blocks + x - 1) / x));
 }
 
-#ifndef STAT_WT
-#define STAT_WT 2
-#define STAT_WR 2
-#define SUM_WT 2
-#define SUM_WR 2
-#endif
-constexpr int kStatWT = STAT_WT, kStatWR = STAT_WR, kSumWT = SUM_WT, kSumWR = SUM_WR, kStatChunk = 64 * kStatWT;
-
 template <int FMT, int D>
 void launch_format(WeightArgs a, hipStream_t stream) {
     constexpr bool kTurned = FMT == kProd || FMT == kMse;
-    constexpr int kStoreMost = kTurned ? 64 : 32;
-    const size_t rows = (size_t)a.tokens * a.hq;
-    // x is stored where that moves fewer bytes than K's second reading.
-    const long long per_seq = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;
-    const size_t padded = ((size_t)a.max_kv + 255) / 256 * 256;
-    const bool store = per_seq <= kStoreMost && rows * padded * 4 <= (size_t(256) << 20), few = store && per_seq <= 16;
-    const float scale = 1.44269504f * inv_sqrt_d(D);
-    a.chunk = store || kTurned ? 256 : kStatChunk;
+    using B = Blocks<FMT, D>;
+    using std::integral_constant;
+    const size_t rows = (size_t)a.tokens * a.hq, padded = ((size_t)a.max_kv + 255) / 256 * 256;
+    const long long heads = (long long)a.seqs * a.g.H, cus = num_cus();
+    const long long per_seq = ((long long)a.tokens * a.group + a.seqs - 1) / a.seqs;  // rows of an average kv head
+    // x is stored where that takes less time than K's second reading, its products and a launch
+    // more: for up to 64 rows; for little of it; for compressed pages, whose products cost more, as
+    // long as each workgroup that adds the rows up has not too many chunks' statistics to go over.
+    // Stored / read again in us, 2 kv heads of 128 dims, sequences x tokens, rows:
+    //   dense     1 x 2K, 128: 13.9 / 16.9   512: 29.5 / 22.7   1 x 8K, 64: 14.0 / 16.1  128: 18.1 / 17.7
+    //             1 x 32K, 64: 27.0 / 24.2   128: 45.8 / 26.8   32 x 8K, 64: 64.1 / 78.0
+    //   prod      1 x 2K, 512: 33.8 / 46.6   1 x 8K, 512: 51.1 / 85.6   8 x 4K, 256: 49.0 / 75.6
+    //             1 x 32K, 64: 34.0 / 32.2   128: 54.3 / 45.5   32 x 8K, 64: 68.0 / 91
+    const size_t stored = rows * padded * 4;
+    const bool store = stored <= (size_t(256) << 20) &&
+                       (per_seq <= 64 || (kTurned ? a.max_kv <= 16384 : stored <= (size_t(4) << 20)));
+    const bool few = store && per_seq <= 16;
+    a.chunk = store || kTurned ? 256 : 128;
     a.logit_stride = (int64_t)padded;
     const auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
     const size_t parts = up(((size_t)a.max_kv + a.chunk - 1) / a.chunk * rows * sizeof(float2));
-    const size_t second = store ? up(rows * padded * 4) : up(rows * sizeof(float2));
+    const size_t second = up(store ? stored : rows * sizeof(float2));
     const size_t turned = kTurned && !few ? up(rows * 4 * D) : 0, scales = kTurned && !few ? up(rows * 4) : 0;
+    const float scale = 1.44269504f * inv_sqrt_d(D);
     const WorkspaceTurn turn(stream);
     uint8_t* ws = static_cast<uint8_t*>(Scratch{}.get(stream, parts + second + turned + scales, "attention weights"));
     a.part = reinterpret_cast<float2*>(ws);
@@ -825,38 +843,64 @@ void launch_format(WeightArgs a, hipStream_t stream) {
                            const_cast<float*>(a.turned_scale), scale * inv_sqrt_d(D));
         check_launch("attention_weights_turn_kernel");
     }
-    const auto pass = [&](auto wt, auto wr, auto mode) {
+    const auto chunks_of = [&](int C) { return ((long long)a.max_kv + C - 1) / C; };
+    const auto pass = [&](auto wt, auto wr, auto mode, auto block, long long split = 1) {
         constexpr int WT = decltype(wt)::value, WR = decltype(wr)::value, MODE = decltype(mode)::value;
-        using S = Shape<FMT, D, WT, WR, MODE>;
-        const long long chunks = ((long long)a.max_kv + S::C - 1) / S::C;
-        hipLaunchKernelGGL((weights_kernel<FMT, D, WT, WR, MODE>), grid_of((a.seqs * chunks + 7) / 8 * 8 * a.g.H),
-                           dim3(S::kThreads), 0, stream, a, kTurned ? scale * inv_sqrt_d(D) : scale);
+        using S = Shape<FMT, D, WT, WR, MODE, decltype(block)::value>;
+        a.row_split = (int)split;
+        hipLaunchKernelGGL((weights_kernel<FMT, D, WT, WR, MODE, decltype(block)::value>),
+                           grid_of((a.seqs * chunks_of(S::C) + 7) / 8 * 8 * a.g.H * split), dim3(S::kThreads), 0, stream, a,
+                           kTurned ? scale * inv_sqrt_d(D) : scale);
         check_launch(MODE == kSum ? "attention_weights_sum_kernel" : "attention_weights_kernel");
     };
-    using std::integral_constant;
     constexpr integral_constant<int, 1> one{};
+    constexpr integral_constant<int, 2> two{};  // (waves for tokens x rows: 2 x 2 17.3 + 18.4 us for 512 rows of
+                                                // 32K tokens, 4 x 2 22.2 + 19.6, 1 x 4 19.7 + 20.7, 2 x 4 23.7 + 23.3)
     constexpr integral_constant<int, 4> four{};
+    // Blocks of few rows or many, and the workgroups that share a chunk's where it has several and
+    // the chunks leave compute units without work (prod, 1 x 2K, 512 rows: 132 us without; dense,
+    // 1 x 2K, 512 rows: the pass 15.4 us, 7.9 with; 1 x 8K, 128: 6.2, 8.5 with).
+    const auto first = [&](auto wt, auto wr, auto mode) {
+        const long long work = heads * chunks_of(a.chunk);
+        if (per_seq <= B::kSmall)
+            pass(wt, wr, mode, integral_constant<int, B::kSmall>{});
+        else if (work < (!kTurned ? cus / 4 : store ? 2 * cus : cus))
+            pass(wt, wr, mode, integral_constant<int, B::kSmall>{},
+                 std::min((per_seq + B::kSmall - 1) / B::kSmall, (4 * cus + work - 1) / work));
+        else
+            pass(wt, wr, mode, integral_constant<int, B::kLarge>{});
+    };
+    constexpr integral_constant<int, kStore> storing{};
+    constexpr integral_constant<int, kStats> counting{};
+    constexpr integral_constant<int, kSum> summing{};
+    constexpr integral_constant<int, B::kLarge> large{};
     if (store) {
-        if (rows) few ? pass(four, one, integral_constant<int, kStoreFew>{}) : pass(four, one, integral_constant<int, kStore>{});
-        const long long heads = (long long)a.seqs * a.g.H, blocks = (a.max_kv + kSumTokens - 1) / kSumTokens;
-        if (blocks * heads >= 4LL * num_cus())
-            hipLaunchKernelGGL(weights_sum_kernel<1>, grid_of(blocks * heads), dim3(256), 0, stream, a);
-        else  // few workgroups: smaller ones
-            hipLaunchKernelGGL(weights_sum_kernel<4>, grid_of((a.max_kv + kSumTokens / 4 - 1) / (kSumTokens / 4) * heads),
-                               dim3(256), 0, stream, a);
+        if (rows && few)
+            pass(four, one, storing, integral_constant<int, B::kFew>{});
+        else if (rows)
+            first(four, one, storing);
+        const long long blocks = chunks_of(1024), smaller = chunks_of(256);
+        if (blocks * heads >= 4 * cus)
+            hipLaunchKernelGGL((weights_sum_kernel<1024, 1>), grid_of(blocks * heads), dim3(256), 0, stream, a);
+        else if (per_seq <= 64)  // few workgroups: smaller ones
+            hipLaunchKernelGGL((weights_sum_kernel<256, 4>), grid_of(smaller * heads), dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL((weights_sum_kernel<256, 16>), grid_of(smaller * heads), dim3(1024), 0, stream, a);
         check_launch("attention_weights_sum_kernel");
         return;
     }
     if constexpr (kTurned)
-        pass(four, one, integral_constant<int, kStats>{});
+        first(four, one, counting);
     else
-        pass(integral_constant<int, kStatWT>{}, integral_constant<int, kStatWR>{}, integral_constant<int, kStats>{});
+        first(two, two, counting);
     hipLaunchKernelGGL(weights_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
     check_launch("attention_weights_rows_kernel");
     if constexpr (kTurned)
-        pass(four, one, integral_constant<int, kSum>{});
+        pass(four, one, summing, large);
+    else if (heads * chunks_of(a.chunk) < cus / 4)  // smaller chunks, whose rows eight waves share: 13.8 us, now 10.9
+        pass(one, integral_constant<int, 8>{}, summing, large);
     else
-        pass(integral_constant<int, kSumWT>{}, integral_constant<int, kSumWR>{}, integral_constant<int, kSum>{});
+        pass(two, two, summing, large);
 }
 
 bool aligned(uint64_t v, uint64_t a) { return (v & (a - 1)) == 0; }
