@@ -252,7 +252,6 @@ struct Keys {
     u4 k[kTurned ? 1 : TT][KK];         // dense: operands
     code_t code[kTurned ? TT : 1];      // compressed: a quarter of a token's codes
     uint32_t scales[kTurned ? TT : 1];  // its RMS, its residual's RMS above
-    KeyParts kp[kTurned ? TT : 1][KK];
     float ks[kTurned ? TT : 1][4], kr[kTurned ? TT : 1][4];  // of the tokens 4 gq + 0..3
 
     __device__ __forceinline__ void pages(const WeightArgs& a, const int32_t* table, int t0, int end, int i) {
@@ -288,12 +287,10 @@ struct Keys {
             }
         }
     }
-    __device__ __forceinline__ void decode(int gq) {
+    __device__ __forceinline__ void scales_of(int gq) {
         if constexpr (kTurned) {
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) kp[tt][kk] = decode8<FMT>(code[tt][kk]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t w = (uint32_t)__shfl((int)scales[tt], 4 * gq + r, 64);
@@ -310,49 +307,59 @@ struct Keys {
         for (int tt = 0; tt < TT; ++tt) all &= live[tt];
         return all == 0xffffu && t0 + T <= L;
     }
-    // Their products with 16 query rows: operand(part, piece) is a row's 16-byte piece.
-    template <class Operand>
-    __device__ __forceinline__ void products(f4 (&x)[TT], int gq, Operand&& operand) const {
-        f4 y[TT];
+    // Their products with N times 16 query rows: operand(n, part, piece) is a row's 16-byte
+    // piece.  Compressed keys are decoded 32 dims at a time, for all the rows.
+    template <int N, class Operand>
+    __device__ __forceinline__ void products(f4 (&x)[N][TT], int gq, Operand&& operand) const {
+        f4 y[N][TT];
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) x[tt] = y[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) x[n][tt] = y[n][tt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         if constexpr (!kTurned) {
-            u4 qf[KK];
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) qf[kk] = operand(0, kk * 4 + gq);
+            for (int n = 0; n < N; ++n) {
+                u4 q[KK];
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
+                for (int kk = 0; kk < KK; ++kk) q[kk] = operand(n, 0, kk * 4 + gq);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<BF>(k[tt][kk], qf[kk], x[tt]);
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) x[n][tt] = mfma<BF>(k[tt][kk], q[kk], x[n][tt]);
+            }
         } else {
-            u4 qh[KK], ql[KK];
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                qh[kk] = operand(0, gq * KK + kk);
-                ql[kk] = operand(1, gq * KK + kk);
-            }
+                __builtin_amdgcn_sched_barrier(0);  // (no operands ahead: registers)
+                KeyParts kp[TT];
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
+                for (int tt = 0; tt < TT; ++tt) kp[tt] = decode8<FMT>(code[tt][kk]);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, qh[kk], x[tt]);
+                for (int n = 0; n < N; ++n) {
+                    const u4 qh = operand(n, 0, gq * KK + kk), ql = operand(n, 1, gq * KK + kk);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, qh[kk], y[tt]);
+                    for (int tt = 0; tt < TT; ++tt) x[n][tt] = mfma<false>(kp[tt].hi, qh, x[n][tt]);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].hi, ql[kk], x[tt]);
+                    for (int tt = 0; tt < TT; ++tt)
+                        if (FMT == kProd) y[n][tt] = mfma<false>(kp[tt].sign, qh, y[n][tt]);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    if (FMT == kProd) y[tt] = mfma<false>(kp[tt][kk].sign, ql[kk], y[tt]);
+                    for (int tt = 0; tt < TT; ++tt) x[n][tt] = mfma<false>(kp[tt].hi, ql, x[n][tt]);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) x[tt] = mfma<false>(kp[tt][kk].lo, qh[kk], x[tt]);
-            }
+                    for (int tt = 0; tt < TT; ++tt)
+                        if (FMT == kProd) y[n][tt] = mfma<false>(kp[tt].sign, ql, y[n][tt]);
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (FMT == kProd) x[tt][r] = fmaf(kr[tt][r], y[tt][r], x[tt][r]);
-                    x[tt][r] *= ks[tt][r];
+                    for (int tt = 0; tt < TT; ++tt) x[n][tt] = mfma<false>(kp[tt].lo, qh, x[n][tt]);
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (FMT == kProd) x[n][tt][r] = fmaf(kr[tt][r], y[n][tt][r], x[n][tt][r]);
+                        x[n][tt][r] *= ks[tt][r];
+                    }
         }
     }
     // -infinity for the tokens that a row of so many does not see.
@@ -435,10 +442,12 @@ struct Shape {
     static constexpr int kRowBlock = RB, kPart = RB * kRowBytes;  // bytes of a block's part
     static constexpr bool kSplits = MODE != kSum && RB == Blocks<FMT, D>::kSmall;
     static constexpr int kThreads = 64 * WT * WR;
+    static constexpr int kTiles = !kTurned ? 1 : RB >= 64 ? 4 : RB / 16;  // of rows that share a decoded key
+    static constexpr int kWaves = kTurned ? (kTiles < 4 ? 5 - kTiles : 2) : MODE == kSum ? 2 : 3;  // of a SIMD, at least
 };
 
 template <int FMT, int D, int WT, int WR, int MODE, int RB>
-__global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightArgs a, float scale) {
+__global__ __launch_bounds__(64 * WT * WR, (Shape<FMT, D, WT, WR, MODE, RB>::kWaves)) void weights_kernel(const WeightArgs a, float scale) {
     using S = Shape<FMT, D, WT, WR, MODE, RB>;
     constexpr bool kTurned = S::kTurned;
     constexpr int TT = S::TT, T = S::T, C = S::C, kRowBlock = S::kRowBlock;
@@ -556,60 +565,67 @@ __global__ __launch_bounds__(64 * WT * WR, 2) void weights_kernel(const WeightAr
                 if (rb != rb0 || u) keys.pages(a, table, t0, q.end, i);
                 keys.fetch(a, h, t0, q.end, i, gq);
             }
-            keys.decode(gq);
+            keys.scales_of(gq);
             const bool plain = keys.plain(t0, q.L);
             if (t0 >= q.end && (MODE == kSum || (MODE == kStats && u))) continue;
 
-            for (int r0 = wr * 16; r0 < n; r0 += 16 * WR) {
-                const int row = min(rb + r0 + i, R - 1);
-                const auto operand = [&](int part, int piece) {
-                    return *reinterpret_cast<const u4*>(rows_mem + part * S::kPart + (r0 + i) * S::kRowBytes +
-                                                        (piece ^ swz(r0 + i)) * 16);
-                };
-                f4 x[TT];
-                keys.products(x, gq, operand);
-                // x rs: the logit in powers of two.
-                float rs = kTurned ? row_scales[r0 + i] : scale;
-                if (!plain) keys.mask(x, t0, limit_of(a, q, row), gq);
-                const auto rounded = [&] {
+            constexpr bool kOnce = kTurned && 16 * S::kTiles == kRowBlock;
+            static_assert(S::kTiles == 1 || WR == 1, "the tiles of a wave lie in a row");
+            for (int r0 = wr * 16; r0 < n; r0 += 16 * WR * S::kTiles) {
+                f4 xs[S::kTiles][TT];
+                keys.products(xs, gq, [&](int k, int part, int piece) {
+                    const int r = r0 + k * 16 + i;
+                    return *reinterpret_cast<const u4*>(rows_mem + part * S::kPart + r * S::kRowBytes + (piece ^ swz(r)) * 16);
+                });
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) x[tt] *= rs;
-                    rs = 1.0f;
-                };
-                if constexpr (MODE == kSum) {
-                    const float2 st = ml[0][r0 + i];
-                    if (__ballot(fabsf(st.x) >= kHuge)) rounded();
+                for (int k = 0; k < S::kTiles; ++k) {
+                    if (k && r0 + 16 * k >= n) break;
+                    f4(&x)[TT] = xs[k];
+                    const int at = r0 + 16 * k + i, row = min(rb + at, R - 1);
+                    // x rs: the logit in powers of two.
+                    float rs = kTurned ? row_scales[at] : scale;
+                    if (!plain) keys.mask(x, t0, limit_of(a, q, row), gq);
+                    const auto rounded = [&] {
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
+                        for (int tt = 0; tt < TT; ++tt) x[tt] *= rs;
+                        rs = 1.0f;
+                    };
+                    if constexpr (MODE == kSum) {
+                        const float2 st = ml[0][at];
+                        if (__ballot(fabsf(st.x) >= kHuge)) rounded();
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
-                } else {
-                    if (MODE == kStore) rounded();
-                    float m = row_max(largest(x)) * rs;
-                    if (MODE == kStats && __ballot(fabsf(m) >= kHuge)) rounded();
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
+                            for (int r = 0; r < 4; ++r)
+                                acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
+                    } else {
+                        if (MODE == kStore) rounded();
+                        float m = row_max(largest(x)) * rs;
+                        if (MODE == kStats && __ballot(fabsf(m) >= kHuge)) rounded();
+                        const float ref = m == -INFINITY ? 0.0f : m;
+                        float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) l4[r] += exp2_hw(fmaf(x[tt][r], rs, -ref));
-                    float l = row_sum((l4[0] + l4[1]) + (l4[2] + l4[3]));
-                    if (gq == 0) {
-                        if (u) {  // (the wave's own entry)
-                            const float2 e = ml[wt][r0 + i];
-                            add_part(m, l, e);
+                        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) l4[r] += exp2_hw(fmaf(x[tt][r], rs, -ref));
+                        float l = row_sum((l4[0] + l4[1]) + (l4[2] + l4[3]));
+                        if (gq == 0) {
+                            if (u) {  // (the wave's own entry)
+                                const float2 e = ml[wt][at];
+                                add_part(m, l, e);
+                            }
+                            ml[wt][at] = make_float2(m, l);
                         }
-                        ml[wt][r0 + i] = make_float2(m, l);
-                    }
-                    if constexpr (MODE == kStore) {
-                        if (rb + r0 + i < R) {
-                            float* to = a.logits + (int64_t)nat_of(row) * a.logit_stride + t0 + 4 * gq;
+                        if constexpr (MODE == kStore) {
+                            if (rb + at < R) {
+                                float* to = a.logits + (int64_t)nat_of(row) * a.logit_stride + t0 + 4 * gq;
 #pragma unroll
-                            for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f4*>(to + tt * 16) = x[tt];
+                                for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f4*>(to + tt * 16) = x[tt];
+                            }
                         }
                     }
                 }
+                if (kOnce) break;
             }
         }
         if constexpr (MODE != kSum) {
