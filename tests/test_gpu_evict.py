@@ -406,3 +406,35 @@ def test_batch_under_a_budget(tq, cuda, scheme):
         assert [batch.table.num_tokens(s) for s in range(3)] == lens
     assert batch.alloc.num_free() > free
     batch.close()
+
+
+def test_batch_evicts_on_another_stream(tq, cuda):
+    """What evict allocates belongs to the stream that it runs on, not to the caller's; it refuses
+    scores and tables that hold fewer tokens than the batch."""
+    batch = PagedBatch(tq, "turbo_mse", [300, 90], [3, 2], kv_heads=2, q_heads=8, head_dim=64)
+    batch.append_new_tokens(seed=7)
+    bt = batch.block_tables()
+    held = [303, 92]
+    full = torch.rand(2, 2, 320, generator=torch.Generator().manual_seed(43))
+    scores = full.to(cuda)
+    with pytest.raises(ValueError, match="303 tokens"):
+        batch.evict(scores[:, :, :302].contiguous(), 64, bt)
+    with pytest.raises(ValueError, match="303 tokens"):
+        batch.evict(scores, 64, bt[:, :18].contiguous())
+    assert [batch.table.num_tokens(s) for s in range(2)] == held
+    torch.cuda.synchronize()
+    pool = batch.pool.cpu()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        busy = torch.randn(2048, 2048, device=cuda)
+        for _ in range(20):  # evict's kernels wait behind these
+            busy = (busy @ busy).clamp(-1.0, 1.0)
+    lens = batch.evict(scores, 64, bt, sink=2, recent=8, stream=side.cuda_stream)
+    other = [torch.full((2, 2, 64), -1, dtype=torch.int32, device=cuda) for _ in range(4)]
+    torch.cuda.synchronize()
+    kept, new, moved = select(full, held, 64, 2, 8)
+    assert lens == new.tolist()
+    assert torch.equal(scores.cpu(), moved)
+    assert torch.equal(batch.pool.cpu(), compact("turbo_mse", pool, bt.cpu(), kept, batch.layout, batch.cfg))
+    assert all(int(x.max()) == -1 for x in other)
+    batch.close()

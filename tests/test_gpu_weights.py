@@ -338,3 +338,19 @@ def test_stream_and_graph(tq, cuda, scheme, dtype, width):
     graph.replay()
     torch.cuda.synchronize()
     w.compare(w.out)
+
+
+def test_two_streams_at_once(tq, cuda):
+    """Calls of different sizes on two streams, several in flight: each has its stream's workspace."""
+    a = Weights(tq, "turbo_prod", FP16, [900, 300], [9, 1], 16, 2, 128, seed=50, before=False)
+    b = Weights(tq, "dense", BF16, [2000], [12], 8, 2, 64, seed=51, before=False)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for w in (a, b):
+        w.upload(cuda)
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for w, st in zip((a, b), streams):
+            w.call(st.cuda_stream)
+    torch.cuda.synchronize()
+    for w in (a, b):
+        w.compare(w.out)

@@ -168,11 +168,17 @@ class PagedBatch:
         Returns their lengths.  Positions go on from the tokens ever appended, not
         from what is left."""
         held = [self.table.num_tokens(s) for s in range(self.S)]
-        kept = torch.empty(self.S, self.H, budget, dtype=torch.int32, device=self.dev)
-        lens = torch.tensor(held, dtype=torch.int32, device=self.dev)
-        self.tq.select_kv(scores, lens, kept, sink=sink, recent=recent, out_scores=scores, stream=stream)
-        self.tq.compact_kv(self.scheme, self.pool, block_tables, kept, self.layout, self.cfg,
-                           stream=stream)
+        if max(held) > scores.shape[-1] or max(held) > block_tables.shape[-1] * self.B:
+            raise ValueError(f"evict: scores and block_tables must hold {max(held)} tokens")
+        # (allocated for the stream that uses them: their memory is given back on it)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.dev) if stream
+                               else torch.cuda.default_stream(self.dev)):
+            kept = torch.empty(self.S, self.H, budget, dtype=torch.int32, device=self.dev)
+            lens = torch.tensor(held, dtype=torch.int32, device=self.dev)
+            self.tq.select_kv(scores, lens, kept, sink=sink, recent=recent, out_scores=scores,
+                              stream=stream)
+            self.tq.compact_kv(self.scheme, self.pool, block_tables, kept, self.layout, self.cfg,
+                               stream=stream)
         self.lens = [min(n, budget) for n in held]
         for s, n in enumerate(self.lens):
             self.table.truncate(s, n)

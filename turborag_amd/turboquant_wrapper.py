@@ -989,7 +989,7 @@ class TurboQuantWrapper:
 
         scheme, query [num_tokens, Hq, D], block_tables, row_start and prefix_len as
         in tree_attn_output; scores (and scores_in) [num_seqs, H, >= max_kv_len] fp32,
-        rows contiguous in their last dimension.  causal: row j of a sequence attends
+        contiguous.  causal: row j of a sequence attends
         its first prefix_len + j + 1 tokens, otherwise the first prefix_len.  Tokens
         past what the last row attends keep their scores."""
         op = "attn_weights"
