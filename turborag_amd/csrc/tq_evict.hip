@@ -304,6 +304,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kMoveThreads = 256, kMoveDeep = 8;
+// Waits of some microseconds are given up after about a second, which takes two graphs of one
+// stream replayed at once, against the rule: their cells are wrong then, but both end.
+constexpr int kMostPolls = 1 << 20;
 
 // Cells of whole cache lines go past the caches (dense, 32 sequences to 4,096 tokens each,
 // 258 MB: 58.6 -> 54.4 us; 8 kv heads 60.2 -> 56.4); parts of lines are put together there
@@ -335,6 +338,7 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactA
         if (tid == 0) ticket = atomicAdd(&a.state[row], 1u);
         __syncthreads();
         c = (int)ticket;
+        if (c >= a.chunks) return;  // (state that another call's kernels share: nothing out of bounds)
     }
     const int s = (int)(row / a.H), h = (int)(row - (long long)s * a.H);
     const int32_t* __restrict__ kept = a.kept + row * a.budget;
@@ -390,8 +394,10 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactA
         if (tid == 0) __hip_atomic_store(&done[c], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         for (int k = tid; k < c; k += kMoveThreads)  // (unsigned: a hole in kept counts as any token)
             if (kept[k * T] < (c + 1) * T && (uint32_t)kept[k * T + T - 1] >= (uint32_t)(c * T))
-                while (!__hip_atomic_load(&done[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+                for (int polls = 0; polls < kMostPolls; ++polls) {
+                    if (__hip_atomic_load(&done[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) break;
                     __builtin_amdgcn_s_sleep(1);
+                }
         __syncthreads();
     }
 #pragma unroll
