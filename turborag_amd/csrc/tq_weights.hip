@@ -419,6 +419,13 @@ __device__ __forceinline__ float largest(const f4 (&x)[TT]) {
 //   kSum: the weights, summed over the rows.
 // Blocks of few rows (of 16 at head_dim 128): compressed pages' queries are rotated here.
 // kSplits: a.row_split workgroups share a chunk's blocks.
+// Bound by: memory with few rows of dense pages (32 sequences, 540K tokens, 8 rows: 277 MB of
+// K and 35 MB of x in 62.5 us, 5.0 TB/s); latency where a workgroup has one chunk and
+// its rows (256 rows of 32K tokens: 17 us a launch, of which the products and exponentials
+// are 5 to 6); for compressed pages decode and matrix instructions, five products where dense
+// keys have one (64 rows of 32 sequences to 8K tokens: 39 us, vector units 34% busy, matrix
+// cores 20%).  A key is decoded 32 dims at a time for all rows of a block, so that three or
+// four waves of a SIMD have registers (32 rows, 32 x 8K tokens: 51.6 -> 46.0 us with the sum).
 // ---------------------------------------------------------------------------
 constexpr int kStats = 0, kStore = 1, kSum = 2;
 template <int FMT, int D>
@@ -717,7 +724,9 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(const WeightArgs a) {
     a.stat[row] = row_stat(m, l);
 }
 
-// The weights of stored x: a workgroup has one kv head and T tokens, four a lane, whose
+// The weights of stored x, 4 bytes a row and token: bound by reading them, mostly out of the
+// caches that they were just written to (32 sequences, 540K tokens, 8 rows: 35 MB in 15.5 us,
+// of which a launch and the statistics are ~5).  A workgroup has one kv head and T tokens, four a lane, whose
 // rows its G groups of waves share.  Eight rows' x are on their way while the rows'
 // statistics are put together.
 constexpr int kSumRows = 64;
@@ -870,7 +879,7 @@ void launch_format(WeightArgs a, hipStream_t stream) {
         check_launch(MODE == kSum ? "attention_weights_sum_kernel" : "attention_weights_kernel");
     };
     constexpr integral_constant<int, 1> one{};
-    constexpr integral_constant<int, 2> two{};  // (waves for tokens x rows: 2 x 2 17.3 + 18.4 us for 512 rows of
+    constexpr integral_constant<int, 2> two{};  // (waves for tokens x rows: 2 x 2 17.3 + 18.4 us for 256 rows of
                                                 // 32K tokens, 4 x 2 22.2 + 19.6, 1 x 4 19.7 + 20.7, 2 x 4 23.7 + 23.3)
     constexpr integral_constant<int, 4> four{};
     // Blocks of few rows or many, and the workgroups that share a chunk's where it has several and
