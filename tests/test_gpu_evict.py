@@ -3,6 +3,8 @@ restatements, value for value and byte for byte; and the eviction of a batch
 with the steps around it."""
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -438,3 +440,35 @@ def test_batch_evicts_on_another_stream(tq, cuda):
     assert torch.equal(batch.pool.cpu(), compact("turbo_mse", pool, bt.cpu(), kept, batch.layout, batch.cfg))
     assert all(int(x.max()) == -1 for x in other)
     batch.close()
+
+
+def test_host_threads_on_one_stream(tq, cuda):
+    """In-place compactions from four threads on one stream: each call's flags are its
+    own until its last launch."""
+    ps = [Problem(tq, "dense", torch.float16, [1500 + 64 * k, 700], [0, 0], 2, 2, 128, seed=70 + k) for k in range(4)]
+    keeps = [_kept(2, 2, [1500 + 64 * k, 700], 900 + k, "random", seed=80 + k) for k in range(4)]
+    want = [compact("dense", p.pool, p.tables, kept, p.layout, p.cfg) for p, kept in zip(ps, keeps)]
+    pools = [[p.pool.to(cuda) for _ in range(6)] for p in ps]
+    tables, kepts = [p.tables.to(cuda) for p in ps], [k.to(cuda) for k in keeps]
+    stream, errors = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+
+    def work(k):
+        try:
+            torch.cuda.set_device(cuda)
+            for pool in pools[k]:
+                tq.compact_kv("dense", pool, tables[k], kepts[k], ps[k].layout, ps[k].cfg,
+                              stream=stream.cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for k in range(4):
+        for pool in pools[k]:
+            assert torch.equal(pool.cpu(), want[k])

@@ -354,3 +354,16 @@ def test_two_streams_at_once(tq, cuda):
     torch.cuda.synchronize()
     for w in (a, b):
         w.compare(w.out)
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("lens,widths", [([300, 90], [2, 1]), ([500], [20]), ([400, 17000], [12, 10])])
+def test_padded_batch(tq, cuda, scheme, dtype, lens, widths):
+    """Rows behind the last sequence's, as a padded batch has them, hold anything and reach nothing;
+    the same pages under two sequences are scored for each."""
+    w = Weights(tq, scheme, dtype, lens, widths, 16, 2, 128, seed=60)
+    p = w.p
+    if len(lens) == 2 and lens[1] < lens[0]:
+        p.tables[1] = p.tables[0]
+    p.query = torch.cat([p.query, torch.full((37, 16, 128), float("nan"), dtype=dtype)])
+    w.check(cuda)
