@@ -367,3 +367,12 @@ def test_padded_batch(tq, cuda, scheme, dtype, lens, widths):
         p.tables[1] = p.tables[0]
     p.query = torch.cat([p.query, torch.full((37, 16, 128), float("nan"), dtype=dtype)])
     w.check(cuda)
+
+
+@pytest.mark.parametrize("scheme,dtype", SCHEMES)
+@pytest.mark.parametrize("S,L,width", [(130, 1300, 1), (130, 700, 3), (70, 5000, 1), (130, 4000, 1)])
+def test_many_sequences(tq, cuda, scheme, dtype, S, L, width):
+    """Sequences enough for the sum's middle and largest workgroups, of uneven lengths."""
+    lens = [(L * (k + 1)) // S for k in range(S)]
+    lens[3] = 0
+    Weights(tq, scheme, dtype, lens, [width] * S, 4, 2, 64, seed=90).check(cuda)

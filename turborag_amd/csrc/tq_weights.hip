@@ -907,6 +907,9 @@ void launch_format(WeightArgs a, hipStream_t stream) {
         const long long blocks = chunks_of(1024), smaller = chunks_of(256);
         if (blocks * heads >= 4 * cus)
             hipLaunchKernelGGL((weights_sum_kernel<1024, 1>), grid_of(blocks * heads), dim3(256), 0, stream, a);
+        else if (blocks * heads >= cus)  // (32 x 8K tokens, 16 rows: 37.1 us with 256 tokens, 35.2, with 1,024 34.5;
+            // 64 rows of compressed pages 53.0, 53.0, 55.1; 32 x 32K, 8 rows: 89.8, 81.2, 78)
+            hipLaunchKernelGGL((weights_sum_kernel<512, 2>), grid_of(chunks_of(512) * heads), dim3(256), 0, stream, a);
         else if (per_seq <= 64)  // few workgroups: smaller ones
             hipLaunchKernelGGL((weights_sum_kernel<256, 4>), grid_of(smaller * heads), dim3(256), 0, stream, a);
         else
