@@ -433,10 +433,18 @@ struct Blocks {  // rows of a block
     static constexpr int kFew = 2048 / D, kSmall = 4096 / D;
     static constexpr int kLarge = (FMT == kProd || FMT == kMse ? 8192 : 16384) / D;
 };
-// x is exact to half an ulp; its difference from a reference of this size on is taken
-// after x itself is rounded, so that no exponent is above 0 (one of up to half an ulp of
-// the reference otherwise, the same in both passes).
+// x rs, the logit in powers of two, is one number in both passes, whatever rows share a tile and
+// whatever the row's maximum is there: exact below kHuge and rounded from there on (its difference
+// from a rounded maximum may be above 0 by half an ulp of that, which would overflow).  A maximum
+// of at least half of kHuge says that a tile may have such logits that count: those of a smaller
+// maximum are at least 2^21 below it, 0 either way.  (An infinite one is a row that sees nothing,
+// or one of NaN.)
 constexpr float kHuge = 4194304.0f;
+__device__ __forceinline__ bool near_huge(float m) { return fabsf(m) >= kHuge / 2 && fabsf(m) < INFINITY; }
+__device__ __forceinline__ float over_huge(float x, float rs, float ref) {
+    const float y = x * rs;
+    return fabsf(y) >= kHuge ? y - ref : fmaf(x, rs, -ref);
+}
 
 template <int FMT, int D, int WT, int WR, int MODE, int RB>
 struct Shape {
@@ -592,24 +600,31 @@ __global__ __launch_bounds__(64 * WT * WR, (Shape<FMT, D, WT, WR, MODE, RB>::kWa
                     // x rs: the logit in powers of two.
                     float rs = kTurned ? row_scales[at] : scale;
                     if (!plain) keys.mask(x, t0, limit_of(a, q, row), gq);
-                    const auto rounded = [&] {
+                    const auto differences = [&](float& ref) {  // into x, for fmaf(x, rs, -ref)
 #pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) x[tt] *= rs;
+                        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[tt][r] = over_huge(x[tt][r], rs, ref);
                         rs = 1.0f;
+                        ref = 0.0f;
                     };
                     if constexpr (MODE == kSum) {
-                        const float2 st = ml[0][at];
-                        if (__ballot(fabsf(st.x) >= kHuge)) rounded();
+                        float2 st = ml[0][at];
+                        if (__ballot(near_huge(st.x))) differences(st.x);
 #pragma unroll
                         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 acc[u][tt][r] = fmaf(exp2_hw(fmaf(x[tt][r], rs, -st.x)), st.y, acc[u][tt][r]);
                     } else {
-                        if (MODE == kStore) rounded();
+                        if (MODE == kStore) {  // (rounded where it is stored)
+#pragma unroll
+                            for (int tt = 0; tt < TT; ++tt) x[tt] *= rs;
+                            rs = 1.0f;
+                        }
                         float m = row_max(largest(x)) * rs;
-                        if (MODE == kStats && __ballot(fabsf(m) >= kHuge)) rounded();
-                        const float ref = m == -INFINITY ? 0.0f : m;
+                        float ref = m == -INFINITY ? 0.0f : m;
+                        if (MODE == kStats && __ballot(near_huge(m))) differences(ref);
                         float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int tt = 0; tt < TT; ++tt)
