@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "tq_device.h"
@@ -340,8 +341,9 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactA
     if constexpr (IN_PLACE) {
         if (tid == 0) ticket = atomicAdd(&a.state[row], 1u);
         __syncthreads();
+        // (state that another call's kernels share may hold any bits: nothing out of bounds)
+        if (ticket >= (uint32_t)a.chunks) return;
         c = (int)ticket;
-        if (c >= a.chunks) return;  // (state that another call's kernels share: nothing out of bounds)
     }
     const int s = (int)(row / a.H), h = (int)(row - (long long)s * a.H);
     const int32_t* __restrict__ kept = a.kept + row * a.budget;
@@ -423,9 +425,14 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactA
     }
 }
 
-__global__ __launch_bounds__(256) void clear_kernel(uint32_t* p, long long n) {
-    for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < n; k += (long long)gridDim.x * 256) p[k] = 0;
+// The tickets (the first `rows` words) and the flags behind them.
+__global__ __launch_bounds__(256) void clear_kernel(uint32_t* p, long long n, long long rows, uint32_t first) {
+    for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < n; k += (long long)gridDim.x * 256)
+        p[k] = k < rows ? first : 0;
 }
+
+// What tests set (tq_test_compact).
+std::atomic<uint32_t> g_first_ticket{0};
 
 dim3 grid_of(long long blocks) {
     const unsigned x = (unsigned)std::min<long long>(blocks, 1 << 23);
@@ -447,7 +454,7 @@ void launch_move(CompactArgs a, bool in_place, hipStream_t stream) {
     const long long words = a.rows + blocks;
     a.state = static_cast<uint32_t*>(Scratch{}.get(stream, (size_t)words * 4, "compact_kv"));
     hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<long long>((words + 255) / 256, 1024)), dim3(256), 0, stream,
-                       a.state, words);
+                       a.state, words, a.rows, g_first_ticket.load(std::memory_order_relaxed));
     check_launch("compact_kv_clear_kernel");
     hipLaunchKernelGGL((compact_kv_kernel<U, NS, true>), grid_of(blocks), dim3(kMoveThreads), 0, stream, a);
     check_launch("compact_kv_kernel");
@@ -535,6 +542,13 @@ void take_geom(CompactArgs& a, const PageGeom& g) {
 
 }  // namespace
 }  // namespace tq
+
+// For tests: the first ticket of in-place moves (0, but for a workspace that another call's
+// kernels have written over).
+extern "C" __attribute__((visibility("default"))) int tq_test_compact(uint32_t first_ticket) {
+    tq::g_first_ticket.store(first_ticket);
+    return 0;
+}
 
 extern "C" int tq_launch_select_kv(const float* scores, int64_t score_stride, const int32_t* kv_len, int num_seqs,
                                    int num_kv_heads, int max_kv_len, int budget, int sink, int recent, int32_t* kept,
