@@ -657,7 +657,11 @@ int tq_launch_select_kv(const float* scores, int64_t score_stride, const int32_t
  * (they may be shared).  Tokens past a table's end, and those whose page id is
  * negative on either side, are not moved.  Cells behind the kept ones stay as
  * they were.  Bytes are copied as they are.  head_dim 64 or 128; alignments as in
- * the tree attention entries.  In place, flags in the per-stream workspace. */
+ * the tree attention entries.  In place, flags in the per-stream workspace: if
+ * another call's kernels write over them (graphs of one stream replayed at once,
+ * against the workspace's rule), cells may stay unmoved, and the next call of
+ * these entries or tq_launch_select_kv returns -2 and says so, once, having done
+ * nothing else. */
 int tq_launch_dense_compact_kv(uint8_t* page_pool, const int32_t* block_tables,
                                int max_blocks_per_seq, const int32_t* kept, int budget,
                                const int32_t* out_block_tables, int out_max_blocks_per_seq,

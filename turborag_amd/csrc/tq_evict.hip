@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "tq_device.h"
@@ -302,6 +303,8 @@ struct CompactArgs {
     int H, block_size;
     long long rows;      // sequences * kv heads
     uint32_t* state;     // in place: [row] its next ticket, [rows + row * chunks + c] reads done
+    uint32_t* lost;      // in place: host memory, set where chunks stay unwritten; or null
+    int polls;           // in place: of a wait, at most
 };
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -309,7 +312,8 @@ typedef uint32_t u4a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kMoveThreads = 256, kMoveDeep = 8;
 // Waits of some microseconds are given up after about a second, which takes two graphs of one
-// stream replayed at once, against the rule: their cells are wrong then, but both end.
+// stream replayed at once, against the rule: both end, no cell that is still to be read is
+// written over, and the next call says that cells were not moved.
 constexpr int kMostPolls = 1 << 20;
 
 // Cells of whole cache lines go past the caches (dense, 32 sequences to 4,096 tokens each,
@@ -323,6 +327,10 @@ __device__ __forceinline__ void store_unit(uint8_t* p, u4 v) {
         *reinterpret_cast<u4a2*>(p) = v;
 }
 
+__device__ __forceinline__ void say_lost(const CompactArgs& a) {
+    if (a.lost) __hip_atomic_store(a.lost, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
 // U: 16-byte units of a K (V) cell; NS: scales; chunk tokens so that a thread has eight units.
 template <int U, int NS, bool IN_PLACE>
 __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactArgs a) {
@@ -332,17 +340,23 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactA
     constexpr uint64_t kNone = ~0ull;
     __shared__ uint64_t page[2][T];  // the page's offset, from and to (kNone: not moved)
     __shared__ uint32_t cell[2][T];
-    __shared__ uint32_t ticket;
+    __shared__ uint32_t ticket, gave_up;
     const int tid = threadIdx.x;
     const long long b = (long long)blockIdx.y * gridDim.x + blockIdx.x;
     if (b >= a.rows * a.chunks) return;
     const long long row = b / a.chunks;
     int c = (int)(b - row * a.chunks);
     if constexpr (IN_PLACE) {
-        if (tid == 0) ticket = atomicAdd(&a.state[row], 1u);
+        if (tid == 0) {
+            ticket = atomicAdd(&a.state[row], 1u);
+            gave_up = 0;
+        }
         __syncthreads();
         // (state that another call's kernels share may hold any bits: nothing out of bounds)
-        if (ticket >= (uint32_t)a.chunks) return;
+        if (ticket >= (uint32_t)a.chunks) {
+            if (tid == 0) say_lost(a);
+            return;
+        }
         c = (int)ticket;
     }
     const int s = (int)(row / a.H), h = (int)(row - (long long)s * a.H);
@@ -398,12 +412,19 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_kernel(const CompactA
         __syncthreads();
         if (tid == 0) __hip_atomic_store(&done[c], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         for (int k = tid; k < c; k += kMoveThreads)  // (unsigned: a hole in kept counts as any token)
-            if (kept[k * T] < (c + 1) * T && (uint32_t)kept[k * T + T - 1] >= (uint32_t)(c * T))
-                for (int polls = 0; polls < kMostPolls; ++polls) {
+            if (kept[k * T] < (c + 1) * T && (uint32_t)kept[k * T + T - 1] >= (uint32_t)(c * T)) {
+                int polls = 0;
+                for (; polls < a.polls; ++polls) {
                     if (__hip_atomic_load(&done[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) break;
                     __builtin_amdgcn_s_sleep(1);
                 }
+                if (polls >= a.polls) gave_up = 1;
+            }
         __syncthreads();
+        if (gave_up) {
+            if (tid == 0) say_lost(a);
+            return;
+        }
     }
 #pragma unroll
     for (int k = 0; k < kMoveDeep; ++k) {
@@ -433,6 +454,39 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* p, long long n, lo
 
 // What tests set (tq_test_compact).
 std::atomic<uint32_t> g_first_ticket{0};
+std::atomic<int> g_polls{kMostPolls};
+
+// A word of host memory for all calls, which kernels write if they leave cells unmoved.  Never
+// freed: graphs hold it.  (Also made within a capture, which nothing that is not recorded ends
+// in the relaxed mode; none to be had: nothing is said.)
+std::atomic<uint32_t*> g_lost{nullptr};
+uint32_t* lost_word() {
+    uint32_t* p = g_lost.load(std::memory_order_acquire);
+    if (p) return p;
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    if ((p = g_lost.load(std::memory_order_acquire))) return p;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    void* mem = nullptr;
+    if (hipHostMalloc(&mem, sizeof(uint32_t), hipHostMallocPortable | hipHostMallocMapped) != hipSuccess) mem = nullptr;
+    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (!mem) {
+        (void)hipGetLastError();
+        return nullptr;
+    }
+    p = static_cast<uint32_t*>(mem);
+    *p = 0;
+    g_lost.store(p, std::memory_order_release);
+    return p;
+}
+// Once for all that were lost before.
+void report_lost() {
+    uint32_t* p = g_lost.load(std::memory_order_acquire);
+    if (p && __atomic_load_n(p, __ATOMIC_RELAXED) && __atomic_exchange_n(p, 0u, __ATOMIC_RELAXED))
+        throw Error("compact_kv: an earlier in-place call left cells unmoved, because another call's kernels wrote over its "
+                    "workspace (graphs of one stream replayed at once?); this call did nothing");
+}
 
 dim3 grid_of(long long blocks) {
     const unsigned x = (unsigned)std::min<long long>(blocks, 1 << 23);
@@ -452,6 +506,8 @@ void launch_move(CompactArgs a, bool in_place, hipStream_t stream) {
     }
     const WorkspaceTurn turn(stream);
     const long long words = a.rows + blocks;
+    a.lost = lost_word();
+    a.polls = g_polls.load(std::memory_order_relaxed);
     a.state = static_cast<uint32_t*>(Scratch{}.get(stream, (size_t)words * 4, "compact_kv"));
     hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<long long>((words + 255) / 256, 1024)), dim3(256), 0, stream,
                        a.state, words, a.rows, g_first_ticket.load(std::memory_order_relaxed));
@@ -466,6 +522,7 @@ bool aligned(const void* p, uint64_t a) { return aligned(reinterpret_cast<uintpt
 template <class F>
 int evict_entry(void* stream, F&& f) {
     try {
+        report_lost();
         f();
         debug_sync(stream);
         return 0;
@@ -544,9 +601,10 @@ void take_geom(CompactArgs& a, const PageGeom& g) {
 }  // namespace tq
 
 // For tests: the first ticket of in-place moves (0, but for a workspace that another call's
-// kernels have written over).
-extern "C" __attribute__((visibility("default"))) int tq_test_compact(uint32_t first_ticket) {
+// kernels have written over), and the polls after which a wait is given up (< 0: as ever).
+extern "C" __attribute__((visibility("default"))) int tq_test_compact(uint32_t first_ticket, int polls) {
     tq::g_first_ticket.store(first_ticket);
+    tq::g_polls.store(polls < 0 ? tq::kMostPolls : polls);
     return 0;
 }
 
