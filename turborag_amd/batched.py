@@ -30,7 +30,10 @@ from turborag_amd.turboquant_wrapper import BlockTable, PageAllocator, TurboQuan
 class PagedBatch:
     def __init__(self, tq: TurboQuantWrapper, scheme: str, lens, widths, *, kv_heads: int = 2,
                  q_heads: int = 16, head_dim: int = 128, block_size: int = 16, seed: int = 500,
-                 device: torch.device | None = None) -> None:
+                 device: torch.device | None = None, capacity: int = 0) -> None:
+        """lens cached tokens and widths new ones of every sequence.  capacity: the tokens that a
+        sequence may come to hold (a budget and a step's new tokens), for which there are pages;
+        otherwise, for those of the first step and a page more for each."""
         self.tq, self.scheme = tq, scheme
         self.dev = device or torch.device("cuda", 0)
         self.lens = [int(x) for x in lens]
@@ -44,16 +47,27 @@ class PagedBatch:
         self.prod = scheme == "turbo_prod"
         self.layout = tq.make_layout_for(cfg) if self.prod else tq.make_mse_layout_for(cfg)
         B = block_size
-        pages = sum((L + w + B - 1) // B for L, w in zip(self.lens, self.widths)) + self.S
+        most = [max(L + w, capacity) for L, w in zip(self.lens, self.widths)]
+        pages = sum(self._pages(n) for n in most) + self.S
         self.pool = torch.zeros(pages * self.layout.page_size_bytes, dtype=torch.uint8,
                                 device=self.dev)
         self.alloc = PageAllocator(tq, self.layout.page_size_bytes, pages, device_pool=self.pool)
         self.table = BlockTable(self.alloc, B)
-        self.max_blocks = max((L + w + B - 1) // B for L, w in zip(self.lens, self.widths))
+        self.max_blocks = max(self._pages(n) for n in most)
         self.seed = seed
         self._prefill()
 
     # ── helpers ─────────────────────────────────────────────────────── #
+
+    def _held(self, s: int) -> int:
+        """Tokens that the block table holds of sequence s."""
+        try:
+            return self.table.num_tokens(s)
+        except KeyError:  # none so far
+            return 0
+
+    def _pages(self, tokens: int) -> int:
+        return (tokens + self.B - 1) // self.B
 
     def _pack(self, k: torch.Tensor, v: torch.Tensor, slots: list[int]) -> None:
         self._last_pack = (k.to(self.dev), v.to(self.dev),
@@ -87,9 +101,10 @@ class PagedBatch:
         self._pack(torch.cat(keys), torch.cat(vals), slots)
 
     def block_tables(self) -> torch.Tensor:
-        bt = torch.full((self.S, self.max_blocks), -1, dtype=torch.int32)
-        for s in range(self.S):
-            b = self.table.blocks(s)
+        """[S, max_blocks], or wider where a sequence has more pages by now; -1 behind them."""
+        blocks = [self.table.blocks(s) for s in range(self.S)]
+        bt = torch.full((self.S, max(self.max_blocks, *map(len, blocks))), -1, dtype=torch.int32)
+        for s, b in enumerate(blocks):
             bt[s, :len(b)] = torch.tensor(b, dtype=torch.int32)
         return bt.to(self.dev)
 
@@ -103,7 +118,12 @@ class PagedBatch:
 
     def append_new_tokens(self, seed: int) -> tuple[list, list]:
         """w_s new tokens per sequence, quantized into (newly allocated)
-        pages with one pack launch; returns the new K/V per sequence."""
+        pages with one pack launch; returns the new K/V per sequence.  Refused,
+        with nothing appended, where the pool has not the pages."""
+        need = sum(self._pages(self._held(s) + w) - self._pages(self._held(s)) for s, w in enumerate(self.widths))
+        if need > self.alloc.num_free():
+            raise RuntimeError(f"append_new_tokens: out of blocks, {need} pages are needed, {self.alloc.num_free()} "
+                               "are free (capacity: tokens that a sequence may come to hold)")
         keys, vals, slots, new = [], [], [], []
         for s, w in enumerate(self.widths):
             k, v = kv_tokens_major(w, self.H, self.D, seed=seed + s)
@@ -164,12 +184,20 @@ class PagedBatch:
         """Cuts every sequence to at most `budget` tokens (its first `sink`, last
         `recent` and highest scores): cells and scores are moved to the front, and
         the pages behind go back to the allocator.  The sequences' tokens are those
-        that their block tables hold; new_widths: the new tokens of the next step.
-        Returns their lengths.  Positions go on from the tokens ever appended, not
-        from what is left."""
-        held = [self.table.num_tokens(s) for s in range(self.S)]
+        that their block tables hold; new_widths: the new tokens of the next step,
+        refused where the pool has not the pages.  Returns their lengths.  Positions
+        go on from the tokens ever appended, not from what is left."""
+        held = [self._held(s) for s in range(self.S)]
         if max(held) > scores.shape[-1] or max(held) > block_tables.shape[-1] * self.B:
             raise ValueError(f"evict: scores and block_tables must hold {max(held)} tokens")
+        left = [min(n, budget) for n in held]
+        if new_widths is not None:
+            new_widths = [int(x) for x in new_widths]
+            if len(new_widths) != self.S or min(new_widths) < 0:
+                raise ValueError(f"evict: new_widths must be {self.S} widths >= 0")
+            need = sum(self._pages(n + w) for n, w in zip(left, new_widths))
+            if need > self.alloc.num_pages:
+                raise ValueError(f"evict: new_widths need {need} pages, the pool has {self.alloc.num_pages}")
         # (allocated for the stream that uses them: their memory is given back on it)
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.dev) if stream
                                else torch.cuda.default_stream(self.dev)):
@@ -179,11 +207,12 @@ class PagedBatch:
                               stream=stream)
             self.tq.compact_kv(self.scheme, self.pool, block_tables, kept, self.layout, self.cfg,
                                stream=stream)
-        self.lens = [min(n, budget) for n in held]
+        self.lens = left
         for s, n in enumerate(self.lens):
-            self.table.truncate(s, n)
+            if n < held[s]:
+                self.table.truncate(s, n)
         if new_widths is not None:
-            self.widths = [int(x) for x in new_widths]
+            self.widths = new_widths
         return list(self.lens)
 
     def close(self) -> None:
