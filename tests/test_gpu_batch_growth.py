@@ -111,3 +111,38 @@ def test_new_widths_refused(tq, cuda, new_widths, match):
     batch.append_new_tokens(seed=953)
     assert [batch.table.num_tokens(s) for s in range(2)] == [62, 52]
     batch.close()
+
+
+def test_repack_after_an_eviction(tq, cuda):
+    """The last append's slots hold other tokens by then, or another sequence's pages: repack refuses
+    until the next append, whose tokens it stores again."""
+    batch = PagedBatch(tq, "turbo_prod", [90, 40], [2, 3], kv_heads=2, q_heads=8, head_dim=64)
+    batch.append_new_tokens(seed=954)
+    batch.repack()
+    scores = torch.rand(2, 2, 100, device=cuda)
+    before = _state(batch, scores)
+    assert batch.evict(scores, 92, batch.block_tables(), sink=2, recent=8) == [92, 43]
+    batch.repack()  # (nothing was evicted)
+    assert torch.equal(_state(batch, scores)[1], before[1])
+    batch.evict(scores, 32, batch.block_tables(), sink=2, recent=8)
+    before = _state(batch, scores)
+    with pytest.raises(RuntimeError, match="repack"):
+        batch.repack()
+    assert _same(_state(batch, scores), before)
+    batch.append_new_tokens(seed=955)
+    after = _state(batch, scores)
+    batch.repack()
+    assert _same(_state(batch, scores), after)
+    batch.close()
+
+
+def test_repack_after_a_refused_eviction(tq, cuda):
+    batch = PagedBatch(tq, "turbo_prod", [90, 40], [2, 3], kv_heads=2, q_heads=8, head_dim=64)
+    batch.append_new_tokens(seed=956)
+    scores = torch.rand(2, 2, 100, device=cuda)
+    before = _state(batch, scores)
+    with pytest.raises(RuntimeError):
+        batch.evict(scores, 8, batch.block_tables(), sink=4, recent=8)
+    batch.repack()
+    assert _same(_state(batch, scores), before)
+    batch.close()

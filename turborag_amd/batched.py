@@ -76,7 +76,10 @@ class PagedBatch:
 
     def repack(self, stream: int = 0) -> None:
         """Issue the last pack launch again (same tokens into the same slots:
-        idempotent), e.g. to time the append of a step."""
+        idempotent), e.g. to time the append of a step.  Not after an eviction of
+        any token: others lie in those slots then, or their pages are given back."""
+        if self._last_pack is None:
+            raise RuntimeError("repack: the last append's tokens have been moved by evict")
         k, v, s = self._last_pack
         (self.tq.pack if self.prod else self.tq.mse_pack)(k, v, s, self.pool, self.layout,
                                                           self.cfg, stream=stream)
@@ -207,6 +210,8 @@ class PagedBatch:
                               stream=stream)
             self.tq.compact_kv(self.scheme, self.pool, block_tables, kept, self.layout, self.cfg,
                                stream=stream)
+        if left != held:
+            self._last_pack = None
         self.lens = left
         for s, n in enumerate(self.lens):
             if n < held[s]:
