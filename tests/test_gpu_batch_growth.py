@@ -146,3 +146,20 @@ def test_repack_after_a_refused_eviction(tq, cuda):
     batch.repack()
     assert _same(_state(batch, scores), before)
     batch.close()
+
+
+@pytest.mark.parametrize("change,match", [
+    (lambda bt: bt.long(), "int32"), (lambda bt: bt.cpu(), "GPU tensor"), (lambda bt: bt[:1], "kept must be"),
+    (lambda bt: bt.repeat_interleave(2, 1)[:, ::2], "contiguous"), (lambda bt: bt[None], "2 dimensions")])
+def test_tables_refused_before_scores_move(tq, cuda, change, match):
+    """What the move would refuse is refused before the selection moves the scores."""
+    batch = PagedBatch(tq, "turbo_mse", [90, 40], [2, 3], kv_heads=2, q_heads=8, head_dim=64)
+    batch.append_new_tokens(seed=957)
+    bt = batch.block_tables()
+    scores = torch.rand(2, 2, 100, device=cuda)
+    before = _state(batch, scores)
+    with pytest.raises(ValueError, match=match):
+        batch.evict(scores, 32, change(bt), sink=2, recent=8)
+    assert _same(_state(batch, scores), before)
+    assert batch.evict(scores, 32, bt, sink=2, recent=8) == [32, 32]
+    batch.close()

@@ -206,6 +206,7 @@ class PagedBatch:
                                else torch.cuda.default_stream(self.dev)):
             kept = torch.empty(self.S, self.H, budget, dtype=torch.int32, device=self.dev)
             lens = torch.tensor(held, dtype=torch.int32, device=self.dev)
+            self.tq._compact_checks(self.scheme, self.pool, block_tables, kept, self.cfg)  # before scores move
             self.tq.select_kv(scores, lens, kept, sink=sink, recent=recent, out_scores=scores,
                               stream=stream)
             self.tq.compact_kv(self.scheme, self.pool, block_tables, kept, self.layout, self.cfg,

@@ -1070,11 +1070,8 @@ class TurboQuantWrapper:
         if rc != 0:
             self._kernel_raise(rc, "evict", op)
 
-    def compact_kv(self, scheme: str, page_pool, block_tables, kept, layout, cfg,
-                   out_block_tables=None, stream: int = 0) -> None:
-        """Moves the kept tokens' cells (select_kv's kept [num_seqs, H, budget]) to the
-        front of their sequences: in place, or (out_block_tables [num_seqs, blocks])
-        into other pages, the originals staying as they are."""
+    def _compact_checks(self, scheme, page_pool, block_tables, kept, cfg, out_block_tables=None):
+        """compact_kv's checks; its entry."""
         op = "compact_kv"
         fn = self._compact.get(scheme)
         if fn is None:
@@ -1099,6 +1096,15 @@ class TurboQuantWrapper:
             wants["out_block_tables"] = (out_block_tables, torch.int32, 0)
         if not self._fit(dev, wants.values()) or dev < 0 or dev != torch.cuda.current_device():
             self._refuse(scheme, op, dev, wants)
+        return fn
+
+    def compact_kv(self, scheme: str, page_pool, block_tables, kept, layout, cfg,
+                   out_block_tables=None, stream: int = 0) -> None:
+        """Moves the kept tokens' cells (select_kv's kept [num_seqs, H, budget]) to the
+        front of their sequences: in place, or (out_block_tables [num_seqs, blocks])
+        into other pages, the originals staying as they are."""
+        fn = self._compact_checks(scheme, page_pool, block_tables, kept, cfg, out_block_tables)
+        S, blocks = block_tables.shape
         if S == 0:
             return
         out, out_blocks = None, 0
@@ -1107,7 +1113,7 @@ class TurboQuantWrapper:
         rc = fn(page_pool.data_ptr(), block_tables.data_ptr(), blocks, kept.data_ptr(), kept.shape[2],
                 out, out_blocks, ctypes.byref(layout), ctypes.byref(cfg), S, self._stream(stream))
         if rc != 0:
-            self._kernel_raise(rc, scheme, op)
+            self._kernel_raise(rc, scheme, "compact_kv")
 
     # ── the reference's unexported kernels ──────────────────────────── #
     # QJL-1b (include/tq_qjl.cuh), legacy INT4 (include/tq_layout.h), dense
