@@ -271,7 +271,7 @@ def test_uneven_rows(tq, cuda, scheme, dtype, D):
 
 
 @pytest.mark.parametrize("scheme,dtype", SCHEMES)
-def test_many_sequences(tq, cuda, scheme, dtype):
+def test_many_sequences_on_large_workgroups(tq, cuda, scheme, dtype):
     """Workgroups enough for large ones in the sum over stored rows."""
     Weights(tq, scheme, dtype, [1500] + [20] * 70, [1] * 71, 16, 8, 64, seed=22, before=True).check(cuda)
 
