@@ -609,9 +609,10 @@ int tq_launch_turbo_mse_tree_attention(const uint16_t* query, const uint8_t* pag
  * attention entries.  num_seqs 0 does nothing; num_tokens * num_q_heads <= 2^25;
  * ceil(max_kv_len / 128) times that, or times num_seqs * H, at most 2^30.  The
  * per-stream workspace holds the rows' statistics (8 bytes for each row and 128
- * or 256 tokens), compressed pages' rotated queries (4 D + 4 bytes a row) and,
- * where that is the faster way, the logits, up to 256 MB: a capture needs an
- * earlier call with the same sizes on its stream. */
+ * or 256 tokens: 1.1 GB for 32,768 tokens of 16 heads over as many), compressed
+ * pages' rotated queries (4 D + 4 bytes a row) and, where that is the faster way,
+ * the logits, up to 256 MB (4 bytes for each row and token below max_kv_len): a
+ * capture needs an earlier call with the same sizes on its stream. */
 int tq_launch_dense_attention_weights(
     const void* query, const uint8_t* page_pool, const int32_t* block_tables,
     int max_blocks_per_seq, const int32_t* row_start, const int32_t* prefix_len, int causal,

@@ -189,7 +189,8 @@ class PagedBatch:
         the pages behind go back to the allocator.  The sequences' tokens are those
         that their block tables hold; new_widths: the new tokens of the next step,
         refused where the pool has not the pages.  Returns their lengths.  Positions
-        go on from the tokens ever appended, not from what is left."""
+        go on from the tokens ever appended, not from what is left.  (On another
+        stream: an append, which stores on the default one, waits for it first.)"""
         held = [self._held(s) for s in range(self.S)]
         if max(held) > scores.shape[-1] or max(held) > block_tables.shape[-1] * self.B:
             raise ValueError(f"evict: scores and block_tables must hold {max(held)} tokens")

@@ -292,7 +292,8 @@ __global__ __launch_bounds__(64 * WAVES) void select_kv_kernel(const SelectArgs 
 // head)'s chunks are taken by tickets in that order, so what a workgroup waits for has
 // begun, and reads wait for nothing: every wait ends.  (Dense, 32
 // sequences to 4,096 tokens in place: 92.7 us with one counter for all, 81.9 with one each,
-// 78.9 without the waits that are not needed; into other pages 54.)
+// 78.9 without the waits that are not needed.  The kernel alone 72, into other pages 56;
+// turbo_prod 30 and 26: what is left is read, then waited for, then written in turn.)
 // ---------------------------------------------------------------------------
 struct CompactArgs {
     uint8_t* pool;

@@ -422,10 +422,14 @@ __device__ __forceinline__ float largest(const f4 (&x)[TT]) {
 // Bound by: memory with few rows of dense pages (32 sequences, 540K tokens, 8 rows: 277 MB of
 // K and 35 MB of x in 62.5 us, 5.0 TB/s); latency where a workgroup has one chunk and
 // its rows (256 rows of 32K tokens: 17 us a launch, of which the products and exponentials
-// are 5 to 6); for compressed pages decode and matrix instructions, five products where dense
-// keys have one (64 rows of 32 sequences to 8K tokens: 39 us, vector units 34% busy, matrix
-// cores 20%).  A key is decoded 32 dims at a time for all rows of a block, so that three or
-// four waves of a SIMD have registers (32 rows, 32 x 8K tokens: 51.6 -> 46.0 us with the sum).
+// are 5 to 6); for compressed pages latency at few waves, one chain page ids -> codes -> decode
+// -> products after the other (64 rows of 32 sequences to 8K tokens: 39 us at two waves a SIMD,
+// which issue in 41% of their cycles, wait for loads in 32% and for a free unit in 27%; vector
+// units 34% busy, matrix cores 20%: five products where dense keys have one).  A key is decoded
+// 32 dims at a time for all rows of a block, so that three or four waves of a SIMD have
+// registers where rows are fewer (32 rows, 32 x 8K tokens: 51.6 -> 46.0 us with the sum).
+// Rows that see nothing of a chunk are worked through as the others are: half of both passes
+// for a whole prompt (2,048 tokens without a prefix 234 us, 8,192 3,039).
 // ---------------------------------------------------------------------------
 constexpr int kStats = 0, kStore = 1, kSum = 2;
 template <int FMT, int D>
@@ -858,6 +862,9 @@ void launch_format(WeightArgs a, hipStream_t stream) {
     //             1 x 32K, 64: 27.0 / 24.2   128: 45.8 / 26.8   32 x 8K, 64: 64.1 / 78.0
     //   prod      1 x 2K, 512: 33.8 / 46.6   1 x 8K, 512: 51.1 / 85.6   8 x 4K, 256: 49.0 / 75.6
     //             1 x 32K, 64: 34.0 / 32.2   128: 54.3 / 45.5   32 x 8K, 64: 68.0 / 91
+    // Not past 256 MB, which are counted by max_kv for every row: with few rows K's second reading
+    // costs far more there, as its blocks are made for many (dense, 8 rows: 32 x 8K tokens 36.5, and
+    // one of 120,000 more 72.7, of 131,072 211; 64 x 16,000, 64 heads on 8 523, 64 x 16,500 1,393).
     const size_t stored = rows * padded * 4;
     const bool store = stored <= (size_t(256) << 20) &&
                        (per_seq <= 64 || (kTurned ? a.max_kv <= 16384 : stored <= (size_t(4) << 20)));
