@@ -485,8 +485,8 @@ uint32_t* lost_word() {
 void report_lost() {
     uint32_t* p = g_lost.load(std::memory_order_acquire);
     if (p && __atomic_load_n(p, __ATOMIC_RELAXED) && __atomic_exchange_n(p, 0u, __ATOMIC_RELAXED))
-        throw Error("compact_kv: an earlier in-place call left cells unmoved, because another call's kernels wrote over its "
-                    "workspace (graphs of one stream replayed at once?); this call did nothing");
+        throw Error("compact_kv: an earlier in-place call left cells unmoved, because another call's kernels wrote over "
+                    "its workspace (graphs of one stream replayed at once?); this call did nothing");
 }
 
 dim3 grid_of(long long blocks) {
